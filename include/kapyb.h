@@ -498,6 +498,165 @@ KAPYB_API kapyb_status kapyb_reduce(kapyb_handle h, const kapyb_tensor2d *src,
                                     const kapyb_tensor2d *dst, int32_t axis,
                                     int32_t combiner, void *stream);
 
+/* -------------------------------------- rows that pick their weights
+ *
+ * Matmuls in which every row names the weights it is multiplied by: tokens routed
+ * to experts, requests with adapters of their own.  No counterpart in the
+ * reference, whose matmul has one rhs per program; these calls stand beside
+ * kapyb_matmul and kapyb_reduce for callers that serve or train such models.
+ *
+ * A training or serving step strings them together:
+ *     kapyb_route         logits [T,E]          -> weights, experts [T,k]
+ *     kapyb_plan_rows     experts as index[T*k] -> order, offsets, slots
+ *     kapyb_matmul_grouped  x, W1 (gathered through order, gate and up fused) -> h [T*k, I]
+ *     kapyb_matmul_grouped  h, W2 (rows already in plan order)                -> y [T*k, N]
+ *     kapyb_combine_rows  y, slots, weights     -> out [T, N]
+ * and backwards kapyb_combine_rows_backward, kapyb_matmul_grouped with transposed
+ * weight descriptors (gradient of the rows), kapyb_matmul_grouped_grad (gradient of
+ * the weights), kapyb_combine_rows without weights (sum over a token's rows) and
+ * kapyb_route_backward.  A plan serves every product of the step.
+ *
+ * Integer and f32 arrays passed as plain pointers are dense device arrays aligned
+ * to their element size.  The calls keep no state between them, use no handle
+ * workspace and may be captured into a graph; `stream` must belong to the handle's
+ * device, whichever device is current.  Indices, orders and offsets are read on the
+ * device and may hold anything: one that leads outside its tensor names no group /
+ * a row of zeros, and no memory outside the tensors is touched.  Outputs must not
+ * overlap inputs (KAPYB_INVALID_ARG where the descriptors show it). */
+
+typedef enum {
+  KAPYB_SCORE_SOFTMAX = 0,
+  KAPYB_SCORE_SIGMOID = 1
+} kapyb_score;
+
+typedef struct {
+  int32_t score;       /* kapyb_score */
+  int32_t top_k;       /* experts per row: 1 .. 32, at most the number of experts */
+  int32_t n_groups;    /* adjacent experts form groups of equal size: 1 .. 32 (1: no groups) */
+  int32_t top_groups;  /* only the experts of this many groups can be chosen */
+  int32_t group_best;  /* a group's rank is its best selection score (1) or the sum of its
+                          two best (2) */
+  int32_t renormalize; /* weights are divided by the sum of the chosen scores */
+  float scale;         /* weights are multiplied by this last */
+} kapyb_routing;
+
+/* Routing of rows to experts.  s = softmax(logits row) or sigmoid(logit), formed in
+ * f32; selection scores c = s + bias (bias: f32 [experts], NULL = none; it decides
+ * who is chosen and is not part of the weights).  experts[t][j] is the expert with
+ * the j-th largest c of row t among the kept groups, ties (of experts and of
+ * groups) go to the lower index, and weights[t][j] = scale * s of it, renormalised
+ * if asked.  The ranking is that of exactly evaluated scores: without a bias the
+ * logits themselves are compared, and where 32 bits cannot tell two scores apart the
+ * row is decided in 64 bits.
+ * A logit of -inf masks its expert: score 0, never chosen.  Where fewer than top_k
+ * experts are left the remaining entries are expert -1, weight 0 (a row of -inf, the
+ * padding of a batch, names no expert at all).  A row with a NaN or +inf logit under
+ * softmax has NaN weights; a NaN score ranks behind every number.
+ * logits: f16 / bf16 / f32 [rows, experts], any strides, up to 1024 experts.
+ * weights f32 and experts int32: dense [rows, top_k]. */
+KAPYB_API kapyb_status kapyb_route(kapyb_handle h, const kapyb_tensor2d *logits, const float *bias,
+                                   const kapyb_routing *routing, float *weights, int32_t *experts,
+                                   void *stream);
+
+/* Gradient of the logits: logits and experts as kapyb_route had and gave them,
+ * grad_weights f32 [rows, top_k], grad_logits f16 / bf16 / f32 [rows, experts], any
+ * strides, written whole.  The choice itself and the bias have no gradient; masked
+ * experts get 0, and so do experts that were not chosen except under a softmax that
+ * is not renormalised.  An expert named twice counts twice, an index outside
+ * 0 .. experts-1 not at all. */
+KAPYB_API kapyb_status kapyb_route_backward(kapyb_handle h, const kapyb_tensor2d *logits,
+                                            const kapyb_routing *routing, const int32_t *experts,
+                                            const float *grad_weights,
+                                            const kapyb_tensor2d *grad_logits, void *stream);
+
+/* Stable counting sort of index[n] into `groups` (1 .. 1024) groups.  order[n]: the
+ * entries of group 0 in ascending order, then group 1's, ...; offsets[groups + 1]:
+ * group g holds positions offsets[g] .. offsets[g+1]-1, offsets[groups] = planned
+ * entries; slots[n] (may be NULL): the position of each entry.  An index outside
+ * 0 .. groups-1 is not planned: slot -1, and order is -1 behind the last planned
+ * position.  n may be 0. */
+KAPYB_API kapyb_status kapyb_plan_rows(kapyb_handle h, const int32_t *index, int32_t n,
+                                       int32_t groups, int32_t *order, int32_t *offsets,
+                                       int32_t *slots, void *stream);
+
+/* out[p] = epilogue(lhs[row(p)] . rhs of p's group) for the planned positions p:
+ * group g holds positions offsets[g] .. offsets[g+1]-1 (device, int32 [groups+1], not
+ * decreasing, at most out->size0), row(p) = order[p] / fan, or p itself when order is
+ * NULL (then fan is ignored).  fan = rows of the plan per row of lhs (the k of a top-k
+ * routing whose index has k entries per token).  A row of lhs that does not exist
+ * counts as zeros.  Rows of out behind the last planned position keep what they hold.
+ * rhs describes ONE group's [K, N] weights, group g starting g * group_stride elements
+ * later; either axis may have the unit stride, so a transposed descriptor computes the
+ * gradient of the rows: out = grad . W^T.
+ * gated != 0: rhs has 2 N columns, gate then up, and the result is
+ * activation(gate) * up, each with its own scale and bias.  epilogue: alpha, bias
+ * (dense [groups, columns of rhs], bias_axis 1), activation, rounding; NULL = none.
+ * lhs and rhs: both f16, both bf16 (tensor cores) or both f32 (CUDA cores, multiplied
+ * as f32), out f16 / bf16 / f32; sums in f32.  16-bit operands with 16-byte aligned
+ * bases, leading dimensions and group stride, lhs with unit stride on K, run on
+ * tcgen05; any other strides run on CUDA cores.  Up to 1024 groups.  The same bits on
+ * every run. */
+KAPYB_API kapyb_status kapyb_matmul_grouped(kapyb_handle h, const kapyb_tensor2d *lhs,
+                                            const kapyb_tensor2d *rhs, int32_t groups,
+                                            int64_t group_stride, const int32_t *offsets,
+                                            const int32_t *order, int32_t fan,
+                                            const kapyb_tensor2d *out,
+                                            const kapyb_epilogue *epilogue, int32_t gated,
+                                            void *stream);
+
+/* Gradient of the groups' weights: out[g] = alpha * sum over group g's positions p of
+ * lhs[row(p)]^T grad[p], [K, N] per group (g * out_group_stride elements apart), zeros
+ * for a group without rows.  lhs [source rows, K], grad [positions, N] (f16, bf16 or
+ * f32, of one type), offsets / order / fan as in kapyb_matmul_grouped; a position whose
+ * row does not exist adds nothing.  Sums in f32, rounded once to out's type. */
+KAPYB_API kapyb_status kapyb_matmul_grouped_grad(kapyb_handle h, const kapyb_tensor2d *lhs,
+                                                 const kapyb_tensor2d *grad, int32_t groups,
+                                                 const int32_t *offsets, const int32_t *order,
+                                                 int32_t fan, const kapyb_tensor2d *out,
+                                                 int64_t out_group_stride, float alpha,
+                                                 int32_t rounding, void *stream);
+
+/* out[t] = sum_j weights[t][j] * rows[slots[t][j]], j < k <= 32, summed in f32 in
+ * ascending j.  slots int32 [tokens, k] (a slot outside 0 .. rows-1 adds nothing and is
+ * not read), weights f32 [tokens, k] or NULL (all one).  rows [positions, N] and out
+ * [tokens, N]: f16 / bf16 / f32, any strides. */
+KAPYB_API kapyb_status kapyb_combine_rows(kapyb_handle h, const kapyb_tensor2d *rows,
+                                          const int32_t *slots, int32_t k, const float *weights,
+                                          const kapyb_tensor2d *out, void *stream);
+
+/* Gradients of kapyb_combine_rows: grad_rows[slots[t][j]] = weights[t][j] * grad_out[t]
+ * (a slot must not occur twice; rows that no slot names keep what they hold) and
+ * grad_weights[t][j] = <grad_out[t], rows[slots[t][j]]> (0 where the slot names no row).
+ * Either may be NULL; rows may be NULL without grad_weights. */
+KAPYB_API kapyb_status kapyb_combine_rows_backward(kapyb_handle h, const kapyb_tensor2d *rows,
+                                                   const int32_t *slots, int32_t k,
+                                                   const float *weights,
+                                                   const kapyb_tensor2d *grad_out,
+                                                   const kapyb_tensor2d *grad_rows,
+                                                   float *grad_weights, void *stream);
+
+/* A shared projection with low-rank adapters of many requests beside it:
+ *     out[t] = epilogue( lhs[t] . rhs ) with scale[i] * (lhs[t] . down[i]) . up[i]
+ * added before the activation, i = index[t] (int32 [rows]); an index outside
+ * 0 .. groups-1 means no adapter.  rhs [K, N]; down / up describe adapter 0's [K, rank]
+ * and [rank, N], the next ones down_stride / up_stride elements later; scale f32
+ * [groups] or NULL (1).  rank 1 .. 128.  alpha and bias apply to the shared part, as
+ * in kapyb_matmul.  lhs, rhs, down, up: all f16, all bf16 or all f32; out f16 / bf16 /
+ * f32.  The inner product lhs . down is kept to at least 16 bits of precision and the
+ * whole sum is formed in f32.  An inference operator: it has no gradient here (rhs,
+ * down and up of a training step are ordinary kapyb_matmul problems).
+ * scratch: device memory of kapyb_matmul_adapters_scratch() bytes, 256-byte aligned,
+ * the call's own until it has run on `stream`. */
+KAPYB_API kapyb_status kapyb_matmul_adapters(kapyb_handle h, const kapyb_tensor2d *lhs,
+                                             const kapyb_tensor2d *rhs, int32_t groups,
+                                             const kapyb_tensor2d *down, int64_t down_stride,
+                                             const kapyb_tensor2d *up, int64_t up_stride,
+                                             const int32_t *index, const float *scale,
+                                             const kapyb_tensor2d *out,
+                                             const kapyb_epilogue *epilogue, void *scratch,
+                                             size_t scratch_bytes, void *stream);
+KAPYB_API size_t kapyb_matmul_adapters_scratch(int32_t rows, int32_t groups, int32_t rank);
+
 /* ------------------------------------------------------------- shard math */
 
 /* Range [begin, end) of `total` units owned by `rank` of `parts` when units

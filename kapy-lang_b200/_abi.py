@@ -33,6 +33,8 @@ RZ, RN = 0, 1
 ACT_NONE, ACT_RELU, ACT_GELU_TANH, ACT_SILU = 0, 1, 2, 3
 # kapyb_combiner
 RED_ADD, RED_MUL, RED_MAX, RED_MIN = 0, 1, 2, 3
+# kapyb_score
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 # kapyb_matmul_impl_way (Enums.td:90-100)
 MMA_ANY, MMA_M16N8K8_F16, MMA_M16N8K16_F16, MMA_M16N8K8_TF32, MMA_M16N8K16_F8 = 0, 1, 2, 3, 4
 
@@ -71,6 +73,12 @@ class Inst(C.Structure):
     _fields_ = [("op", C.c_int32), ("dtype", C.c_int32), ("dst", C.c_int32),
                 ("a", C.c_int32), ("b", C.c_int32), ("c", C.c_int32),
                 ("imm", C.c_float), ("flags", C.c_int32)]
+
+
+class Routing(C.Structure):
+    _fields_ = [("score", C.c_int32), ("top_k", C.c_int32), ("n_groups", C.c_int32),
+                ("top_groups", C.c_int32), ("group_best", C.c_int32),
+                ("renormalize", C.c_int32), ("scale", C.c_float)]
 
 
 # name -> (restype, argtypes); every symbol include/kapyb.h declares.
@@ -112,6 +120,31 @@ PROTOTYPES = {
                                     C.c_int32, C.POINTER(Tensor2d), C.c_void_p]),
     "kapyb_reduce": (C.c_int, [C.c_void_p, C.POINTER(Tensor2d), C.POINTER(Tensor2d), C.c_int32,
                                C.c_int32, C.c_void_p]),
+    "kapyb_route": (C.c_int, [C.c_void_p, C.POINTER(Tensor2d), C.c_void_p, C.POINTER(Routing),
+                              C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kapyb_route_backward": (C.c_int, [C.c_void_p, C.POINTER(Tensor2d), C.POINTER(Routing),
+                                       C.c_void_p, C.c_void_p, C.POINTER(Tensor2d), C.c_void_p]),
+    "kapyb_plan_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
+                                  C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kapyb_matmul_grouped": (C.c_int, [C.c_void_p, C.POINTER(Tensor2d), C.POINTER(Tensor2d),
+                                       C.c_int32, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32,
+                                       C.POINTER(Tensor2d), C.POINTER(Epilogue), C.c_int32,
+                                       C.c_void_p]),
+    "kapyb_matmul_grouped_grad": (C.c_int, [C.c_void_p, C.POINTER(Tensor2d), C.POINTER(Tensor2d),
+                                            C.c_int32, C.c_void_p, C.c_void_p, C.c_int32,
+                                            C.POINTER(Tensor2d), C.c_int64, C.c_float, C.c_int32,
+                                            C.c_void_p]),
+    "kapyb_combine_rows": (C.c_int, [C.c_void_p, C.POINTER(Tensor2d), C.c_void_p, C.c_int32,
+                                     C.c_void_p, C.POINTER(Tensor2d), C.c_void_p]),
+    "kapyb_combine_rows_backward": (C.c_int, [C.c_void_p, C.POINTER(Tensor2d), C.c_void_p,
+                                              C.c_int32, C.c_void_p, C.POINTER(Tensor2d),
+                                              C.POINTER(Tensor2d), C.c_void_p, C.c_void_p]),
+    "kapyb_matmul_adapters": (C.c_int, [C.c_void_p, C.POINTER(Tensor2d), C.POINTER(Tensor2d),
+                                        C.c_int32, C.POINTER(Tensor2d), C.c_int64,
+                                        C.POINTER(Tensor2d), C.c_int64, C.c_void_p, C.c_void_p,
+                                        C.POINTER(Tensor2d), C.POINTER(Epilogue), C.c_void_p,
+                                        C.c_size_t, C.c_void_p]),
+    "kapyb_matmul_adapters_scratch": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
     "kapyb_shard_range": (C.c_int, [C.c_int64, C.c_int32, C.c_int32, C.c_int64,
                                     C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
     "kapyb_last_kernel": (C.c_char_p, [C.c_void_p]),

@@ -1,0 +1,693 @@
+// C ABI of the operators whose rows pick their weights (include/kapyb.h): argument
+// checks, choice of kernel and launch.  The arithmetic lives in route.cuh,
+// plan_rows.cuh, combine_rows.cuh, rows_simt.cuh and grouped_sm100.cuh.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "../../include/kapyb.h"
+#include "combine_rows.cuh"
+#include "context.cuh"
+#include "plan_rows.cuh"
+#include "route.cuh"
+#include "rows_simt.cuh"
+
+using namespace kapyb;
+
+namespace {
+
+// Launches go to the handle's device; the caller's current device comes back on the
+// way out.
+class OnDevice {
+ public:
+  explicit OnDevice(kapyb_handle h) {
+    error_ = cudaGetDevice(&before_);
+    if (error_ == cudaSuccess && before_ != h->device) {
+      error_ = cudaSetDevice(h->device);
+      moved_ = error_ == cudaSuccess;
+    }
+  }
+  ~OnDevice() {
+    if (moved_) cudaSetDevice(before_);
+  }
+  cudaError_t error() const { return error_; }
+
+ private:
+  int before_ = 0;
+  bool moved_ = false;
+  cudaError_t error_ = cudaSuccess;
+};
+
+// The arguments are checked before the handle, so that the checks need no GPU.
+#define HAVE_HANDLE(h) \
+  if (!h) return fail(nullptr, KAPYB_INVALID_ARG, "%s: NULL handle", call)
+
+#define ON_DEVICE(h)       \
+  HAVE_HANDLE(h);          \
+  OnDevice on_device_(h);  \
+  CUDA_TRY(h, on_device_.error())
+
+kapyb_status launched(kapyb_handle h, const char *name, int kernels = 1) {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(h, KAPYB_CUDA_ERROR, "%s: launch failed: %s", name, cudaGetErrorString(e));
+  h->last_kernel = name;
+  h->launches += kernels;
+  return KAPYB_OK;
+}
+
+bool empty(const kapyb_tensor2d *t) { return t->size0 == 0 || t->size1 == 0; }
+
+kapyb_status check_tensor(kapyb_handle h, const char *call, const char *what, const kapyb_tensor2d *t) {
+  if (!t) return fail(h, KAPYB_INVALID_ARG, "%s: %s is NULL", call, what);
+  if (t->size0 < 0 || t->size1 < 0 || t->stride0 < 0 || t->stride1 < 0 || t->offset_elems < 0)
+    return fail(h, KAPYB_INVALID_ARG, "%s: %s has a negative size, stride or offset", call, what);
+  if (!valid_dtype(t->dtype))
+    return fail(h, KAPYB_INVALID_ARG, "%s: %s must have f16, bf16 or f32 element type", call, what);
+  if (!t->ptr && !empty(t)) return fail(h, KAPYB_INVALID_ARG, "%s: %s has no data pointer", call, what);
+  if (reinterpret_cast<uintptr_t>(t->ptr) % dtype_size(t->dtype) != 0)
+    return fail(h, KAPYB_INVALID_ARG, "%s: %s is not aligned to its element size", call, what);
+  if (!valid_cache(t->cache))
+    return fail(h, KAPYB_INVALID_ARG, "%s: %s has an unknown cache operator or eviction priority", call, what);
+  return KAPYB_OK;
+}
+
+kapyb_status check_output(kapyb_handle h, const char *call, const char *what, const kapyb_tensor2d *t) {
+  const kapyb_status st = check_tensor(h, call, what, t);
+  if (st != KAPYB_OK) return st;
+  // two elements of an output must not share an address
+  const bool a = t->size0 > 1 && t->stride0 == 0, b = t->size1 > 1 && t->stride1 == 0;
+  if (a || b) return fail(h, KAPYB_INVALID_ARG, "%s: %s has a stride of 0", call, what);
+  return KAPYB_OK;
+}
+
+bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+// First and last byte behind a descriptor repeated `batch` times.
+struct Span {
+  uintptr_t lo, hi;
+};
+Span span_of(const kapyb_tensor2d *t, int64_t batch = 1, int64_t batch_stride = 0) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(elem_ptr(t));
+  if (empty(t) || batch == 0) return {lo, lo};
+  const int64_t last = (t->size0 - 1ll) * t->stride0 + (t->size1 - 1ll) * t->stride1 + (batch - 1) * batch_stride;
+  return {lo, lo + static_cast<uintptr_t>(last + 1) * dtype_size(t->dtype)};
+}
+Span span_of(const void *p, size_t bytes) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+  return {lo, p ? lo + bytes : lo};
+}
+bool meet(const Span &a, const Span &b) { return a.lo < a.hi && b.lo < b.hi && a.lo < b.hi && b.lo < a.hi; }
+
+bool rounding_ok(int r) { return r == KAPYB_RZ || r == KAPYB_RN; }
+
+kapyb_status check_epilogue(kapyb_handle h, const char *call, const kapyb_epilogue *ep) {
+  if (!ep) return KAPYB_OK;
+  if (ep->bias && !valid_dtype(ep->bias_dtype))
+    return fail(h, KAPYB_INVALID_ARG, "%s: bias must have f16, bf16 or f32 element type", call);
+  if (ep->bias_axis != 0 && ep->bias_axis != 1) return fail(h, KAPYB_INVALID_ARG, "%s: bias_axis must be 0 or 1", call);
+  if (ep->activation < KAPYB_ACT_NONE || ep->activation > KAPYB_ACT_SILU)
+    return fail(h, KAPYB_INVALID_ARG, "%s: unknown activation %d", call, ep->activation);
+  if (!rounding_ok(ep->rounding))
+    return fail(h, KAPYB_INVALID_ARG, "%s: rounding mode must be set for down cast", call);
+  return KAPYB_OK;
+}
+
+const kapyb_epilogue kPlainEpilogue = {1.0f, nullptr, KAPYB_F32, 1, KAPYB_ACT_NONE, KAPYB_RN};
+
+#define TRY(expr)                          \
+  do {                                     \
+    const kapyb_status st_ = (expr);       \
+    if (st_ != KAPYB_OK) return st_;       \
+  } while (0)
+
+// ------------------------------------------------------------------- routing
+
+kapyb_status check_routing(kapyb_handle h, const char *call, const kapyb_tensor2d *logits, const kapyb_routing *r) {
+  if (!r) return fail(h, KAPYB_INVALID_ARG, "%s: routing is NULL", call);
+  const int experts = logits->size1;
+  if (experts < 1 || experts > kRouteMaxExperts)
+    return fail(h, experts < 1 ? KAPYB_INVALID_ARG : KAPYB_UNSUPPORTED, "%s: 1 to %d experts (got %d)", call,
+                kRouteMaxExperts, experts);
+  if (r->score != KAPYB_SCORE_SOFTMAX && r->score != KAPYB_SCORE_SIGMOID)
+    return fail(h, KAPYB_INVALID_ARG, "%s: unknown score %d", call, r->score);
+  if (r->top_k < 1 || r->top_k > kRouteMaxTopK || r->top_k > experts)
+    return fail(h, KAPYB_INVALID_ARG, "%s: top_k must be 1 to %d and at most the number of experts (got %d of %d)",
+                call, kRouteMaxTopK, r->top_k, experts);
+  if (r->n_groups < 1 || r->n_groups > kRouteMaxGroups || experts % r->n_groups != 0)
+    return fail(h, KAPYB_INVALID_ARG, "%s: n_groups must be 1 to %d and divide the number of experts (got %d of %d)",
+                call, kRouteMaxGroups, r->n_groups, experts);
+  if (r->top_groups < 1 || r->top_groups > r->n_groups)
+    return fail(h, KAPYB_INVALID_ARG, "%s: top_groups must be 1 to n_groups (got %d of %d)", call, r->top_groups,
+                r->n_groups);
+  if (r->group_best != 1 && r->group_best != 2)
+    return fail(h, KAPYB_INVALID_ARG, "%s: group_best must be 1 or 2 (got %d)", call, r->group_best);
+  return KAPYB_OK;
+}
+
+RouteParams route_params(const kapyb_tensor2d *logits, const kapyb_routing *r) {
+  RouteParams p{};
+  p.x = elem_ptr(logits);
+  p.x_s0 = logits->stride0;
+  p.x_s1 = logits->stride1;
+  p.x_dtype = logits->dtype;
+  p.rows = logits->size0;
+  p.experts = logits->size1;
+  p.sigmoid = r->score == KAPYB_SCORE_SIGMOID;
+  p.top_k = r->top_k;
+  p.n_groups = r->n_groups;
+  p.group_size = logits->size1 / r->n_groups;
+  p.top_groups = r->top_groups;
+  p.group_best = r->group_best;
+  p.renormalize = r->renormalize != 0;
+  p.scale = r->scale;
+  return p;
+}
+
+// experts per lane, rounded up to a compiled width
+template <template <int> class Launch>
+void by_width(int experts, const RouteParams &p, int grid, cudaStream_t stream) {
+  if (experts <= 64) Launch<2>::go(p, grid, stream);
+  else if (experts <= 128) Launch<4>::go(p, grid, stream);
+  else if (experts <= 256) Launch<8>::go(p, grid, stream);
+  else if (experts <= 512) Launch<16>::go(p, grid, stream);
+  else Launch<32>::go(p, grid, stream);
+}
+template <int VPT>
+struct LaunchRoute {
+  static void go(const RouteParams &p, int grid, cudaStream_t s) { route_kernel<VPT><<<grid, 256, 0, s>>>(p); }
+};
+template <int VPT>
+struct LaunchRouteBackward {
+  static void go(const RouteParams &p, int grid, cudaStream_t s) { route_backward_kernel<VPT><<<grid, 256, 0, s>>>(p); }
+};
+
+int warp_grid(int rows) { return static_cast<int>((rows + 7ll) / 8); }
+
+}  // namespace
+
+extern "C" KAPYB_API kapyb_status kapyb_route(kapyb_handle h, const kapyb_tensor2d *logits, const float *bias,
+                                              const kapyb_routing *routing, float *weights, int32_t *experts,
+                                              void *stream) {
+  const char *call = "route";
+  TRY(check_tensor(h, "route", "logits", logits));
+  TRY(check_routing(h, "route", logits, routing));
+  if (logits->size0 == 0) {
+    HAVE_HANDLE(h);
+    return KAPYB_OK;
+  }
+  if (!weights || !experts) return fail(h, KAPYB_INVALID_ARG, "route: weights or experts is NULL");
+  if (!aligned4(weights) || !aligned4(experts) || !aligned4(bias))
+    return fail(h, KAPYB_INVALID_ARG, "route: bias, weights and experts must be 4-byte aligned");
+  const size_t bytes = static_cast<size_t>(logits->size0) * routing->top_k * 4;
+  const Span w = span_of(weights, bytes), e = span_of(experts, bytes), x = span_of(logits),
+             b = span_of(bias, static_cast<size_t>(logits->size1) * 4);
+  if (meet(w, e) || meet(w, x) || meet(e, x) || meet(w, b) || meet(e, b))
+    return fail(h, KAPYB_INVALID_ARG, "route: an output overlaps another tensor of the call");
+  ON_DEVICE(h);
+  RouteParams p = route_params(logits, routing);
+  p.bias = bias;
+  p.weights = weights;
+  p.chosen = experts;
+  by_width<LaunchRoute>(p.experts, p, warp_grid(p.rows), static_cast<cudaStream_t>(stream));
+  return launched(h, "route");
+}
+
+extern "C" KAPYB_API kapyb_status kapyb_route_backward(kapyb_handle h, const kapyb_tensor2d *logits,
+                                                       const kapyb_routing *routing, const int32_t *experts,
+                                                       const float *grad_weights, const kapyb_tensor2d *grad_logits,
+                                                       void *stream) {
+  const char *call = "route_backward";
+  TRY(check_tensor(h, "route_backward", "logits", logits));
+  TRY(check_routing(h, "route_backward", logits, routing));
+  TRY(check_output(h, "route_backward", "grad_logits", grad_logits));
+  if (grad_logits->size0 != logits->size0 || grad_logits->size1 != logits->size1)
+    return fail(h, KAPYB_INVALID_ARG, "route_backward: grad_logits must have the shape of logits");
+  if (logits->size0 == 0) {
+    HAVE_HANDLE(h);
+    return KAPYB_OK;
+  }
+  if (!experts || !grad_weights) return fail(h, KAPYB_INVALID_ARG, "route_backward: experts or grad_weights is NULL");
+  if (!aligned4(experts) || !aligned4(grad_weights))
+    return fail(h, KAPYB_INVALID_ARG, "route_backward: experts and grad_weights must be 4-byte aligned");
+  const size_t bytes = static_cast<size_t>(logits->size0) * routing->top_k * 4;
+  const Span out = span_of(grad_logits);
+  if (meet(out, span_of(logits)) || meet(out, span_of(experts, bytes)) || meet(out, span_of(grad_weights, bytes)))
+    return fail(h, KAPYB_INVALID_ARG, "route_backward: grad_logits overlaps an input");
+  ON_DEVICE(h);
+  RouteParams p = route_params(logits, routing);
+  p.picked = experts;
+  p.grad_weights = grad_weights;
+  p.grad = const_cast<void *>(elem_ptr(grad_logits));
+  p.g_s0 = grad_logits->stride0;
+  p.g_s1 = grad_logits->stride1;
+  p.g_dtype = grad_logits->dtype;
+  by_width<LaunchRouteBackward>(p.experts, p, warp_grid(p.rows), static_cast<cudaStream_t>(stream));
+  return launched(h, "route_backward");
+}
+
+// ---------------------------------------------------------------------- plan
+
+extern "C" KAPYB_API kapyb_status kapyb_plan_rows(kapyb_handle h, const int32_t *index, int32_t n, int32_t groups,
+                                                  int32_t *order, int32_t *offsets, int32_t *slots, void *stream) {
+  const char *call = "plan_rows";
+  if (n < 0) return fail(h, KAPYB_INVALID_ARG, "plan_rows: n is negative");
+  if (groups < 1 || groups > kPlanMaxGroups)
+    return fail(h, groups < 1 ? KAPYB_INVALID_ARG : KAPYB_UNSUPPORTED, "plan_rows: 1 to %d groups (got %d)",
+                kPlanMaxGroups, groups);
+  if (!offsets || (n > 0 && (!index || !order)))
+    return fail(h, KAPYB_INVALID_ARG, "plan_rows: index, order or offsets is NULL");
+  if (!aligned4(index) || !aligned4(order) || !aligned4(offsets) || !aligned4(slots))
+    return fail(h, KAPYB_INVALID_ARG, "plan_rows: arrays must be 4-byte aligned");
+  const size_t bytes = static_cast<size_t>(n) * 4;
+  const Span s[4] = {span_of(index, bytes), span_of(order, bytes), span_of(offsets, (groups + 1ull) * 4),
+                     span_of(slots, bytes)};
+  for (int i = 0; i < 4; ++i)
+    for (int j = i + 1; j < 4; ++j)
+      if (meet(s[i], s[j])) return fail(h, KAPYB_INVALID_ARG, "plan_rows: two arrays of the call overlap");
+  ON_DEVICE(h);
+  const size_t smem = plan_smem_bytes(groups);
+  CUDA_TRY(h, cudaFuncSetAttribute(plan_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(plan_smem_bytes(kPlanMaxGroups))));
+  // A warp's piece is a whole number of 32-entry steps.  One CTA takes up to four
+  // steps a warp; beyond that the work is spread over the cluster.
+  int ctas = 1;
+  while (ctas < kPlanMaxCtas && static_cast<long long>(n) > ctas * kPlanWarps * 128ll) ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(ctas, 1, 1);
+  cfg.blockDim = dim3(kPlanWarps * 32, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const PlanParams p{index, n, groups, order, offsets, slots};
+  CUDA_TRY(h, cudaLaunchKernelEx(&cfg, plan_rows_kernel, p));
+  return launched(h, "plan_rows");
+}
+
+// ------------------------------------------------------------------- products
+
+namespace {
+
+constexpr int kMaxRowGroups = 1024;
+
+// What the two grouped products check alike.
+kapyb_status check_grouped(kapyb_handle h, const char *call, const kapyb_tensor2d *lhs, const kapyb_tensor2d *other,
+                           int groups, const int32_t *offsets, const int32_t *order, int fan) {
+  if (lhs->dtype != other->dtype)
+    return fail(h, KAPYB_INVALID_ARG, "%s: operands must have same element type", call);
+  if (lhs->padding != KAPYB_PAD_ZERO || other->padding != KAPYB_PAD_ZERO)
+    return fail(h, KAPYB_UNSUPPORTED, "%s: operands are padded with zeros only", call);
+  if (groups < 1 || groups > kMaxRowGroups)
+    return fail(h, groups < 1 ? KAPYB_INVALID_ARG : KAPYB_UNSUPPORTED, "%s: 1 to %d groups (got %d)", call,
+                kMaxRowGroups, groups);
+  if (!offsets) return fail(h, KAPYB_INVALID_ARG, "%s: offsets is NULL", call);
+  if (order && fan < 1) return fail(h, KAPYB_INVALID_ARG, "%s: fan must be at least 1", call);
+  if (!aligned4(offsets) || !aligned4(order))
+    return fail(h, KAPYB_INVALID_ARG, "%s: offsets and order must be 4-byte aligned", call);
+  return KAPYB_OK;
+}
+
+}  // namespace
+
+extern "C" KAPYB_API kapyb_status kapyb_matmul_grouped(kapyb_handle h, const kapyb_tensor2d *lhs,
+                                                       const kapyb_tensor2d *rhs, int32_t groups,
+                                                       int64_t group_stride, const int32_t *offsets,
+                                                       const int32_t *order, int32_t fan, const kapyb_tensor2d *out,
+                                                       const kapyb_epilogue *epilogue, int32_t gated, void *stream) {
+  const char *call = "matmul_grouped";
+  TRY(check_tensor(h, call, "lhs", lhs));
+  TRY(check_tensor(h, call, "rhs", rhs));
+  TRY(check_output(h, call, "out", out));
+  TRY(check_grouped(h, call, lhs, rhs, groups, offsets, order, fan));
+  TRY(check_epilogue(h, call, epilogue));
+  if (epilogue && epilogue->bias && epilogue->bias_axis != 1)
+    return fail(h, KAPYB_UNSUPPORTED, "%s: bias_axis must be 1 (one value per column of each group)", call);
+  if (group_stride < 0) return fail(h, KAPYB_INVALID_ARG, "%s: group_stride is negative", call);
+  if (lhs->size1 != rhs->size0)
+    return fail(h, KAPYB_INVALID_ARG, "%s: number of columns of lhs must be equal to number of rows of rhs", call);
+  const int64_t cols_w = static_cast<int64_t>(out->size1) * (gated ? 2 : 1);
+  if (rhs->size1 != cols_w)
+    return fail(h, KAPYB_INVALID_ARG, "%s: rhs must have %s columns of out", call, gated ? "twice the" : "the");
+  if (!order && lhs->size0 != out->size0)
+    return fail(h, KAPYB_INVALID_ARG, "%s: without order lhs must have as many rows as out", call);
+  if (empty(out)) {
+    HAVE_HANDLE(h);
+    return KAPYB_OK;
+  }
+  const Span o = span_of(out);
+  if (meet(o, span_of(lhs)) || meet(o, span_of(rhs, groups, group_stride)) ||
+      meet(o, span_of(offsets, (groups + 1ull) * 4)) || meet(o, span_of(order, order ? out->size0 * 4ull : 0)) ||
+      (epilogue && meet(o, span_of(epilogue->bias, groups * cols_w * dtype_size(epilogue->bias_dtype)))))
+    return fail(h, KAPYB_INVALID_ARG, "%s: out overlaps an input", call);
+  ON_DEVICE(h);
+  const kapyb_epilogue &ep = epilogue ? *epilogue : kPlainEpilogue;
+  RowsSimtParams p{};
+  p.x = elem_ptr(lhs);
+  p.x_s0 = lhs->stride0;
+  p.x_s1 = lhs->stride1;
+  p.src_rows = lhs->size0;
+  p.w = elem_ptr(rhs);
+  p.w_s0 = rhs->stride0;
+  p.w_s1 = rhs->stride1;
+  p.w_group = group_stride;
+  p.in_dtype = lhs->dtype;
+  p.groups = groups;
+  p.rows = out->size0;
+  p.K = lhs->size1;
+  p.cols = out->size1;
+  p.cols_w = rhs->size1;
+  p.offsets = offsets;
+  p.order = order;
+  p.fan = fan;
+  p.gated = gated != 0;
+  p.out = const_cast<void *>(elem_ptr(out));
+  p.out_s0 = out->stride0;
+  p.out_s1 = out->stride1;
+  p.out_dtype = out->dtype;
+  p.alpha = ep.alpha;
+  p.bias = ep.bias;
+  p.bias_dtype = ep.bias_dtype;
+  p.activation = ep.activation;
+  p.rounding = ep.rounding;
+  const long long blocks = (p.rows + 31ll) / 32 + std::min(groups, p.rows);
+  const dim3 grid((p.cols + 31) / 32, static_cast<unsigned>(std::min<long long>(blocks, 65535)));
+  rows_simt_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return launched(h, "grouped_simt");
+}
+
+extern "C" KAPYB_API kapyb_status kapyb_matmul_grouped_grad(kapyb_handle h, const kapyb_tensor2d *lhs,
+                                                            const kapyb_tensor2d *grad, int32_t groups,
+                                                            const int32_t *offsets, const int32_t *order, int32_t fan,
+                                                            const kapyb_tensor2d *out, int64_t out_group_stride,
+                                                            float alpha, int32_t rounding, void *stream) {
+  const char *call = "matmul_grouped_grad";
+  TRY(check_tensor(h, call, "lhs", lhs));
+  TRY(check_tensor(h, call, "grad", grad));
+  TRY(check_output(h, call, "out", out));
+  TRY(check_grouped(h, call, lhs, grad, groups, offsets, order, fan));
+  if (!rounding_ok(rounding))
+    return fail(h, KAPYB_INVALID_ARG, "%s: rounding mode must be set for down cast", call);
+  if (out->size0 != lhs->size1 || out->size1 != grad->size1)
+    return fail(h, KAPYB_INVALID_ARG, "%s: out must have a row per column of lhs and a column per column of grad", call);
+  if (!order && lhs->size0 != grad->size0)
+    return fail(h, KAPYB_INVALID_ARG, "%s: without order lhs must have as many rows as grad", call);
+  if (empty(out)) {
+    HAVE_HANDLE(h);
+    return KAPYB_OK;
+  }
+  // groups of the output must not share addresses: behind one another, or interleaved
+  // by whole rows / columns that another group cannot reach
+  const int64_t extent = (out->size0 - 1ll) * out->stride0 + (out->size1 - 1ll) * out->stride1 + 1;
+  if (groups > 1 && out_group_stride < extent)
+    return fail(h, KAPYB_INVALID_ARG, "%s: out_group_stride (%lld) lets the groups of out overlap", call,
+                static_cast<long long>(out_group_stride));
+  const Span o = span_of(out, groups, out_group_stride);
+  if (meet(o, span_of(lhs)) || meet(o, span_of(grad)) || meet(o, span_of(offsets, (groups + 1ull) * 4)) ||
+      meet(o, span_of(order, order ? grad->size0 * 4ull : 0)))
+    return fail(h, KAPYB_INVALID_ARG, "%s: out overlaps an input", call);
+  ON_DEVICE(h);
+  RowsSimtParams p{};
+  p.x = elem_ptr(lhs);
+  p.x_s0 = lhs->stride0;
+  p.x_s1 = lhs->stride1;
+  p.src_rows = lhs->size0;
+  p.w = elem_ptr(grad);
+  p.w_s0 = grad->stride0;
+  p.w_s1 = grad->stride1;
+  p.in_dtype = lhs->dtype;
+  p.groups = groups;
+  p.rows = grad->size0;
+  p.K = lhs->size1;
+  p.cols = grad->size1;
+  p.offsets = offsets;
+  p.order = order;
+  p.fan = fan;
+  p.out = const_cast<void *>(elem_ptr(out));
+  p.out_s0 = out->stride0;
+  p.out_s1 = out->stride1;
+  p.out_group = out_group_stride;
+  p.out_dtype = out->dtype;
+  p.alpha = alpha;
+  p.rounding = rounding;
+  const int k_blocks = (p.K + 31) / 32;
+  if (k_blocks > 65535)
+    return fail(h, KAPYB_UNSUPPORTED, "%s: more than %d columns of lhs on the CUDA-core path", call, 65535 * 32);
+  const dim3 grid((p.cols + 31) / 32, k_blocks, groups);
+  rows_grad_simt_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return launched(h, "grouped_grad_simt");
+}
+
+// -------------------------------------------------------------------- combine
+
+namespace {
+
+// 16-byte pieces: unit column stride, 16-byte aligned base and row pitch
+bool pieces_ok(const kapyb_tensor2d *t) {
+  const int64_t esz = dtype_size(t->dtype);
+  return t->stride1 == 1 && aligned16(elem_ptr(t)) && (t->stride0 * esz) % 16 == 0 && (t->size1 * esz) % 16 == 0;
+}
+
+kapyb_status check_slots(kapyb_handle h, const char *call, const int32_t *slots, int k, const float *weights) {
+  if (k < 1 || k > kCombineMaxK)
+    return fail(h, KAPYB_INVALID_ARG, "%s: k must be 1 to %d (got %d)", call, kCombineMaxK, k);
+  if (!slots) return fail(h, KAPYB_INVALID_ARG, "%s: slots is NULL", call);
+  if (!aligned4(slots) || !aligned4(weights))
+    return fail(h, KAPYB_INVALID_ARG, "%s: slots and weights must be 4-byte aligned", call);
+  return KAPYB_OK;
+}
+
+}  // namespace
+
+extern "C" KAPYB_API kapyb_status kapyb_combine_rows(kapyb_handle h, const kapyb_tensor2d *rows, const int32_t *slots,
+                                                     int32_t k, const float *weights, const kapyb_tensor2d *out,
+                                                     void *stream) {
+  const char *call = "combine_rows";
+  TRY(check_tensor(h, call, "rows", rows));
+  TRY(check_output(h, call, "out", out));
+  if (rows->size1 != out->size1)
+    return fail(h, KAPYB_INVALID_ARG, "%s: rows and out must have as many columns", call);
+  if (empty(out)) {
+    HAVE_HANDLE(h);
+    return KAPYB_OK;
+  }
+  TRY(check_slots(h, call, slots, k, weights));
+  const size_t entries = static_cast<size_t>(out->size0) * k;
+  const Span o = span_of(out);
+  if (meet(o, span_of(rows)) || meet(o, span_of(slots, entries * 4)) || meet(o, span_of(weights, entries * 4)))
+    return fail(h, KAPYB_INVALID_ARG, "%s: out overlaps an input", call);
+  ON_DEVICE(h);
+  CombineParams p{};
+  p.rows = elem_ptr(rows);
+  p.rows_s0 = rows->stride0;
+  p.rows_s1 = rows->stride1;
+  p.rows_dtype = rows->dtype;
+  p.n_rows = rows->size0;
+  p.slots = slots;
+  p.weights = weights;
+  p.tokens = out->size0;
+  p.k = k;
+  p.cols = out->size1;
+  p.out = const_cast<void *>(elem_ptr(out));
+  p.out_s0 = out->stride0;
+  p.out_s1 = out->stride1;
+  p.out_dtype = out->dtype;
+  p.rounding = KAPYB_RN;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool vec = rows->dtype == out->dtype && pieces_ok(rows) && pieces_ok(out);
+  const uint32_t per_row = vec ? static_cast<uint32_t>(p.cols * dtype_size(rows->dtype) / 16) : p.cols;
+  const unsigned long long threads = static_cast<unsigned long long>(p.tokens) * per_row;
+  const unsigned long long blocks = (threads + 255) / 256;
+  if (blocks > 0x7fffffffull) return fail(h, KAPYB_UNSUPPORTED, "%s: output too large", call);
+  const int grid = static_cast<int>(blocks);
+  if (!vec)
+    combine_any_kernel<<<grid, 256, 0, s>>>(p);
+  else if (rows->dtype == KAPYB_F32)
+    combine_vec_kernel<KAPYB_F32><<<grid, 256, 0, s>>>(p, per_row);
+  else if (rows->dtype == KAPYB_BF16)
+    combine_vec_kernel<KAPYB_BF16><<<grid, 256, 0, s>>>(p, per_row);
+  else
+    combine_vec_kernel<KAPYB_F16><<<grid, 256, 0, s>>>(p, per_row);
+  return launched(h, vec ? "combine_vec" : "combine_any");
+}
+
+extern "C" KAPYB_API kapyb_status kapyb_combine_rows_backward(kapyb_handle h, const kapyb_tensor2d *rows,
+                                                              const int32_t *slots, int32_t k, const float *weights,
+                                                              const kapyb_tensor2d *grad_out,
+                                                              const kapyb_tensor2d *grad_rows, float *grad_weights,
+                                                              void *stream) {
+  const char *call = "combine_rows_backward";
+  TRY(check_tensor(h, call, "grad_out", grad_out));
+  if (grad_weights && !rows) return fail(h, KAPYB_INVALID_ARG, "%s: grad_weights needs rows", call);
+  if (rows) TRY(check_tensor(h, call, "rows", rows));
+  if (grad_rows) TRY(check_output(h, call, "grad_rows", grad_rows));
+  if ((rows && rows->size1 != grad_out->size1) || (grad_rows && grad_rows->size1 != grad_out->size1))
+    return fail(h, KAPYB_INVALID_ARG, "%s: rows, grad_out and grad_rows must have as many columns", call);
+  if (rows && grad_rows && rows->size0 != grad_rows->size0)
+    return fail(h, KAPYB_INVALID_ARG, "%s: grad_rows must have the shape of rows", call);
+  if (grad_out->size0 == 0 || (!grad_rows && !grad_weights)) {
+    HAVE_HANDLE(h);
+    return KAPYB_OK;
+  }
+  TRY(check_slots(h, call, slots, k, weights));
+  if (!aligned4(grad_weights)) return fail(h, KAPYB_INVALID_ARG, "%s: grad_weights must be 4-byte aligned", call);
+  const size_t bytes = static_cast<size_t>(grad_out->size0) * k * 4;
+  const Span gw = span_of(grad_weights, bytes);
+  const Span gr = grad_rows ? span_of(grad_rows) : Span{0, 0};
+  const Span in[4] = {rows ? span_of(rows) : Span{0, 0}, span_of(slots, bytes), span_of(weights, bytes),
+                      span_of(grad_out)};
+  if (meet(gw, gr)) return fail(h, KAPYB_INVALID_ARG, "%s: grad_weights overlaps grad_rows", call);
+  for (const Span &i : in)
+    if (meet(gw, i) || meet(gr, i)) return fail(h, KAPYB_INVALID_ARG, "%s: an output overlaps an input", call);
+  ON_DEVICE(h);
+  CombineParams p{};
+  if (rows) {
+    p.rows = elem_ptr(rows);
+    p.rows_s0 = rows->stride0;
+    p.rows_s1 = rows->stride1;
+    p.rows_dtype = rows->dtype;
+  }
+  p.n_rows = rows ? rows->size0 : grad_rows->size0;
+  p.slots = slots;
+  p.weights = weights;
+  p.tokens = grad_out->size0;
+  p.k = k;
+  p.cols = grad_out->size1;
+  p.grad_out = elem_ptr(grad_out);
+  p.go_s0 = grad_out->stride0;
+  p.go_s1 = grad_out->stride1;
+  p.go_dtype = grad_out->dtype;
+  p.rounding = KAPYB_RN;
+  if (grad_rows) {
+    p.grad_rows = const_cast<void *>(elem_ptr(grad_rows));
+    p.gr_s0 = grad_rows->stride0;
+    p.gr_s1 = grad_rows->stride1;
+    p.gr_dtype = grad_rows->dtype;
+  }
+  p.grad_weights = grad_weights;
+  const int dt = grad_out->dtype;
+  const bool vec = pieces_ok(grad_out) && (!rows || (rows->dtype == dt && pieces_ok(rows))) &&
+                   (!grad_rows || (grad_rows->dtype == dt && pieces_ok(grad_rows)));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const long long units = vec ? static_cast<long long>(p.cols) * dtype_size(dt) / 16 : p.cols;
+  const int threads = static_cast<int>(std::min(256ll, std::max(32ll, (units + 31) / 32 * 32)));
+  if (!vec)
+    combine_backward_kernel<KAPYB_F32, false><<<p.tokens, threads, 0, s>>>(p);
+  else if (dt == KAPYB_F32)
+    combine_backward_kernel<KAPYB_F32, true><<<p.tokens, threads, 0, s>>>(p);
+  else if (dt == KAPYB_BF16)
+    combine_backward_kernel<KAPYB_BF16, true><<<p.tokens, threads, 0, s>>>(p);
+  else
+    combine_backward_kernel<KAPYB_F16, true><<<p.tokens, threads, 0, s>>>(p);
+  return launched(h, vec ? "combine_backward_vec" : "combine_backward_any");
+}
+
+// ------------------------------------------------------------------- adapters
+
+namespace {
+constexpr int kMaxAdapterRank = 128;
+}  // namespace
+
+extern "C" KAPYB_API size_t kapyb_matmul_adapters_scratch(int32_t rows, int32_t groups, int32_t rank) {
+  if (rows <= 0 || groups <= 0 || rank <= 0) return 0;
+  return static_cast<size_t>(rows) * rank * sizeof(float);
+}
+
+extern "C" KAPYB_API kapyb_status kapyb_matmul_adapters(kapyb_handle h, const kapyb_tensor2d *lhs,
+                                                        const kapyb_tensor2d *rhs, int32_t groups,
+                                                        const kapyb_tensor2d *down, int64_t down_stride,
+                                                        const kapyb_tensor2d *up, int64_t up_stride,
+                                                        const int32_t *index, const float *scale,
+                                                        const kapyb_tensor2d *out, const kapyb_epilogue *epilogue,
+                                                        void *scratch, size_t scratch_bytes, void *stream) {
+  const char *call = "matmul_adapters";
+  TRY(check_tensor(h, call, "lhs", lhs));
+  TRY(check_tensor(h, call, "rhs", rhs));
+  TRY(check_tensor(h, call, "down", down));
+  TRY(check_tensor(h, call, "up", up));
+  TRY(check_output(h, call, "out", out));
+  TRY(check_epilogue(h, call, epilogue));
+  if (lhs->dtype != rhs->dtype || lhs->dtype != down->dtype || lhs->dtype != up->dtype)
+    return fail(h, KAPYB_INVALID_ARG, "%s: lhs, rhs, down and up must have same element type", call);
+  for (const kapyb_tensor2d *t : {lhs, rhs, down, up})
+    if (t->padding != KAPYB_PAD_ZERO)
+      return fail(h, KAPYB_UNSUPPORTED, "%s: operands are padded with zeros only", call);
+  if (groups < 1 || groups > kMaxRowGroups)
+    return fail(h, groups < 1 ? KAPYB_INVALID_ARG : KAPYB_UNSUPPORTED, "%s: 1 to %d adapters (got %d)", call,
+                kMaxRowGroups, groups);
+  if (down_stride < 0 || up_stride < 0)
+    return fail(h, KAPYB_INVALID_ARG, "%s: down_stride or up_stride is negative", call);
+  if (lhs->size1 != rhs->size0)
+    return fail(h, KAPYB_INVALID_ARG, "%s: number of columns of lhs must be equal to number of rows of rhs", call);
+  if (out->size0 != lhs->size0 || out->size1 != rhs->size1)
+    return fail(h, KAPYB_INVALID_ARG, "%s: out must have the rows of lhs and the columns of rhs", call);
+  if (down->size0 != lhs->size1 || up->size1 != rhs->size1 || down->size1 != up->size0)
+    return fail(h, KAPYB_INVALID_ARG, "%s: down must be [columns of lhs, rank] and up [rank, columns of rhs]", call);
+  if (down->size1 < 1 || down->size1 > kMaxAdapterRank)
+    return fail(h, down->size1 < 1 ? KAPYB_INVALID_ARG : KAPYB_UNSUPPORTED, "%s: rank must be 1 to %d (got %d)", call,
+                kMaxAdapterRank, down->size1);
+  if (empty(out)) {
+    HAVE_HANDLE(h);
+    return KAPYB_OK;
+  }
+  if (!index) return fail(h, KAPYB_INVALID_ARG, "%s: index is NULL", call);
+  if (!aligned4(index) || !aligned4(scale))
+    return fail(h, KAPYB_INVALID_ARG, "%s: index and scale must be 4-byte aligned", call);
+  const size_t need = kapyb_matmul_adapters_scratch(lhs->size0, groups, down->size1);
+  if (!scratch || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 256 != 0)
+    return fail(h, KAPYB_INVALID_ARG, "%s: scratch must be %zu bytes, 256-byte aligned", call, need);
+  const kapyb_epilogue &ep = epilogue ? *epilogue : kPlainEpilogue;
+  const Span o = span_of(out), sc = span_of(scratch, need);
+  const Span in[8] = {span_of(lhs), span_of(rhs), span_of(down, groups, down_stride), span_of(up, groups, up_stride),
+                      span_of(index, lhs->size0 * 4ull), span_of(scale, scale ? groups * 4ull : 0),
+                      span_of(ep.bias, static_cast<size_t>(ep.bias_axis == 1 ? out->size1 : out->size0) *
+                                           dtype_size(ep.bias_dtype)),
+                      Span{0, 0}};
+  if (meet(o, sc)) return fail(h, KAPYB_INVALID_ARG, "%s: out overlaps scratch", call);
+  for (const Span &i : in)
+    if (meet(o, i) || meet(sc, i)) return fail(h, KAPYB_INVALID_ARG, "%s: out or scratch overlaps an input", call);
+  ON_DEVICE(h);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  AdapterSimtParams p{};
+  p.x = elem_ptr(lhs);
+  p.x_s0 = lhs->stride0;
+  p.x_s1 = lhs->stride1;
+  p.w = elem_ptr(rhs);
+  p.w_s0 = rhs->stride0;
+  p.w_s1 = rhs->stride1;
+  p.down = elem_ptr(down);
+  p.d_s0 = down->stride0;
+  p.d_s1 = down->stride1;
+  p.d_group = down_stride;
+  p.up = elem_ptr(up);
+  p.u_s0 = up->stride0;
+  p.u_s1 = up->stride1;
+  p.u_group = up_stride;
+  p.in_dtype = lhs->dtype;
+  p.groups = groups;
+  p.rows = lhs->size0;
+  p.K = lhs->size1;
+  p.cols = rhs->size1;
+  p.rank = down->size1;
+  p.index = index;
+  p.scale = scale;
+  p.low = static_cast<float *>(scratch);
+  p.out = const_cast<void *>(elem_ptr(out));
+  p.out_s0 = out->stride0;
+  p.out_s1 = out->stride1;
+  p.out_dtype = out->dtype;
+  p.alpha = ep.alpha;
+  p.bias = ep.bias;
+  p.bias_dtype = ep.bias_dtype;
+  p.bias_axis = ep.bias_axis;
+  p.activation = ep.activation;
+  p.rounding = ep.rounding;
+  adapter_low_simt_kernel<<<p.rows, 256, 0, s>>>(p);
+  TRY(launched(h, "adapter_low_simt"));
+  const dim3 grid((p.cols + 31) / 32, static_cast<unsigned>(std::min((p.rows + 31ll) / 32, 65535ll)));
+  adapter_simt_kernel<<<grid, 256, 0, s>>>(p);
+  return launched(h, "adapter_simt");
+}

@@ -1,0 +1,132 @@
+// Row plan: a stable counting sort of n indices into groups.
+//
+//   order[p]   = the entry at position p (entries of group 0 first, each group's in
+//                ascending order of entry), -1 behind the last planned position
+//   offsets[g] = first position of group g; offsets[groups] = number of planned entries
+//   slots[i]   = position of entry i, -1 when its index names no group
+//
+// One launch without scratch memory: a cluster of CTAs splits the entries, every
+// warp counts a contiguous piece of them in its own row of a shared-memory table
+// (match.any finds equal groups in a step, so nothing is atomic and the order is
+// that of the entries), the CTAs read one another's totals through distributed
+// shared memory, and each warp walks its piece again to place it.
+#pragma once
+
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace kapyb {
+
+constexpr int kPlanWarps = 16;
+constexpr int kPlanMaxGroups = 1024;
+constexpr int kPlanMaxCtas = 8;
+
+struct PlanParams {
+  const int32_t *index;
+  int n, groups;
+  int32_t *order, *offsets, *slots;
+};
+
+inline size_t plan_smem_bytes(int groups) {
+  // per-warp counters, this CTA's totals, first positions
+  return static_cast<size_t>(kPlanWarps + 2) * groups * sizeof(int32_t);
+}
+
+__global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanParams p) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ int32_t plan_smem[];
+  __shared__ int scan_part[kPlanWarps];
+  const int G = p.groups;
+  int32_t *count = plan_smem;                  // [kPlanWarps][G]
+  int32_t *total = plan_smem + kPlanWarps * G;  // [G]
+  int32_t *first = total + G;                   // [G]
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int ctas = static_cast<int>(cluster.num_blocks()), me = static_cast<int>(cluster.block_rank());
+  const int pieces = ctas * kPlanWarps;
+  const long long step = ((static_cast<long long>(p.n) + pieces - 1) / pieces + 31) / 32 * 32;
+  const long long lo = min(static_cast<long long>(p.n), (me * kPlanWarps + w) * step);
+  const long long hi = min(static_cast<long long>(p.n), lo + step);
+
+  for (int i = threadIdx.x; i < kPlanWarps * G; i += blockDim.x) count[i] = 0;
+  __syncthreads();
+  int32_t *mine = count + w * G;
+  for (long long i0 = lo; i0 < hi; i0 += 32) {
+    const long long i = i0 + lane;
+    int g = i < hi ? p.index[i] : -1;
+    if (g < 0 || g >= G) g = -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, g);
+    if (g >= 0 && lane == __ffs(same) - 1) mine[g] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < G; g += blockDim.x) {
+    int run = 0;
+#pragma unroll
+    for (int k = 0; k < kPlanWarps; ++k) {
+      const int c = count[k * G + g];
+      count[k * G + g] = run;
+      run += c;
+    }
+    total[g] = run;
+  }
+  cluster.sync();
+  // first position of every group: exclusive scan over the groups of the cluster's
+  // totals, plus what the CTAs in front of this one hold of the group.  A thread
+  // owns a run of adjacent groups.
+  const int per = (G + blockDim.x - 1) / blockDim.x;
+  const int g0 = min(G, static_cast<int>(threadIdx.x) * per), g1 = min(G, g0 + per);
+  int sum = 0;
+  for (int g = g0; g < g1; ++g) {
+    int all = 0, before = 0;
+    for (int c = 0; c < ctas; ++c) {
+      const int t = cluster.map_shared_rank(total, c)[g];
+      if (c < me) before += t;
+      all += t;
+    }
+    first[g] = sum + before;
+    if (me == 0) p.offsets[g] = sum;  // completed below
+    sum += all;
+  }
+  int scan = sum;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, scan, off);
+    if (lane >= off) scan += o;
+  }
+  if (lane == 31) scan_part[w] = scan;
+  __syncthreads();
+  int base = scan - sum, planned = 0;
+  for (int k = 0; k < kPlanWarps; ++k) {
+    if (k < w) base += scan_part[k];
+    planned += scan_part[k];
+  }
+  for (int g = g0; g < g1; ++g) {
+    first[g] += base;
+    if (me == 0) p.offsets[g] += base;
+  }
+  if (me == 0 && threadIdx.x == 0) p.offsets[G] = planned;
+  // the others' totals have been read: nobody leaves while they still may be
+  cluster.sync();
+  for (long long i0 = lo; i0 < hi; i0 += 32) {
+    const long long i = i0 + lane;
+    int g = i < hi ? p.index[i] : -1;
+    if (g < 0 || g >= G) g = -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, g);
+    int pos = -1;
+    if (g >= 0) pos = first[g] + mine[g] + __popc(same & ((1u << lane) - 1u));
+    __syncwarp();
+    if (g >= 0 && lane == __ffs(same) - 1) mine[g] += __popc(same);
+    __syncwarp();
+    if (i < hi) {
+      if (pos >= 0) p.order[pos] = static_cast<int32_t>(i);
+      if (p.slots) p.slots[i] = pos;
+    }
+  }
+  for (long long q = planned + static_cast<long long>(me) * blockDim.x + threadIdx.x; q < p.n;
+       q += static_cast<long long>(ctas) * blockDim.x)
+    p.order[q] = -1;
+}
+
+}  // namespace kapyb

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from contextlib import nullcontext
 from typing import Optional, Sequence
 
 from . import _abi as abi
@@ -431,6 +432,284 @@ class Handle:
         ts, td = tensor2d(src), tensor2d(out)
         st = self._lib.kapyb_reduce(self._h, C.byref(ts), C.byref(td), int(axis), int(combiner),
                                     self._stream(stream))
+        if st != abi.OK:
+            self._raise(st)
+        return out
+
+    # ------------------------------------------- rows that pick their weights
+    def _launch_stream(self, stream):
+        """(ctypes stream, context in which tensors the call allocates belong to it)."""
+        torch = _torch()
+        if stream is None:
+            return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream), nullcontext()
+        if not hasattr(stream, "cuda_stream"):
+            stream = torch.cuda.ExternalStream(int(stream), device=self.device)
+        return C.c_void_p(stream.cuda_stream), torch.cuda.stream(stream)
+
+    def _on_device(self, **tensors):
+        for name, t in tensors.items():
+            if t is None:
+                continue
+            if not t.is_cuda:
+                raise ValueError(f"{name} must be a CUDA tensor")
+            if t.device.index != self.device:
+                raise ValueError(f"{name} is on {t.device}, the handle on cuda:{self.device}")
+
+    def _dense(self, dtype, **tensors):
+        """Plain device arrays: right element type, contiguous, on the handle's GPU."""
+        self._on_device(**tensors)
+        for name, t in tensors.items():
+            if t is None:
+                continue
+            if t.dtype != dtype:
+                raise ValueError(f"{name} must have element type {dtype}, not {t.dtype}")
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+
+    @staticmethod
+    def _ptr(t):
+        return None if t is None else C.c_void_p(t.data_ptr())
+
+    @staticmethod
+    def _grouped2d(t, name):
+        """Descriptor of the first matrix of [groups, rows, cols] and the group stride."""
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be [groups, rows, columns]")
+        d = abi.Tensor2d(t.data_ptr(), 0, t.shape[1], t.shape[2], t.stride(1), t.stride(2),
+                         dtype_code(t.dtype), abi.PAD_ZERO, 0, 0)
+        for v in (t.shape[1], t.shape[2], t.stride(1), t.stride(2)):
+            if v >= 2 ** 31:
+                raise ValueError("sizes and strides must fit i32")
+        return d, t.stride(0)
+
+    def _routing(self, top_k, score, groups, top_groups, group_best, renormalize, scale):
+        return abi.Routing(int(score), int(top_k), int(groups), int(top_groups), int(group_best),
+                           1 if renormalize else 0, float(scale))
+
+    def route(self, logits, top_k: int, *, bias=None, score: int = abi.SCORE_SOFTMAX,
+              groups: int = 1, top_groups: Optional[int] = None, group_best: int = 1,
+              renormalize: bool = True, scale: float = 1.0, weights=None, experts=None,
+              stream=None):
+        """Routing of rows to experts (kapyb_route): (weights f32 [T, k], experts int32
+        [T, k]) of logits [T, E]; the bias (f32 [E]) takes part in the choice only."""
+        torch = _torch()
+        self._on_device(logits=logits)
+        self._dense(torch.float32, bias=bias, weights=weights)
+        self._dense(torch.int32, experts=experts)
+        tl = tensor2d(logits)
+        shape = (logits.shape[0], int(top_k))
+        if bias is not None and tuple(bias.shape) != (logits.shape[1],):
+            raise ValueError("bias must have one value per expert")
+        for name, t in (("weights", weights), ("experts", experts)):
+            if t is not None and tuple(t.shape) != shape:
+                raise ValueError(f"{name} must have shape {shape}")
+        r = self._routing(top_k, score, groups, groups if top_groups is None else top_groups,
+                          group_best, renormalize, scale)
+        s, where = self._launch_stream(stream)
+        with where:
+            if weights is None:
+                weights = torch.empty(max(0, shape[0]), max(0, shape[1]), device=logits.device)
+            if experts is None:
+                experts = torch.empty(max(0, shape[0]), max(0, shape[1]), device=logits.device,
+                                      dtype=torch.int32)
+        st = self._lib.kapyb_route(self._h, C.byref(tl), self._ptr(bias), C.byref(r),
+                                   self._ptr(weights), self._ptr(experts), s)
+        if st != abi.OK:
+            self._raise(st)
+        return weights, experts
+
+    def route_backward(self, logits, experts, grad_weights, *, score: int = abi.SCORE_SOFTMAX,
+                       renormalize: bool = True, scale: float = 1.0, out=None, stream=None):
+        """Gradient of the logits (kapyb_route_backward) from the gradient of route's
+        weights; `experts`, score, renormalize and scale as in the forward call."""
+        torch = _torch()
+        self._on_device(logits=logits, out=out)
+        self._dense(torch.int32, experts=experts)
+        self._dense(torch.float32, grad_weights=grad_weights)
+        if experts.dim() != 2 or experts.shape[0] != logits.shape[0] or \
+                grad_weights.shape != experts.shape:
+            raise ValueError("experts and grad_weights must be [rows of logits, k]")
+        tl = tensor2d(logits)
+        r = self._routing(experts.shape[1], score, 1, 1, 1, renormalize, scale)
+        s, where = self._launch_stream(stream)
+        if out is None:
+            with where:
+                out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+        to = tensor2d(out)
+        st = self._lib.kapyb_route_backward(self._h, C.byref(tl), C.byref(r), self._ptr(experts),
+                                            self._ptr(grad_weights), C.byref(to), s)
+        if st != abi.OK:
+            self._raise(st)
+        return out
+
+    def plan_rows(self, index, groups: int, *, order=None, offsets=None, slots=None, stream=None):
+        """Stable counting sort of an int32 index (any shape) into groups
+        (kapyb_plan_rows): (order [n], offsets [groups + 1], slots of index's shape)."""
+        torch = _torch()
+        self._dense(torch.int32, index=index, order=order, offsets=offsets, slots=slots)
+        n = index.numel()
+        for name, t, want in (("order", order, n), ("offsets", offsets, int(groups) + 1),
+                              ("slots", slots, n)):
+            if t is not None and t.numel() != want:
+                raise ValueError(f"{name} must have {want} elements")
+        s, where = self._launch_stream(stream)
+        with where:
+            new = lambda *shape: torch.empty(*shape, device=index.device, dtype=torch.int32)
+            order = new(n) if order is None else order
+            offsets = new(max(0, int(groups)) + 1) if offsets is None else offsets
+            slots = new(index.shape) if slots is None else slots
+        st = self._lib.kapyb_plan_rows(self._h, self._ptr(index), n, int(groups),
+                                       self._ptr(order), self._ptr(offsets), self._ptr(slots), s)
+        if st != abi.OK:
+            self._raise(st)
+        return order, offsets, slots
+
+    def _check_plan(self, offsets, order, fan, groups, rows):
+        torch = _torch()
+        self._dense(torch.int32, offsets=offsets, order=order)
+        if offsets.numel() != groups + 1:
+            raise ValueError(f"offsets must have {groups + 1} elements")
+        if order is not None and order.numel() != rows:
+            raise ValueError(f"order must have {rows} elements")
+        if order is not None and int(fan) < 1:
+            raise ValueError("fan must be at least 1")
+
+    def matmul_grouped(self, lhs, rhs, offsets, out=None, *, order=None, fan: int = 1,
+                       alpha: float = 1.0, bias=None, activation: int = abi.ACT_NONE,
+                       gated: bool = False, rounding: int = abi.RN, out_dtype=None, stream=None):
+        """out[p] = epilogue(lhs[row] . rhs[g]) for every planned position p of group g
+        (kapyb_matmul_grouped): row = order[p] // fan, or p without an order.  rhs is
+        [groups, K, N]; gated: [groups, K, 2 N], gate columns then up columns, out =
+        activation(gate) * up.  bias: [groups, columns of rhs]."""
+        torch = _torch()
+        self._on_device(lhs=lhs, rhs=rhs, out=out, bias=bias)
+        tr, stride = self._grouped2d(rhs, "rhs")
+        rows = order.numel() if order is not None else lhs.shape[0]
+        self._check_plan(offsets, order, fan, rhs.shape[0], rows)
+        if bias is not None and tuple(bias.shape) != (rhs.shape[0], rhs.shape[2]):
+            raise ValueError("bias must be [groups, columns of rhs]")
+        if out is not None and out.shape[0] != rows:
+            raise ValueError(f"out must have {rows} rows")
+        s, where = self._launch_stream(stream)
+        if out is None:
+            with where:
+                out = torch.empty(rows, rhs.shape[2] // 2 if gated else rhs.shape[2],
+                                  device=lhs.device, dtype=out_dtype or lhs.dtype)
+        tl, to = tensor2d(lhs), tensor2d(out)
+        ep = self._epilogue(alpha, bias, 1, activation, rounding)
+        st = self._lib.kapyb_matmul_grouped(self._h, C.byref(tl), C.byref(tr), rhs.shape[0], stride,
+                                            self._ptr(offsets), self._ptr(order), int(fan),
+                                            C.byref(to), C.byref(ep), 1 if gated else 0, s)
+        if st != abi.OK:
+            self._raise(st)
+        return out
+
+    def matmul_grouped_grad(self, lhs, grad, offsets, out=None, *, order=None, fan: int = 1,
+                            alpha: float = 1.0, rounding: int = abi.RN, out_dtype=None,
+                            stream=None):
+        """Gradient of matmul_grouped's weights (kapyb_matmul_grouped_grad): [groups, K, N]
+        from lhs, the gradient of the products [positions, N] and the plan they ran on."""
+        torch = _torch()
+        self._on_device(lhs=lhs, grad=grad, out=out)
+        groups = offsets.numel() - 1
+        self._check_plan(offsets, order, fan, groups, grad.shape[0])
+        s, where = self._launch_stream(stream)
+        if out is None:
+            with where:
+                out = torch.empty(groups, lhs.shape[1], grad.shape[1], device=lhs.device,
+                                  dtype=out_dtype or lhs.dtype)
+        if out.shape[0] != groups:
+            raise ValueError(f"out must have {groups} groups")
+        tl, tg = tensor2d(lhs), tensor2d(grad)
+        to, stride = self._grouped2d(out, "out")
+        st = self._lib.kapyb_matmul_grouped_grad(self._h, C.byref(tl), C.byref(tg), groups,
+                                                 self._ptr(offsets), self._ptr(order), int(fan),
+                                                 C.byref(to), stride, float(alpha), int(rounding), s)
+        if st != abi.OK:
+            self._raise(st)
+        return out
+
+    def combine_rows(self, rows, slots, out=None, *, weights=None, out_dtype=None, stream=None):
+        """out[t] = sum_j weights[t, j] * rows[slots[t, j]] (kapyb_combine_rows)."""
+        torch = _torch()
+        self._on_device(rows=rows, out=out)
+        self._dense(torch.int32, slots=slots)
+        self._dense(torch.float32, weights=weights)
+        if slots.dim() != 2 or (weights is not None and weights.shape != slots.shape):
+            raise ValueError("slots and weights must be [tokens, k]")
+        s, where = self._launch_stream(stream)
+        if out is None:
+            with where:
+                out = torch.empty(slots.shape[0], rows.shape[1], device=rows.device,
+                                  dtype=out_dtype or rows.dtype)
+        if out.shape[0] != slots.shape[0]:
+            raise ValueError("out must have a row per token")
+        tr, to = tensor2d(rows), tensor2d(out)
+        st = self._lib.kapyb_combine_rows(self._h, C.byref(tr), self._ptr(slots), slots.shape[1],
+                                          self._ptr(weights), C.byref(to), s)
+        if st != abi.OK:
+            self._raise(st)
+        return out
+
+    def combine_rows_backward(self, rows, slots, grad_out, *, weights=None, grad_rows=None,
+                              grad_weights=None, stream=None):
+        """Gradients of combine_rows (kapyb_combine_rows_backward): (grad_rows,
+        grad_weights); the latter is None for a sum without weights.  A given grad_rows
+        keeps the rows no slot names; an allocated one starts as zeros."""
+        torch = _torch()
+        self._on_device(rows=rows, grad_out=grad_out, grad_rows=grad_rows)
+        self._dense(torch.int32, slots=slots)
+        self._dense(torch.float32, weights=weights, grad_weights=grad_weights)
+        if slots.dim() != 2 or grad_out.shape[0] != slots.shape[0] or \
+                any(t is not None and t.shape != slots.shape for t in (weights, grad_weights)):
+            raise ValueError("slots, weights and grad_weights must be [rows of grad_out, k]")
+        s, where = self._launch_stream(stream)
+        with where:
+            if grad_rows is None:
+                grad_rows = torch.zeros(rows.shape, device=rows.device, dtype=rows.dtype)
+            if grad_weights is None and weights is not None:
+                grad_weights = torch.empty(slots.shape, device=rows.device, dtype=torch.float32)
+        tr, tg, td = tensor2d(rows), tensor2d(grad_out), tensor2d(grad_rows)
+        st = self._lib.kapyb_combine_rows_backward(
+            self._h, C.byref(tr), self._ptr(slots), slots.shape[1], self._ptr(weights),
+            C.byref(tg), C.byref(td), self._ptr(grad_weights), s)
+        if st != abi.OK:
+            self._raise(st)
+        return grad_rows, grad_weights
+
+    def matmul_adapters(self, lhs, rhs, down, up, index, out=None, *, scale=None,
+                        alpha: float = 1.0, bias=None, bias_axis: int = 1,
+                        activation: int = abi.ACT_NONE, rounding: int = abi.RN, out_dtype=None,
+                        stream=None):
+        """lhs . rhs with every row's low-rank adapter beside it (kapyb_matmul_adapters):
+        row t adds scale[i] * (lhs[t] . down[i]) . up[i], i = index[t]; an index outside
+        the adapters adds nothing.  down [groups, K, rank], up [groups, rank, N]."""
+        torch = _torch()
+        self._on_device(lhs=lhs, rhs=rhs, down=down, up=up, out=out, bias=bias)
+        self._dense(torch.int32, index=index)
+        self._dense(torch.float32, scale=scale)
+        td, d_stride = self._grouped2d(down, "down")
+        tu, u_stride = self._grouped2d(up, "up")
+        groups = down.shape[0]
+        if up.shape[0] != groups or (scale is not None and scale.numel() != groups):
+            raise ValueError("down, up and scale must have as many adapters")
+        if index.numel() != lhs.shape[0]:
+            raise ValueError("index must have an element per row of lhs")
+        if bias is not None and bias.numel() != (rhs.shape[1] if bias_axis == 1 else lhs.shape[0]):
+            raise ValueError("bias must have a value per column (bias_axis 1) or row (0)")
+        s, where = self._launch_stream(stream)
+        nbytes = int(self._lib.kapyb_matmul_adapters_scratch(lhs.shape[0], groups, down.shape[2]))
+        with where:
+            scratch = torch.empty(nbytes, device=lhs.device, dtype=torch.uint8)
+            if out is None:
+                out = torch.empty(lhs.shape[0], rhs.shape[1], device=lhs.device,
+                                  dtype=out_dtype or lhs.dtype)
+        tl, tr, to = tensor2d(lhs), tensor2d(rhs), tensor2d(out)
+        ep = self._epilogue(alpha, bias, bias_axis, activation, rounding)
+        st = self._lib.kapyb_matmul_adapters(
+            self._h, C.byref(tl), C.byref(tr), groups, C.byref(td), d_stride, C.byref(tu), u_stride,
+            self._ptr(index), self._ptr(scale), C.byref(to), C.byref(ep), self._ptr(scratch), nbytes,
+            s)
         if st != abi.OK:
             self._raise(st)
         return out
