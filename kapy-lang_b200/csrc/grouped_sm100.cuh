@@ -1,0 +1,525 @@
+// Products of rows that pick their weights, on tcgen05:
+//   forward   out[p, n]    = epilogue( sum_k lhs[row(p), k] * rhs[g(p)][k, n] )
+//   gradient  out[g][k, n] = alpha * sum over p of group g  lhs[row(p), k] * grad[p, n]
+//
+// The output columns n always fill the 128-row side of the MMA (TMEM lanes) and the
+// output rows its N side:  D[n, r] = sum A[n, .] B[r, .].  The N side of a tcgen05.mma
+// is any multiple of 16 up to 256, so a group of three rows costs a 16-wide MMA and
+// not a 128-row tile, and one kernel serves a decode step (a few rows per group,
+// bound by streaming the weights) and a prompt (hundreds of rows, bound by the tensor
+// cores).  A group's rows are dealt out in equal tiles of at most BT.
+//
+// Rows named by a plan are fetched by TMA where they lie (tile::gather4: four row
+// numbers per instruction, one lane each), so no permuted copy of lhs is written.
+// Rows outside lhs, and the K tail of both operands, arrive as zeros.  A tile's rows
+// behind the end of its group may be those of the next group: they only reach output
+// rows that are not stored.  In the gradient the rows are the contraction, so there
+// everything behind a group's end is fetched as zeros on both sides (a zero on one
+// side alone would still let a NaN through).
+//
+// Persistent CTAs; warp 0 produces (the whole warp, one TMA instruction per lane),
+// warp 1 issues the MMAs, warps 2..5 drain: two accumulator slots in TMEM let the
+// drain of one tile run under the next one's main loop.  MSETS = 2 multiplies the
+// same rows with two column blocks, gate and up, and joins them in the drain.
+//
+// The table of tiles depends on the plan, which only the device knows: every CTA
+// builds it in shared memory from the offsets (a scan over at most 1024 groups).
+#pragma once
+
+#include <cuda.h>
+
+#include "common.cuh"
+#include "ptx_sm100.cuh"
+#include "rows_simt.cuh"
+
+namespace kapyb {
+
+// Four rows of a 2-D tensor (map with a box one row high), named one by one: they land
+// behind one another in shared memory, under the map's swizzle.  Rows outside the
+// tensor are filled with zeros.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const void *tmap, uint32_t bar, int x, int r0,
+                                            int r1, int r2, int r3) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      :
+      : "r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2),
+        "r"(r3)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *tmap, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      :
+      : "r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+struct GroupedParams {
+  int groups, rows;      // rows: positions of the plan
+  int cols;              // output columns (of one group)
+  int K;                 // forward: contraction length; gradient: output rows of one group
+  int n_tiles;           // ceil(cols / 128)
+  int k_tiles;           // gradient: ceil(K / BT)
+  int num_kb;            // forward: ceil(K / 64)
+  const int32_t *offsets, *order;
+  int fan, src_rows;     // row(p) = order[p] / fan (order may be nullptr: p); rows of lhs
+  int a_mn_major;        // forward: rhs has its unit stride on n
+  int bf16;
+  void *out;
+  long long out_s0, out_group;  // unit stride on n
+  int out_dtype, pair_stores;   // pair_stores: two 16-bit columns may be stored as one word
+  float alpha;
+  const void *bias;      // [groups, bias_cols]
+  int bias_dtype, bias_cols, activation, rounding;
+  uint32_t *status;
+  uint32_t wait_limit_us;
+};
+
+constexpr int kGroupedThreads = 192;
+constexpr int kGroupedMaxGroups = 1024;
+
+template <int BT, int MSETS>
+struct GroupedCfg {
+  static constexpr int A_BYTES = MSETS * 128 * 128;  // 128 columns x 64 of the contraction, 16-bit
+  static constexpr int B_BYTES = BT * 128;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int CTRL_BYTES = 1024;
+  static constexpr int TABLE_BYTES = (3 * kGroupedMaxGroups + 4) * 4;
+  static constexpr int SMEM_LIMIT = 232448;
+  static constexpr int STAGES_RAW = (SMEM_LIMIT - 1024 - CTRL_BYTES - TABLE_BYTES) / STAGE_BYTES;
+  static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + CTRL_BYTES + TABLE_BYTES;
+  static constexpr int SLOT_COLS = BT * MSETS;
+  static constexpr int TMEM_COLS = 2 * SLOT_COLS;
+  static_assert(BT % 32 == 0 && BT <= 256 && TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
+  static_assert(STAGES >= 3, "pipeline too shallow");
+};
+
+// One output tile.
+struct GroupedTile {
+  int g;        // group
+  int n0;       // first output column
+  int r0;       // forward: first position; gradient: first output row
+  int rows;     // output rows of the tile
+  int wide;     // the MMA's N: rows rounded up to 16
+  int num_kb;   // K blocks
+  int p0, p1;   // gradient: the group's positions
+};
+
+__device__ __forceinline__ int round16(int v) { return (v + 15) & ~15; }
+
+// The tile table in shared memory: first[g] = tiles of output rows in front of group
+// g, begin[g] / count[g] its positions.
+struct GroupedTable {
+  int *first, *begin, *count;
+};
+
+template <int BT, bool GRAD>
+__device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams &p, const GroupedTable &t, int idx) {
+  GroupedTile r;
+  if constexpr (GRAD) {
+    // group by group; row tiles of one column block next to one another
+    const int per = p.n_tiles * p.k_tiles;
+    r.g = idx / per;
+    const int in = idx - r.g * per;
+    const int n = in / p.k_tiles;
+    r.r0 = (in - n * p.k_tiles) * BT;
+    r.n0 = n * 128;
+    r.rows = min(BT, p.K - r.r0);
+    r.wide = round16(r.rows);
+    r.p0 = t.begin[r.g];
+    r.p1 = r.p0 + t.count[r.g];
+    r.num_kb = (t.count[r.g] + 63) >> 6;
+  } else {
+    const int q = idx / p.n_tiles;
+    int lo = 0, hi = p.groups;  // the group g with first[g] <= q < first[g + 1]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (t.first[mid] <= q) lo = mid;
+      else hi = mid;
+    }
+    r.g = lo;
+    const int tiles = t.first[lo + 1] - t.first[lo];
+    const int in = idx - t.first[lo] * p.n_tiles;
+    const int n = in / tiles, m = in - n * tiles;
+    const int cnt = t.count[lo];
+    const int each = round16((cnt + tiles - 1) / tiles);
+    r.n0 = n * 128;
+    r.r0 = t.begin[lo] + m * each;
+    r.rows = min(each, cnt - m * each);
+    r.wide = round16(r.rows);
+    r.num_kb = p.num_kb;
+    r.p0 = r.p1 = 0;
+  }
+  return r;
+}
+
+// Activation, scale and bias of 32 values of one output column.
+template <int MSETS>
+__device__ __forceinline__ void grouped_finish32(const GroupedParams &p, float (&f)[32], const float *up,
+                                                 float bias, float bias_up) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f[i] = f[i] * p.alpha + bias;
+  switch (p.activation) {
+  case KAPYB_ACT_RELU:
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = apply_activation_t<KAPYB_ACT_RELU>(f[i]);
+    break;
+  case KAPYB_ACT_GELU_TANH:
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = apply_activation_t<KAPYB_ACT_GELU_TANH>(f[i]);
+    break;
+  case KAPYB_ACT_SILU:
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = apply_activation_t<KAPYB_ACT_SILU>(f[i]);
+    break;
+  default: break;
+  }
+  if constexpr (MSETS == 2) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] *= up[i] * p.alpha + bias_up;
+  }
+}
+
+// 32 output rows of one column per lane -> memory.  `row0` points at (first row,
+// column n); rows_left of the 32 exist.  Neighbouring lanes swap half of their values
+// so that each stores two adjacent columns of every other row as one word: half the
+// store instructions of one value each, and 64-byte runs either way.
+template <int DT, int RN>
+__device__ __forceinline__ void store_rows16(uint16_t *at, long long s0, const float (&f)[32], int rows_left,
+                                             int lane, bool mine, bool both, bool pairs) {
+  if (pairs) {
+    const bool odd = lane & 1;
+    uint16_t *base = odd ? at - 1 + s0 : at;  // (first row + odd, even column)
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float give = odd ? f[j] : f[j + 1];
+      const float take = __shfl_xor_sync(0xffffffffu, give, 1);
+      const uint32_t w = odd ? cvt_pack2_t<DT, RN>(take, f[j + 1]) : cvt_pack2_t<DT, RN>(f[j], take);
+      if (j + (odd ? 1 : 0) < rows_left) {
+        if (both)
+          *reinterpret_cast<uint32_t *>(base + j * s0) = w;
+        else if (!odd && mine)  // the last column of an odd number has no neighbour
+          base[j * s0] = static_cast<uint16_t>(w & 0xffffu);
+      }
+    }
+    // ... and its odd rows are stored by itself
+    if (!odd && mine && !both) {
+#pragma unroll
+      for (int j = 1; j < 32; j += 2)
+        if (j < rows_left) at[j * s0] = static_cast<uint16_t>(cvt_pack2_t<DT, RN>(f[j], 0.0f) & 0xffffu);
+    }
+  } else if (mine) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < rows_left) at[j * s0] = static_cast<uint16_t>(cvt_pack2_t<DT, RN>(f[j], 0.0f) & 0xffffu);
+  }
+}
+
+__device__ __forceinline__ void grouped_store32(const GroupedParams &p, void *out, long long idx, const float (&f)[32],
+                                                int rows_left, int lane, bool mine, bool both) {
+  if (p.out_dtype == KAPYB_F32) {
+    if (mine) {
+      float *at = static_cast<float *>(out) + idx;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j < rows_left) at[j * p.out_s0] = f[j];
+    }
+    return;
+  }
+  uint16_t *at = static_cast<uint16_t *>(out) + idx;
+  const bool pairs = p.pair_stores != 0;
+  if (p.out_dtype == KAPYB_BF16) {
+    if (p.rounding) store_rows16<KAPYB_BF16, 1>(at, p.out_s0, f, rows_left, lane, mine, both, pairs);
+    else store_rows16<KAPYB_BF16, 0>(at, p.out_s0, f, rows_left, lane, mine, both, pairs);
+  } else {
+    if (p.rounding) store_rows16<KAPYB_F16, 1>(at, p.out_s0, f, rows_left, lane, mine, both, pairs);
+    else store_rows16<KAPYB_F16, 0>(at, p.out_s0, f, rows_left, lane, mine, both, pairs);
+  }
+}
+
+// tmA: forward: rhs, 3-D (unit axis, other axis, group), boxes of 64 x 128 (K-major) or
+// 64 x 64 (MN-major); gradient: grad [positions, cols], one-row boxes of 64 columns.
+// tmB: lhs [source rows, K]: one-row boxes of 64 columns (gathered, and the gradient),
+// or 64 x 32 boxes (rows already in plan order).
+template <int BT, int MSETS, bool GRAD>
+__global__ void __launch_bounds__(kGroupedThreads, 1)
+grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                       const GroupedParams p) {
+  using Cfg = GroupedCfg<BT, MSETS>;
+  constexpr int STAGES = Cfg::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                              ~static_cast<uintptr_t>(1023));
+  uint8_t *sA = smem;
+  uint8_t *sB = sA + STAGES * Cfg::A_BYTES;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sB + STAGES * Cfg::B_BYTES);
+  uint64_t *full_bar = bars, *empty_bar = bars + STAGES, *tfull_bar = bars + 2 * STAGES, *tempty_bar = tfull_bar + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty_bar + 2);
+  volatile uint32_t *abort_flag = tmem_slot + 1;  // two words
+  int *table_mem = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(bars) + Cfg::CTRL_BYTES);
+  GroupedTable table{table_mem, table_mem + kGroupedMaxGroups + 1, table_mem + 2 * kGroupedMaxGroups + 1};
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&full_bar[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(ptx::smem_u32(&tfull_bar[a]), 1);
+      ptx::mbar_init(ptx::smem_u32(&tempty_bar[a]), 4);
+    }
+    abort_flag[0] = 0u;
+    abort_flag[1] = p.wait_limit_us;
+    ptx::fence_barrier_init();
+    ptx::prefetch_tensormap(&tmA);
+    ptx::prefetch_tensormap(&tmB);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<1>(ptx::smem_u32(tmem_slot), Cfg::TMEM_COLS);
+    ptx::tmem_relinquish<1>();
+  }
+  if (warp == 0) {
+    int before = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+      const int g = g0 + lane;
+      int b = 0, e = 0;
+      if (g < p.groups) group_range(p.offsets, g, p.rows, b, e);
+      const int cnt = max(0, e - b);
+      const int tiles = GRAD ? 0 : (cnt + BT - 1) / BT;
+      int scan = tiles;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, scan, off);
+        if (lane >= off) scan += o;
+      }
+      if (g < p.groups) {
+        table.first[g] = before + scan - tiles;
+        table.begin[g] = b;
+        table.count[g] = cnt;
+      }
+      before += __shfl_sync(0xffffffffu, scan, 31);
+    }
+    if (lane == 0) table.first[p.groups] = before;
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int total = GRAD ? p.groups * p.n_tiles * p.k_tiles : table.first[p.groups] * p.n_tiles;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    // the source row of position q, src_rows (a row of zeros) where there is none
+    auto row_of = [&](int q, int end) -> int {
+      if (q >= end) return p.src_rows;
+      const long long r = source_row(p.order, p.fan, p.src_rows, q);
+      return r < 0 ? p.src_rows : static_cast<int>(r);
+    };
+    const bool gather = GRAD || p.order != nullptr;
+    for (int idx = blockIdx.x; ok && idx < total; idx += gridDim.x) {
+      const GroupedTile t = grouped_tile<BT, GRAD>(p, table, idx);
+      // forward: this lane's rows of the tile, four per gather instruction
+      constexpr int kMine = GRAD ? 1 : BT / 128 > 0 ? BT / 128 : 1;
+      int rows4[kMine][4];
+      if (!GRAD && gather) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = (i * 32 + lane) * 4 + j;
+            rows4[i][j] = r < t.wide ? row_of(t.r0 + r, t.r0 + t.rows) : p.src_rows;
+          }
+      }
+      const int boxes = gather ? t.wide / 4 : (t.wide + 31) / 32;  // forward, token side
+      const uint32_t b_bytes = GRAD ? static_cast<uint32_t>((t.rows + 63) / 64) * 8192u
+                                    : static_cast<uint32_t>(boxes) * (gather ? 512u : 4096u);
+      for (int kb = 0; kb < t.num_kb; ++kb) {
+        const bool got = ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag);
+        if (!__all_sync(0xffffffffu, got)) {
+          ok = false;
+          break;
+        }
+        const uint32_t fb = ptx::smem_u32(&full_bar[stage]);
+        const uint32_t a_dst = ptx::smem_u32(sA + stage * Cfg::A_BYTES);
+        const uint32_t b_dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES);
+        if (lane == 0) ptx::mbar_arrive_expect_tx(fb, Cfg::A_BYTES + b_bytes);
+        __syncwarp();
+        if constexpr (GRAD) {
+          // 64 positions: 16 groups of four rows; lane l fetches rows 4 (l % 16) .. + 3
+          // of every other 64-column chunk
+          const int q = t.p0 + kb * 64 + (lane & 15) * 4;
+          int src[4], own[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            src[j] = row_of(q + j, t.p1);
+            own[j] = src[j] < p.src_rows ? q + j : p.rows;  // zeros on both sides
+          }
+          const uint32_t off = static_cast<uint32_t>(lane & 15) * 512u;
+          const int c0 = lane >> 4;
+          tma_gather4(a_dst + c0 * 8192 + off, &tmA, fb, t.n0 + c0 * 64, own[0], own[1], own[2], own[3]);
+#pragma unroll
+          for (int c = c0; c < BT / 64; c += 2)
+            if (c * 64 < t.rows)
+              tma_gather4(b_dst + c * 8192 + off, &tmB, fb, t.r0 + c * 64, src[0], src[1], src[2], src[3]);
+        } else {
+          const int k0 = kb * 64;
+          if (p.a_mn_major) {
+            if (lane < 2 * MSETS)
+              ptx::tma_load_3d(a_dst + lane * 8192, &tmA, fb, t.n0 + (lane & 1) * 64 + (lane >> 1) * p.cols, k0, t.g);
+          } else {
+            if (lane < MSETS) ptx::tma_load_3d(a_dst + lane * 16384, &tmA, fb, k0, t.n0 + lane * p.cols, t.g);
+          }
+          if (gather) {
+#pragma unroll
+            for (int i = 0; i < kMine; ++i)
+              if (i * 32 + lane < boxes)
+                tma_gather4(b_dst + (i * 32 + lane) * 512, &tmB, fb, k0, rows4[i][0], rows4[i][1], rows4[i][2],
+                            rows4[i][3]);
+          } else if (lane < boxes) {
+            tma_load_2d(b_dst + lane * 4096, &tmB, fb, k0, t.r0 + lane * 32);
+          }
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------- MMA issuer
+    auto wait_all = [&](uint32_t bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag)) != 0;
+    };
+    // K-major tile: 128-byte rows, 8-row groups 1024 bytes apart, a K step is 32 bytes.
+    // MN-major tile: 64-column chunks 8192 bytes apart, a K step is 16 rows of 128 bytes.
+    const bool a_mn = GRAD || p.a_mn_major;
+    constexpr bool b_mn = GRAD;
+    const uint32_t a_lo0 = ((a_mn ? 8192u : 16u) >> 4) << 16 | (ptx::smem_u32(sA) >> 4);
+    const uint32_t b_lo0 = ((b_mn ? 8192u : 16u) >> 4) << 16 | (ptx::smem_u32(sB) >> 4);
+    constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    const uint32_t a_step = (a_mn ? 2048u : 32u) >> 4, b_step = (b_mn ? 2048u : 32u) >> 4;
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (int idx = blockIdx.x; ok && idx < total; idx += gridDim.x) {
+      const GroupedTile t = grouped_tile<BT, GRAD>(p, table, idx);
+      const uint32_t idesc = ptx::make_idesc_f16(p.bf16, a_mn, b_mn, 128, t.wide);
+      if (!wait_all(ptx::smem_u32(&tempty_bar[acc]), acc_phase ^ 1u)) break;
+      ptx::tc_fence_after();
+      const uint32_t d = tmem_base + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
+      for (int kb = 0; kb < t.num_kb; ++kb) {
+        if (!wait_all(ptx::smem_u32(&full_bar[stage]), phase)) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        if (ptx::elect_one()) {
+          const uint32_t a_lo = a_lo0 + static_cast<uint32_t>(stage) * (Cfg::A_BYTES >> 4);
+          const uint32_t b_lo = b_lo0 + static_cast<uint32_t>(stage) * (Cfg::B_BYTES >> 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t bd = (static_cast<uint64_t>(hi) << 32) | (b_lo + k * b_step);
+#pragma unroll
+            for (int s = 0; s < MSETS; ++s) {
+              const uint64_t ad = (static_cast<uint64_t>(hi) << 32) | (a_lo + s * (16384u >> 4) + k * a_step);
+              ptx::umma_k<1, 0>(d + s * BT, ad, bd, idesc, (kb | k) != 0 ? 1u : 0u);
+            }
+          }
+          ptx::umma_commit<1>(ptx::smem_u32(&empty_bar[stage]));
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      if (ptx::elect_one()) ptx::umma_commit<1>(ptx::smem_u32(&tfull_bar[acc]));
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;  // TMEM lane quarter this warp may touch
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int idx = blockIdx.x; idx < total; idx += gridDim.x) {
+      const GroupedTile t = grouped_tile<BT, GRAD>(p, table, idx);
+      const int n = t.n0 + q * 32 + lane;
+      const bool mine = n < p.cols, both = (n | 1) < p.cols;
+      float bias = 0.0f, bias_up = 0.0f;
+      if (p.bias != nullptr && mine) {
+        const long long at = static_cast<long long>(t.g) * p.bias_cols + n;
+        bias = load_as_f32(p.bias, p.bias_dtype, at);
+        if constexpr (MSETS == 2) bias_up = load_as_f32(p.bias, p.bias_dtype, at + p.cols);
+      }
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc]), acc_phase, abort_flag))) break;
+      ptx::tc_fence_after();
+      const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
+      const bool warp_has = t.n0 + q * 32 < p.cols;
+      const long long out0 = GRAD ? t.g * p.out_group : 0ll;
+      for (int c = 0; c < t.rows && warp_has; c += 32) {
+        float f[32], u[MSETS == 2 ? 32 : 1];
+        if (!GRAD || t.num_kb > 0) {
+          uint32_t v[32];
+          ptx::tmem_ld_32x32(src + c, v);
+          if constexpr (MSETS == 2) {
+            uint32_t w[32];
+            ptx::tmem_ld_32x32(src + BT + c, w);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(w[i]);
+          } else {
+            ptx::tmem_ld_wait();
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+        } else {
+          // a group without rows: no MMA has written the accumulator
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+        }
+        if (c + 32 >= t.rows) {
+          // the accumulator has been read: the slot is the MMA warp's again
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&tempty_bar[acc]));
+        }
+        grouped_finish32<MSETS>(p, f, u, bias, bias_up);
+        grouped_store32(p, p.out, out0 + static_cast<long long>(t.r0 + c) * p.out_s0 + n, f, t.rows - c, lane, mine,
+                        both);
+      }
+      if (!warp_has) {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&tempty_bar[acc]));
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+  }
+
+  // ---------------------------------------------------------------- teardown
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0u) {
+    if (threadIdx.x == 0) atomicExch(p.status, kStatusTimeout);
+    // loads in flight land before the shared memory they target is released
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 200000ull) {
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<1>(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+}  // namespace kapyb

@@ -7,6 +7,7 @@
 #include "../../include/kapyb.h"
 #include "combine_rows.cuh"
 #include "context.cuh"
+#include "grouped_sm100.cuh"
 #include "plan_rows.cuh"
 #include "route.cuh"
 #include "rows_simt.cuh"
@@ -292,7 +293,143 @@ extern "C" KAPYB_API kapyb_status kapyb_plan_rows(kapyb_handle h, const int32_t 
 
 namespace {
 
-constexpr int kMaxRowGroups = 1024;
+constexpr int kMaxRowGroups = kGroupedMaxGroups;
+
+// 2-D map over 16-bit rows of `inner` unit-stride elements, boxes of 64 elements x box_rows.
+kapyb_status make_row_tmap(kapyb_handle h, CUtensorMap *map, const void *base, int dtype, uint64_t inner,
+                           uint64_t rows, uint64_t ld, uint32_t box_rows) {
+  cuuint64_t dims[2] = {inner, rows};
+  cuuint64_t strides[1] = {ld * 2};
+  cuuint32_t box[2] = {64, box_rows}, step[2] = {1, 1};
+  const CUresult r = h->encode(map, tmap_dtype(dtype), 2, const_cast<void *>(base), dims, strides, box, step,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(h, KAPYB_CUDA_ERROR, "cuTensorMapEncodeTiled failed (%d): rows of %llu, %llu of them, ld %llu", (int)r,
+                (unsigned long long)inner, (unsigned long long)rows, (unsigned long long)ld);
+  return KAPYB_OK;
+}
+
+bool half_type(int dtype) { return dtype == KAPYB_F16 || dtype == KAPYB_BF16; }
+
+// Two neighbouring 16-bit columns of the output may be written as one aligned word.
+bool pair_stores_ok(const void *out, int dtype, int64_t s0, int64_t group) {
+  return half_type(dtype) && reinterpret_cast<uintptr_t>(out) % 4 == 0 && s0 % 2 == 0 && group % 2 == 0;
+}
+
+template <int BT, int MSETS, bool GRAD>
+kapyb_status launch_grouped(kapyb_handle h, const CUtensorMap &tmA, const CUtensorMap &tmB, const GroupedParams &gp,
+                            long long tiles, cudaStream_t stream) {
+  using Cfg = GroupedCfg<BT, MSETS>;
+  auto kern = grouped_tcgen05_kernel<BT, MSETS, GRAD>;
+  CUDA_TRY(h, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+  const int grid = static_cast<int>(std::min<long long>(tiles, h->sm_count));
+  kern<<<grid, kGroupedThreads, Cfg::SMEM_BYTES, stream>>>(tmA, tmB, gp);
+  return launched(h, GRAD ? "grouped_grad_tcgen05" : "grouped_tcgen05");
+}
+
+// Rows of lhs as TMA can fetch them: 16-bit, unit stride along K, 16-byte rows.
+bool rows_tma_ok(const kapyb_tensor2d *t) {
+  return half_type(t->dtype) && t->stride1 == 1 && tma_ok(elem_ptr(t), t->dtype, t->size1, t->size0, t->stride0, 1, 0);
+}
+
+// The tensor-core path of kapyb_matmul_grouped; *taken = false when the operands are
+// not for it.
+kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const kapyb_tensor2d *rhs, int groups,
+                                int64_t group_stride, const int32_t *offsets, const int32_t *order, int fan,
+                                const kapyb_tensor2d *out, const kapyb_epilogue &ep, bool gated, cudaStream_t stream,
+                                bool *taken) {
+  *taken = false;
+  if (!rows_tma_ok(lhs) || out->stride1 != 1) return KAPYB_OK;
+  const bool mn = rhs->stride1 == 1;
+  if (!mn && rhs->stride0 != 1) return KAPYB_OK;
+  const int64_t unit = mn ? rhs->size1 : rhs->size0, other = mn ? rhs->size0 : rhs->size1;
+  const int64_t ld = mn ? rhs->stride0 : rhs->stride1;
+  if (!tma_ok(elem_ptr(rhs), rhs->dtype, unit, other, ld, groups, group_stride)) return KAPYB_OK;
+  // the up columns' tiles start at column cols: a TMA start on 16 bytes
+  if (gated && mn && out->size1 % 8 != 0) return KAPYB_OK;
+  GroupedParams gp{};
+  gp.groups = groups;
+  gp.rows = out->size0;
+  gp.cols = out->size1;
+  gp.K = lhs->size1;
+  gp.n_tiles = (gp.cols + 127) / 128;
+  gp.num_kb = (gp.K + 63) / 64;
+  gp.offsets = offsets;
+  gp.order = order;
+  gp.fan = order ? fan : 1;
+  gp.src_rows = lhs->size0;
+  gp.a_mn_major = mn;
+  gp.bf16 = lhs->dtype == KAPYB_BF16;
+  gp.out = const_cast<void *>(elem_ptr(out));
+  gp.out_s0 = out->stride0;
+  gp.out_dtype = out->dtype;
+  gp.pair_stores = pair_stores_ok(gp.out, out->dtype, out->stride0, 0);
+  gp.alpha = ep.alpha;
+  gp.bias = ep.bias;
+  gp.bias_dtype = ep.bias_dtype;
+  gp.bias_cols = rhs->size1;
+  gp.activation = ep.activation;
+  gp.rounding = ep.rounding;
+  gp.status = h->status;
+  gp.wait_limit_us = h->wait_limit_us;
+  const long long busy = std::min(groups, gp.rows);
+  const bool narrow = gp.rows <= 32 * busy;  // rows per group that has any, at most
+  const int bt = narrow ? 64 : gated ? 128 : 256;
+  const long long tiles = ((gp.rows + bt - 1ll) / bt + busy) * gp.n_tiles;
+  if (tiles >= (1ll << 31)) return KAPYB_OK;
+  CUtensorMap tmA, tmB;
+  TRY(make_tmap(h, &tmA, elem_ptr(rhs), rhs->dtype, unit, other, groups, ld, group_stride, 64, mn ? 64 : 128));
+  TRY(make_row_tmap(h, &tmB, elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
+                    lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, order ? 1 : 32));
+  *taken = true;
+  if (gated)
+    return narrow ? launch_grouped<64, 2, false>(h, tmA, tmB, gp, tiles, stream)
+                  : launch_grouped<128, 2, false>(h, tmA, tmB, gp, tiles, stream);
+  return narrow ? launch_grouped<64, 1, false>(h, tmA, tmB, gp, tiles, stream)
+                : launch_grouped<256, 1, false>(h, tmA, tmB, gp, tiles, stream);
+}
+
+kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const kapyb_tensor2d *grad,
+                                     int groups, const int32_t *offsets, const int32_t *order, int fan,
+                                     const kapyb_tensor2d *out, int64_t out_group_stride, float alpha, int rounding,
+                                     cudaStream_t stream, bool *taken) {
+  *taken = false;
+  if (!rows_tma_ok(lhs) || !rows_tma_ok(grad) || out->stride1 != 1) return KAPYB_OK;
+  GroupedParams gp{};
+  gp.groups = groups;
+  gp.rows = grad->size0;
+  gp.cols = out->size1;
+  gp.K = out->size0;
+  gp.n_tiles = (gp.cols + 127) / 128;
+  const int bt = gp.K <= 64 ? 64 : 256;
+  gp.k_tiles = (gp.K + bt - 1) / bt;
+  gp.offsets = offsets;
+  gp.order = order;
+  gp.fan = order ? fan : 1;
+  gp.src_rows = lhs->size0;
+  gp.bf16 = lhs->dtype == KAPYB_BF16;
+  gp.out = const_cast<void *>(elem_ptr(out));
+  gp.out_s0 = out->stride0;
+  gp.out_group = out_group_stride;
+  gp.out_dtype = out->dtype;
+  gp.pair_stores = pair_stores_ok(gp.out, out->dtype, out->stride0, groups > 1 ? out_group_stride : 0);
+  gp.alpha = alpha;
+  gp.activation = KAPYB_ACT_NONE;
+  gp.rounding = rounding;
+  gp.status = h->status;
+  gp.wait_limit_us = h->wait_limit_us;
+  const long long tiles = static_cast<long long>(groups) * gp.n_tiles * gp.k_tiles;
+  if (tiles >= (1ll << 31)) return KAPYB_OK;
+  CUtensorMap tmA, tmB;
+  TRY(make_row_tmap(h, &tmA, elem_ptr(grad), grad->dtype, grad->size1, grad->size0,
+                    grad->size0 > 1 ? grad->stride0 : (grad->size1 + 7) / 8 * 8, 1));
+  TRY(make_row_tmap(h, &tmB, elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
+                    lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, 1));
+  *taken = true;
+  return bt == 64 ? launch_grouped<64, 1, true>(h, tmA, tmB, gp, tiles, stream)
+                  : launch_grouped<256, 1, true>(h, tmA, tmB, gp, tiles, stream);
+}
 
 // What the two grouped products check alike.
 kapyb_status check_grouped(kapyb_handle h, const char *call, const kapyb_tensor2d *lhs, const kapyb_tensor2d *other,
@@ -345,6 +482,10 @@ extern "C" KAPYB_API kapyb_status kapyb_matmul_grouped(kapyb_handle h, const kap
     return fail(h, KAPYB_INVALID_ARG, "%s: out overlaps an input", call);
   ON_DEVICE(h);
   const kapyb_epilogue &ep = epilogue ? *epilogue : kPlainEpilogue;
+  bool taken = false;
+  const kapyb_status st = grouped_on_tcgen05(h, lhs, rhs, groups, group_stride, offsets, order, fan, out, ep,
+                                             gated != 0, static_cast<cudaStream_t>(stream), &taken);
+  if (taken || st != KAPYB_OK) return st;
   RowsSimtParams p{};
   p.x = elem_ptr(lhs);
   p.x_s0 = lhs->stride0;
@@ -410,6 +551,10 @@ extern "C" KAPYB_API kapyb_status kapyb_matmul_grouped_grad(kapyb_handle h, cons
       meet(o, span_of(order, order ? grad->size0 * 4ull : 0)))
     return fail(h, KAPYB_INVALID_ARG, "%s: out overlaps an input", call);
   ON_DEVICE(h);
+  bool taken = false;
+  const kapyb_status st = grouped_grad_on_tcgen05(h, lhs, grad, groups, offsets, order, fan, out, out_group_stride,
+                                                  alpha, rounding, static_cast<cudaStream_t>(stream), &taken);
+  if (taken || st != KAPYB_OK) return st;
   RowsSimtParams p{};
   p.x = elem_ptr(lhs);
   p.x_s0 = lhs->stride0;
