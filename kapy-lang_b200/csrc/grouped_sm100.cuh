@@ -29,6 +29,7 @@
 #include <cuda.h>
 
 #include "common.cuh"
+#include "gemm_sm100.cuh"
 #include "ptx_sm100.cuh"
 #include "rows_simt.cuh"
 
@@ -67,7 +68,8 @@ struct GroupedParams {
   int a_mn_major;        // forward: rhs has its unit stride on n
   int bf16;
   void *out;
-  long long out_s0, out_group;  // unit stride on n
+  uint32_t row_pitch;           // bytes between output rows, below 2^26; unit stride on n
+  long long group_bytes;        // gradient: bytes between groups
   int out_dtype, pair_stores;   // pair_stores: two 16-bit columns may be stored as one word
   float alpha;
   const void *bias;      // [groups, bias_cols]
@@ -182,60 +184,75 @@ __device__ __forceinline__ void grouped_finish32(const GroupedParams &p, float (
   }
 }
 
-// 32 output rows of one column per lane -> memory.  `row0` points at (first row,
-// column n); rows_left of the 32 exist.  Neighbouring lanes swap half of their values
-// so that each stores two adjacent columns of every other row as one word: half the
-// store instructions of one value each, and 64-byte runs either way.
+// 32 output rows of one column per lane -> memory.  `at` points at (first row, column
+// n), rows are `pitch` bytes apart, `left` of the 32 exist (ALL: all of them).
+// Neighbouring lanes swap half of their 16-bit values so that each stores two adjacent
+// columns of every other row as one word: half the store instructions of one value
+// each.  The common case (32 rows, 32 columns) carries no conditions and 32-bit row
+// offsets: the drain of a short main loop is bound by the instructions of this loop.
+template <int DT, int RN, bool ALL>
+__device__ __forceinline__ void store_pairs16(char *at, uint32_t pitch, const float (&f)[32], int left, int lane,
+                                              bool both) {
+  const bool odd = lane & 1;
+  char *base = odd ? at - 2 + pitch : at;  // (first row + odd, even column)
+  uint32_t off = 0u;
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    const float give = odd ? f[j] : f[j + 1];
+    const float take = __shfl_xor_sync(0xffffffffu, give, 1);
+    const uint32_t w = odd ? cvt_pack2_t<DT, RN>(take, f[j + 1]) : cvt_pack2_t<DT, RN>(f[j], take);
+    if (ALL || (both && j + (odd ? 1 : 0) < left)) *reinterpret_cast<uint32_t *>(base + off) = w;
+    off += 2u * pitch;
+  }
+}
 template <int DT, int RN>
-__device__ __forceinline__ void store_rows16(uint16_t *at, long long s0, const float (&f)[32], int rows_left,
-                                             int lane, bool mine, bool both, bool pairs) {
-  if (pairs) {
-    const bool odd = lane & 1;
-    uint16_t *base = odd ? at - 1 + s0 : at;  // (first row + odd, even column)
+__device__ __forceinline__ void store_single16(char *at, uint32_t pitch, const float (&f)[32], int left, bool on) {
+  if (!on) return;
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      const float give = odd ? f[j] : f[j + 1];
-      const float take = __shfl_xor_sync(0xffffffffu, give, 1);
-      const uint32_t w = odd ? cvt_pack2_t<DT, RN>(take, f[j + 1]) : cvt_pack2_t<DT, RN>(f[j], take);
-      if (j + (odd ? 1 : 0) < rows_left) {
-        if (both)
-          *reinterpret_cast<uint32_t *>(base + j * s0) = w;
-        else if (!odd && mine)  // the last column of an odd number has no neighbour
-          base[j * s0] = static_cast<uint16_t>(w & 0xffffu);
-      }
-    }
-    // ... and its odd rows are stored by itself
-    if (!odd && mine && !both) {
-#pragma unroll
-      for (int j = 1; j < 32; j += 2)
-        if (j < rows_left) at[j * s0] = static_cast<uint16_t>(cvt_pack2_t<DT, RN>(f[j], 0.0f) & 0xffffu);
-    }
-  } else if (mine) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < rows_left) at[j * s0] = static_cast<uint16_t>(cvt_pack2_t<DT, RN>(f[j], 0.0f) & 0xffffu);
+  for (int j = 0; j < 32; ++j)
+    if (j < left)
+      *reinterpret_cast<uint16_t *>(at + static_cast<unsigned long long>(j) * pitch) =
+          static_cast<uint16_t>(cvt_pack2_t<DT, RN>(f[j], 0.0f) & 0xffffu);
+}
+template <int DT, int RN>
+__device__ __forceinline__ void store_rows16(char *at, uint32_t pitch, const float (&f)[32], int left, int lane,
+                                             bool mine, bool both, bool pairs) {
+  if (!pairs) {
+    store_single16<DT, RN>(at, pitch, f, left, mine);
+  } else if (left >= 32 && __all_sync(0xffffffffu, both)) {
+    store_pairs16<DT, RN, true>(at, pitch, f, left, lane, both);
+  } else {
+    store_pairs16<DT, RN, false>(at, pitch, f, left, lane, both);
+    store_single16<DT, RN>(at, pitch, f, left, mine && !both);  // the last of an odd number of columns
   }
 }
 
-__device__ __forceinline__ void grouped_store32(const GroupedParams &p, void *out, long long idx, const float (&f)[32],
-                                                int rows_left, int lane, bool mine, bool both) {
+// p.row_pitch (bytes) is below 2^26, so 32 rows span less than 2^31.
+__device__ __forceinline__ void grouped_store32(const GroupedParams &p, char *at, const float (&f)[32], int left,
+                                                int lane, bool mine, bool both) {
+  const uint32_t pitch = p.row_pitch;
   if (p.out_dtype == KAPYB_F32) {
-    if (mine) {
-      float *at = static_cast<float *>(out) + idx;
+    if (left >= 32 && __all_sync(0xffffffffu, mine)) {
+      uint32_t off = 0u;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        *reinterpret_cast<float *>(at + off) = f[j];
+        off += pitch;
+      }
+    } else if (mine) {
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (j < rows_left) at[j * p.out_s0] = f[j];
+        if (j < left) *reinterpret_cast<float *>(at + static_cast<unsigned long long>(j) * pitch) = f[j];
     }
     return;
   }
-  uint16_t *at = static_cast<uint16_t *>(out) + idx;
   const bool pairs = p.pair_stores != 0;
   if (p.out_dtype == KAPYB_BF16) {
-    if (p.rounding) store_rows16<KAPYB_BF16, 1>(at, p.out_s0, f, rows_left, lane, mine, both, pairs);
-    else store_rows16<KAPYB_BF16, 0>(at, p.out_s0, f, rows_left, lane, mine, both, pairs);
+    if (p.rounding) store_rows16<KAPYB_BF16, 1>(at, pitch, f, left, lane, mine, both, pairs);
+    else store_rows16<KAPYB_BF16, 0>(at, pitch, f, left, lane, mine, both, pairs);
   } else {
-    if (p.rounding) store_rows16<KAPYB_F16, 1>(at, p.out_s0, f, rows_left, lane, mine, both, pairs);
-    else store_rows16<KAPYB_F16, 0>(at, p.out_s0, f, rows_left, lane, mine, both, pairs);
+    if (p.rounding) store_rows16<KAPYB_F16, 1>(at, pitch, f, left, lane, mine, both, pairs);
+    else store_rows16<KAPYB_F16, 0>(at, pitch, f, left, lane, mine, both, pairs);
   }
 }
 
@@ -463,7 +480,8 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
       ptx::tc_fence_after();
       const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
       const bool warp_has = t.n0 + q * 32 < p.cols;
-      const long long out0 = GRAD ? t.g * p.out_group : 0ll;
+      char *out = static_cast<char *>(p.out) + (GRAD ? t.g * p.group_bytes : 0ll) +
+                  static_cast<long long>(t.r0) * p.row_pitch + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll);
       for (int c = 0; c < t.rows && warp_has; c += 32) {
         float f[32], u[MSETS == 2 ? 32 : 1];
         if (!GRAD || t.num_kb > 0) {
@@ -492,8 +510,7 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
           if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&tempty_bar[acc]));
         }
         grouped_finish32<MSETS>(p, f, u, bias, bias_up);
-        grouped_store32(p, p.out, out0 + static_cast<long long>(t.r0 + c) * p.out_s0 + n, f, t.rows - c, lane, mine,
-                        both);
+        grouped_store32(p, out + static_cast<long long>(c) * p.row_pitch, f, t.rows - c, lane, mine, both);
       }
       if (!warp_has) {
         ptx::tc_fence_before();
@@ -519,6 +536,508 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
   if (warp == 1) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc<1>(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------- CTA pairs
+//
+// The kernel for many rows per group: two CTAs of a cluster share one tile through
+// tcgen05.mma.cta_group::2.  Each holds 128 of the tile's 256 output columns (its M
+// half) and fetches half of its rows (its half of the N side), so a row is pulled
+// from L2 once per 256 columns and an SM reads a third fewer operand bytes from
+// shared memory per flop than alone.
+//
+// Gathered rows.  tile::gather4 costs about 70 clocks per four rows here (measured:
+// 37 ns with every lane of a warp issuing), four times the MMA time of the tile they
+// feed, so eight more warps gather with 16-byte cp.async, eight lanes a row, straight
+// into the swizzled layout, as far ahead as there are free stages.  Their copies
+// complete on a barrier of their CTA (cp.async.mbarrier.arrive); one more warp waits
+// there, fences the generic proxy that wrote the rows against the async proxy the MMA
+// reads them through, and arrives on the leader's barrier, whichever CTA it sits in.
+// What has to be ordered are finished copies into an SM's shared memory against the
+// tensor core's reads of the same memory, and the proxy fence does that; the arrival
+// itself carries the default semantics.  (With a release at cluster scope it waited for
+// all copies in flight, 1 to 1.5 us a stage, three times the whole kernel's time.)  Four
+// warps fetch 16 KB a stage in 1070 clocks, twice the MMA's time for it (8192 x 4096 x
+// 4096 as one group: 259 us); eight keep up with it (193 us, rows in plan order 183).
+//
+// In the gradient the rows are the contraction: lhs is always gathered (zeros behind
+// the group's end), grad lies in plan order and comes by TMA, whole 64-row boxes while
+// they last and then 8-row and 1-row boxes, so that what is behind the end is fetched
+// as zeros as well.
+
+struct PairParams {
+  GroupedParams g;
+  int gather;            // rows of lhs by cp.async: a plan's order, and always the gradient
+  const uint8_t *lhs;    // element (0, 0)
+  long long lhs_pitch;   // bytes between rows
+  FastDiv div_fan;
+};
+
+constexpr int kPairThreads = 192 + 256 + 32;
+
+template <int BT, int MSETS>
+struct PairCfg {
+  static constexpr int A_BYTES = MSETS * 128 * 128;  // per CTA
+  static constexpr int B_BYTES = BT / 2 * 128;       // per CTA: half of the tile's rows
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int CTRL_BYTES = 1024;
+  static constexpr int TABLE_BYTES = (3 * kGroupedMaxGroups + 4) * 4;
+  static constexpr int SMEM_LIMIT = 232448;
+  static constexpr int STAGES_RAW = (SMEM_LIMIT - 1024 - CTRL_BYTES - TABLE_BYTES) / STAGE_BYTES;
+  static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + CTRL_BYTES + TABLE_BYTES;
+  static constexpr int SLOT_COLS = BT * MSETS;
+  static constexpr int TMEM_COLS = 2 * SLOT_COLS;
+  static_assert(TMEM_COLS == 512 && BT % 64 == 0 && STAGES >= 3, "tile");
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// Arrives on `bar` once every cp.async this thread has issued so far is complete.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void *tmap, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];"
+      :
+      : "r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+__device__ __forceinline__ int round32(int v) { return (v + 31) & ~31; }
+
+// The tile of a pair: as grouped_tile, for blocks of 256 columns, rows rounded to 32
+// (the N side of a pair's MMA is a multiple of 32).
+template <int BT, bool GRAD>
+__device__ __forceinline__ GroupedTile pair_tile(const GroupedParams &p, const GroupedTable &t, int idx) {
+  GroupedTile r;
+  if constexpr (GRAD) {
+    const int per = p.n_tiles * p.k_tiles;
+    r.g = idx / per;
+    const int in = idx - r.g * per;
+    const int n = in / p.k_tiles;
+    r.r0 = (in - n * p.k_tiles) * BT;
+    r.n0 = n * 256;
+    r.rows = min(BT, p.K - r.r0);
+    r.p0 = t.begin[r.g];
+    r.p1 = r.p0 + t.count[r.g];
+    r.num_kb = (t.count[r.g] + 63) >> 6;
+  } else {
+    const int q = idx / p.n_tiles;
+    int lo = 0, hi = p.groups;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (t.first[mid] <= q) lo = mid;
+      else hi = mid;
+    }
+    r.g = lo;
+    const int tiles = t.first[lo + 1] - t.first[lo];
+    const int in = idx - t.first[lo] * p.n_tiles;
+    const int n = in / tiles, m = in - n * tiles;
+    const int cnt = t.count[lo];
+    const int each = round32((cnt + tiles - 1) / tiles);
+    r.n0 = n * 256;
+    r.r0 = t.begin[lo] + m * each;
+    r.rows = min(each, cnt - m * each);
+    r.num_kb = p.num_kb;
+    r.p0 = r.p1 = 0;
+  }
+  r.wide = round32(r.rows);
+  return r;
+}
+
+// tmA: forward: rhs as in grouped_tcgen05_kernel; gradient: grad in boxes of 64 x 64,
+// tmA8 and tmA1 the same in boxes 8 rows and 1 row high.  Forward without a gather: lhs
+// in boxes of 64 x 32 (tmB) and 64 x BT / 2 (tmA8).
+template <int BT, int MSETS, bool GRAD>
+__global__ void __launch_bounds__(kPairThreads, 1)
+grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmA8, const __grid_constant__ CUtensorMap tmA1,
+                    const PairParams pp) {
+  using Cfg = PairCfg<BT, MSETS>;
+  constexpr int STAGES = Cfg::STAGES;
+  const GroupedParams &p = pp.g;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                              ~static_cast<uintptr_t>(1023));
+  uint8_t *sA = smem;
+  uint8_t *sB = sA + STAGES * Cfg::A_BYTES;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(sB + STAGES * Cfg::B_BYTES);
+  uint64_t *full_bar = bars, *empty_bar = bars + STAGES, *tfull_bar = bars + 2 * STAGES, *tempty_bar = tfull_bar + 2;
+  uint64_t *rows_bar = tempty_bar + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(rows_bar + STAGES);
+  volatile uint32_t *abort_flag = tmem_slot + 1;  // two words
+  int *table_mem = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(bars) + Cfg::CTRL_BYTES);
+  GroupedTable table{table_mem, table_mem + kGroupedMaxGroups + 1, table_mem + 2 * kGroupedMaxGroups + 1};
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(ptx::cluster_ctarank());
+  const int unit = blockIdx.x >> 1, units = gridDim.x >> 1;
+  const bool gather = GRAD || pp.gather;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      // the leader's expect_tx, and with a gather one arrival from each CTA
+      ptx::mbar_init(ptx::smem_u32(&full_bar[s]), gather ? 3 : 1);
+      ptx::mbar_init(ptx::smem_u32(&rows_bar[s]), 256);  // every gathering thread
+      ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(ptx::smem_u32(&tfull_bar[a]), 1);
+      ptx::mbar_init(ptx::smem_u32(&tempty_bar[a]), 8);  // four epilogue warps of each CTA
+    }
+    abort_flag[0] = 0u;
+    abort_flag[1] = p.wait_limit_us;
+    ptx::fence_barrier_init();
+    ptx::prefetch_tensormap(&tmA);
+    ptx::prefetch_tensormap(&tmB);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<2>(ptx::smem_u32(tmem_slot), Cfg::TMEM_COLS);
+    ptx::tmem_relinquish<2>();
+  }
+  if (warp == 0) {
+    int before = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+      const int g = g0 + lane;
+      int b = 0, e = 0;
+      if (g < p.groups) group_range(p.offsets, g, p.rows, b, e);
+      const int cnt = max(0, e - b);
+      const int tiles = GRAD ? 0 : (cnt + BT - 1) / BT;
+      int scan = tiles;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, scan, off);
+        if (lane >= off) scan += o;
+      }
+      if (g < p.groups) {
+        table.first[g] = before + scan - tiles;
+        table.begin[g] = b;
+        table.count[g] = cnt;
+      }
+      before += __shfl_sync(0xffffffffu, scan, 31);
+    }
+    if (lane == 0) table.first[p.groups] = before;
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int total = GRAD ? p.groups * p.n_tiles * p.k_tiles : table.first[p.groups] * p.n_tiles;
+  auto leader = [](const void *bar) { return ptx::mapa(ptx::smem_u32(bar), 0); };
+
+  if (warp == 0) {
+    // ------------------------------------- TMA: the columns' side, and rows in plan order
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int idx = unit; ok && idx < total; idx += units) {
+      const GroupedTile t = pair_tile<BT, GRAD>(p, table, idx);
+      const int half = t.wide >> 1;                         // rows this CTA fetches
+      // rows in plan order: one tall box, or boxes of 32 rows where it would fetch too much
+      const bool tall = half > BT / 2 - 32;
+      const int boxes = gather ? 0 : tall ? 1 : (half + 31) >> 5;
+      const uint32_t b_bytes = gather ? 0u : tall ? static_cast<uint32_t>(Cfg::B_BYTES) : boxes * 4096u;
+      const int n0 = t.n0 + rank * 128;
+      for (int kb = 0; kb < t.num_kb; ++kb) {
+        const bool got = ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag);
+        if (!__all_sync(0xffffffffu, got)) {
+          ok = false;
+          break;
+        }
+        const uint32_t fb = leader(&full_bar[stage]);
+        const uint32_t a_dst = ptx::smem_u32(sA + stage * Cfg::A_BYTES);
+        const uint32_t b_dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES);
+        if (rank == 0 && lane == 0)
+          ptx::mbar_arrive_expect_tx(ptx::smem_u32(&full_bar[stage]), 2u * (Cfg::A_BYTES + b_bytes));
+        __syncwarp();
+        if constexpr (GRAD) {
+          const int q = t.p0 + kb * 64;
+          const int live = t.p1 - q;  // positions of this block that are the group's
+          if (live >= 64) {
+            if (lane < 2) tma_load_2d_pair(a_dst + lane * 8192, &tmA, fb, n0 + lane * 64, q);
+          } else if (lane < 16) {
+            // eight rows per lane: all of the group, none of it, or the border
+            const int c = lane >> 3, r = (lane & 7) * 8;
+            const uint32_t dst = a_dst + c * 8192 + r * 128;
+            if (r + 8 <= live || r >= live) {
+              tma_load_2d_pair(dst, &tmA8, fb, n0 + c * 64, r < live ? q + r : p.rows);
+            } else {
+              for (int j = 0; j < 8; ++j)
+                tma_load_2d_pair(dst + j * 128, &tmA1, fb, n0 + c * 64, r + j < live ? q + r + j : p.rows);
+            }
+          }
+        } else {
+          const int k0 = kb * 64;
+          if (p.a_mn_major) {
+            if (lane < 2 * MSETS)
+              ptx::tma_load_3d_pair(a_dst + lane * 8192, &tmA, fb, n0 + (lane & 1) * 64 + (lane >> 1) * p.cols, k0, t.g);
+          } else {
+            if (lane < MSETS) ptx::tma_load_3d_pair(a_dst + lane * 16384, &tmA, fb, k0, n0 + lane * p.cols, t.g);
+          }
+          if (tall) {
+            if (boxes && lane == 0) tma_load_2d_pair(b_dst, &tmA8, fb, k0, t.r0 + rank * half);
+          } else if (lane < boxes) {
+            tma_load_2d_pair(b_dst + lane * 4096, &tmB, fb, k0, t.r0 + rank * half + lane * 32);
+          }
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1 && rank == 0) {
+    // ---------------------------------------------------------- MMA issuer
+    auto wait_all = [&](uint32_t bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag)) != 0;
+    };
+    const bool a_mn = GRAD || p.a_mn_major;
+    constexpr bool b_mn = GRAD;
+    const uint32_t a_lo0 = ((a_mn ? 8192u : 16u) >> 4) << 16 | (ptx::smem_u32(sA) >> 4);
+    const uint32_t b_lo0 = ((b_mn ? 8192u : 16u) >> 4) << 16 | (ptx::smem_u32(sB) >> 4);
+    constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    const uint32_t a_step = (a_mn ? 2048u : 32u) >> 4, b_step = (b_mn ? 2048u : 32u) >> 4;
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (int idx = unit; ok && idx < total; idx += units) {
+      const GroupedTile t = pair_tile<BT, GRAD>(p, table, idx);
+      const uint32_t idesc = ptx::make_idesc_f16(p.bf16, a_mn, b_mn, 256, t.wide);
+      if (!wait_all(ptx::smem_u32(&tempty_bar[acc]), acc_phase ^ 1u)) break;
+      ptx::tc_fence_after();
+      const uint32_t d = tmem_base + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
+      for (int kb = 0; kb < t.num_kb; ++kb) {
+        if (!wait_all(ptx::smem_u32(&full_bar[stage]), phase)) {
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        if (ptx::elect_one()) {
+          const uint32_t a_lo = a_lo0 + static_cast<uint32_t>(stage) * (Cfg::A_BYTES >> 4);
+          const uint32_t b_lo = b_lo0 + static_cast<uint32_t>(stage) * (Cfg::B_BYTES >> 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t bd = (static_cast<uint64_t>(hi) << 32) | (b_lo + k * b_step);
+#pragma unroll
+            for (int s = 0; s < MSETS; ++s) {
+              const uint64_t ad = (static_cast<uint64_t>(hi) << 32) | (a_lo + s * (16384u >> 4) + k * a_step);
+              ptx::umma_k<2, 0>(d + s * BT, ad, bd, idesc, (kb | k) != 0 ? 1u : 0u);
+            }
+          }
+          ptx::umma_commit<2>(ptx::smem_u32(&empty_bar[stage]));
+          ptx::umma_commit<2>(ptx::mapa(ptx::smem_u32(&empty_bar[stage]), 1));
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      if (ptx::elect_one()) {
+        ptx::umma_commit<2>(ptx::smem_u32(&tfull_bar[acc]));
+        ptx::umma_commit<2>(ptx::mapa(ptx::smem_u32(&tfull_bar[acc]), 1));
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+  } else if (warp >= 2 && warp < 6) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int idx = unit; idx < total; idx += units) {
+      const GroupedTile t = pair_tile<BT, GRAD>(p, table, idx);
+      const int warp_n = t.n0 + rank * 128 + q * 32;
+      const int n = warp_n + lane;
+      const bool mine = n < p.cols, both = (n | 1) < p.cols;
+      float bias = 0.0f, bias_up = 0.0f;
+      if (p.bias != nullptr && mine) {
+        const long long at = static_cast<long long>(t.g) * p.bias_cols + n;
+        bias = load_as_f32(p.bias, p.bias_dtype, at);
+        if constexpr (MSETS == 2) bias_up = load_as_f32(p.bias, p.bias_dtype, at + p.cols);
+      }
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc]), acc_phase, abort_flag))) break;
+      ptx::tc_fence_after();
+      const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
+      const uint32_t tempty = leader(&tempty_bar[acc]);
+      const bool warp_has = warp_n < p.cols;
+      char *out = static_cast<char *>(p.out) + (GRAD ? t.g * p.group_bytes : 0ll) +
+                  static_cast<long long>(t.r0) * p.row_pitch + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll);
+      for (int c = 0; c < t.rows && warp_has; c += 32) {
+        float f[32], u[MSETS == 2 ? 32 : 1];
+        if (!GRAD || t.num_kb > 0) {
+          uint32_t v[32];
+          ptx::tmem_ld_32x32(src + c, v);
+          if constexpr (MSETS == 2) {
+            uint32_t w[32];
+            ptx::tmem_ld_32x32(src + BT + c, w);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(w[i]);
+          } else {
+            ptx::tmem_ld_wait();
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+        }
+        if (c + 32 >= t.rows) {
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive_cluster(tempty);
+        }
+        grouped_finish32<MSETS>(p, f, u, bias, bias_up);
+        grouped_store32(p, out + static_cast<long long>(c) * p.row_pitch, f, t.rows - c, lane, mine, both);
+      }
+      if (!warp_has) {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(tempty);
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+  } else if (warp == 14 && gather) {
+    // ------------------------- finished copies of this CTA -> the leader's barrier
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int idx = unit; ok && idx < total; idx += units) {
+      const GroupedTile t = pair_tile<BT, GRAD>(p, table, idx);
+      for (int kb = 0; kb < t.num_kb; ++kb) {
+        if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&rows_bar[stage]), phase, abort_flag))) {
+          ok = false;
+          break;
+        }
+        ptx::fence_proxy_async_smem();
+        if (lane == 0) ptx::mbar_arrive_cluster(leader(&full_bar[stage]));
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp >= 6 && gather) {
+    // -------------------------------------------------------------- gather
+    const int tid = threadIdx.x - 192;  // 0 .. 255
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int idx = unit; ok && idx < total; idx += units) {
+      const GroupedTile t = pair_tile<BT, GRAD>(p, table, idx);
+      const int half = t.wide >> 1;
+      if constexpr (GRAD) {
+        // thread: 16-byte piece `piece` of this CTA's columns, rows row0, row0 + 16, ...
+        const int piece = tid & 15, row0 = tid >> 4;
+        const int col = t.r0 + rank * half + piece * 8;
+        const uint32_t bytes = static_cast<uint32_t>(max(0, min(16, (p.K - col) * 2)));
+        const bool need = piece * 8 < half;
+        const uint8_t *base = pp.lhs + static_cast<long long>(bytes ? col : 0) * 2;
+        // Plan entries are loaded two blocks ahead, into two sets of registers that take
+        // turns, and turned into row numbers when they are needed: no block waits for
+        // the load that names its rows.
+        int even[4], odd[4];
+        auto fetch = [&](int kb, int (&entry)[4]) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int q = t.p0 + kb * 64 + row0 + 16 * i;
+            entry[i] = q >= t.p1 ? -1 : p.order ? __ldg(p.order + q) : q;
+          }
+        };
+        auto copy = [&](const int (&entry)[4]) -> bool {
+          if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)))
+            return false;
+          const uint32_t dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES) + (piece >> 3) * 8192;
+          if (need) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = row0 + 16 * i;
+              const int from = entry[i] < 0 ? -1 : p.order ? pp.div_fan.div(entry[i]) : entry[i];
+              const bool live = from >= 0 && from < p.src_rows;
+              cp_async16(dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4), base + (live ? from * pp.lhs_pitch : 0ll),
+                         live ? bytes : 0u);
+            }
+          }
+          cp_async_arrive(ptx::smem_u32(&rows_bar[stage]));
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          return true;
+        };
+        fetch(0, even);
+        fetch(1, odd);
+        for (int kb = 0; ok && kb < t.num_kb; kb += 2) {
+          ok = copy(even);
+          fetch(kb + 2, even);
+          if (ok && kb + 1 < t.num_kb) {
+            ok = copy(odd);
+            fetch(kb + 3, odd);
+          }
+        }
+      } else {
+        // thread: 16-byte piece tid % 8 of rows tid / 8, + 32, ...
+        constexpr int kRows = BT / 64;
+        const int piece = tid & 7, row0 = tid >> 3;
+        const uint8_t *row[kRows];
+        bool live[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const int r = rank * half + row0 + 32 * i;  // row of the tile
+          long long s = -1;
+          if (row0 + 32 * i < half && r < t.rows) s = source_row(p.order, p.fan, p.src_rows, t.r0 + r);
+          live[i] = s >= 0;
+          row[i] = pp.lhs + (live[i] ? s * pp.lhs_pitch : 0);
+        }
+        for (int kb = 0; kb < t.num_kb; ++kb) {
+          if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag))) {
+            ok = false;
+            break;
+          }
+          const int k = kb * 64 + piece * 8;
+          const uint32_t bytes = static_cast<uint32_t>(max(0, min(16, (p.K - k) * 2)));
+          const uint32_t dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES) + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
+          const long long at = bytes ? k * 2ll : 0ll;
+#pragma unroll
+          for (int i = 0; i < kRows; ++i)
+            if (row0 + 32 * i < half) cp_async16(dst + i * 4096, row[i] + at, live[i] ? bytes : 0u);
+          cp_async_arrive(ptx::smem_u32(&rows_bar[stage]));
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+    cp_async_wait_all();
+  }
+
+  // ---------------------------------------------------------------- teardown
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0u) {
+    if (threadIdx.x == 0) atomicExch(p.status, kStatusTimeout);
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 200000ull) {
+    }
+    __syncthreads();
+  }
+  // the peer may still address this CTA's barriers and shared memory
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<2>(tmem_base, Cfg::TMEM_COLS);
   }
 }
 

@@ -4,6 +4,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../../include/kapyb.h"
 #include "combine_rows.cuh"
 #include "context.cuh"
@@ -163,23 +165,29 @@ RouteParams route_params(const kapyb_tensor2d *logits, const kapyb_routing *r) {
   return p;
 }
 
-// experts per lane, rounded up to a compiled width
-template <template <int> class Launch>
-void by_width(int experts, const RouteParams &p, int grid, cudaStream_t stream) {
-  if (experts <= 64) Launch<2>::go(p, grid, stream);
-  else if (experts <= 128) Launch<4>::go(p, grid, stream);
-  else if (experts <= 256) Launch<8>::go(p, grid, stream);
-  else if (experts <= 512) Launch<16>::go(p, grid, stream);
-  else Launch<32>::go(p, grid, stream);
+// Experts per lane, rounded up to a compiled width; VEC: a lane's experts are one aligned
+// run that exists as a whole.
+template <int VPT>
+bool row_vec_ok(const RouteParams &p) {
+  const int64_t esz = dtype_size(p.x_dtype);
+  const int64_t align = std::min<int64_t>(16, VPT * esz);
+  return p.x_s1 == 1 && p.experts % VPT == 0 && reinterpret_cast<uintptr_t>(p.x) % align == 0 &&
+         (p.x_s0 * esz) % align == 0;
 }
 template <int VPT>
-struct LaunchRoute {
-  static void go(const RouteParams &p, int grid, cudaStream_t s) { route_kernel<VPT><<<grid, 256, 0, s>>>(p); }
-};
+void launch_route(const RouteParams &p, int grid, cudaStream_t s) {
+  const bool scored = p.bias != nullptr || (p.n_groups > 1 && p.group_best > 1);
+  const bool vec = row_vec_ok<VPT>(p);
+  if (scored && vec) route_kernel<VPT, true, true><<<grid, 256, 0, s>>>(p);
+  else if (scored) route_kernel<VPT, true, false><<<grid, 256, 0, s>>>(p);
+  else if (vec) route_kernel<VPT, false, true><<<grid, 256, 0, s>>>(p);
+  else route_kernel<VPT, false, false><<<grid, 256, 0, s>>>(p);
+}
 template <int VPT>
-struct LaunchRouteBackward {
-  static void go(const RouteParams &p, int grid, cudaStream_t s) { route_backward_kernel<VPT><<<grid, 256, 0, s>>>(p); }
-};
+void launch_route_backward(const RouteParams &p, int grid, cudaStream_t s) {
+  if (row_vec_ok<VPT>(p)) route_backward_kernel<VPT, true><<<grid, 256, 0, s>>>(p);
+  else route_backward_kernel<VPT, false><<<grid, 256, 0, s>>>(p);
+}
 
 int warp_grid(int rows) { return static_cast<int>((rows + 7ll) / 8); }
 
@@ -208,7 +216,13 @@ extern "C" KAPYB_API kapyb_status kapyb_route(kapyb_handle h, const kapyb_tensor
   p.bias = bias;
   p.weights = weights;
   p.chosen = experts;
-  by_width<LaunchRoute>(p.experts, p, warp_grid(p.rows), static_cast<cudaStream_t>(stream));
+  const int grid = warp_grid(p.rows);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p.experts <= 64) launch_route<2>(p, grid, s);
+  else if (p.experts <= 128) launch_route<4>(p, grid, s);
+  else if (p.experts <= 256) launch_route<8>(p, grid, s);
+  else if (p.experts <= 512) launch_route<16>(p, grid, s);
+  else launch_route<32>(p, grid, s);
   return launched(h, "route");
 }
 
@@ -241,7 +255,16 @@ extern "C" KAPYB_API kapyb_status kapyb_route_backward(kapyb_handle h, const kap
   p.g_s0 = grad_logits->stride0;
   p.g_s1 = grad_logits->stride1;
   p.g_dtype = grad_logits->dtype;
-  by_width<LaunchRouteBackward>(p.experts, p, warp_grid(p.rows), static_cast<cudaStream_t>(stream));
+  const int64_t esz = dtype_size(p.g_dtype);
+  p.vec_out = p.g_s1 == 1 && p.experts % 4 == 0 && p.g_s0 % 4 == 0 &&
+              reinterpret_cast<uintptr_t>(p.grad) % (4 * esz) == 0;
+  const int grid = warp_grid(p.rows);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p.experts <= 64) launch_route_backward<2>(p, grid, s);
+  else if (p.experts <= 128) launch_route_backward<4>(p, grid, s);
+  else if (p.experts <= 256) launch_route_backward<8>(p, grid, s);
+  else if (p.experts <= 512) launch_route_backward<16>(p, grid, s);
+  else launch_route_backward<32>(p, grid, s);
   return launched(h, "route_backward");
 }
 
@@ -268,10 +291,12 @@ extern "C" KAPYB_API kapyb_status kapyb_plan_rows(kapyb_handle h, const int32_t 
   const size_t smem = plan_smem_bytes(groups);
   CUDA_TRY(h, cudaFuncSetAttribute(plan_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    static_cast<int>(plan_smem_bytes(kPlanMaxGroups))));
-  // A warp's piece is a whole number of 32-entry steps.  One CTA takes up to four
-  // steps a warp; beyond that the work is spread over the cluster.
+  // A warp's piece is a whole number of 32-entry steps.  One CTA takes up to two steps a
+  // warp; beyond that the work is spread over the cluster.
   int ctas = 1;
-  while (ctas < kPlanMaxCtas && static_cast<long long>(n) > ctas * kPlanWarps * 128ll) ctas *= 2;
+  while (ctas < kPlanMaxCtas && static_cast<long long>(n) > ctas * kPlanWarps * 64ll) ctas *= 2;
+  if (ctas > 8)
+    CUDA_TRY(h, cudaFuncSetAttribute(plan_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3(ctas, 1, 1);
@@ -312,6 +337,8 @@ kapyb_status make_row_tmap(kapyb_handle h, CUtensorMap *map, const void *base, i
 
 bool half_type(int dtype) { return dtype == KAPYB_F16 || dtype == KAPYB_BF16; }
 
+constexpr int64_t kMaxRowPitch = 1 << 26;  // bytes between output rows on the tcgen05 paths
+
 // Two neighbouring 16-bit columns of the output may be written as one aligned word.
 bool pair_stores_ok(const void *out, int dtype, int64_t s0, int64_t group) {
   return half_type(dtype) && reinterpret_cast<uintptr_t>(out) % 4 == 0 && s0 % 2 == 0 && group % 2 == 0;
@@ -328,6 +355,41 @@ kapyb_status launch_grouped(kapyb_handle h, const CUtensorMap &tmA, const CUtens
   return launched(h, GRAD ? "grouped_grad_tcgen05" : "grouped_tcgen05");
 }
 
+// The pair kernel: `tiles` pairs of CTAs at most, as many as the device holds at once
+// (the tile loop is statically strided).
+template <int BT, int MSETS, bool GRAD>
+kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmA8,
+                          const CUtensorMap &tmA1, const PairParams &pp, long long tiles, cudaStream_t stream) {
+  using Cfg = PairCfg<BT, MSETS>;
+  auto kern = grouped_pair_kernel<BT, MSETS, GRAD>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  static std::atomic<int> resident[kMaxDevices];  // 0: not asked yet
+  int pairs = resident[h->device].load();
+  if (pairs == 0) {
+    CUDA_TRY(h, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+    cfg.gridDim = dim3(2 * (h->sm_count / 2), 1, 1);
+    if (cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg) != cudaSuccess || pairs < 1) {
+      cudaGetLastError();
+      pairs = h->sm_count / 2;
+    }
+    pairs = std::min(pairs, h->sm_count / 2);
+    resident[h->device].store(pairs);
+  }
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min<long long>(tiles, pairs)), 1, 1);
+  CUDA_TRY(h, cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmA8, tmA1, pp));
+  return launched(h, GRAD ? "grouped_grad_pair" : "grouped_pair");
+}
+
 // Rows of lhs as TMA can fetch them: 16-bit, unit stride along K, 16-byte rows.
 bool rows_tma_ok(const kapyb_tensor2d *t) {
   return half_type(t->dtype) && t->stride1 == 1 && tma_ok(elem_ptr(t), t->dtype, t->size1, t->size0, t->stride0, 1, 0);
@@ -341,6 +403,8 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
                                 bool *taken) {
   *taken = false;
   if (!rows_tma_ok(lhs) || out->stride1 != 1) return KAPYB_OK;
+  const int64_t pitch = static_cast<int64_t>(out->stride0) * dtype_size(out->dtype);
+  if (pitch >= kMaxRowPitch) return KAPYB_OK;
   const bool mn = rhs->stride1 == 1;
   if (!mn && rhs->stride0 != 1) return KAPYB_OK;
   const int64_t unit = mn ? rhs->size1 : rhs->size0, other = mn ? rhs->size0 : rhs->size1;
@@ -362,7 +426,7 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
   gp.a_mn_major = mn;
   gp.bf16 = lhs->dtype == KAPYB_BF16;
   gp.out = const_cast<void *>(elem_ptr(out));
-  gp.out_s0 = out->stride0;
+  gp.row_pitch = static_cast<uint32_t>(pitch);
   gp.out_dtype = out->dtype;
   gp.pair_stores = pair_stores_ok(gp.out, out->dtype, out->stride0, 0);
   gp.alpha = ep.alpha;
@@ -376,18 +440,24 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
   const long long busy = std::min(groups, gp.rows);
   const bool narrow = gp.rows <= 32 * busy;  // rows per group that has any, at most
   const int bt = narrow ? 64 : gated ? 128 : 256;
+  if (!narrow) gp.n_tiles = (gp.cols + 255) / 256;
   const long long tiles = ((gp.rows + bt - 1ll) / bt + busy) * gp.n_tiles;
   if (tiles >= (1ll << 31)) return KAPYB_OK;
   CUtensorMap tmA, tmB;
   TRY(make_tmap(h, &tmA, elem_ptr(rhs), rhs->dtype, unit, other, groups, ld, group_stride, 64, mn ? 64 : 128));
   TRY(make_row_tmap(h, &tmB, elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
-                    lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, order ? 1 : 32));
+                    lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, order && narrow ? 1 : 32));
   *taken = true;
-  if (gated)
-    return narrow ? launch_grouped<64, 2, false>(h, tmA, tmB, gp, tiles, stream)
-                  : launch_grouped<128, 2, false>(h, tmA, tmB, gp, tiles, stream);
-  return narrow ? launch_grouped<64, 1, false>(h, tmA, tmB, gp, tiles, stream)
-                : launch_grouped<256, 1, false>(h, tmA, tmB, gp, tiles, stream);
+  if (narrow)
+    return gated ? launch_grouped<64, 2, false>(h, tmA, tmB, gp, tiles, stream)
+                 : launch_grouped<64, 1, false>(h, tmA, tmB, gp, tiles, stream);
+  const PairParams pp{gp, order != nullptr, static_cast<const uint8_t *>(elem_ptr(lhs)), lhs->stride0 * 2ll,
+                    FastDiv::make(static_cast<uint32_t>(gp.fan))};
+  CUtensorMap tall;
+  TRY(make_row_tmap(h, &tall, elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
+                    lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, bt / 2));
+  return gated ? launch_pairs<128, 2, false>(h, tmA, tmB, tall, tmA, pp, tiles, stream)
+               : launch_pairs<256, 1, false>(h, tmA, tmB, tall, tmA, pp, tiles, stream);
 }
 
 kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const kapyb_tensor2d *grad,
@@ -396,22 +466,23 @@ kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, 
                                      cudaStream_t stream, bool *taken) {
   *taken = false;
   if (!rows_tma_ok(lhs) || !rows_tma_ok(grad) || out->stride1 != 1) return KAPYB_OK;
+  const int64_t pitch = static_cast<int64_t>(out->stride0) * dtype_size(out->dtype);
+  if (pitch >= kMaxRowPitch) return KAPYB_OK;
   GroupedParams gp{};
   gp.groups = groups;
   gp.rows = grad->size0;
   gp.cols = out->size1;
   gp.K = out->size0;
-  gp.n_tiles = (gp.cols + 127) / 128;
-  const int bt = gp.K <= 64 ? 64 : 256;
-  gp.k_tiles = (gp.K + bt - 1) / bt;
+  gp.n_tiles = (gp.cols + 255) / 256;
+  gp.k_tiles = (gp.K + 255) / 256;
   gp.offsets = offsets;
   gp.order = order;
   gp.fan = order ? fan : 1;
   gp.src_rows = lhs->size0;
   gp.bf16 = lhs->dtype == KAPYB_BF16;
   gp.out = const_cast<void *>(elem_ptr(out));
-  gp.out_s0 = out->stride0;
-  gp.out_group = out_group_stride;
+  gp.row_pitch = static_cast<uint32_t>(pitch);
+  gp.group_bytes = groups > 1 ? out_group_stride * dtype_size(out->dtype) : 0;
   gp.out_dtype = out->dtype;
   gp.pair_stores = pair_stores_ok(gp.out, out->dtype, out->stride0, groups > 1 ? out_group_stride : 0);
   gp.alpha = alpha;
@@ -421,14 +492,15 @@ kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, 
   gp.wait_limit_us = h->wait_limit_us;
   const long long tiles = static_cast<long long>(groups) * gp.n_tiles * gp.k_tiles;
   if (tiles >= (1ll << 31)) return KAPYB_OK;
-  CUtensorMap tmA, tmB;
-  TRY(make_row_tmap(h, &tmA, elem_ptr(grad), grad->dtype, grad->size1, grad->size0,
-                    grad->size0 > 1 ? grad->stride0 : (grad->size1 + 7) / 8 * 8, 1));
-  TRY(make_row_tmap(h, &tmB, elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
-                    lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, 1));
+  CUtensorMap tmA, tmA8, tmA1;
+  const uint64_t ld = grad->size0 > 1 ? grad->stride0 : (grad->size1 + 7) / 8 * 8;
+  TRY(make_row_tmap(h, &tmA, elem_ptr(grad), grad->dtype, grad->size1, grad->size0, ld, 64));
+  TRY(make_row_tmap(h, &tmA8, elem_ptr(grad), grad->dtype, grad->size1, grad->size0, ld, 8));
+  TRY(make_row_tmap(h, &tmA1, elem_ptr(grad), grad->dtype, grad->size1, grad->size0, ld, 1));
   *taken = true;
-  return bt == 64 ? launch_grouped<64, 1, true>(h, tmA, tmB, gp, tiles, stream)
-                  : launch_grouped<256, 1, true>(h, tmA, tmB, gp, tiles, stream);
+  const PairParams pp{gp, 1, static_cast<const uint8_t *>(elem_ptr(lhs)), lhs->stride0 * 2ll,
+                    FastDiv::make(static_cast<uint32_t>(gp.fan))};
+  return launch_pairs<256, 1, true>(h, tmA, tmA, tmA8, tmA1, pp, tiles, stream);
 }
 
 // What the two grouped products check alike.

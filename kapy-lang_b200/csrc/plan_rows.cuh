@@ -6,9 +6,10 @@
 //   slots[i]   = position of entry i, -1 when its index names no group
 //
 // One launch without scratch memory: a cluster of CTAs splits the entries, every
-// warp counts a contiguous piece of them in its own row of a shared-memory table
-// (match.any finds equal groups in a step, so nothing is atomic and the order is
-// that of the entries), the CTAs read one another's totals through distributed
+// warp counts a contiguous piece of them in its own row of a shared-memory table (the
+// lanes of a step that name one group find each other by a ballot per bit of the group
+// number, so nothing is atomic and the order is that of the entries; match.any does the
+// same in one instruction that takes some 240 clocks), the CTAs read one another's totals through distributed
 // shared memory, and each warp walks its piece again to place it.
 #pragma once
 
@@ -18,9 +19,10 @@
 
 namespace kapyb {
 
-constexpr int kPlanWarps = 16;
+constexpr int kPlanWarps = 32;
+constexpr int kPlanBatch = 8;  // index loads in flight per lane
 constexpr int kPlanMaxGroups = 1024;
-constexpr int kPlanMaxCtas = 8;
+constexpr int kPlanMaxCtas = 16;
 
 struct PlanParams {
   const int32_t *index;
@@ -28,9 +30,13 @@ struct PlanParams {
   int32_t *order, *offsets, *slots;
 };
 
+// Counters of one warp, an odd number of words so that a column of the table (one group,
+// all warps) is free of bank conflicts.
+__host__ __device__ inline int plan_pitch(int groups) { return groups | 1; }
+
 inline size_t plan_smem_bytes(int groups) {
   // per-warp counters, this CTA's totals, first positions
-  return static_cast<size_t>(kPlanWarps + 2) * groups * sizeof(int32_t);
+  return (static_cast<size_t>(kPlanWarps) * plan_pitch(groups) + 2 * groups) * sizeof(int32_t);
 }
 
 __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanParams p) {
@@ -39,9 +45,10 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
   extern __shared__ int32_t plan_smem[];
   __shared__ int scan_part[kPlanWarps];
   const int G = p.groups;
-  int32_t *count = plan_smem;                  // [kPlanWarps][G]
-  int32_t *total = plan_smem + kPlanWarps * G;  // [G]
-  int32_t *first = total + G;                   // [G]
+  const int pitch = plan_pitch(G);
+  int32_t *count = plan_smem;                       // [kPlanWarps][pitch]
+  int32_t *total = plan_smem + kPlanWarps * pitch;  // [G]
+  int32_t *first = total + G;                       // [G]
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int ctas = static_cast<int>(cluster.num_blocks()), me = static_cast<int>(cluster.block_rank());
   const int pieces = ctas * kPlanWarps;
@@ -49,27 +56,54 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
   const long long lo = min(static_cast<long long>(p.n), (me * kPlanWarps + w) * step);
   const long long hi = min(static_cast<long long>(p.n), lo + step);
 
-  for (int i = threadIdx.x; i < kPlanWarps * G; i += blockDim.x) count[i] = 0;
+  for (int i = threadIdx.x; i < kPlanWarps * pitch; i += blockDim.x) count[i] = 0;
   __syncthreads();
-  int32_t *mine = count + w * G;
-  for (long long i0 = lo; i0 < hi; i0 += 32) {
-    const long long i = i0 + lane;
-    int g = i < hi ? p.index[i] : -1;
-    if (g < 0 || g >= G) g = -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, g);
+  int32_t *mine = count + w * pitch;
+  // walks this warp's piece, kPlanBatch steps of 32 entries at a time so that their loads
+  // overlap; step(i, g): entry i of group g (-1: none)
+  auto walk = [&](auto &&step) {
+    for (long long i0 = lo; i0 < hi; i0 += 32 * kPlanBatch) {
+      int g[kPlanBatch];
+#pragma unroll
+      for (int u = 0; u < kPlanBatch; ++u) {
+        const long long i = i0 + 32 * u + lane;
+        g[u] = i < hi ? __ldg(p.index + i) : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < kPlanBatch; ++u)
+        if (i0 + 32 * u < hi) step(i0 + 32 * u + lane, g[u] < 0 || g[u] >= G ? -1 : g[u]);
+    }
+  };
+  const int bits = 32 - __clz(G);  // of 0 .. G, G standing for "no group"
+  auto lanes_like = [&](int g) {
+    const uint32_t code = g < 0 ? G : g;
+    uint32_t same = 0xffffffffu;
+    for (int b = 0; b < bits; ++b) {
+      const bool one = (code >> b) & 1u;
+      const uint32_t ones = __ballot_sync(0xffffffffu, one);
+      same &= one ? ones : ~ones;
+    }
+    return same;
+  };
+  walk([&](long long, int g) {
+    const uint32_t same = lanes_like(g);
     if (g >= 0 && lane == __ffs(same) - 1) mine[g] += __popc(same);
     __syncwarp();
-  }
+  });
   __syncthreads();
-  for (int g = threadIdx.x; g < G; g += blockDim.x) {
-    int run = 0;
+  // a group's counters over the CTA's warps -> their exclusive sums: one warp per group,
+  // lane k holding warp k's
+  static_assert(kPlanWarps == 32, "one lane per warp");
+  for (int g = w; g < G; g += kPlanWarps) {
+    const int c = count[lane * pitch + g];
+    int run = c;
 #pragma unroll
-    for (int k = 0; k < kPlanWarps; ++k) {
-      const int c = count[k * G + g];
-      count[k * G + g] = run;
-      run += c;
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, run, off);
+      if (lane >= off) run += o;
     }
-    total[g] = run;
+    count[lane * pitch + g] = run - c;
+    if (lane == 31) total[g] = run;
   }
   cluster.sync();
   // first position of every group: exclusive scan over the groups of the cluster's
@@ -109,11 +143,8 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
   if (me == 0 && threadIdx.x == 0) p.offsets[G] = planned;
   // the others' totals have been read: nobody leaves while they still may be
   cluster.sync();
-  for (long long i0 = lo; i0 < hi; i0 += 32) {
-    const long long i = i0 + lane;
-    int g = i < hi ? p.index[i] : -1;
-    if (g < 0 || g >= G) g = -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, g);
+  walk([&](long long i, int g) {
+    const uint32_t same = lanes_like(g);
     int pos = -1;
     if (g >= 0) pos = first[g] + mine[g] + __popc(same & ((1u << lane) - 1u));
     __syncwarp();
@@ -123,7 +154,7 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
       if (pos >= 0) p.order[pos] = static_cast<int32_t>(i);
       if (p.slots) p.slots[i] = pos;
     }
-  }
+  });
   for (long long q = planned + static_cast<long long>(me) * blockDim.x + threadIdx.x; q < p.n;
        q += static_cast<long long>(ctas) * blockDim.x)
     p.order[q] = -1;

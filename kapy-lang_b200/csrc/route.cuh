@@ -4,18 +4,25 @@
 //   s = softmax(x) or sigmoid(x)        c = s + bias   (c only decides who is chosen)
 //   w_j = scale * s_j [/ sum of the chosen s]
 //
-// One warp owns one row and keeps it in registers (expert e sits in lane e % 32),
-// so the row is read once and nothing but k weights and k indices leaves the warp.
-// A pick is two warp-wide integer reductions (redux.sync): the largest key, then
-// the lowest index that has it, which is the rule for ties.
+// One warp owns one row and keeps it in registers, every lane a run of VPT adjacent
+// experts (one vector load), so the row is read once and only k weights and k indices
+// leave the warp.  A lane ranks its own two best; a pick is one redux.sync over the
+// lanes' best, and the lowest lane that has it wins, which is the rule for ties.  A lane
+// whose two best are gone looks for its next two (about one row in two, once).
 //
-// Keys.  A choice between experts must not depend on how an exponential was
-// rounded.  Without a bias the order of the scores is the order of the logits, so
-// the logits themselves are the keys, which is exact.  With a bias (or with groups
-// ranked by a sum of two scores) c is formed in 32 bits together with a bound on
-// its error, and a row in which two neighbours of the ranking lie within that bound
-// of one another is decided again in 64 bits (choose_f64).  On normally
-// distributed logits that is about one row in a thousand.
+// Keys.  A choice between experts must not depend on how an exponential was rounded.
+// Without a bias the order of the scores is the order of the logits, so the logits
+// themselves are the keys, which is exact.  With a bias (or with groups ranked by a sum
+// of two scores) c is formed in 32 bits with a bound on its error, and a row in which
+// two neighbours of the ranking lie within that bound of one another is decided again
+// in 64 bits (choose_f64), about one row in a thousand on normally distributed logits.
+// The bound for a sigmoid: with e = ex2.approx of a rounded product the relative error
+// of e is (|x| + 4) 2^-24, so s = 1 / (1 + e) is off by s (1 - s) (|x| + 4) 2^-24 for e
+// and 4 s 2^-24 for the sum and the reciprocal, below 6 2^-24 in all; 16 2^-24 is used.
+// For a softmax: s = e / z, e off by (d + 4) 2^-24 relative, d = max - x; z by the mean of
+// that over the row, at most ln(1024) + 4, and 37 roundings of its sum; s is at most 1 / z
+// and (d + 4) exp(-d) at most 4, so 64 2^-24 / z covers it.  The sum with the bias adds one
+// rounding of c.
 #pragma once
 
 #include "common.cuh"
@@ -42,6 +49,7 @@ struct RouteParams {
   void *grad;
   long long g_s0, g_s1;
   int g_dtype;
+  int vec_out;  // grad: unit stride, four experts at a time on aligned addresses
 };
 
 // Ranks as unsigned integers: 0 = masked (never chosen), 1 = NaN (behind every
@@ -89,6 +97,66 @@ __device__ __forceinline__ float route_logit(const RouteParams &p, long long row
   return load_as_f32(p.x, p.x_dtype, row * p.x_s0 + e * p.x_s1);
 }
 
+// A lane's VPT experts lane * VPT ..; experts that do not exist read as masked.  VEC: the
+// row has unit stride, VPT * element size alignment and a multiple of VPT experts.
+template <int VPT, bool VEC>
+__device__ __forceinline__ void load_row(const RouteParams &p, long long row, int lane, float (&x)[VPT]) {
+  const int e0 = lane * VPT;
+  if constexpr (VEC) {
+    if (e0 >= p.experts) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) x[i] = -INFINITY;
+      return;
+    }
+    if (p.x_dtype == KAPYB_F32) {
+      const float *src = static_cast<const float *>(p.x) + row * p.x_s0 + e0;
+      if constexpr (VPT == 2) {
+        const float2 v = __ldg(reinterpret_cast<const float2 *>(src));
+        x[0] = v.x;
+        x[1] = v.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPT / 4; ++i) {
+          const float4 v = __ldg(reinterpret_cast<const float4 *>(src) + i);
+          x[4 * i] = v.x;
+          x[4 * i + 1] = v.y;
+          x[4 * i + 2] = v.z;
+          x[4 * i + 3] = v.w;
+        }
+      }
+    } else {
+      const uint16_t *src = static_cast<const uint16_t *>(p.x) + row * p.x_s0 + e0;
+      uint32_t w[VPT / 2];
+      if constexpr (VPT == 2) {
+        w[0] = __ldg(reinterpret_cast<const uint32_t *>(src));
+      } else if constexpr (VPT == 4) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(src));
+        w[0] = v.x;
+        w[1] = v.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPT / 8; ++i) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src) + i);
+          w[4 * i] = v.x;
+          w[4 * i + 1] = v.y;
+          w[4 * i + 2] = v.z;
+          w[4 * i + 3] = v.w;
+        }
+      }
+      if (p.x_dtype == KAPYB_BF16) {
+#pragma unroll
+        for (int i = 0; i < VPT / 2; ++i) unpack2_16<KAPYB_BF16>(w[i], x[2 * i], x[2 * i + 1]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPT / 2; ++i) unpack2_16<KAPYB_F16>(w[i], x[2 * i], x[2 * i + 1]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) x[i] = e0 + i < p.experts ? route_logit(p, row, e0 + i) : -INFINITY;
+  }
+}
+
 // The kept groups of a row as a bit mask, from the lanes' group keys (lane q holds
 // group q; 0 = the group has nothing to choose from).
 template <class Key>
@@ -108,48 +176,51 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteParams &p, Key key, i
   return kept;
 }
 
-// One row's choice with every score in 64 bits: lane j < top_k returns the j-th
-// choice, or -1.  Walks the row again per step instead of keeping it: rare.
+// One row's choice with every score in 64 bits: lane j < top_k returns the j-th choice, or
+// -1.  Every score is formed once, a lane's in parallel.
+template <int VPT>
 __device__ __noinline__ int choose_f64(const RouteParams &p, long long row) {
   const int lane = threadIdx.x & 31;
-  double top = -INFINITY, z = 1.0;
-  if (!p.sigmoid) {
-    float m = -INFINITY;
-    for (int e = lane; e < p.experts; e += 32) m = fmaxf(m, route_logit(p, row, e));
-    top = warp_max(m);
-    double s = 0.0;
-    for (int e = lane; e < p.experts; e += 32) {
-      const float x = route_logit(p, row, e);
-      if (x != -INFINITY) s += exp(static_cast<double>(x) - top);
+  const int e0 = lane * VPT;
+  unsigned long long key[VPT];  // rank of expert e0 + i, 0 when it is masked
+  {
+    double top = 0.0, z = 1.0;
+    if (!p.sigmoid) {
+      float m = -INFINITY;
+      for (int i = 0; i < VPT; ++i)
+        if (e0 + i < p.experts) m = fmaxf(m, route_logit(p, row, e0 + i));
+      top = warp_max(m);
+      double s = 0.0;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const float x = e0 + i < p.experts ? route_logit(p, row, e0 + i) : -INFINITY;
+        if (x != -INFINITY) s += exp(static_cast<double>(x) - top);
+      }
+      z = warp_sum64(s);
     }
-    z = warp_sum64(s);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const float x = e0 + i < p.experts ? route_logit(p, row, e0 + i) : -INFINITY;
+      const double xd = x;
+      double c = p.sigmoid ? 1.0 / (1.0 + exp(-xd)) : exp(xd - top) / z;
+      if (p.bias && e0 + i < p.experts) c += static_cast<double>(p.bias[e0 + i]);
+      key[i] = x == -INFINITY ? 0ull : rank_key64(c);
+    }
   }
-  // rank of expert e, 0 when it is masked
-  auto key_of = [&](int e) -> unsigned long long {
-    const float x = route_logit(p, row, e);
-    if (x == -INFINITY) return 0ull;
-    const double xd = x;
-    double c = p.sigmoid ? 1.0 / (1.0 + exp(-xd)) : exp(xd - top) / z;
-    if (p.bias) c += static_cast<double>(p.bias[e]);
-    return rank_key64(c);
+  auto value_of = [](unsigned long long k) -> double {
+    if (k == 1ull) return __longlong_as_double(0x7fffffffffffffffll);
+    return __longlong_as_double(static_cast<long long>(k >> 63 ? (k & 0x7fffffffffffffffull) : ~k));
   };
-  auto value_of = [&](unsigned long long key) -> double {
-    if (key == 1ull) return __longlong_as_double(0x7fffffffffffffffll);
-    return __longlong_as_double(static_cast<long long>(key >> 63 ? (key & 0x7fffffffffffffffull) : ~key));
-  };
-  uint32_t kept = 0xffffffffu;
   if (p.n_groups > 1) {
     unsigned long long mine = 0ull;
     for (int q = 0; q < p.n_groups; ++q) {
-      unsigned long long k1 = 0ull, k2 = 0ull;  // this lane's two best
-      for (int e = q * p.group_size + lane; e < (q + 1) * p.group_size; e += 32) {
-        const unsigned long long k = key_of(e);
-        if (k > k1) {
-          k2 = k1;
-          k1 = k;
-        } else if (k > k2) {
-          k2 = k;
-        }
+      const int lo = q * p.group_size, hi = lo + p.group_size;
+      unsigned long long k1 = 0ull, k2 = 0ull;  // this lane's two best of the group
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const unsigned long long k = e0 + i >= lo && e0 + i < hi ? key[i] : 0ull;
+        k2 = k > k1 ? k1 : k > k2 ? k : k2;
+        k1 = k > k1 ? k : k1;
       }
       const unsigned long long g1 = warp_max64(k1);
       unsigned long long gk = g1;
@@ -160,201 +231,230 @@ __device__ __noinline__ int choose_f64(const RouteParams &p, long long row) {
       }
       if (lane == q) mine = gk;
     }
-    kept = keep_groups(p, mine, lane);
+    const uint32_t kept = keep_groups(p, mine, lane);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (e0 + i < p.experts && !((kept >> ((e0 + i) / p.group_size)) & 1u)) key[i] = 0ull;
   }
   int pick = -1;
-  unsigned long long last = ~0ull;  // the previous choice's rank and index: the next one is behind it
-  int last_e = -1;
   for (int j = 0; j < p.top_k; ++j) {
     unsigned long long best = 0ull;
-    int best_e = 0x7fffffff;
-    for (int e = lane; e < p.experts; e += 32) {
-      if (p.n_groups > 1 && !((kept >> (e / p.group_size)) & 1u)) continue;
-      const unsigned long long k = key_of(e);
-      if (k == 0ull || k > last || (k == last && e <= last_e)) continue;
-      if (k > best) {
-        best = k;
-        best_e = e;
+    int at = -1;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        at = i;
       }
+    const unsigned long long g = warp_max64(best);
+    if (g == 0ull) break;
+    const int w = __ffs(__ballot_sync(0xffffffffu, best == g)) - 1;
+    const int i_w = __shfl_sync(0xffffffffu, at, w);
+    if (lane == j) pick = w * VPT + i_w;
+    if (lane == w) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        if (i == at) key[i] = 0ull;
     }
-    const unsigned long long top_key = warp_max64(best);
-    if (top_key == 0ull) break;
-    const int e = static_cast<int>(
-        __reduce_min_sync(0xffffffffu, best == top_key ? static_cast<uint32_t>(best_e) : 0x7fffffffu));
-    if (lane == j) pick = e;
-    last = top_key;
-    last_e = e;
   }
   return pick;
 }
 
-// exp(x - shift) and the like for the weights: full-precision expf and division,
-// f32 throughout.
-// VPT experts per lane.
+// A lane's two best of what is behind (bound, index) in the ranking.
+struct LaneBest {
+  uint32_t k1, k2;
+  int i1, i2;
+};
 template <int VPT>
+__device__ __forceinline__ LaneBest two_best(const uint32_t (&key)[VPT], uint32_t bound, int behind) {
+  LaneBest b{0u, 0u, 0, 0};
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const uint32_t k = key[i] < bound || (key[i] == bound && i > behind) ? key[i] : 0u;
+    const bool first = k > b.k1, second = k > b.k2;
+    b.k2 = first ? b.k1 : second ? k : b.k2;
+    b.i2 = first ? b.i1 : second ? i : b.i2;
+    b.k1 = first ? k : b.k1;
+    b.i1 = first ? i : b.i1;
+  }
+  return b;
+}
+
+// Weights from full-precision expf and division, f32 throughout.  SCORED: experts (or
+// groups) are ranked by their scores, not by their logits.
+template <int VPT, bool SCORED, bool VEC>
 __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
   const int lane = threadIdx.x & 31;
-  const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
-  for (long long row = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-       row < p.rows; row += warps) {
+  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const int e0 = lane * VPT;
+  uint32_t key[VPT];
+  float top = 0.0f, z = 1.0f, err = 0.0f;
+  bool bad;  // a NaN or +inf among the logits: softmax weights are NaN
+  {
     float x[VPT];
+    load_row<VPT, VEC>(p, row, lane, x);
+    bool off = false;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int e = i * 32 + lane;
-      x[i] = e < p.experts ? route_logit(p, row, e) : -INFINITY;
-    }
-    float top = 0.0f, z = 1.0f;
-    const bool by_score = p.bias != nullptr || (p.n_groups > 1 && p.group_best > 1);
-    if (!p.sigmoid) {
+    for (int i = 0; i < VPT; ++i) off |= !(x[i] < INFINITY);
+    bad = __any_sync(0xffffffffu, off);
+    if (!p.sigmoid && (SCORED || !p.renormalize)) {
       float m = x[0];
 #pragma unroll
       for (int i = 1; i < VPT; ++i) m = fmaxf(m, x[i]);
       top = warp_max(m);
       float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) s += x[i] == -INFINITY ? 0.0f : expf(x[i] - top);
+      for (int i = 0; i < VPT; ++i) s += x[i] == -INFINITY ? 0.0f : kapy_exp(x[i] - top);
       z = warp_sum(s);
     }
-    // c and the bound on its error, from the 32-bit evaluation: a few roundings of
-    // s (relative), the rounding of the exponent's argument (|x - top| 2^-24,
-    // absolute in the exponent, so relative in s), one rounding of the sum with the bias
-    auto score_of = [&](float xv, int e) -> float {
-      float s = p.sigmoid ? 1.0f / (1.0f + expf(-xv)) : expf(xv - top) / z;
-      return p.bias != nullptr ? s + p.bias[e] : s;
-    };
-    auto error_of = [&](float xv, float c) -> float {
-      const float s = p.sigmoid ? 1.0f / (1.0f + expf(-xv)) : expf(xv - top) / z;
-      const float rel = p.sigmoid ? 16.0f : 24.0f + fabsf(xv - top);
-      return s * rel * 5.9604645e-8f + fabsf(c) * 1.1920929e-7f + 1e-37f;
-    };
-    uint32_t key[VPT];
+    if constexpr (SCORED) {
+      err = (p.sigmoid ? 16.0f : 64.0f / z) * 5.9604645e-8f + 1e-37f;
+      const float rz = 1.0f / z;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int e = i * 32 + lane;
-      key[i] = x[i] == -INFINITY ? 0u : rank_key(by_score ? score_of(x[i], e) : x[i]);
+      for (int i = 0; i < VPT; ++i) {
+        const float s = p.sigmoid ? __fdividef(1.0f, 1.0f + kapy_exp(-x[i])) : kapy_exp(x[i] - top) * rz;
+        const float c = p.bias != nullptr && e0 + i < p.experts ? s + __ldg(p.bias + e0 + i) : s;
+        key[i] = x[i] == -INFINITY ? 0u : rank_key(c);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) key[i] = x[i] == -INFINITY ? 0u : rank_key(x[i]);
     }
-    bool unsure = false;
-    if (p.n_groups > 1) {
-      uint32_t mine = 0u;
-      float err = 0.0f;
+  }
+  bool unsure = false;
+  LaneBest b = two_best<VPT>(key, 0xffffffffu, VPT);
+  if (p.n_groups > 1) {
+    uint32_t mine = 0u;
+    float slack = 0.0f;  // error of this lane's group
+    auto sum_key = [&](uint32_t g1, uint32_t g2, uint32_t &gk, float &ge) {
+      gk = g1;
+      ge = 0.0f;
+      if (SCORED && g1 != 0u) {
+        ge = err + fabsf(key_value(g1)) * 1.1920929e-7f;
+        if (p.group_best == 2 && g2 != 0u) {
+          const float sum = key_value(g1) + key_value(g2);
+          ge += err + (fabsf(key_value(g2)) + fabsf(sum)) * 1.1920929e-7f;
+          gk = rank_key(sum);
+        }
+      }
+    };
+    const int lanes = p.group_size / VPT;  // lanes per group, when groups are whole lanes
+    if (lanes * VPT == p.group_size && (lanes & (lanes - 1)) == 0 && lanes <= 32) {
+      // every lane's two best belong to one group: join them over its lanes
+      uint32_t k1 = b.k1, k2 = b.k2;
+      for (int off = 1; off < lanes; off <<= 1) {
+        const uint32_t o1 = __shfl_xor_sync(0xffffffffu, k1, off), o2 = __shfl_xor_sync(0xffffffffu, k2, off);
+        k2 = max(min(k1, o1), max(k2, o2));
+        k1 = max(k1, o1);
+      }
+      uint32_t gk;
+      float ge;
+      sum_key(k1, k2, gk, ge);
+      const int from = lane * lanes;  // a lane of group `lane`
+      mine = __shfl_sync(0xffffffffu, gk, from & 31);
+      slack = __shfl_sync(0xffffffffu, ge, from & 31);
+      if (lane >= p.n_groups) {
+        mine = 0u;
+        slack = 0.0f;
+      }
+    } else {
       for (int q = 0; q < p.n_groups; ++q) {
-        const int lo = q * p.group_size, hi = lo + p.group_size;
+        const int lo = q * p.group_size - e0, hi = lo + p.group_size;
         uint32_t k1 = 0u, k2 = 0u;
-        float e1 = 0.0f, e2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-          const int e = i * 32 + lane;
-          const uint32_t k = e >= lo && e < hi ? key[i] : 0u;
-          const float er = by_score ? error_of(x[i], key_value(k)) : 0.0f;
-          if (k > k1) {
-            k2 = k1;
-            e2 = e1;
-            k1 = k;
-            e1 = er;
-          } else if (k > k2) {
-            k2 = k;
-            e2 = er;
-          }
+          const uint32_t k = i >= lo && i < hi ? key[i] : 0u;
+          k2 = k > k1 ? k1 : max(k2, k);
+          k1 = max(k1, k);
         }
         const uint32_t g1 = __reduce_max_sync(0xffffffffu, k1);
-        uint32_t gk = g1;
-        float ge = 0.0f;
-        if (g1 != 0u) {
-          const int owner = __ffs(__ballot_sync(0xffffffffu, k1 == g1)) - 1;
-          ge = __shfl_sync(0xffffffffu, e1, owner);
-          if (p.group_best == 2) {
-            const uint32_t r1 = lane == owner ? k2 : k1;
-            const float re = lane == owner ? e2 : e1;
-            const uint32_t g2 = __reduce_max_sync(0xffffffffu, r1);
-            if (g2 != 0u) {
-              const int owner2 = __ffs(__ballot_sync(0xffffffffu, r1 == g2)) - 1;
-              const float sum = key_value(g1) + key_value(g2);
-              ge += __shfl_sync(0xffffffffu, re, owner2) + fabsf(sum) * 1.1920929e-7f;
-              gk = rank_key(sum);
-            }
-          }
-        }
+        const uint32_t owners = __ballot_sync(0xffffffffu, k1 == g1);
+        const uint32_t g2 = __reduce_max_sync(0xffffffffu, lane == __ffs(owners) - 1 ? k2 : k1);
+        uint32_t gk;
+        float ge;
+        sum_key(g1, g2, gk, ge);
         if (lane == q) {
           mine = gk;
-          err = ge;
+          slack = ge;
         }
-      }
-      const uint32_t kept = keep_groups(p, mine, lane);
-      if (by_score && p.top_groups < p.n_groups) {
-        // the weakest kept group against the strongest one left out
-        const bool in = (kept >> lane) & 1u;
-        const uint32_t low = __reduce_min_sync(0xffffffffu, in ? mine : 0xffffffffu);
-        const uint32_t high = __reduce_max_sync(0xffffffffu, in ? 0u : mine);
-        if (kept != 0u && high != 0u) {
-          const float e_max = warp_max(err);
-          unsure = !(key_value(low) - key_value(high) > 2.0f * e_max);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int e = i * 32 + lane;
-        if (e < p.experts && !((kept >> (e / p.group_size)) & 1u)) key[i] = 0u;
       }
     }
-    int pick = -1;
-    float prev = 0.0f, prev_err = 0.0f;
-    // with scores as keys one more rank is looked at: the best expert left out
-    const int steps = by_score ? p.top_k + 1 : p.top_k;
-    for (int j = 0; j < steps && !unsure; ++j) {
-      uint32_t best = key[0];
-#pragma unroll
-      for (int i = 1; i < VPT; ++i) best = key[i] > best ? key[i] : best;
-      const uint32_t g = __reduce_max_sync(0xffffffffu, best);
-      if (g == 0u) break;
-      uint32_t at = 0x7fffffffu;
-      float er = 0.0f;
-#pragma unroll
-      for (int i = VPT - 1; i >= 0; --i)
-        if (key[i] == g) at = static_cast<uint32_t>(i * 32 + lane);
-      const int e = static_cast<int>(__reduce_min_sync(0xffffffffu, at));
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        if (i * 32 + lane == e) {
-          if (by_score) er = error_of(x[i], key_value(g));
-          key[i] = 0u;
-        }
-      }
-      if (by_score) {
-        er = __shfl_sync(0xffffffffu, er, e & 31);
-        const float c = key_value(g);
-        if (j > 0 && !(prev - c > prev_err + er)) unsure = true;
-        prev = c;
-        prev_err = er;
-      }
-      if (lane == j && j < p.top_k) pick = e;
+    const uint32_t kept = keep_groups(p, mine, lane);
+    if (SCORED && p.top_groups < p.n_groups) {
+      // the weakest kept group against the strongest one left out
+      const bool in = (kept >> lane) & 1u;
+      const uint32_t low = __reduce_min_sync(0xffffffffu, in ? mine : 0xffffffffu);
+      const uint32_t high = __reduce_max_sync(0xffffffffu, in ? 0u : mine);
+      if (kept != 0u && high != 0u) unsure = !(key_value(low) - key_value(high) > 2.0f * warp_max(slack));
     }
-    if (unsure) pick = choose_f64(p, row);
-
-    // weights of the choices, lane j the j-th
-    const bool on = lane < p.top_k && pick >= 0;
-    const float xv = on ? route_logit(p, row, pick) : -INFINITY;
-    float w = 0.0f;
-    if (p.renormalize) {
-      // only ratios matter, so both scores are divided by e^shift, which keeps the
-      // sum away from zero: softmax  exp(x - shift), sigmoid exp(x - shift) / (1 + exp(x))
-      const float big = warp_max(xv);
-      float r;
-      if (p.sigmoid) {
-        const float shift = fminf(big, 0.0f);
-        r = xv > 0.0f ? 1.0f / (1.0f + expf(-xv)) : expf(xv - shift) / (1.0f + expf(xv));
-        if (xv != xv) r = xv;
+    int q = e0 / p.group_size, next = (q + 1) * p.group_size - e0;  // group of expert e0 + i
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      while (i >= next) {
+        ++q;
+        next += p.group_size;
+      }
+      if (q < 32 && !((kept >> q) & 1u)) key[i] = 0u;
+    }
+    b = two_best<VPT>(key, 0xffffffffu, VPT);
+  }
+  int pick = -1;
+  float prev = 0.0f;
+  bool spent = false;  // this lane's second best is its candidate already
+  // with scores as keys one more rank is looked at: the best expert left out
+  const int steps = SCORED ? p.top_k + 1 : p.top_k;
+  for (int j = 0; j < steps && !unsure; ++j) {
+    const uint32_t g = __reduce_max_sync(0xffffffffu, b.k1);
+    if (g == 0u) break;
+    const int w = __ffs(__ballot_sync(0xffffffffu, b.k1 == g)) - 1;
+    const int i_w = __shfl_sync(0xffffffffu, b.i1, w);
+    if constexpr (SCORED) {
+      const float c = key_value(g);
+      if (j > 0 && !(prev - c > 2.0f * err + (fabsf(prev) + fabsf(c)) * 1.1920929e-7f)) unsure = true;
+      prev = c;
+    }
+    if (lane == j && j < p.top_k) pick = w * VPT + i_w;
+    if (lane == w) {
+      if (spent) {
+        b = two_best<VPT>(key, g, i_w);
+        spent = false;
       } else {
-        r = expf(xv - big) + (z - z);  // a row whose scores are NaN has NaN weights
+        b.k1 = b.k2;
+        b.i1 = b.i2;
+        spent = true;
       }
-      if (!on) r = 0.0f;
-      w = r / warp_sum(r);
+    }
+    __syncwarp();
+  }
+  if constexpr (SCORED) {
+    if (unsure) pick = choose_f64<VPT>(p, row);
+  }
+
+  // weights of the choices, lane j the j-th
+  const bool on = lane < p.top_k && pick >= 0;
+  const float xv = on ? route_logit(p, row, pick) : -INFINITY;
+  float w = 0.0f;
+  if (p.renormalize) {
+    // only ratios matter, so both scores are divided by e^shift, which keeps the sum away
+    // from zero: softmax  exp(x - shift), sigmoid  exp(x - shift) / (1 + exp(x))
+    const float big = warp_max(xv);
+    float r;
+    if (p.sigmoid) {
+      const float shift = fminf(big, 0.0f);
+      r = xv > 0.0f ? 1.0f / (1.0f + expf(-xv)) : expf(xv - shift) / (1.0f + expf(xv));
+      if (xv != xv) r = xv;
     } else {
-      w = p.sigmoid ? 1.0f / (1.0f + expf(-xv)) : expf(xv - top) / z;
+      r = bad ? __uint_as_float(0x7fffffffu) : expf(xv - big);
     }
-    if (lane < p.top_k) {
-      p.weights[row * p.top_k + lane] = on ? w * p.scale : 0.0f;
-      p.chosen[row * p.top_k + lane] = pick;
-    }
+    if (!on) r = 0.0f;
+    w = r / warp_sum(r);
+  } else {
+    w = p.sigmoid ? 1.0f / (1.0f + expf(-xv)) : expf(xv - top) / z;
+  }
+  if (lane < p.top_k) {
+    p.weights[row * p.top_k + lane] = on ? w * p.scale : 0.0f;
+    p.chosen[row * p.top_k + lane] = pick;
   }
 }
 
@@ -365,92 +465,110 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
 //   plain sigmoid          dx_j = scale g_j s_j (1 - s_j)              others 0
 //   plain softmax          dx_e = s_e (scale g_e [e chosen] - scale sum_j g_j s_j)
 // (the softmax's own normaliser cancels in the renormalised form), so only the last
-// one reads whole rows; the others read k logits a row and write the row once.
-// A choice that names an expert twice counts twice; one outside 0..experts-1 not at
-// all.  The sums run in lane order of a fixed tree: the same bits every time.
-template <int VPT>
+// one reads whole rows; the others read k logits a row and write the row once, put
+// together in shared memory.  A choice that names an expert twice counts twice: its
+// terms are summed in the order of the choices by the lane of its first mention.  One
+// outside 0..experts-1 does not count.  No atomics: the same bits every time.
+template <int VPT, bool VEC>
 __global__ void __launch_bounds__(256) route_backward_kernel(const RouteParams p) {
+  __shared__ __align__(16) float rows_mem[8][VPT * 32];
   const int lane = threadIdx.x & 31;
-  const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
-  for (long long row = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-       row < p.rows; row += warps) {
-    int e = -1;
-    float g = 0.0f;
-    if (lane < p.top_k) {
-      e = p.picked[row * p.top_k + lane];
-      g = p.grad_weights[row * p.top_k + lane];
-    }
-    float xv = -INFINITY;
-    if (e >= 0 && e < p.experts) xv = route_logit(p, row, e);
-    if (xv == -INFINITY) {  // masked, or no expert: no part in anything
-      e = -1;
-      g = 0.0f;
-    }
-    float x[VPT];
-    float top = 0.0f, z = 1.0f;
-    const bool dense = !p.sigmoid && !p.renormalize;
-    if (dense) {
+  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  float *mem = rows_mem[threadIdx.x >> 5];
+  int e = -1;
+  float g = 0.0f;
+  if (lane < p.top_k) {
+    e = p.picked[row * p.top_k + lane];
+    g = p.grad_weights[row * p.top_k + lane];
+  }
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int c = i * 32 + lane;
-        x[i] = c < p.experts ? route_logit(p, row, c) : -INFINITY;
-      }
-      float m = x[0];
+  for (int i = 0; i < VPT; ++i) mem[i * 32 + lane] = 0.0f;
+  float xv = -INFINITY;
+  if (e >= 0 && e < p.experts) xv = route_logit(p, row, e);
+  if (xv == -INFINITY) {  // masked, or no expert: no part in anything
+    e = -1;
+    g = 0.0f;
+  }
+  float x[VPT];
+  float top = 0.0f, z = 1.0f;
+  const bool dense = !p.sigmoid && !p.renormalize;
+  if (dense) {
+    load_row<VPT, VEC>(p, row, lane, x);
+    float m = x[0];
 #pragma unroll
-      for (int i = 1; i < VPT; ++i) m = fmaxf(m, x[i]);
-      top = warp_max(m);
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        x[i] = x[i] == -INFINITY ? 0.0f : expf(x[i] - top);
-        s += x[i];
-      }
-      z = warp_sum(s);
-    }
-    float d = 0.0f;      // what lane j adds to the gradient of its expert
-    float common = 0.0f;  // dense: subtracted from every expert's
-    if (p.renormalize) {
-      const float big = warp_max(xv);
-      float r, one_minus = 1.0f;
-      if (p.sigmoid) {
-        const float shift = fminf(big, 0.0f);
-        r = xv > 0.0f ? 1.0f / (1.0f + expf(-xv)) : expf(xv - shift) / (1.0f + expf(xv));
-        if (xv != xv) r = xv;
-        one_minus = 1.0f / (1.0f + expf(xv));
-      } else {
-        r = expf(xv - big);
-      }
-      if (e < 0) r = 0.0f;
-      const float total = warp_sum(r);
-      if (e >= 0) r /= total;
-      const float mean = warp_sum(g * r);
-      if (e >= 0) d = p.scale * r * one_minus * (g - mean);
-    } else if (p.sigmoid) {
-      if (e >= 0) d = p.scale * g / (1.0f + expf(-xv)) / (1.0f + expf(xv));
-    } else {
-      const float s = e >= 0 ? expf(xv - top) / z : 0.0f;
-      common = p.scale * warp_sum(g * s);
-      d = p.scale * g;
-    }
-    float out[VPT];
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) out[i] = 0.0f;
-    for (int j = 0; j < p.top_k; ++j) {
-      const int ej = __shfl_sync(0xffffffffu, e, j);
-      const float dj = __shfl_sync(0xffffffffu, d, j);
-#pragma unroll
-      for (int i = 0; i < VPT; ++i)
-        if (ej == i * 32 + lane) out[i] += dj;
-    }
-    if (dense) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) out[i] = x[i] == 0.0f ? 0.0f : x[i] / z * (out[i] - common);
-    }
+    for (int i = 1; i < VPT; ++i) m = fmaxf(m, x[i]);
+    top = warp_max(m);
+    float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = i * 32 + lane;
-      if (c < p.experts) store_from_f32(p.grad, p.g_dtype, row * p.g_s0 + c * p.g_s1, out[i], 1);
+      x[i] = x[i] == -INFINITY ? 0.0f : expf(x[i] - top);
+      s += x[i];
     }
+    z = warp_sum(s);
+  }
+  float d = 0.0f;       // what lane j adds to the gradient of its expert
+  float common = 0.0f;  // dense: subtracted from every expert's
+  if (p.renormalize) {
+    const float big = warp_max(xv);
+    float r, one_minus = 1.0f;
+    if (p.sigmoid) {
+      const float shift = fminf(big, 0.0f);
+      r = xv > 0.0f ? 1.0f / (1.0f + expf(-xv)) : expf(xv - shift) / (1.0f + expf(xv));
+      if (xv != xv) r = xv;
+      one_minus = 1.0f / (1.0f + expf(xv));
+    } else {
+      r = expf(xv - big);
+    }
+    if (e < 0) r = 0.0f;
+    const float total = warp_sum(r);
+    if (e >= 0) r /= total;
+    const float mean = warp_sum(g * r);
+    if (e >= 0) d = p.scale * r * one_minus * (g - mean);
+  } else if (p.sigmoid) {
+    if (e >= 0) d = p.scale * g / (1.0f + expf(-xv)) / (1.0f + expf(xv));
+  } else {
+    const float s = e >= 0 ? expf(xv - top) / z : 0.0f;
+    common = p.scale * warp_sum(g * s);
+    d = p.scale * g;
+  }
+  float total_d = 0.0f;
+  bool first = e >= 0;
+  for (int j = 0; j < p.top_k; ++j) {
+    const int ej = __shfl_sync(0xffffffffu, e, j);
+    const float dj = __shfl_sync(0xffffffffu, d, j);
+    if (ej == e) {
+      total_d += dj;
+      if (j < lane) first = false;
+    }
+  }
+  __syncwarp();
+  if (first) mem[e] = total_d;
+  __syncwarp();
+  if (dense) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      mem[lane * VPT + i] = x[i] == 0.0f ? 0.0f : x[i] / z * (mem[lane * VPT + i] - common);
+    __syncwarp();
+  }
+  if (p.vec_out) {
+    // four experts per lane and step: 16 bytes of f32, 8 of a 16-bit type
+    for (int c = lane * 4; c < p.experts; c += 128) {
+      const float4 v = *reinterpret_cast<const float4 *>(mem + c);
+      if (p.g_dtype == KAPYB_F32) {
+        __stcs(reinterpret_cast<float4 *>(static_cast<float *>(p.grad) + row * p.g_s0 + c), v);
+      } else {
+        uint2 w;
+        if (p.g_dtype == KAPYB_BF16)
+          w = make_uint2(cvt_pack2_t<KAPYB_BF16, 1>(v.x, v.y), cvt_pack2_t<KAPYB_BF16, 1>(v.z, v.w));
+        else
+          w = make_uint2(cvt_pack2_t<KAPYB_F16, 1>(v.x, v.y), cvt_pack2_t<KAPYB_F16, 1>(v.z, v.w));
+        __stcs(reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.grad) + row * p.g_s0 + c), w);
+      }
+    }
+  } else {
+    for (int c = lane; c < p.experts; c += 32)
+      store_from_f32(p.grad, p.g_dtype, row * p.g_s0 + c * p.g_s1, mem[c], 1);
   }
 }
 
