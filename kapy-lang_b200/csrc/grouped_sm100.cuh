@@ -72,8 +72,12 @@ struct GroupedParams {
   long long group_bytes;        // gradient: bytes between groups
   int out_dtype, pair_stores;   // pair_stores: two 16-bit columns may be stored as one word
   float alpha;
-  const void *bias;      // [groups, bias_cols]
-  int bias_dtype, bias_cols, activation, rounding;
+  const void *bias;      // [groups, bias_cols]; adapters: [cols], or [source rows] with bias_axis 0
+  int bias_dtype, bias_cols, bias_axis, activation, rounding;
+  // pairs, forward: the result as two 16-bit halves, v rounded and what that left, the
+  // second array lo_bytes behind the first (0: off); scaled by alpha * group_scale[g]
+  long long lo_bytes;
+  const float *group_scale;
   uint32_t *status;
   uint32_t wait_limit_us;
 };
@@ -87,7 +91,7 @@ struct GroupedCfg {
   static constexpr int B_BYTES = BT * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int CTRL_BYTES = 1024;
-  static constexpr int TABLE_BYTES = (3 * kGroupedMaxGroups + 4) * 4;
+  static constexpr int TABLE_BYTES = (3 * kGroupedMaxGroups + 8) * 4;
   static constexpr int SMEM_LIMIT = 232448;
   static constexpr int STAGES_RAW = (SMEM_LIMIT - 1024 - CTRL_BYTES - TABLE_BYTES) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
@@ -108,6 +112,18 @@ struct GroupedTile {
   int num_kb;   // K blocks
   int p0, p1;   // gradient: the group's positions
 };
+
+// Which of a group's tiles (`tiles` row tiles x n_tiles column blocks) is number `in`:
+// row tiles next to one another, eight at a time, so that CTAs running at the same time
+// share rows and columns in L2 (eight row tiles and some nine column blocks at once
+// instead of all row tiles of a long group and one or two column blocks).
+__device__ __forceinline__ void raster(int in, int tiles, int n_tiles, int &m, int &n) {
+  const int block = in / (8 * n_tiles), first = block * 8;
+  const int high = min(8, tiles - first);
+  const int r = in - block * 8 * n_tiles;
+  n = r / high;
+  m = first + r - n * high;
+}
 
 __device__ __forceinline__ int round16(int v) { return (v + 15) & ~15; }
 
@@ -144,7 +160,8 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams &p, cons
     r.g = lo;
     const int tiles = t.first[lo + 1] - t.first[lo];
     const int in = idx - t.first[lo] * p.n_tiles;
-    const int n = in / tiles, m = in - n * tiles;
+    int m, n;
+    raster(in, tiles, p.n_tiles, m, n);
     const int cnt = t.count[lo];
     const int each = round16((cnt + tiles - 1) / tiles);
     r.n0 = n * 128;
@@ -157,13 +174,8 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams &p, cons
   return r;
 }
 
-// Activation, scale and bias of 32 values of one output column.
-template <int MSETS>
-__device__ __forceinline__ void grouped_finish32(const GroupedParams &p, float (&f)[32], const float *up,
-                                                 float bias, float bias_up) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = f[i] * p.alpha + bias;
-  switch (p.activation) {
+__device__ __forceinline__ void grouped_activation32(int activation, float (&f)[32]) {
+  switch (activation) {
   case KAPYB_ACT_RELU:
 #pragma unroll
     for (int i = 0; i < 32; ++i) f[i] = apply_activation_t<KAPYB_ACT_RELU>(f[i]);
@@ -178,9 +190,18 @@ __device__ __forceinline__ void grouped_finish32(const GroupedParams &p, float (
     break;
   default: break;
   }
+}
+
+// Scale, bias and activation of 32 values of one output column.
+template <int MSETS>
+__device__ __forceinline__ void grouped_finish32(const GroupedParams &p, float alpha, float (&f)[32], const float *up,
+                                                 float bias, float bias_up) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f[i] = f[i] * alpha + bias;
+  grouped_activation32(p.activation, f);
   if constexpr (MSETS == 2) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] *= up[i] * p.alpha + bias_up;
+    for (int i = 0; i < 32; ++i) f[i] *= up[i] * alpha + bias_up;
   }
 }
 
@@ -253,6 +274,53 @@ __device__ __forceinline__ void grouped_store32(const GroupedParams &p, char *at
   } else {
     if (p.rounding) store_rows16<KAPYB_F16, 1>(at, pitch, f, left, lane, mine, both, pairs);
     else store_rows16<KAPYB_F16, 0>(at, pitch, f, left, lane, mine, both, pairs);
+  }
+}
+
+// The same rows to places of their own: lane j of the warp holds the output row of f[j],
+// -1 for none.
+template <int DT, int RN>
+__device__ __forceinline__ void scatter_rows16(char *col, uint32_t pitch, const float (&f)[32], int to, int lane,
+                                               bool mine, bool both, bool pairs) {
+  const bool odd = lane & 1;
+  if (pairs) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float give = odd ? f[j] : f[j + 1];
+      const float take = __shfl_xor_sync(0xffffffffu, give, 1);
+      const uint32_t w = odd ? cvt_pack2_t<DT, RN>(take, f[j + 1]) : cvt_pack2_t<DT, RN>(f[j], take);
+      const int even_row = __shfl_sync(0xffffffffu, to, j), odd_row = __shfl_sync(0xffffffffu, to, j + 1);
+      const int row = odd ? odd_row : even_row;
+      char *at = col + static_cast<long long>(row) * pitch;
+      if (both && row >= 0) *reinterpret_cast<uint32_t *>(odd ? at - 2 : at) = w;
+    }
+    if (!__any_sync(0xffffffffu, mine && !both)) return;
+  }
+  const bool on = mine && !(pairs && both);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const int row = __shfl_sync(0xffffffffu, to, j);
+    if (on && row >= 0)
+      *reinterpret_cast<uint16_t *>(col + static_cast<long long>(row) * pitch) =
+          static_cast<uint16_t>(cvt_pack2_t<DT, RN>(f[j], 0.0f) & 0xffffu);
+  }
+}
+__device__ __forceinline__ void grouped_scatter32(const GroupedParams &p, char *col, const float (&f)[32], int to,
+                                                  int lane, bool mine, bool both) {
+  const uint32_t pitch = p.row_pitch;
+  const bool pairs = p.pair_stores != 0;
+  if (p.out_dtype == KAPYB_F32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const int row = __shfl_sync(0xffffffffu, to, j);
+      if (mine && row >= 0) *reinterpret_cast<float *>(col + static_cast<long long>(row) * pitch) = f[j];
+    }
+  } else if (p.out_dtype == KAPYB_BF16) {
+    if (p.rounding) scatter_rows16<KAPYB_BF16, 1>(col, pitch, f, to, lane, mine, both, pairs);
+    else scatter_rows16<KAPYB_BF16, 0>(col, pitch, f, to, lane, mine, both, pairs);
+  } else {
+    if (p.rounding) scatter_rows16<KAPYB_F16, 1>(col, pitch, f, to, lane, mine, both, pairs);
+    else scatter_rows16<KAPYB_F16, 0>(col, pitch, f, to, lane, mine, both, pairs);
   }
 }
 
@@ -509,7 +577,7 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&tempty_bar[acc]));
         }
-        grouped_finish32<MSETS>(p, f, u, bias, bias_up);
+        grouped_finish32<MSETS>(p, p.alpha, f, u, bias, bias_up);
         grouped_store32(p, out + static_cast<long long>(c) * p.row_pitch, f, t.rows - c, lane, mine, both);
       }
       if (!warp_has) {
@@ -566,12 +634,26 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 // they last and then 8-row and 1-row boxes, so that what is behind the end is fetched
 // as zeros as well.
 
+// Adapters: the rows are a plan sorted by adapter whose groups start at multiples of 32
+// (gaps and rows without an adapter included), and the tile's main loop over the shared
+// weights is followed by more K blocks, for each adapter that has rows in the tile: its
+// `up` block times the rows' low-rank products (scale x . down, computed before), into
+// exactly the accumulator columns those rows own.  The products come in two 16-bit
+// halves, so the second factor is exact to 16 bits and more.  Nothing is added twice to
+// memory and one rounding remains; what a broken adapter produces stays in its own rows.
+
+enum PairMode { PAIR_FORWARD = 0, PAIR_GRADIENT = 1, PAIR_ADAPTERS = 2 };
+
 struct PairParams {
   GroupedParams g;
   int gather;            // rows of lhs by cp.async: a plan's order, and always the gradient
   const uint8_t *lhs;    // element (0, 0)
   long long lhs_pitch;   // bytes between rows
   FastDiv div_fan;
+  int tile_rows;         // forward: most rows of a tile, at most BT and a multiple of 32
+  // adapters: g.groups = adapters + 1 (the last group: rows without one)
+  int rank, up_mn_major;
+  int low_rows;          // rows of one half of the low-rank products
 };
 
 constexpr int kPairThreads = 192 + 256 + 32;
@@ -582,7 +664,7 @@ struct PairCfg {
   static constexpr int B_BYTES = BT / 2 * 128;       // per CTA: half of the tile's rows
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int CTRL_BYTES = 1024;
-  static constexpr int TABLE_BYTES = (3 * kGroupedMaxGroups + 4) * 4;
+  static constexpr int TABLE_BYTES = (3 * kGroupedMaxGroups + 8) * 4;
   static constexpr int SMEM_LIMIT = 232448;
   static constexpr int STAGES_RAW = (SMEM_LIMIT - 1024 - CTRL_BYTES - TABLE_BYTES) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
@@ -613,10 +695,20 @@ __device__ __forceinline__ int round32(int v) { return (v + 31) & ~31; }
 
 // The tile of a pair: as grouped_tile, for blocks of 256 columns, rows rounded to 32
 // (the N side of a pair's MMA is a multiple of 32).
-template <int BT, bool GRAD>
+template <int BT, int MODE>
 __device__ __forceinline__ GroupedTile pair_tile(const GroupedParams &p, const GroupedTable &t, int idx) {
   GroupedTile r;
-  if constexpr (GRAD) {
+  if constexpr (MODE == PAIR_ADAPTERS) {
+    const int all = t.begin[p.groups];  // positions, gaps included
+    int m, n;
+    raster(idx, (all + BT - 1) / BT, p.n_tiles, m, n);
+    r.g = 0;
+    r.n0 = n * 256;
+    r.r0 = m * BT;
+    r.rows = min(BT, all - r.r0);
+    r.num_kb = p.num_kb;
+    r.p0 = r.p1 = 0;
+  } else if constexpr (MODE == PAIR_GRADIENT) {
     const int per = p.n_tiles * p.k_tiles;
     r.g = idx / per;
     const int in = idx - r.g * per;
@@ -638,7 +730,8 @@ __device__ __forceinline__ GroupedTile pair_tile(const GroupedParams &p, const G
     r.g = lo;
     const int tiles = t.first[lo + 1] - t.first[lo];
     const int in = idx - t.first[lo] * p.n_tiles;
-    const int n = in / tiles, m = in - n * tiles;
+    int m, n;
+    raster(in, tiles, p.n_tiles, m, n);
     const int cnt = t.count[lo];
     const int each = round32((cnt + tiles - 1) / tiles);
     r.n0 = n * 256;
@@ -651,16 +744,35 @@ __device__ __forceinline__ GroupedTile pair_tile(const GroupedParams &p, const G
   return r;
 }
 
+// The adapters that have rows in [c0, c1): f(g, first position, last position + 1) for
+// each; returns false as soon as f does.
+template <class F>
+__device__ __forceinline__ bool each_adapter(const GroupedTable &t, int adapters, int c0, int c1, F &&f) {
+  int lo = 0, hi = adapters;  // the first adapter that ends behind c0
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (t.begin[mid + 1] > c0) hi = mid;
+    else lo = mid + 1;
+  }
+  for (int g = lo; g < adapters && t.begin[g] < c1; ++g) {
+    const int s0 = max(t.begin[g], c0), s1 = min(t.begin[g + 1], c1);
+    if (s1 > s0 && !f(g, s0, s1)) return false;
+  }
+  return true;
+}
+
 // tmA: forward: rhs as in grouped_tcgen05_kernel; gradient: grad in boxes of 64 x 64,
 // tmA8 and tmA1 the same in boxes 8 rows and 1 row high.  Forward without a gather: lhs
-// in boxes of 64 x 32 (tmB) and 64 x BT / 2 (tmA8).
-template <int BT, int MSETS, bool GRAD>
+// in boxes of 64 x 32 (tmB) and 64 x BT / 2 (tmA8).  Adapters: tmA8 up, 3-D as rhs, tmA1
+// the low-rank products, both halves behind one another, in boxes of 64 x 16.
+template <int BT, int MSETS, int MODE>
 __global__ void __launch_bounds__(kPairThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmA8, const __grid_constant__ CUtensorMap tmA1,
                     const PairParams pp) {
   using Cfg = PairCfg<BT, MSETS>;
   constexpr int STAGES = Cfg::STAGES;
+  constexpr bool GRAD = MODE == PAIR_GRADIENT, ADAPT = MODE == PAIR_ADAPTERS;
   const GroupedParams &p = pp.g;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -673,13 +785,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(rows_bar + STAGES);
   volatile uint32_t *abort_flag = tmem_slot + 1;  // two words
   int *table_mem = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(bars) + Cfg::CTRL_BYTES);
-  GroupedTable table{table_mem, table_mem + kGroupedMaxGroups + 1, table_mem + 2 * kGroupedMaxGroups + 1};
+  GroupedTable table{table_mem, table_mem + kGroupedMaxGroups + 2, table_mem + 2 * kGroupedMaxGroups + 4};
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
   const int unit = blockIdx.x >> 1, units = gridDim.x >> 1;
-  const bool gather = GRAD || pp.gather;
+  const bool gather = GRAD || ADAPT || pp.gather;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       // the leader's expect_tx, and with a gather one arrival from each CTA
@@ -701,14 +813,31 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     ptx::tmem_alloc<2>(ptx::smem_u32(tmem_slot), Cfg::TMEM_COLS);
     ptx::tmem_relinquish<2>();
   }
-  if (warp == 0) {
+  if constexpr (ADAPT) {
+    // group starts only, made ascending whatever the memory holds
+    if (warp == 0) {
+      int high = 0;
+      for (int g0 = 0; g0 <= p.groups; g0 += 32) {
+        const int g = g0 + lane;
+        int b = g <= p.groups ? min(max(p.offsets[g], 0), p.rows) & ~31 : 0;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const int o = __shfl_up_sync(0xffffffffu, b, off);
+          if (lane >= off) b = max(b, o);
+        }
+        b = max(b, high);
+        if (g <= p.groups) table.begin[g] = b;
+        high = __shfl_sync(0xffffffffu, b, 31);
+      }
+    }
+  } else if (warp == 0) {
     int before = 0;
     for (int g0 = 0; g0 < p.groups; g0 += 32) {
       const int g = g0 + lane;
       int b = 0, e = 0;
       if (g < p.groups) group_range(p.offsets, g, p.rows, b, e);
       const int cnt = max(0, e - b);
-      const int tiles = GRAD ? 0 : (cnt + BT - 1) / BT;
+      const int tiles = GRAD ? 0 : (cnt + pp.tile_rows - 1) / pp.tile_rows;
       int scan = tiles;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -730,7 +859,20 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   ptx::cluster_wait();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int total = GRAD ? p.groups * p.n_tiles * p.k_tiles : table.first[p.groups] * p.n_tiles;
+  const int total = GRAD    ? p.groups * p.n_tiles * p.k_tiles
+                    : ADAPT ? (table.begin[p.groups] + BT - 1) / BT * p.n_tiles
+                            : table.first[p.groups] * p.n_tiles;
+  const int low_blocks = ADAPT ? (pp.rank + 63) >> 6 : 0;  // K blocks of an adapter, each twice
+  // adapters: K blocks of a tile behind its main loop
+  auto extra = [&](const GroupedTile &t) {
+    int n = 0;
+    if constexpr (ADAPT)
+      each_adapter(table, p.groups - 1, t.r0, t.r0 + t.rows, [&](int, int, int) {
+        n += 2 * low_blocks;
+        return true;
+      });
+    return n;
+  };
   auto leader = [](const void *bar) { return ptx::mapa(ptx::smem_u32(bar), 0); };
 
   if (warp == 0) {
@@ -739,7 +881,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     uint32_t phase = 0;
     bool ok = true;
     for (int idx = unit; ok && idx < total; idx += units) {
-      const GroupedTile t = pair_tile<BT, GRAD>(p, table, idx);
+      const GroupedTile t = pair_tile<BT, MODE>(p, table, idx);
       const int half = t.wide >> 1;                         // rows this CTA fetches
       // rows in plan order: one tall box, or boxes of 32 rows where it would fetch too much
       const bool tall = half > BT / 2 - 32;
@@ -793,6 +935,36 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           phase ^= 1u;
         }
       }
+      if constexpr (ADAPT) {
+        if (!ok) break;
+        ok = each_adapter(table, p.groups - 1, t.r0, t.r0 + t.rows, [&](int g, int s0, int s1) {
+          const int mine = (s1 - s0) >> 1;  // rows this CTA fetches: a multiple of 16
+          for (int b = 0; b < 2 * low_blocks; ++b) {
+            const bool got = ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag);
+            if (!__all_sync(0xffffffffu, got)) return false;
+            const uint32_t fb = leader(&full_bar[stage]);
+            const uint32_t a_dst = ptx::smem_u32(sA + stage * Cfg::A_BYTES);
+            const uint32_t b_dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES);
+            if (rank == 0 && lane == 0)
+              ptx::mbar_arrive_expect_tx(ptx::smem_u32(&full_bar[stage]), 2u * (Cfg::A_BYTES + mine * 128u));
+            __syncwarp();
+            const int k0 = (b >> 1) * 64;
+            if (pp.up_mn_major) {
+              if (lane < 2) ptx::tma_load_3d_pair(a_dst + lane * 8192, &tmA8, fb, n0 + lane * 64, k0, g);
+            } else {
+              if (lane == 0) ptx::tma_load_3d_pair(a_dst, &tmA8, fb, k0, n0, g);
+            }
+            if (lane < (mine >> 4))
+              tma_load_2d_pair(b_dst + lane * 2048, &tmA1, fb, k0,
+                               (b & 1) * pp.low_rows + s0 + rank * mine + lane * 16);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+          return true;
+        });
+      }
     }
   } else if (warp == 1 && rank == 0) {
     // ---------------------------------------------------------- MMA issuer
@@ -809,7 +981,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
     for (int idx = unit; ok && idx < total; idx += units) {
-      const GroupedTile t = pair_tile<BT, GRAD>(p, table, idx);
+      const GroupedTile t = pair_tile<BT, MODE>(p, table, idx);
       const uint32_t idesc = ptx::make_idesc_f16(p.bf16, a_mn, b_mn, 256, t.wide);
       if (!wait_all(ptx::smem_u32(&tempty_bar[acc]), acc_phase ^ 1u)) break;
       ptx::tc_fence_after();
@@ -840,6 +1012,33 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           phase ^= 1u;
         }
       }
+      if constexpr (ADAPT) {
+        if (!ok) break;
+        const uint32_t u_step = (pp.up_mn_major ? 2048u : 32u) >> 4;
+        const uint32_t u_lo0 = ((pp.up_mn_major ? 8192u : 16u) >> 4) << 16 | (ptx::smem_u32(sA) >> 4);
+        ok = each_adapter(table, p.groups - 1, t.r0, t.r0 + t.rows, [&](int, int s0, int s1) {
+          const uint32_t idesc_s = ptx::make_idesc_f16(p.bf16, pp.up_mn_major, 0, 256, s1 - s0);
+          for (int b = 0; b < 2 * low_blocks; ++b) {
+            if (!wait_all(ptx::smem_u32(&full_bar[stage]), phase)) return false;
+            ptx::tc_fence_after();
+            const int steps = (min(64, pp.rank - (b >> 1) * 64) + 15) >> 4;
+            if (ptx::elect_one()) {
+              const uint32_t a_lo = u_lo0 + static_cast<uint32_t>(stage) * (Cfg::A_BYTES >> 4);
+              const uint32_t b_lo = b_lo0 + static_cast<uint32_t>(stage) * (Cfg::B_BYTES >> 4);
+              for (int k = 0; k < steps; ++k)
+                ptx::umma_k<2, 0>(d + (s0 - t.r0), (static_cast<uint64_t>(hi) << 32) | (a_lo + k * u_step),
+                                  (static_cast<uint64_t>(hi) << 32) | (b_lo + k * 2u), idesc_s, 1u);
+              ptx::umma_commit<2>(ptx::smem_u32(&empty_bar[stage]));
+              ptx::umma_commit<2>(ptx::mapa(ptx::smem_u32(&empty_bar[stage]), 1));
+            }
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+          return true;
+        });
+      }
       if (!ok) break;
       if (ptx::elect_one()) {
         ptx::umma_commit<2>(ptx::smem_u32(&tfull_bar[acc]));
@@ -854,16 +1053,17 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int idx = unit; idx < total; idx += units) {
-      const GroupedTile t = pair_tile<BT, GRAD>(p, table, idx);
+      const GroupedTile t = pair_tile<BT, MODE>(p, table, idx);
       const int warp_n = t.n0 + rank * 128 + q * 32;
       const int n = warp_n + lane;
       const bool mine = n < p.cols, both = (n | 1) < p.cols;
       float bias = 0.0f, bias_up = 0.0f;
-      if (p.bias != nullptr && mine) {
-        const long long at = static_cast<long long>(t.g) * p.bias_cols + n;
+      if (p.bias != nullptr && mine && (!ADAPT || p.bias_axis == 1)) {
+        const long long at = (ADAPT ? 0ll : static_cast<long long>(t.g) * p.bias_cols) + n;
         bias = load_as_f32(p.bias, p.bias_dtype, at);
         if constexpr (MSETS == 2) bias_up = load_as_f32(p.bias, p.bias_dtype, at + p.cols);
       }
+      const float alpha = !ADAPT && p.group_scale != nullptr ? p.alpha * p.group_scale[t.g] : p.alpha;
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc]), acc_phase, abort_flag))) break;
       ptx::tc_fence_after();
       const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
@@ -896,8 +1096,30 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive_cluster(tempty);
         }
-        grouped_finish32<MSETS>(p, f, u, bias, bias_up);
-        grouped_store32(p, out + static_cast<long long>(c) * p.row_pitch, f, t.rows - c, lane, mine, both);
+        if constexpr (ADAPT) {
+          // rows go where the plan took them from; lane l holds row c + l's number
+          int to = c + lane < t.rows ? p.order[t.r0 + c + lane] : -1;
+          if (to >= p.src_rows) to = -1;
+          if (p.bias != nullptr && p.bias_axis == 0) {
+            const float row_bias = to >= 0 ? load_as_f32(p.bias, p.bias_dtype, to) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = f[j] * alpha + __shfl_sync(0xffffffffu, row_bias, j);
+            grouped_activation32(p.activation, f);
+          } else {
+            grouped_finish32<1>(p, alpha, f, nullptr, bias, 0.0f);
+          }
+          grouped_scatter32(p, static_cast<char *>(p.out) + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll), f, to, lane,
+                            mine, both);
+        } else {
+          grouped_finish32<MSETS>(p, alpha, f, u, bias, bias_up);
+          char *at = out + static_cast<long long>(c) * p.row_pitch;
+          grouped_store32(p, at, f, t.rows - c, lane, mine, both);
+          if (MODE == PAIR_FORWARD && MSETS == 1 && p.lo_bytes != 0) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] -= cvt_16_to_f32(cvt_f32_to_16(f[j], p.out_dtype, 1), p.out_dtype);
+            grouped_store32(p, at + p.lo_bytes, f, t.rows - c, lane, mine, both);
+          }
+        }
       }
       if (!warp_has) {
         ptx::tc_fence_before();
@@ -913,8 +1135,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     uint32_t phase = 0;
     bool ok = true;
     for (int idx = unit; ok && idx < total; idx += units) {
-      const GroupedTile t = pair_tile<BT, GRAD>(p, table, idx);
-      for (int kb = 0; kb < t.num_kb; ++kb) {
+      const GroupedTile t = pair_tile<BT, MODE>(p, table, idx);
+      const int blocks = t.num_kb + extra(t);
+      for (int kb = 0; kb < blocks; ++kb) {
         if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&rows_bar[stage]), phase, abort_flag))) {
           ok = false;
           break;
@@ -934,7 +1157,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     uint32_t phase = 0;
     bool ok = true;
     for (int idx = unit; ok && idx < total; idx += units) {
-      const GroupedTile t = pair_tile<BT, GRAD>(p, table, idx);
+      const GroupedTile t = pair_tile<BT, MODE>(p, table, idx);
       const int half = t.wide >> 1;
       if constexpr (GRAD) {
         // thread: 16-byte piece `piece` of this CTA's columns, rows row0, row0 + 16, ...
@@ -999,7 +1222,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           live[i] = s >= 0;
           row[i] = pp.lhs + (live[i] ? s * pp.lhs_pitch : 0);
         }
-        for (int kb = 0; kb < t.num_kb; ++kb) {
+        const int blocks = t.num_kb + extra(t);
+        for (int kb = 0; kb < blocks; ++kb) {
           if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag))) {
             ok = false;
             break;
@@ -1008,9 +1232,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           const uint32_t bytes = static_cast<uint32_t>(max(0, min(16, (p.K - k) * 2)));
           const uint32_t dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES) + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
           const long long at = bytes ? k * 2ll : 0ll;
+          // (the adapters' blocks bring their rows by TMA: nothing to copy, only to arrive)
 #pragma unroll
           for (int i = 0; i < kRows; ++i)
-            if (row0 + 32 * i < half) cp_async16(dst + i * 4096, row[i] + at, live[i] ? bytes : 0u);
+            if (row0 + 32 * i < half && kb < t.num_kb) cp_async16(dst + i * 4096, row[i] + at, live[i] ? bytes : 0u);
           cp_async_arrive(ptx::smem_u32(&rows_bar[stage]));
           if (++stage == STAGES) {
             stage = 0;

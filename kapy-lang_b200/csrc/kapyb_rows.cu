@@ -5,8 +5,10 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cmath>
 
 #include "../../include/kapyb.h"
+#include "adapters_sm100.cuh"
 #include "combine_rows.cuh"
 #include "context.cuh"
 #include "grouped_sm100.cuh"
@@ -270,6 +272,36 @@ extern "C" KAPYB_API kapyb_status kapyb_route_backward(kapyb_handle h, const kap
 
 // ---------------------------------------------------------------------- plan
 
+namespace {
+
+kapyb_status launch_plan(kapyb_handle h, const PlanParams &p, cudaStream_t stream) {
+  const size_t smem = plan_smem_bytes(p.groups);
+  CUDA_TRY(h, cudaFuncSetAttribute(plan_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(plan_smem_bytes(kPlanMaxGroups + 1))));
+  // A warp's piece is a whole number of 32-entry steps.  One CTA takes up to two steps a
+  // warp; beyond that the work is spread over the cluster.
+  int ctas = 1;
+  while (ctas < kPlanMaxCtas && static_cast<long long>(p.n) > ctas * kPlanWarps * 64ll) ctas *= 2;
+  if (ctas > 8)
+    CUDA_TRY(h, cudaFuncSetAttribute(plan_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(ctas, 1, 1);
+  cfg.blockDim = dim3(kPlanWarps * 32, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CUDA_TRY(h, cudaLaunchKernelEx(&cfg, plan_rows_kernel, p));
+  return launched(h, "plan_rows");
+}
+
+}  // namespace
+
 extern "C" KAPYB_API kapyb_status kapyb_plan_rows(kapyb_handle h, const int32_t *index, int32_t n, int32_t groups,
                                                   int32_t *order, int32_t *offsets, int32_t *slots, void *stream) {
   const char *call = "plan_rows";
@@ -288,30 +320,8 @@ extern "C" KAPYB_API kapyb_status kapyb_plan_rows(kapyb_handle h, const int32_t 
     for (int j = i + 1; j < 4; ++j)
       if (meet(s[i], s[j])) return fail(h, KAPYB_INVALID_ARG, "plan_rows: two arrays of the call overlap");
   ON_DEVICE(h);
-  const size_t smem = plan_smem_bytes(groups);
-  CUDA_TRY(h, cudaFuncSetAttribute(plan_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   static_cast<int>(plan_smem_bytes(kPlanMaxGroups))));
-  // A warp's piece is a whole number of 32-entry steps.  One CTA takes up to two steps a
-  // warp; beyond that the work is spread over the cluster.
-  int ctas = 1;
-  while (ctas < kPlanMaxCtas && static_cast<long long>(n) > ctas * kPlanWarps * 64ll) ctas *= 2;
-  if (ctas > 8)
-    CUDA_TRY(h, cudaFuncSetAttribute(plan_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(ctas, 1, 1);
-  cfg.blockDim = dim3(kPlanWarps * 32, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const PlanParams p{index, n, groups, order, offsets, slots};
-  CUDA_TRY(h, cudaLaunchKernelEx(&cfg, plan_rows_kernel, p));
-  return launched(h, "plan_rows");
+  return launch_plan(h, PlanParams{index, n, groups, order, offsets, slots, n, 1, 0},
+                     static_cast<cudaStream_t>(stream));
 }
 
 // ------------------------------------------------------------------- products
@@ -355,13 +365,24 @@ kapyb_status launch_grouped(kapyb_handle h, const CUtensorMap &tmA, const CUtens
   return launched(h, GRAD ? "grouped_grad_tcgen05" : "grouped_tcgen05");
 }
 
+PairParams pair_params(const GroupedParams &gp, const kapyb_tensor2d *lhs, bool gather, int tile_rows) {
+  PairParams pp{};
+  pp.g = gp;
+  pp.gather = gather;
+  pp.lhs = static_cast<const uint8_t *>(elem_ptr(lhs));
+  pp.lhs_pitch = lhs->stride0 * 2ll;
+  pp.div_fan = FastDiv::make(static_cast<uint32_t>(gp.fan));
+  pp.tile_rows = tile_rows;
+  return pp;
+}
+
 // The pair kernel: `tiles` pairs of CTAs at most, as many as the device holds at once
 // (the tile loop is statically strided).
-template <int BT, int MSETS, bool GRAD>
+template <int BT, int MSETS, int MODE>
 kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmA8,
                           const CUtensorMap &tmA1, const PairParams &pp, long long tiles, cudaStream_t stream) {
   using Cfg = PairCfg<BT, MSETS>;
-  auto kern = grouped_pair_kernel<BT, MSETS, GRAD>;
+  auto kern = grouped_pair_kernel<BT, MSETS, MODE>;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.blockDim = dim3(kPairThreads, 1, 1);
@@ -387,7 +408,7 @@ kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensor
   }
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min<long long>(tiles, pairs)), 1, 1);
   CUDA_TRY(h, cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmA8, tmA1, pp));
-  return launched(h, GRAD ? "grouped_grad_pair" : "grouped_pair");
+  return launched(h, MODE == PAIR_GRADIENT ? "grouped_grad_pair" : MODE == PAIR_ADAPTERS ? "adapters_pair" : "grouped_pair");
 }
 
 // Rows of lhs as TMA can fetch them: 16-bit, unit stride along K, 16-byte rows.
@@ -451,13 +472,12 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
   if (narrow)
     return gated ? launch_grouped<64, 2, false>(h, tmA, tmB, gp, tiles, stream)
                  : launch_grouped<64, 1, false>(h, tmA, tmB, gp, tiles, stream);
-  const PairParams pp{gp, order != nullptr, static_cast<const uint8_t *>(elem_ptr(lhs)), lhs->stride0 * 2ll,
-                    FastDiv::make(static_cast<uint32_t>(gp.fan))};
+  const PairParams pp = pair_params(gp, lhs, order != nullptr, bt);
   CUtensorMap tall;
   TRY(make_row_tmap(h, &tall, elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
                     lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, bt / 2));
-  return gated ? launch_pairs<128, 2, false>(h, tmA, tmB, tall, tmA, pp, tiles, stream)
-               : launch_pairs<256, 1, false>(h, tmA, tmB, tall, tmA, pp, tiles, stream);
+  return gated ? launch_pairs<128, 2, PAIR_FORWARD>(h, tmA, tmB, tall, tmA, pp, tiles, stream)
+               : launch_pairs<256, 1, PAIR_FORWARD>(h, tmA, tmB, tall, tmA, pp, tiles, stream);
 }
 
 kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const kapyb_tensor2d *grad,
@@ -498,9 +518,8 @@ kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, 
   TRY(make_row_tmap(h, &tmA8, elem_ptr(grad), grad->dtype, grad->size1, grad->size0, ld, 8));
   TRY(make_row_tmap(h, &tmA1, elem_ptr(grad), grad->dtype, grad->size1, grad->size0, ld, 1));
   *taken = true;
-  const PairParams pp{gp, 1, static_cast<const uint8_t *>(elem_ptr(lhs)), lhs->stride0 * 2ll,
-                    FastDiv::make(static_cast<uint32_t>(gp.fan))};
-  return launch_pairs<256, 1, true>(h, tmA, tmA, tmA8, tmA1, pp, tiles, stream);
+  const PairParams pp = pair_params(gp, lhs, true, 256);
+  return launch_pairs<256, 1, PAIR_GRADIENT>(h, tmA, tmA, tmA8, tmA1, pp, tiles, stream);
 }
 
 // What the two grouped products check alike.
@@ -805,12 +824,269 @@ extern "C" KAPYB_API kapyb_status kapyb_combine_rows_backward(kapyb_handle h, co
 // ------------------------------------------------------------------- adapters
 
 namespace {
+
 constexpr int kMaxAdapterRank = 128;
+
+size_t up256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+
+// Scratch of the call: f32 products for few rows and the CUDA-core path, else the plan
+// (order, offsets) and the products' two 16-bit halves.
+struct AdapterScratch {
+  int64_t positions;   // of the padded plan: groups start at multiples of 32
+  size_t order, offsets, low, total;
+  AdapterScratch(int rows, int groups, int rank) {
+    positions = (rows + 31ll * std::min(groups + 1, rows) + 31) / 32 * 32;
+    order = 0;
+    offsets = up256(static_cast<size_t>(positions) * 4);
+    low = offsets + up256((groups + 2ull) * 4);
+    const size_t halves = static_cast<size_t>(positions) * ((rank + 7) / 8 * 8) * 2 * 2;
+    total = std::max(low + halves, static_cast<size_t>(rows) * rank * sizeof(float));
+  }
+};
+
+struct AdapterCall {
+  const kapyb_tensor2d *lhs, *rhs, *down, *up, *out;
+  int groups;
+  int64_t down_stride, up_stride;
+  const int32_t *index;
+  const float *scale;
+  const kapyb_epilogue &ep;
+  void *scratch;
+};
+
+// One matrix of a stack as TMA can fetch it; `mn`: unit stride on the second axis.
+bool stack_tma_ok(const kapyb_tensor2d *t, int groups, int64_t stride, bool &mn, int64_t &unit, int64_t &other,
+                  int64_t &ld) {
+  mn = t->stride1 == 1;
+  if (!half_type(t->dtype) || (!mn && t->stride0 != 1)) return false;
+  unit = mn ? t->size1 : t->size0;
+  other = mn ? t->size0 : t->size1;
+  ld = mn ? t->stride0 : t->stride1;
+  return tma_ok(elem_ptr(t), t->dtype, unit, other, ld, groups, stride);
+}
+
+// At most 64 rows: the weight stream with the adapters' part beside it.
+kapyb_status adapters_decode(kapyb_handle h, const AdapterCall &c, cudaStream_t stream, bool *taken) {
+  *taken = false;
+  bool mn;
+  int64_t unit, other, ld;
+  if (c.lhs->size0 > kDecodeMaxRows || !rows_tma_ok(c.lhs) || !stack_tma_ok(c.rhs, 1, 0, mn, unit, other, ld))
+    return KAPYB_OK;
+  const int rows = c.lhs->size0, rank = c.down->size1;
+  const uint16_t *down = static_cast<const uint16_t *>(elem_ptr(c.down));
+  float *low = static_cast<float *>(c.scratch);
+  const bool bf = c.lhs->dtype == KAPYB_BF16;
+
+  // low = scale * x . down
+  const bool d_aligned = aligned16(down) && c.down_stride % 8 == 0;
+  const bool d_k = c.down->stride0 == 1 && c.down->stride1 % 8 == 0 && d_aligned;
+  const bool d_r = c.down->stride1 == 1 && c.down->stride0 % 8 == 0 && d_aligned && rank % 8 == 0;
+  if (d_k || d_r) {
+    const LowParams lp{static_cast<const uint16_t *>(elem_ptr(c.lhs)), c.lhs->stride0, down, c.down->stride0,
+                       c.down->stride1, c.down_stride, bf, c.groups, rows, c.lhs->size1, rank, c.index, c.scale, low};
+    if (d_r)
+      bf ? adapter_low_kernel<true, false><<<rows, kLowThreads, 0, stream>>>(lp)
+         : adapter_low_kernel<false, false><<<rows, kLowThreads, 0, stream>>>(lp);
+    else
+      bf ? adapter_low_kernel<true, true><<<rows, kLowThreads, 0, stream>>>(lp)
+         : adapter_low_kernel<false, true><<<rows, kLowThreads, 0, stream>>>(lp);
+  } else {
+    AdapterSimtParams sp{};
+    sp.x = elem_ptr(c.lhs);
+    sp.x_s0 = c.lhs->stride0;
+    sp.x_s1 = c.lhs->stride1;
+    sp.down = down;
+    sp.d_s0 = c.down->stride0;
+    sp.d_s1 = c.down->stride1;
+    sp.d_group = c.down_stride;
+    sp.in_dtype = c.lhs->dtype;
+    sp.groups = c.groups;
+    sp.rows = rows;
+    sp.K = c.lhs->size1;
+    sp.rank = rank;
+    sp.index = c.index;
+    sp.scale = c.scale;
+    sp.low = low;
+    adapter_low_simt_kernel<<<rows, 256, 0, stream>>>(sp);
+  }
+  TRY(launched(h, "adapter_low"));
+
+  DecodeParams p{};
+  p.rows = rows;
+  p.wide = (rows + 15) / 16 * 16;
+  p.cols = c.out->size1;
+  p.num_kb = (c.lhs->size1 + 63) / 64;
+  p.w_mn_major = mn;
+  p.bf16 = bf;
+  p.tmem_cols = p.wide <= 32 ? 32 : 64;
+  p.low = low;
+  p.index = c.index;
+  p.groups = c.groups;
+  p.rank = rank;
+  p.up = static_cast<const uint16_t *>(elem_ptr(c.up));
+  p.u_s0 = c.up->stride0;
+  p.u_s1 = c.up->stride1;
+  p.u_group = c.up_stride;
+  const bool u_aligned = aligned16(p.up) && c.up_stride % 8 == 0;
+  p.up_form = u_aligned && p.u_s1 == 1 && p.u_s0 % 8 == 0 && p.cols % 8 == 0 ? 1
+              : u_aligned && p.u_s0 == 1 && p.u_s1 % 8 == 0 && rank % 8 == 0 ? 2
+                                                                             : 0;
+  p.out = const_cast<void *>(elem_ptr(c.out));
+  p.out_s0 = c.out->stride0;
+  p.out_s1 = c.out->stride1;
+  p.out_dtype = c.out->dtype;
+  p.alpha = c.ep.alpha;
+  p.bias = c.ep.bias;
+  p.bias_dtype = c.ep.bias_dtype;
+  p.bias_axis = c.ep.bias_axis;
+  p.activation = c.ep.activation;
+  p.rounding = c.ep.rounding;
+  p.status = h->status;
+  p.wait_limit_us = h->wait_limit_us;
+  // CTAs per column block: the share of the SMs' time that is used, units over whole
+  // waves, decides; more CTAs must gain a tenth.  Each keeps at least four K blocks.
+  const int tiles = (p.cols + 127) / 128;
+  int split = 1;
+  double best = 0.0;
+  for (int s = 1; s <= 8 && s * 4 <= std::max(4, p.num_kb); s *= 2) {
+    const long long units = static_cast<long long>(tiles) * s;
+    const long long waves = (units + h->sm_count - 1) / h->sm_count;
+    const double used = static_cast<double>(units) / (waves * h->sm_count);
+    if (used > best * 1.1) {
+      best = used;
+      split = s;
+    }
+  }
+  const int delta = (rows + split - 1) / split * 512;
+  p.stage_bytes = 16384 + p.wide * 128;
+  const int budget = 232448 - 2048 - delta;
+  p.stages = std::min(8, budget / p.stage_bytes);
+  // the ring also takes the partial sums
+  const int ring = std::max(p.stages * p.stage_bytes, p.wide * 512);
+  const int smem = 1024 + ring + delta;
+  CUtensorMap tmW, tmX;
+  TRY(make_tmap(h, &tmW, elem_ptr(c.rhs), c.rhs->dtype, unit, other, 1, ld, 0, 64, mn ? 64 : 128));
+  TRY(make_row_tmap(h, &tmX, elem_ptr(c.lhs), c.lhs->dtype, c.lhs->size1, rows,
+                    rows > 1 ? c.lhs->stride0 : (c.lhs->size1 + 7) / 8 * 8, p.wide));
+  auto kern = bf ? adapter_decode_kernel<true> : adapter_decode_kernel<false>;
+  CUDA_TRY(h, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448 - 512));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles) * split, 1, 1);
+  cfg.blockDim = dim3(192, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see adapters_sm100.cuh
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  *taken = true;
+  CUDA_TRY(h, cudaLaunchKernelEx(&cfg, kern, tmW, tmX, p));
+  return launched(h, "adapters_decode");
+}
+
+// More rows: sorted by adapter, products down on the pair kernel, then one pass over the
+// shared weights that takes the adapters' K blocks along.
+kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t stream, bool *taken) {
+  *taken = false;
+  bool w_mn, d_mn, u_mn;
+  int64_t w_unit, w_other, w_ld, d_unit, d_other, d_ld, u_unit, u_other, u_ld;
+  const int rank = c.down->size1, K = c.lhs->size1, rows = c.lhs->size0;
+  const int64_t pitch = static_cast<int64_t>(c.out->stride0) * dtype_size(c.out->dtype);
+  if (!rows_tma_ok(c.lhs) || c.out->stride1 != 1 || pitch >= kMaxRowPitch ||
+      !stack_tma_ok(c.rhs, 1, 0, w_mn, w_unit, w_other, w_ld) ||
+      !stack_tma_ok(c.down, c.groups, c.down_stride, d_mn, d_unit, d_other, d_ld) ||
+      !stack_tma_ok(c.up, c.groups, c.up_stride, u_mn, u_unit, u_other, u_ld))
+    return KAPYB_OK;
+  // the accumulator is scaled as a whole: the adapters' part is divided by alpha first,
+  // which needs an alpha that division does not push out of the 16-bit types' ranges
+  const float size = std::fabs(c.ep.alpha);
+  if (!(size >= 0.00390625f && size <= 256.0f)) return KAPYB_OK;
+  const AdapterScratch sc(rows, c.groups, rank);
+  const int n_tiles = (c.out->size1 + 255) / 256;
+  if (sc.positions >= (1ll << 30) || (sc.positions / 256 + 1) * n_tiles >= (1ll << 31)) return KAPYB_OK;
+  char *scratch = static_cast<char *>(c.scratch);
+  int32_t *order = reinterpret_cast<int32_t *>(scratch + sc.order);
+  int32_t *offsets = reinterpret_cast<int32_t *>(scratch + sc.offsets);
+  const int low_pitch = (rank + 7) / 8 * 8;
+  const int positions = static_cast<int>(sc.positions);
+
+  *taken = true;
+  TRY(launch_plan(h, PlanParams{c.index, rows, c.groups + 1, order, offsets, nullptr, positions, 32, 1}, stream));
+
+  // the rows' products with their adapter's down, in two halves
+  GroupedParams gp{};
+  gp.groups = c.groups;
+  gp.rows = positions;
+  gp.cols = rank;
+  gp.K = K;
+  gp.n_tiles = 1;
+  gp.num_kb = (K + 63) / 64;
+  gp.offsets = offsets;
+  gp.order = order;
+  gp.fan = 1;
+  gp.src_rows = rows;
+  gp.a_mn_major = d_mn;
+  gp.bf16 = c.lhs->dtype == KAPYB_BF16;
+  gp.out = scratch + sc.low;
+  gp.row_pitch = static_cast<uint32_t>(low_pitch) * 2u;
+  gp.out_dtype = c.lhs->dtype;
+  gp.pair_stores = 1;
+  gp.alpha = 1.0f / c.ep.alpha;
+  gp.bias_axis = 1;
+  gp.activation = KAPYB_ACT_NONE;
+  gp.rounding = KAPYB_RN;
+  gp.lo_bytes = static_cast<long long>(positions) * low_pitch * 2;
+  gp.group_scale = c.scale;
+  gp.status = h->status;
+  gp.wait_limit_us = h->wait_limit_us;
+  CUtensorMap tmD, tmW, tmU, tmL;
+  TRY(make_tmap(h, &tmD, elem_ptr(c.down), c.down->dtype, d_unit, d_other, c.groups, d_ld, c.down_stride, 64,
+                d_mn ? 64 : 128));
+  // narrow tiles while a wave of pairs holds them all
+  const int pairs = h->sm_count / 2;
+  int tile_rows = 64;
+  while (tile_rows < 256 && (positions + tile_rows - 1) / tile_rows > pairs) tile_rows *= 2;
+  PairParams pp = pair_params(gp, c.lhs, true, tile_rows);
+  TRY((launch_pairs<256, 1, PAIR_FORWARD>(h, tmD, tmD, tmD, tmD, pp, (positions + tile_rows - 1ll) / tile_rows + c.groups,
+                                          stream)));
+
+  gp.groups = c.groups + 1;
+  gp.cols = c.out->size1;
+  gp.n_tiles = n_tiles;
+  gp.a_mn_major = w_mn;
+  gp.out = const_cast<void *>(elem_ptr(c.out));
+  gp.row_pitch = static_cast<uint32_t>(pitch);
+  gp.out_dtype = c.out->dtype;
+  gp.pair_stores = pair_stores_ok(gp.out, c.out->dtype, c.out->stride0, 0);
+  gp.alpha = c.ep.alpha;
+  gp.bias = c.ep.bias;
+  gp.bias_dtype = c.ep.bias_dtype;
+  gp.bias_axis = c.ep.bias_axis;
+  gp.activation = c.ep.activation;
+  gp.rounding = c.ep.rounding;
+  gp.lo_bytes = 0;
+  gp.group_scale = nullptr;
+  pp = pair_params(gp, c.lhs, true, 256);
+  pp.rank = rank;
+  pp.up_mn_major = u_mn;
+  pp.low_rows = positions;
+  TRY(make_tmap(h, &tmW, elem_ptr(c.rhs), c.rhs->dtype, w_unit, w_other, 1, w_ld, 0, 64, w_mn ? 64 : 128));
+  TRY(make_tmap(h, &tmU, elem_ptr(c.up), c.up->dtype, u_unit, u_other, c.groups, u_ld, c.up_stride, 64,
+                u_mn ? 64 : 128));
+  TRY(make_row_tmap(h, &tmL, scratch + sc.low, c.lhs->dtype, rank, 2ull * positions, low_pitch, 16));
+  return launch_pairs<256, 1, PAIR_ADAPTERS>(h, tmW, tmW, tmU, tmL, pp, (positions / 256 + 1ll) * n_tiles, stream);
+}
+
 }  // namespace
 
 extern "C" KAPYB_API size_t kapyb_matmul_adapters_scratch(int32_t rows, int32_t groups, int32_t rank) {
   if (rows <= 0 || groups <= 0 || rank <= 0) return 0;
-  return static_cast<size_t>(rows) * rank * sizeof(float);
+  return AdapterScratch(rows, groups, rank).total;
 }
 
 extern "C" KAPYB_API kapyb_status kapyb_matmul_adapters(kapyb_handle h, const kapyb_tensor2d *lhs,
@@ -868,6 +1144,14 @@ extern "C" KAPYB_API kapyb_status kapyb_matmul_adapters(kapyb_handle h, const ka
     if (meet(o, i) || meet(sc, i)) return fail(h, KAPYB_INVALID_ARG, "%s: out or scratch overlaps an input", call);
   ON_DEVICE(h);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (lhs->size1 > 0) {
+    const AdapterCall c{lhs, rhs, down, up, out, groups, down_stride, up_stride, index, scale, ep, scratch};
+    bool taken = false;
+    kapyb_status st = adapters_decode(h, c, s, &taken);
+    if (st != KAPYB_OK || taken) return st;
+    if (lhs->size0 > kDecodeMaxRows) st = adapters_pairs(h, c, s, &taken);
+    if (st != KAPYB_OK || taken) return st;
+  }
   AdapterSimtParams p{};
   p.x = elem_ptr(lhs);
   p.x_s0 = lhs->stride0;

@@ -21,13 +21,16 @@ namespace kapyb {
 
 constexpr int kPlanWarps = 32;
 constexpr int kPlanBatch = 8;  // index loads in flight per lane
-constexpr int kPlanMaxGroups = 1024;
+constexpr int kPlanMaxGroups = 1024;  // and one more for the rows of no adapter
 constexpr int kPlanMaxCtas = 16;
 
 struct PlanParams {
   const int32_t *index;
   int n, groups;
   int32_t *order, *offsets, *slots;
+  int capacity;  // entries of order: n, more when groups are padded
+  int align;     // groups start at multiples of this (a power of two); the gaps are -1
+  int rest;      // 1: an index outside 0 .. groups - 2 names the last group
 };
 
 // Counters of one warp, an odd number of words so that a column of the table (one group,
@@ -71,7 +74,10 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
       }
 #pragma unroll
       for (int u = 0; u < kPlanBatch; ++u)
-        if (i0 + 32 * u < hi) step(i0 + 32 * u + lane, g[u] < 0 || g[u] >= G ? -1 : g[u]);
+        if (i0 + 32 * u < hi) {
+          const bool out = g[u] < 0 || g[u] >= G;
+          step(i0 + 32 * u + lane, !out ? g[u] : p.rest && i0 + 32 * u + lane < hi ? G - 1 : -1);
+        }
     }
   };
   const int bits = 32 - __clz(G);  // of 0 .. G, G standing for "no group"
@@ -112,7 +118,12 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
   const int per = (G + blockDim.x - 1) / blockDim.x;
   const int g0 = min(G, static_cast<int>(threadIdx.x) * per), g1 = min(G, g0 + per);
   int sum = 0;
-  for (int g = g0; g < g1; ++g) {
+  int held[2];  // entries of this thread's groups (at most two: see kPlanMaxGroups)
+  static_assert(kPlanMaxGroups + 1 <= 2 * kPlanWarps * 32, "two groups a thread");
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int g = g0 + h;
+    if (g >= g1) break;
     int all = 0, before = 0;
     for (int c = 0; c < ctas; ++c) {
       const int t = cluster.map_shared_rank(total, c)[g];
@@ -121,7 +132,8 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
     }
     first[g] = sum + before;
     if (me == 0) p.offsets[g] = sum;  // completed below
-    sum += all;
+    held[h] = all;
+    sum += (all + p.align - 1) & ~(p.align - 1);
   }
   int scan = sum;
 #pragma unroll
@@ -136,9 +148,17 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
     if (k < w) base += scan_part[k];
     planned += scan_part[k];
   }
-  for (int g = g0; g < g1; ++g) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int g = g0 + h;
+    if (g >= g1) break;
     first[g] += base;
-    if (me == 0) p.offsets[g] += base;
+    if (me == 0) {
+      const int at = p.offsets[g] + base;
+      p.offsets[g] = at;
+      const int end = at + ((held[h] + p.align - 1) & ~(p.align - 1));
+      for (int q = at + held[h]; q < end; ++q) p.order[q] = -1;
+    }
   }
   if (me == 0 && threadIdx.x == 0) p.offsets[G] = planned;
   // the others' totals have been read: nobody leaves while they still may be
@@ -155,7 +175,7 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
       if (p.slots) p.slots[i] = pos;
     }
   });
-  for (long long q = planned + static_cast<long long>(me) * blockDim.x + threadIdx.x; q < p.n;
+  for (long long q = planned + static_cast<long long>(me) * blockDim.x + threadIdx.x; q < p.capacity;
        q += static_cast<long long>(ctas) * blockDim.x)
     p.order[q] = -1;
 }
