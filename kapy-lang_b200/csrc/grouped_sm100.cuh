@@ -1160,36 +1160,37 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       const GroupedTile t = pair_tile<BT, MODE>(p, table, idx);
       const int half = t.wide >> 1;
       if constexpr (GRAD) {
-        // thread: 16-byte piece `piece` of this CTA's columns, rows row0, row0 + 16, ...
-        const int piece = tid & 15, row0 = tid >> 4;
+        // thread: 16-byte piece tid % 8 of both 64-column chunks, rows tid / 8 and + 32
+        const int piece = tid & 7, row0 = tid >> 3;
         const int col = t.r0 + rank * half + piece * 8;
-        const uint32_t bytes = static_cast<uint32_t>(max(0, min(16, (p.K - col) * 2)));
-        const bool need = piece * 8 < half;
-        const uint8_t *base = pp.lhs + static_cast<long long>(bytes ? col : 0) * 2;
+        uint32_t bytes[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) bytes[c] = static_cast<uint32_t>(max(0, min(16, (p.K - col - c * 64) * 2)));
+        const bool need[2] = {piece * 8 < half, 64 + piece * 8 < half};
+        const uint8_t *base = pp.lhs + (bytes[0] ? col * 2ll : 0ll);
+        const uint32_t next_chunk = bytes[1] ? 128u : 0u;
         // Plan entries are loaded two blocks ahead, into two sets of registers that take
         // turns, and turned into row numbers when they are needed: no block waits for
         // the load that names its rows.
-        int even[4], odd[4];
-        auto fetch = [&](int kb, int (&entry)[4]) {
+        int even[2], odd[2];
+        auto fetch = [&](int kb, int (&entry)[2]) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int q = t.p0 + kb * 64 + row0 + 16 * i;
+          for (int i = 0; i < 2; ++i) {
+            const int q = t.p0 + kb * 64 + row0 + 32 * i;
             entry[i] = q >= t.p1 ? -1 : p.order ? __ldg(p.order + q) : q;
           }
         };
-        auto copy = [&](const int (&entry)[4]) -> bool {
+        auto copy = [&](const int (&entry)[2]) -> bool {
           if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)))
             return false;
-          const uint32_t dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES) + (piece >> 3) * 8192;
-          if (need) {
+          const uint32_t dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES) + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = row0 + 16 * i;
-              const int from = entry[i] < 0 ? -1 : p.order ? pp.div_fan.div(entry[i]) : entry[i];
-              const bool live = from >= 0 && from < p.src_rows;
-              cp_async16(dst + r * 128 + (((piece & 7) ^ (r & 7)) << 4), base + (live ? from * pp.lhs_pitch : 0ll),
-                         live ? bytes : 0u);
-            }
+          for (int i = 0; i < 2; ++i) {
+            const int from = entry[i] < 0 ? -1 : p.order ? pp.div_fan.div(entry[i]) : entry[i];
+            const bool live = from >= 0 && from < p.src_rows;
+            const uint8_t *src = base + (live ? from * pp.lhs_pitch : 0ll);
+            if (need[0]) cp_async16(dst + i * 4096, src, live ? bytes[0] : 0u);
+            if (need[1]) cp_async16(dst + 8192 + i * 4096, src + next_chunk, live ? bytes[1] : 0u);
           }
           cp_async_arrive(ptx::smem_u32(&rows_bar[stage]));
           if (++stage == STAGES) {
