@@ -174,19 +174,20 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams &p, cons
   return r;
 }
 
-__device__ __forceinline__ void grouped_activation32(int activation, float (&f)[32]) {
+template <int R>
+__device__ __forceinline__ void grouped_activation(int activation, float (&f)[R]) {
   switch (activation) {
   case KAPYB_ACT_RELU:
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = apply_activation_t<KAPYB_ACT_RELU>(f[i]);
+    for (int i = 0; i < R; ++i) f[i] = apply_activation_t<KAPYB_ACT_RELU>(f[i]);
     break;
   case KAPYB_ACT_GELU_TANH:
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = apply_activation_t<KAPYB_ACT_GELU_TANH>(f[i]);
+    for (int i = 0; i < R; ++i) f[i] = apply_activation_t<KAPYB_ACT_GELU_TANH>(f[i]);
     break;
   case KAPYB_ACT_SILU:
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = apply_activation_t<KAPYB_ACT_SILU>(f[i]);
+    for (int i = 0; i < R; ++i) f[i] = apply_activation_t<KAPYB_ACT_SILU>(f[i]);
     break;
   default: break;
   }
@@ -198,27 +199,27 @@ __device__ __forceinline__ void grouped_finish32(const GroupedParams &p, float a
                                                  float bias, float bias_up) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) f[i] = f[i] * alpha + bias;
-  grouped_activation32(p.activation, f);
+  grouped_activation(p.activation, f);
   if constexpr (MSETS == 2) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) f[i] *= up[i] * alpha + bias_up;
   }
 }
 
-// 32 output rows of one column per lane -> memory.  `at` points at (first row, column
-// n), rows are `pitch` bytes apart, `left` of the 32 exist (ALL: all of them).
+// R output rows of one column per lane -> memory.  `at` points at (first row, column n),
+// rows are `pitch` bytes apart, `left` of them exist (ALL: all of them).
 // Neighbouring lanes swap half of their 16-bit values so that each stores two adjacent
 // columns of every other row as one word: half the store instructions of one value
 // each.  The common case (32 rows, 32 columns) carries no conditions and 32-bit row
 // offsets: the drain of a short main loop is bound by the instructions of this loop.
-template <int DT, int RN, bool ALL>
-__device__ __forceinline__ void store_pairs16(char *at, uint32_t pitch, const float (&f)[32], int left, int lane,
+template <int DT, int RN, bool ALL, int R>
+__device__ __forceinline__ void store_pairs16(char *at, uint32_t pitch, const float (&f)[R], int left, int lane,
                                               bool both) {
   const bool odd = lane & 1;
   char *base = odd ? at - 2 + pitch : at;  // (first row + odd, even column)
   uint32_t off = 0u;
 #pragma unroll
-  for (int j = 0; j < 32; j += 2) {
+  for (int j = 0; j < R; j += 2) {
     const float give = odd ? f[j] : f[j + 1];
     const float take = __shfl_xor_sync(0xffffffffu, give, 1);
     const uint32_t w = odd ? cvt_pack2_t<DT, RN>(take, f[j + 1]) : cvt_pack2_t<DT, RN>(f[j], take);
@@ -226,21 +227,21 @@ __device__ __forceinline__ void store_pairs16(char *at, uint32_t pitch, const fl
     off += 2u * pitch;
   }
 }
-template <int DT, int RN>
-__device__ __forceinline__ void store_single16(char *at, uint32_t pitch, const float (&f)[32], int left, bool on) {
+template <int DT, int RN, int R>
+__device__ __forceinline__ void store_single16(char *at, uint32_t pitch, const float (&f)[R], int left, bool on) {
   if (!on) return;
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
+  for (int j = 0; j < R; ++j)
     if (j < left)
       *reinterpret_cast<uint16_t *>(at + static_cast<unsigned long long>(j) * pitch) =
           static_cast<uint16_t>(cvt_pack2_t<DT, RN>(f[j], 0.0f) & 0xffffu);
 }
-template <int DT, int RN>
-__device__ __forceinline__ void store_rows16(char *at, uint32_t pitch, const float (&f)[32], int left, int lane,
+template <int DT, int RN, int R>
+__device__ __forceinline__ void store_rows16(char *at, uint32_t pitch, const float (&f)[R], int left, int lane,
                                              bool mine, bool both, bool pairs) {
   if (!pairs) {
     store_single16<DT, RN>(at, pitch, f, left, mine);
-  } else if (left >= 32 && __all_sync(0xffffffffu, both)) {
+  } else if (left >= R && __all_sync(0xffffffffu, both)) {
     store_pairs16<DT, RN, true>(at, pitch, f, left, lane, both);
   } else {
     store_pairs16<DT, RN, false>(at, pitch, f, left, lane, both);
@@ -249,20 +250,21 @@ __device__ __forceinline__ void store_rows16(char *at, uint32_t pitch, const flo
 }
 
 // p.row_pitch (bytes) is below 2^26, so 32 rows span less than 2^31.
-__device__ __forceinline__ void grouped_store32(const GroupedParams &p, char *at, const float (&f)[32], int left,
-                                                int lane, bool mine, bool both) {
+template <int R>
+__device__ __forceinline__ void grouped_store(const GroupedParams &p, char *at, const float (&f)[R], int left,
+                                              int lane, bool mine, bool both) {
   const uint32_t pitch = p.row_pitch;
   if (p.out_dtype == KAPYB_F32) {
-    if (left >= 32 && __all_sync(0xffffffffu, mine)) {
+    if (left >= R && __all_sync(0xffffffffu, mine)) {
       uint32_t off = 0u;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
+      for (int j = 0; j < R; ++j) {
         *reinterpret_cast<float *>(at + off) = f[j];
         off += pitch;
       }
     } else if (mine) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
+      for (int j = 0; j < R; ++j)
         if (j < left) *reinterpret_cast<float *>(at + static_cast<unsigned long long>(j) * pitch) = f[j];
     }
     return;
@@ -578,7 +580,7 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
           if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&tempty_bar[acc]));
         }
         grouped_finish32<MSETS>(p, p.alpha, f, u, bias, bias_up);
-        grouped_store32(p, out + static_cast<long long>(c) * p.row_pitch, f, t.rows - c, lane, mine, both);
+        grouped_store(p, out + static_cast<long long>(c) * p.row_pitch, f, t.rows - c, lane, mine, both);
       }
       if (!warp_has) {
         ptx::tc_fence_before();
@@ -642,7 +644,13 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 // halves, so the second factor is exact to 16 bits and more.  Nothing is added twice to
 // memory and one rounding remains; what a broken adapter produces stays in its own rows.
 
-enum PairMode { PAIR_FORWARD = 0, PAIR_GRADIENT = 1, PAIR_ADAPTERS = 2 };
+// Gated products: the 128 columns a CTA holds are 64 gate columns and the 64 up columns
+// that go with them, so the tile keeps its 256-wide MMA (two sets of columns beside one
+// another would take two 128-wide ones and a quarter more operand bytes).  Gate and up
+// of one output then sit 64 TMEM lanes apart, in two epilogue warps: they swap half of a
+// chunk's rows through shared memory and each finishes 16.
+
+enum PairMode { PAIR_FORWARD = 0, PAIR_GRADIENT = 1, PAIR_ADAPTERS = 2, PAIR_GATED = 3 };
 
 struct PairParams {
   GroupedParams g;
@@ -658,20 +666,19 @@ struct PairParams {
 
 constexpr int kPairThreads = 192 + 256 + 32;
 
-template <int BT, int MSETS>
 struct PairCfg {
-  static constexpr int A_BYTES = MSETS * 128 * 128;  // per CTA
-  static constexpr int B_BYTES = BT / 2 * 128;       // per CTA: half of the tile's rows
+  static constexpr int BT = 256;             // rows of a tile
+  static constexpr int A_BYTES = 128 * 128;  // per CTA: 128 columns x 64 of the contraction
+  static constexpr int B_BYTES = BT / 2 * 128;  // per CTA: half of the tile's rows
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int CTRL_BYTES = 1024;
   static constexpr int TABLE_BYTES = (3 * kGroupedMaxGroups + 8) * 4;
+  static constexpr int SWAP_BYTES = 2 * 2 * 2 * 16 * 32 * 4;  // warp pairs, buffers, directions x 16 rows x 32 lanes
   static constexpr int SMEM_LIMIT = 232448;
-  static constexpr int STAGES_RAW = (SMEM_LIMIT - 1024 - CTRL_BYTES - TABLE_BYTES) / STAGE_BYTES;
-  static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + CTRL_BYTES + TABLE_BYTES;
-  static constexpr int SLOT_COLS = BT * MSETS;
-  static constexpr int TMEM_COLS = 2 * SLOT_COLS;
-  static_assert(TMEM_COLS == 512 && BT % 64 == 0 && STAGES >= 3, "tile");
+  static constexpr int STAGES = (SMEM_LIMIT - 1024 - CTRL_BYTES - TABLE_BYTES - SWAP_BYTES) / STAGE_BYTES;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + CTRL_BYTES + TABLE_BYTES + SWAP_BYTES;
+  static constexpr int TMEM_COLS = 2 * BT;   // two accumulator slots
+  static_assert(STAGES >= 4, "pipeline too shallow");
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
@@ -693,17 +700,19 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void *tmap,
 
 __device__ __forceinline__ int round32(int v) { return (v + 31) & ~31; }
 
-// The tile of a pair: as grouped_tile, for blocks of 256 columns, rows rounded to 32
-// (the N side of a pair's MMA is a multiple of 32).
-template <int BT, int MODE>
+// The tile of a pair: as grouped_tile, for blocks of 256 columns (128 gated ones), rows
+// rounded to 32 (the N side of a pair's MMA is a multiple of 32).
+template <int MODE>
 __device__ __forceinline__ GroupedTile pair_tile(const GroupedParams &p, const GroupedTable &t, int idx) {
+  constexpr int BT = PairCfg::BT;
+  constexpr int COLS = MODE == PAIR_GATED ? 128 : 256;  // output columns of a tile
   GroupedTile r;
   if constexpr (MODE == PAIR_ADAPTERS) {
     const int all = t.begin[p.groups];  // positions, gaps included
     int m, n;
     raster(idx, (all + BT - 1) / BT, p.n_tiles, m, n);
     r.g = 0;
-    r.n0 = n * 256;
+    r.n0 = n * COLS;
     r.r0 = m * BT;
     r.rows = min(BT, all - r.r0);
     r.num_kb = p.num_kb;
@@ -714,7 +723,7 @@ __device__ __forceinline__ GroupedTile pair_tile(const GroupedParams &p, const G
     const int in = idx - r.g * per;
     const int n = in / p.k_tiles;
     r.r0 = (in - n * p.k_tiles) * BT;
-    r.n0 = n * 256;
+    r.n0 = n * COLS;
     r.rows = min(BT, p.K - r.r0);
     r.p0 = t.begin[r.g];
     r.p1 = r.p0 + t.count[r.g];
@@ -734,7 +743,7 @@ __device__ __forceinline__ GroupedTile pair_tile(const GroupedParams &p, const G
     raster(in, tiles, p.n_tiles, m, n);
     const int cnt = t.count[lo];
     const int each = round32((cnt + tiles - 1) / tiles);
-    r.n0 = n * 256;
+    r.n0 = n * COLS;
     r.r0 = t.begin[lo] + m * each;
     r.rows = min(each, cnt - m * each);
     r.num_kb = p.num_kb;
@@ -765,14 +774,14 @@ __device__ __forceinline__ bool each_adapter(const GroupedTable &t, int adapters
 // tmA8 and tmA1 the same in boxes 8 rows and 1 row high.  Forward without a gather: lhs
 // in boxes of 64 x 32 (tmB) and 64 x BT / 2 (tmA8).  Adapters: tmA8 up, 3-D as rhs, tmA1
 // the low-rank products, both halves behind one another, in boxes of 64 x 16.
-template <int BT, int MSETS, int MODE>
+template <int MODE>
 __global__ void __launch_bounds__(kPairThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmA8, const __grid_constant__ CUtensorMap tmA1,
                     const PairParams pp) {
-  using Cfg = PairCfg<BT, MSETS>;
-  constexpr int STAGES = Cfg::STAGES;
-  constexpr bool GRAD = MODE == PAIR_GRADIENT, ADAPT = MODE == PAIR_ADAPTERS;
+  using Cfg = PairCfg;
+  constexpr int STAGES = Cfg::STAGES, BT = Cfg::BT;
+  constexpr bool GRAD = MODE == PAIR_GRADIENT, ADAPT = MODE == PAIR_ADAPTERS, GATED = MODE == PAIR_GATED;
   const GroupedParams &p = pp.g;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -782,10 +791,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   uint64_t *bars = reinterpret_cast<uint64_t *>(sB + STAGES * Cfg::B_BYTES);
   uint64_t *full_bar = bars, *empty_bar = bars + STAGES, *tfull_bar = bars + 2 * STAGES, *tempty_bar = tfull_bar + 2;
   uint64_t *rows_bar = tempty_bar + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(rows_bar + STAGES);
+  uint64_t *swap_bar = rows_bar + STAGES;  // [warp pair][buffer]
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(swap_bar + 4);
   volatile uint32_t *abort_flag = tmem_slot + 1;  // two words
   int *table_mem = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(bars) + Cfg::CTRL_BYTES);
   GroupedTable table{table_mem, table_mem + kGroupedMaxGroups + 2, table_mem + 2 * kGroupedMaxGroups + 4};
+
+  float *swap_mem = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(table_mem) + Cfg::TABLE_BYTES);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
@@ -803,6 +815,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       ptx::mbar_init(ptx::smem_u32(&tfull_bar[a]), 1);
       ptx::mbar_init(ptx::smem_u32(&tempty_bar[a]), 8);  // four epilogue warps of each CTA
     }
+    for (int i = 0; i < 4; ++i) ptx::mbar_init(ptx::smem_u32(&swap_bar[i]), 2);  // both warps
     abort_flag[0] = 0u;
     abort_flag[1] = p.wait_limit_us;
     ptx::fence_barrier_init();
@@ -881,13 +894,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     uint32_t phase = 0;
     bool ok = true;
     for (int idx = unit; ok && idx < total; idx += units) {
-      const GroupedTile t = pair_tile<BT, MODE>(p, table, idx);
+      const GroupedTile t = pair_tile<MODE>(p, table, idx);
       const int half = t.wide >> 1;                         // rows this CTA fetches
       // rows in plan order: one tall box, or boxes of 32 rows where it would fetch too much
       const bool tall = half > BT / 2 - 32;
       const int boxes = gather ? 0 : tall ? 1 : (half + 31) >> 5;
       const uint32_t b_bytes = gather ? 0u : tall ? static_cast<uint32_t>(Cfg::B_BYTES) : boxes * 4096u;
-      const int n0 = t.n0 + rank * 128;
+      const int n0 = t.n0 + rank * (GATED ? 64 : 128);
+      const int second = GATED ? p.cols : 64;  // from the first 64 columns to the other 64
       for (int kb = 0; kb < t.num_kb; ++kb) {
         const bool got = ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag);
         if (!__all_sync(0xffffffffu, got)) {
@@ -919,10 +933,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         } else {
           const int k0 = kb * 64;
           if (p.a_mn_major) {
-            if (lane < 2 * MSETS)
-              ptx::tma_load_3d_pair(a_dst + lane * 8192, &tmA, fb, n0 + (lane & 1) * 64 + (lane >> 1) * p.cols, k0, t.g);
+            if (lane < 2) ptx::tma_load_3d_pair(a_dst + lane * 8192, &tmA, fb, n0 + lane * second, k0, t.g);
+          } else if (GATED) {
+            if (lane < 2) ptx::tma_load_3d_pair(a_dst + lane * 8192, &tmA, fb, k0, n0 + lane * second, t.g);
           } else {
-            if (lane < MSETS) ptx::tma_load_3d_pair(a_dst + lane * 16384, &tmA, fb, k0, n0 + lane * p.cols, t.g);
+            if (lane == 0) ptx::tma_load_3d_pair(a_dst, &tmA, fb, k0, n0, t.g);
           }
           if (tall) {
             if (boxes && lane == 0) tma_load_2d_pair(b_dst, &tmA8, fb, k0, t.r0 + rank * half);
@@ -981,11 +996,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
     for (int idx = unit; ok && idx < total; idx += units) {
-      const GroupedTile t = pair_tile<BT, MODE>(p, table, idx);
+      const GroupedTile t = pair_tile<MODE>(p, table, idx);
       const uint32_t idesc = ptx::make_idesc_f16(p.bf16, a_mn, b_mn, 256, t.wide);
       if (!wait_all(ptx::smem_u32(&tempty_bar[acc]), acc_phase ^ 1u)) break;
       ptx::tc_fence_after();
-      const uint32_t d = tmem_base + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
+      const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BT);
       for (int kb = 0; kb < t.num_kb; ++kb) {
         if (!wait_all(ptx::smem_u32(&full_bar[stage]), phase)) {
           ok = false;
@@ -997,12 +1012,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           const uint32_t b_lo = b_lo0 + static_cast<uint32_t>(stage) * (Cfg::B_BYTES >> 4);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
+            const uint64_t ad = (static_cast<uint64_t>(hi) << 32) | (a_lo + k * a_step);
             const uint64_t bd = (static_cast<uint64_t>(hi) << 32) | (b_lo + k * b_step);
-#pragma unroll
-            for (int s = 0; s < MSETS; ++s) {
-              const uint64_t ad = (static_cast<uint64_t>(hi) << 32) | (a_lo + s * (16384u >> 4) + k * a_step);
-              ptx::umma_k<2, 0>(d + s * BT, ad, bd, idesc, (kb | k) != 0 ? 1u : 0u);
-            }
+            ptx::umma_k<2, 0>(d, ad, bd, idesc, (kb | k) != 0 ? 1u : 0u);
           }
           ptx::umma_commit<2>(ptx::smem_u32(&empty_bar[stage]));
           ptx::umma_commit<2>(ptx::mapa(ptx::smem_u32(&empty_bar[stage]), 1));
@@ -1052,39 +1064,33 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const int q = warp & 3;
     int acc = 0;
     uint32_t acc_phase = 0;
+    uint32_t swaps = 0;  // gated: exchanges so far
+    bool alive = true;
+    (void)swaps;
     for (int idx = unit; idx < total; idx += units) {
-      const GroupedTile t = pair_tile<BT, MODE>(p, table, idx);
-      const int warp_n = t.n0 + rank * 128 + q * 32;
+      const GroupedTile t = pair_tile<MODE>(p, table, idx);
+      const int warp_n = GATED ? t.n0 + rank * 64 + (q & 1) * 32 : t.n0 + rank * 128 + q * 32;
       const int n = warp_n + lane;
       const bool mine = n < p.cols, both = (n | 1) < p.cols;
-      float bias = 0.0f, bias_up = 0.0f;
+      float bias = 0.0f;  // gated: of this warp's side
       if (p.bias != nullptr && mine && (!ADAPT || p.bias_axis == 1)) {
         const long long at = (ADAPT ? 0ll : static_cast<long long>(t.g) * p.bias_cols) + n;
-        bias = load_as_f32(p.bias, p.bias_dtype, at);
-        if constexpr (MSETS == 2) bias_up = load_as_f32(p.bias, p.bias_dtype, at + p.cols);
+        bias = load_as_f32(p.bias, p.bias_dtype, GATED && q >= 2 ? at + p.cols : at);
       }
       const float alpha = !ADAPT && p.group_scale != nullptr ? p.alpha * p.group_scale[t.g] : p.alpha;
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc]), acc_phase, abort_flag))) break;
       ptx::tc_fence_after();
-      const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
+      const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BT);
       const uint32_t tempty = leader(&tempty_bar[acc]);
       const bool warp_has = warp_n < p.cols;
       char *out = static_cast<char *>(p.out) + (GRAD ? t.g * p.group_bytes : 0ll) +
                   static_cast<long long>(t.r0) * p.row_pitch + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll);
       for (int c = 0; c < t.rows && warp_has; c += 32) {
-        float f[32], u[MSETS == 2 ? 32 : 1];
+        float f[32];
         if (!GRAD || t.num_kb > 0) {
           uint32_t v[32];
           ptx::tmem_ld_32x32(src + c, v);
-          if constexpr (MSETS == 2) {
-            uint32_t w[32];
-            ptx::tmem_ld_32x32(src + BT + c, w);
-            ptx::tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(w[i]);
-          } else {
-            ptx::tmem_ld_wait();
-          }
+          ptx::tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
         } else {
@@ -1104,23 +1110,53 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             const float row_bias = to >= 0 ? load_as_f32(p.bias, p.bias_dtype, to) : 0.0f;
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] = f[j] * alpha + __shfl_sync(0xffffffffu, row_bias, j);
-            grouped_activation32(p.activation, f);
+            grouped_activation(p.activation, f);
           } else {
             grouped_finish32<1>(p, alpha, f, nullptr, bias, 0.0f);
           }
           grouped_scatter32(p, static_cast<char *>(p.out) + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll), f, to, lane,
                             mine, both);
+        } else if constexpr (GATED) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = f[j] * alpha + bias;
+          // the gate's warp hands over its rows 16 .. 31 and finishes 0 .. 15, the up
+          // columns' warp the other way round; two buffers take turns
+          const bool up_side = q >= 2;
+          float *box = swap_mem + ((q & 1) * 2 + (swaps & 1)) * 1024;
+          float g[16], u[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) (up_side ? box : box + 512)[j * 32 + lane] = up_side ? f[j] : f[16 + j];
+          __syncwarp();
+          const uint32_t bar = ptx::smem_u32(&swap_bar[(q & 1) * 2 + (swaps & 1)]);
+          if (lane == 0) ptx::mbar_arrive(bar);
+          if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar, (swaps >> 1) & 1, abort_flag))) {
+            alive = false;
+            break;
+          }
+          ++swaps;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float other = (up_side ? box + 512 : box)[j * 32 + lane];
+            g[j] = up_side ? other : f[j];
+            u[j] = up_side ? f[16 + j] : other;
+          }
+          grouped_activation(p.activation, g);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) g[j] *= u[j];
+          const int first = c + (up_side ? 16 : 0);
+          grouped_store(p, out + static_cast<long long>(first) * p.row_pitch, g, t.rows - first, lane, mine, both);
         } else {
-          grouped_finish32<MSETS>(p, alpha, f, u, bias, bias_up);
+          grouped_finish32<1>(p, alpha, f, nullptr, bias, 0.0f);
           char *at = out + static_cast<long long>(c) * p.row_pitch;
-          grouped_store32(p, at, f, t.rows - c, lane, mine, both);
-          if (MODE == PAIR_FORWARD && MSETS == 1 && p.lo_bytes != 0) {
+          grouped_store(p, at, f, t.rows - c, lane, mine, both);
+          if (MODE == PAIR_FORWARD && p.lo_bytes != 0) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] -= cvt_16_to_f32(cvt_f32_to_16(f[j], p.out_dtype, 1), p.out_dtype);
-            grouped_store32(p, at + p.lo_bytes, f, t.rows - c, lane, mine, both);
+            grouped_store(p, at + p.lo_bytes, f, t.rows - c, lane, mine, both);
           }
         }
       }
+      if (!alive) break;
       if (!warp_has) {
         ptx::tc_fence_before();
         __syncwarp();
@@ -1135,7 +1171,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     uint32_t phase = 0;
     bool ok = true;
     for (int idx = unit; ok && idx < total; idx += units) {
-      const GroupedTile t = pair_tile<BT, MODE>(p, table, idx);
+      const GroupedTile t = pair_tile<MODE>(p, table, idx);
       const int blocks = t.num_kb + extra(t);
       for (int kb = 0; kb < blocks; ++kb) {
         if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&rows_bar[stage]), phase, abort_flag))) {
@@ -1157,7 +1193,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     uint32_t phase = 0;
     bool ok = true;
     for (int idx = unit; ok && idx < total; idx += units) {
-      const GroupedTile t = pair_tile<BT, MODE>(p, table, idx);
+      const GroupedTile t = pair_tile<MODE>(p, table, idx);
       const int half = t.wide >> 1;
       if constexpr (GRAD) {
         // thread: 16-byte piece tid % 8 of both 64-column chunks, rows tid / 8 and + 32

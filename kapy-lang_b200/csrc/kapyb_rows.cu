@@ -378,11 +378,11 @@ PairParams pair_params(const GroupedParams &gp, const kapyb_tensor2d *lhs, bool 
 
 // The pair kernel: `tiles` pairs of CTAs at most, as many as the device holds at once
 // (the tile loop is statically strided).
-template <int BT, int MSETS, int MODE>
+template <int MODE>
 kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmA8,
                           const CUtensorMap &tmA1, const PairParams &pp, long long tiles, cudaStream_t stream) {
-  using Cfg = PairCfg<BT, MSETS>;
-  auto kern = grouped_pair_kernel<BT, MSETS, MODE>;
+  using Cfg = PairCfg;
+  auto kern = grouped_pair_kernel<MODE>;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.blockDim = dim3(kPairThreads, 1, 1);
@@ -460,12 +460,13 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
   gp.wait_limit_us = h->wait_limit_us;
   const long long busy = std::min(groups, gp.rows);
   const bool narrow = gp.rows <= 32 * busy;  // rows per group that has any, at most
-  const int bt = narrow ? 64 : gated ? 128 : 256;
-  if (!narrow) gp.n_tiles = (gp.cols + 255) / 256;
+  const int bt = narrow ? 64 : PairCfg::BT;
+  if (!narrow) gp.n_tiles = gated ? (gp.cols + 127) / 128 : (gp.cols + 255) / 256;
   const long long tiles = ((gp.rows + bt - 1ll) / bt + busy) * gp.n_tiles;
   if (tiles >= (1ll << 31)) return KAPYB_OK;
   CUtensorMap tmA, tmB;
-  TRY(make_tmap(h, &tmA, elem_ptr(rhs), rhs->dtype, unit, other, groups, ld, group_stride, 64, mn ? 64 : 128));
+  TRY(make_tmap(h, &tmA, elem_ptr(rhs), rhs->dtype, unit, other, groups, ld, group_stride, 64,
+                mn || (gated && !narrow) ? 64 : 128));
   TRY(make_row_tmap(h, &tmB, elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
                     lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, order && narrow ? 1 : 32));
   *taken = true;
@@ -476,8 +477,8 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
   CUtensorMap tall;
   TRY(make_row_tmap(h, &tall, elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
                     lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, bt / 2));
-  return gated ? launch_pairs<128, 2, PAIR_FORWARD>(h, tmA, tmB, tall, tmA, pp, tiles, stream)
-               : launch_pairs<256, 1, PAIR_FORWARD>(h, tmA, tmB, tall, tmA, pp, tiles, stream);
+  return gated ? launch_pairs<PAIR_GATED>(h, tmA, tmB, tall, tmA, pp, tiles, stream)
+               : launch_pairs<PAIR_FORWARD>(h, tmA, tmB, tall, tmA, pp, tiles, stream);
 }
 
 kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const kapyb_tensor2d *grad,
@@ -519,7 +520,7 @@ kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, 
   TRY(make_row_tmap(h, &tmA1, elem_ptr(grad), grad->dtype, grad->size1, grad->size0, ld, 1));
   *taken = true;
   const PairParams pp = pair_params(gp, lhs, true, 256);
-  return launch_pairs<256, 1, PAIR_GRADIENT>(h, tmA, tmA, tmA8, tmA1, pp, tiles, stream);
+  return launch_pairs<PAIR_GRADIENT>(h, tmA, tmA, tmA8, tmA1, pp, tiles, stream);
 }
 
 // What the two grouped products check alike.
@@ -1052,7 +1053,7 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
   int tile_rows = 64;
   while (tile_rows < 256 && (positions + tile_rows - 1) / tile_rows > pairs) tile_rows *= 2;
   PairParams pp = pair_params(gp, c.lhs, true, tile_rows);
-  TRY((launch_pairs<256, 1, PAIR_FORWARD>(h, tmD, tmD, tmD, tmD, pp, (positions + tile_rows - 1ll) / tile_rows + c.groups,
+  TRY((launch_pairs<PAIR_FORWARD>(h, tmD, tmD, tmD, tmD, pp, (positions + tile_rows - 1ll) / tile_rows + c.groups,
                                           stream)));
 
   gp.groups = c.groups + 1;
@@ -1079,7 +1080,7 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
   TRY(make_tmap(h, &tmU, elem_ptr(c.up), c.up->dtype, u_unit, u_other, c.groups, u_ld, c.up_stride, 64,
                 u_mn ? 64 : 128));
   TRY(make_row_tmap(h, &tmL, scratch + sc.low, c.lhs->dtype, rank, 2ull * positions, low_pitch, 16));
-  return launch_pairs<256, 1, PAIR_ADAPTERS>(h, tmW, tmW, tmU, tmL, pp, (positions / 256 + 1ll) * n_tiles, stream);
+  return launch_pairs<PAIR_ADAPTERS>(h, tmW, tmW, tmU, tmL, pp, (positions / 256 + 1ll) * n_tiles, stream);
 }
 
 }  // namespace
