@@ -629,12 +629,11 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 // itself carries the default semantics.  (With a release at cluster scope it waited for
 // all copies in flight, 1 to 1.5 us a stage, three times the whole kernel's time.)  Four
 // warps fetch 16 KB a stage in 1070 clocks, twice the MMA's time for it (8192 x 4096 x
-// 4096 as one group: 259 us); eight keep up with it (193 us, rows in plan order 183).
+// 4096 as one group: 259 us); eight nearly keep up.
 //
 // In the gradient the rows are the contraction: lhs is always gathered (zeros behind
-// the group's end), grad lies in plan order and comes by TMA, whole 64-row boxes while
-// they last and then 8-row and 1-row boxes, so that what is behind the end is fetched
-// as zeros as well.
+// the group's end); grad lies in plan order and comes by TMA, but for the block that
+// holds the group's end, which the gathering warps bring as well, with zeros behind it.
 
 // Adapters: the rows are a plan sorted by adapter whose groups start at multiples of 32
 // (gaps and rows without an adapter included), and the tile's main loop over the shared
@@ -657,6 +656,8 @@ struct PairParams {
   int gather;            // rows of lhs by cp.async: a plan's order, and always the gradient
   const uint8_t *lhs;    // element (0, 0)
   long long lhs_pitch;   // bytes between rows
+  const uint8_t *grad;   // gradient: the same of grad
+  long long grad_pitch;
   FastDiv div_fan;
   int tile_rows;         // forward: most rows of a tile, at most BT and a multiple of 32
   // adapters: g.groups = adapters + 1 (the last group: rows without one)
@@ -770,14 +771,14 @@ __device__ __forceinline__ bool each_adapter(const GroupedTable &t, int adapters
   return true;
 }
 
-// tmA: forward: rhs as in grouped_tcgen05_kernel; gradient: grad in boxes of 64 x 64,
-// tmA8 and tmA1 the same in boxes 8 rows and 1 row high.  Forward without a gather: lhs
-// in boxes of 64 x 32 (tmB) and 64 x BT / 2 (tmA8).  Adapters: tmA8 up, 3-D as rhs, tmA1
-// the low-rank products, both halves behind one another, in boxes of 64 x 16.
+// tmA: forward: rhs as in grouped_tcgen05_kernel; gradient: grad in boxes of 64 x 64.
+// Rows that come by TMA: lhs in plan order in boxes of 64 x 128 (tmB), 64 x 64 (tmR) and
+// 64 x 32 (tmU); adapters: the low-rank products, both halves behind one another, in boxes
+// of 64 x 128 (tmB) and 64 x 16 (tmR), and tmU up, 3-D as rhs.
 template <int MODE>
 __global__ void __launch_bounds__(kPairThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                    const __grid_constant__ CUtensorMap tmA8, const __grid_constant__ CUtensorMap tmA1,
+                    const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmU,
                     const PairParams pp) {
   using Cfg = PairCfg;
   constexpr int STAGES = Cfg::STAGES, BT = Cfg::BT;
@@ -806,9 +807,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const bool gather = GRAD || ADAPT || pp.gather;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      // the leader's expect_tx, and with a gather one arrival from each CTA
-      ptx::mbar_init(ptx::smem_u32(&full_bar[s]), gather ? 3 : 1);
-      ptx::mbar_init(ptx::smem_u32(&rows_bar[s]), 256);  // every gathering thread
+      // the columns' expect_tx in the leader, and the rows': another one there, or with a
+      // gather one arrival from each CTA
+      ptx::mbar_init(ptx::smem_u32(&full_bar[s]), gather ? 3 : 2);
+      ptx::mbar_init(ptx::smem_u32(&rows_bar[s]), 128);  // every thread of a gathering team
       ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -886,99 +888,119 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       });
     return n;
   };
+  const uint32_t full0 = ptx::mapa(ptx::smem_u32(full_bar), 0);  // the leader's barriers
   auto leader = [](const void *bar) { return ptx::mapa(ptx::smem_u32(bar), 0); };
 
   if (warp == 0) {
-    // ------------------------------------- TMA: the columns' side, and rows in plan order
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int idx = unit; ok && idx < total; idx += units) {
-      const GroupedTile t = pair_tile<MODE>(p, table, idx);
-      const int half = t.wide >> 1;                         // rows this CTA fetches
-      // rows in plan order: one tall box, or boxes of 32 rows where it would fetch too much
-      const bool tall = half > BT / 2 - 32;
-      const int boxes = gather ? 0 : tall ? 1 : (half + 31) >> 5;
-      const uint32_t b_bytes = gather ? 0u : tall ? static_cast<uint32_t>(Cfg::B_BYTES) : boxes * 4096u;
-      const int n0 = t.n0 + rank * (GATED ? 64 : 128);
-      const int second = GATED ? p.cols : 64;  // from the first 64 columns to the other 64
-      for (int kb = 0; kb < t.num_kb; ++kb) {
-        const bool got = ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag);
-        if (!__all_sync(0xffffffffu, got)) {
-          ok = false;
-          break;
+    // -------------------------------------------------- TMA: the columns' side
+    // One lane walks the loop: a load issued by several lanes at once is serialised with
+    // its operands moved to uniform registers lane by lane, some 150 clocks each, and at
+    // 512 clocks of MMA a stage this role's own time is what the pipeline waits for.
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      // a free stage, its barrier told to expect `bytes` from both CTAs together
+      auto open = [&](uint32_t bytes) -> bool {
+        if (!ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) return false;
+        if (rank == 0) {
+          if (bytes) ptx::mbar_arrive_expect_tx(ptx::smem_u32(&full_bar[stage]), bytes);
+          else ptx::mbar_arrive(ptx::smem_u32(&full_bar[stage]));
         }
-        const uint32_t fb = leader(&full_bar[stage]);
-        const uint32_t a_dst = ptx::smem_u32(sA + stage * Cfg::A_BYTES);
-        const uint32_t b_dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES);
-        if (rank == 0 && lane == 0)
-          ptx::mbar_arrive_expect_tx(ptx::smem_u32(&full_bar[stage]), 2u * (Cfg::A_BYTES + b_bytes));
-        __syncwarp();
-        if constexpr (GRAD) {
-          const int q = t.p0 + kb * 64;
-          const int live = t.p1 - q;  // positions of this block that are the group's
-          if (live >= 64) {
-            if (lane < 2) tma_load_2d_pair(a_dst + lane * 8192, &tmA, fb, n0 + lane * 64, q);
-          } else if (lane < 16) {
-            // eight rows per lane: all of the group, none of it, or the border
-            const int c = lane >> 3, r = (lane & 7) * 8;
-            const uint32_t dst = a_dst + c * 8192 + r * 128;
-            if (r + 8 <= live || r >= live) {
-              tma_load_2d_pair(dst, &tmA8, fb, n0 + c * 64, r < live ? q + r : p.rows);
-            } else {
-              for (int j = 0; j < 8; ++j)
-                tma_load_2d_pair(dst + j * 128, &tmA1, fb, n0 + c * 64, r + j < live ? q + r + j : p.rows);
-            }
-          }
-        } else {
-          const int k0 = kb * 64;
-          if (p.a_mn_major) {
-            if (lane < 2) ptx::tma_load_3d_pair(a_dst + lane * 8192, &tmA, fb, n0 + lane * second, k0, t.g);
-          } else if (GATED) {
-            if (lane < 2) ptx::tma_load_3d_pair(a_dst + lane * 8192, &tmA, fb, k0, n0 + lane * second, t.g);
-          } else {
-            if (lane == 0) ptx::tma_load_3d_pair(a_dst, &tmA, fb, k0, n0, t.g);
-          }
-          if (tall) {
-            if (boxes && lane == 0) tma_load_2d_pair(b_dst, &tmA8, fb, k0, t.r0 + rank * half);
-          } else if (lane < boxes) {
-            tma_load_2d_pair(b_dst + lane * 4096, &tmB, fb, k0, t.r0 + rank * half + lane * 32);
-          }
-        }
+        return true;
+      };
+      auto advance = [&]() {
         if (++stage == STAGES) {
           stage = 0;
           phase ^= 1u;
         }
-      }
-      if constexpr (ADAPT) {
-        if (!ok) break;
-        ok = each_adapter(table, p.groups - 1, t.r0, t.r0 + t.rows, [&](int g, int s0, int s1) {
-          const int mine = (s1 - s0) >> 1;  // rows this CTA fetches: a multiple of 16
-          for (int b = 0; b < 2 * low_blocks; ++b) {
-            const bool got = ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag);
-            if (!__all_sync(0xffffffffu, got)) return false;
-            const uint32_t fb = leader(&full_bar[stage]);
-            const uint32_t a_dst = ptx::smem_u32(sA + stage * Cfg::A_BYTES);
-            const uint32_t b_dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES);
-            if (rank == 0 && lane == 0)
-              ptx::mbar_arrive_expect_tx(ptx::smem_u32(&full_bar[stage]), 2u * (Cfg::A_BYTES + mine * 128u));
-            __syncwarp();
-            const int k0 = (b >> 1) * 64;
-            if (pp.up_mn_major) {
-              if (lane < 2) ptx::tma_load_3d_pair(a_dst + lane * 8192, &tmA8, fb, n0 + lane * 64, k0, g);
-            } else {
-              if (lane == 0) ptx::tma_load_3d_pair(a_dst, &tmA8, fb, k0, n0, g);
-            }
-            if (lane < (mine >> 4))
-              tma_load_2d_pair(b_dst + lane * 2048, &tmA1, fb, k0,
-                               (b & 1) * pp.low_rows + s0 + rank * mine + lane * 16);
-            if (++stage == STAGES) {
-              stage = 0;
-              phase ^= 1u;
-            }
+      };
+      for (int idx = unit; ok && idx < total; idx += units) {
+        const GroupedTile t = pair_tile<MODE>(p, table, idx);
+        const int n0 = t.n0 + rank * (GATED ? 64 : 128);
+        const int second = GATED ? p.cols : 64;  // from the first 64 columns to the other 64
+        for (int kb = 0; kb < t.num_kb; ++kb) {
+          const int q = t.p0 + kb * 64;
+          const bool tail = GRAD && t.p1 - q < 64;  // the gathering warps bring grad's rows as well
+          if (!open(tail ? 0u : 2u * Cfg::A_BYTES)) {
+            ok = false;
+            break;
           }
-          return true;
-        });
+          const uint32_t fb = full0 + stage * 8u;
+          const uint32_t a_dst = ptx::smem_u32(sA) + stage * Cfg::A_BYTES;
+          if constexpr (GRAD) {
+            if (!tail) {
+              tma_load_2d_pair(a_dst, &tmA, fb, n0, q);
+              tma_load_2d_pair(a_dst + 8192, &tmA, fb, n0 + 64, q);
+            }
+          } else if (p.a_mn_major) {
+            ptx::tma_load_3d_pair(a_dst, &tmA, fb, n0, kb * 64, t.g);
+            ptx::tma_load_3d_pair(a_dst + 8192, &tmA, fb, n0 + second, kb * 64, t.g);
+          } else if (GATED) {
+            ptx::tma_load_3d_pair(a_dst, &tmA, fb, kb * 64, n0, t.g);
+            ptx::tma_load_3d_pair(a_dst + 8192, &tmA, fb, kb * 64, n0 + second, t.g);
+          } else {
+            ptx::tma_load_3d_pair(a_dst, &tmA, fb, kb * 64, n0, t.g);
+          }
+          advance();
+        }
+        if constexpr (ADAPT) {
+          if (!ok) break;
+          ok = each_adapter(table, p.groups - 1, t.r0, t.r0 + t.rows, [&](int g, int s0, int s1) {
+            const int mine = (s1 - s0) >> 1;  // rows this CTA fetches: a multiple of 16
+            for (int b = 0; b < 2 * low_blocks; ++b) {
+              if (!open(2u * (Cfg::A_BYTES + mine * 128u))) return false;
+              const uint32_t fb = full0 + stage * 8u;
+              const uint32_t a_dst = ptx::smem_u32(sA) + stage * Cfg::A_BYTES;
+              const uint32_t b_dst = ptx::smem_u32(sB) + stage * Cfg::B_BYTES;
+              const int k0 = (b >> 1) * 64, y = (b & 1) * pp.low_rows + s0 + rank * mine;
+              if (pp.up_mn_major) {
+                ptx::tma_load_3d_pair(a_dst, &tmU, fb, n0, k0, g);
+                ptx::tma_load_3d_pair(a_dst + 8192, &tmU, fb, n0 + 64, k0, g);
+              } else {
+                ptx::tma_load_3d_pair(a_dst, &tmU, fb, k0, n0, g);
+              }
+              if (mine == BT / 2) {
+                tma_load_2d_pair(b_dst, &tmB, fb, k0, y);
+              } else {
+                for (int r = 0; r < mine; r += 16) tma_load_2d_pair(b_dst + r * 128, &tmR, fb, k0, y + r);
+              }
+              advance();
+            }
+            return true;
+          });
+        }
+      }
+    }
+  } else if (warp == 6 && !gather) {
+    // ------------------------------------------- TMA: rows that lie in plan order
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int idx = unit; ok && idx < total; idx += units) {
+        const GroupedTile t = pair_tile<MODE>(p, table, idx);
+        const int half = t.wide >> 1;  // rows this CTA fetches
+        // one box of 128, 64 or 32 rows, the first that holds them: a load costs its
+        // issuing lane more than the rows too many cost
+        const int height = half > 64 ? 128 : half > 32 ? 64 : 32;
+        const int y = t.r0 + rank * half;
+        for (int kb = 0; kb < t.num_kb; ++kb) {
+          if (!ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) ptx::mbar_arrive_expect_tx(ptx::smem_u32(&full_bar[stage]), 2u * height * 128u);
+          const uint32_t fb = full0 + stage * 8u;
+          const uint32_t b_dst = ptx::smem_u32(sB) + stage * Cfg::B_BYTES;
+          if (height == 128) tma_load_2d_pair(b_dst, &tmB, fb, kb * 64, y);
+          else if (height == 64) tma_load_2d_pair(b_dst, &tmR, fb, kb * 64, y);
+          else tma_load_2d_pair(b_dst, &tmU, fb, kb * 64, y);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
       }
     }
   } else if (warp == 1 && rank == 0) {
@@ -1179,7 +1201,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           break;
         }
         ptx::fence_proxy_async_smem();
-        if (lane == 0) ptx::mbar_arrive_cluster(leader(&full_bar[stage]));
+        if (lane == 0) ptx::mbar_arrive_cluster(full0 + stage * 8u);
         if (++stage == STAGES) {
           stage = 0;
           phase ^= 1u;
@@ -1188,96 +1210,130 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
   } else if (warp >= 6 && gather) {
     // -------------------------------------------------------------- gather
-    const int tid = threadIdx.x - 192;  // 0 .. 255
+    // Two teams of four warps take stages in turn, so that one waits and reports while
+    // the other keeps the copies coming: the copies alone take 460 clocks of a 512-clock
+    // stage (36 bytes a clock), all eight warps on every stage 630 with the rest.
+    const int tid = (threadIdx.x - 192) & 127, team = (threadIdx.x - 192) >> 7;
+    const int piece = tid & 7, row0 = tid >> 3;  // 16-byte piece of rows row0, + 16, ...
     int stage = 0;
-    uint32_t phase = 0;
+    uint32_t phase = 0, turn = 0;  // turn: stages so far
     bool ok = true;
-    for (int idx = unit; ok && idx < total; idx += units) {
-      const GroupedTile t = pair_tile<MODE>(p, table, idx);
-      const int half = t.wide >> 1;
-      if constexpr (GRAD) {
-        // thread: 16-byte piece tid % 8 of both 64-column chunks, rows tid / 8 and + 32
-        const int piece = tid & 7, row0 = tid >> 3;
-        const int col = t.r0 + rank * half + piece * 8;
-        uint32_t bytes[2];
+    auto wait_slot = [&]() {
+      return __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) != 0;
+    };
+    auto advance = [&]() {
+      ++turn;
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    };
+    // source row of a plan entry, -1 for none
+    auto row_of = [&](int entry) -> int {
+      if (entry < 0) return -1;
+      const int r = p.order ? pp.div_fan.div(entry) : entry;
+      return r < p.src_rows ? r : -1;
+    };
+    if constexpr (GRAD) {
+      for (int idx = unit; ok && idx < total; idx += units) {
+        const GroupedTile t = pair_tile<MODE>(p, table, idx);
+        const int half = t.wide >> 1;
+        const int col = t.r0 + rank * half + piece * 8, n = t.n0 + rank * 128 + piece * 8;
+        uint32_t bytes[2], n_bytes[2];  // of the two 64-column chunks
 #pragma unroll
-        for (int c = 0; c < 2; ++c) bytes[c] = static_cast<uint32_t>(max(0, min(16, (p.K - col - c * 64) * 2)));
+        for (int c = 0; c < 2; ++c) {
+          bytes[c] = static_cast<uint32_t>(max(0, min(16, (p.K - col - c * 64) * 2)));
+          n_bytes[c] = static_cast<uint32_t>(max(0, min(16, (p.cols - n - c * 64) * 2)));
+        }
         const bool need[2] = {piece * 8 < half, 64 + piece * 8 < half};
         const uint8_t *base = pp.lhs + (bytes[0] ? col * 2ll : 0ll);
         const uint32_t next_chunk = bytes[1] ? 128u : 0u;
-        // Plan entries are loaded two blocks ahead, into two sets of registers that take
-        // turns, and turned into row numbers when they are needed: no block waits for
-        // the load that names its rows.
-        int even[2], odd[2];
-        auto fetch = [&](int kb, int (&entry)[2]) {
+        // the plan's entries of this team's next block are loaded as soon as it has issued
+        // one, and only turned into row numbers when they are needed
+        int entry[4];
+        auto fetch = [&](int kb) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int q = t.p0 + kb * 64 + row0 + 32 * i;
+          for (int i = 0; i < 4; ++i) {
+            const int q = t.p0 + kb * 64 + row0 + 16 * i;
             entry[i] = q >= t.p1 ? -1 : p.order ? __ldg(p.order + q) : q;
           }
         };
-        auto copy = [&](const int (&entry)[2]) -> bool {
-          if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)))
-            return false;
-          const uint32_t dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES) + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
+        fetch((turn & 1u) == static_cast<uint32_t>(team) ? 0 : 1);
+        for (int kb = 0; kb < t.num_kb; ++kb, advance()) {
+          if ((turn & 1u) != static_cast<uint32_t>(team)) continue;
+          if (!wait_slot()) {
+            ok = false;
+            break;
+          }
+          const uint32_t off = row0 * 128 + ((piece ^ (row0 & 7)) << 4);
+          const uint32_t dst = ptx::smem_u32(sB) + stage * Cfg::B_BYTES + off;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int from = entry[i] < 0 ? -1 : p.order ? pp.div_fan.div(entry[i]) : entry[i];
-            const bool live = from >= 0 && from < p.src_rows;
-            const uint8_t *src = base + (live ? from * pp.lhs_pitch : 0ll);
-            if (need[0]) cp_async16(dst + i * 4096, src, live ? bytes[0] : 0u);
-            if (need[1]) cp_async16(dst + 8192 + i * 4096, src + next_chunk, live ? bytes[1] : 0u);
+          for (int i = 0; i < 4; ++i) {
+            const int from = row_of(entry[i]);
+            const uint8_t *src = base + (from >= 0 ? from * pp.lhs_pitch : 0ll);
+            if (need[0]) cp_async16(dst + i * 2048, src, from >= 0 ? bytes[0] : 0u);
+            if (need[1]) cp_async16(dst + 8192 + i * 2048, src + next_chunk, from >= 0 ? bytes[1] : 0u);
+          }
+          const int q0 = t.p0 + kb * 64;
+          if (t.p1 - q0 < 64) {  // grad's rows of the block with the group's end
+            const uint32_t a_dst = ptx::smem_u32(sA) + stage * Cfg::A_BYTES + off;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int q = q0 + row0 + 16 * i;
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const uint32_t have = q < t.p1 ? n_bytes[c] : 0u;
+                cp_async16(a_dst + c * 8192 + i * 2048,
+                           pp.grad + (have ? q * pp.grad_pitch + (n + c * 64) * 2ll : 0ll), have);
+              }
+            }
           }
           cp_async_arrive(ptx::smem_u32(&rows_bar[stage]));
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
-          return true;
-        };
-        fetch(0, even);
-        fetch(1, odd);
-        for (int kb = 0; ok && kb < t.num_kb; kb += 2) {
-          ok = copy(even);
-          fetch(kb + 2, even);
-          if (ok && kb + 1 < t.num_kb) {
-            ok = copy(odd);
-            fetch(kb + 3, odd);
-          }
+          fetch(kb + 2);
         }
-      } else {
-        // thread: 16-byte piece tid % 8 of rows tid / 8, + 32, ...
-        constexpr int kRows = BT / 64;
-        const int piece = tid & 7, row0 = tid >> 3;
-        const uint8_t *row[kRows];
-        bool live[kRows];
+      }
+    } else {
+      constexpr int kRows = BT / 32;
+      // this thread's entries of a tile, loaded while the tile in front of it is fetched
+      int entry[kRows];
+      auto fetch = [&](int idx) {
+        if (idx >= total) return;
+        const GroupedTile t = pair_tile<MODE>(p, table, idx);
+        const int half = t.wide >> 1;
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-          const int r = rank * half + row0 + 32 * i;  // row of the tile
-          long long s = -1;
-          if (row0 + 32 * i < half && r < t.rows) s = source_row(p.order, p.fan, p.src_rows, t.r0 + r);
-          live[i] = s >= 0;
-          row[i] = pp.lhs + (live[i] ? s * pp.lhs_pitch : 0);
+          const int r = rank * half + row0 + 16 * i;  // row of the tile
+          entry[i] = row0 + 16 * i < half && r < t.rows ? p.order ? __ldg(p.order + t.r0 + r) : t.r0 + r : -1;
         }
+      };
+      fetch(unit);
+      for (int idx = unit; ok && idx < total; idx += units) {
+        const GroupedTile t = pair_tile<MODE>(p, table, idx);
+        const int half = t.wide >> 1;
+        const uint8_t *row[kRows];  // nullptr: zeros
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const int from = row_of(entry[i]);
+          row[i] = from >= 0 ? pp.lhs + from * pp.lhs_pitch : nullptr;
+        }
+        fetch(idx + units);
         const int blocks = t.num_kb + extra(t);
-        for (int kb = 0; kb < blocks; ++kb) {
-          if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag))) {
+        for (int kb = 0; kb < blocks; ++kb, advance()) {
+          if ((turn & 1u) != static_cast<uint32_t>(team)) continue;
+          if (!wait_slot()) {
             ok = false;
             break;
           }
           const int k = kb * 64 + piece * 8;
           const uint32_t bytes = static_cast<uint32_t>(max(0, min(16, (p.K - k) * 2)));
-          const uint32_t dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES) + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
+          const uint32_t dst = ptx::smem_u32(sB) + stage * Cfg::B_BYTES + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
           const long long at = bytes ? k * 2ll : 0ll;
           // (the adapters' blocks bring their rows by TMA: nothing to copy, only to arrive)
 #pragma unroll
           for (int i = 0; i < kRows; ++i)
-            if (row0 + 32 * i < half && kb < t.num_kb) cp_async16(dst + i * 4096, row[i] + at, live[i] ? bytes : 0u);
+            if (row0 + 16 * i < half && kb < t.num_kb)
+              cp_async16(dst + i * 2048, row[i] ? row[i] + at : pp.lhs, row[i] ? bytes : 0u);
           cp_async_arrive(ptx::smem_u32(&rows_bar[stage]));
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
         }
       }
     }

@@ -379,8 +379,8 @@ PairParams pair_params(const GroupedParams &gp, const kapyb_tensor2d *lhs, bool 
 // The pair kernel: `tiles` pairs of CTAs at most, as many as the device holds at once
 // (the tile loop is statically strided).
 template <int MODE>
-kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmA8,
-                          const CUtensorMap &tmA1, const PairParams &pp, long long tiles, cudaStream_t stream) {
+kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensorMap &tmB, const CUtensorMap &tmR,
+                          const CUtensorMap &tmU, const PairParams &pp, long long tiles, cudaStream_t stream) {
   using Cfg = PairCfg;
   auto kern = grouped_pair_kernel<MODE>;
   cudaLaunchConfig_t cfg = {};
@@ -407,7 +407,7 @@ kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensor
     resident[h->device].store(pairs);
   }
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min<long long>(tiles, pairs)), 1, 1);
-  CUDA_TRY(h, cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmA8, tmA1, pp));
+  CUDA_TRY(h, cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmR, tmU, pp));
   return launched(h, MODE == PAIR_GRADIENT ? "grouped_grad_pair" : MODE == PAIR_ADAPTERS ? "adapters_pair" : "grouped_pair");
 }
 
@@ -474,11 +474,12 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
     return gated ? launch_grouped<64, 2, false>(h, tmA, tmB, gp, tiles, stream)
                  : launch_grouped<64, 1, false>(h, tmA, tmB, gp, tiles, stream);
   const PairParams pp = pair_params(gp, lhs, order != nullptr, bt);
-  CUtensorMap tall;
-  TRY(make_row_tmap(h, &tall, elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
-                    lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, bt / 2));
-  return gated ? launch_pairs<PAIR_GATED>(h, tmA, tmB, tall, tmA, pp, tiles, stream)
-               : launch_pairs<PAIR_FORWARD>(h, tmA, tmB, tall, tmA, pp, tiles, stream);
+  CUtensorMap box[2];
+  for (int i = 0; i < 2; ++i)
+    TRY(make_row_tmap(h, &box[i], elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
+                      lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, i == 0 ? 128 : 64));
+  return gated ? launch_pairs<PAIR_GATED>(h, tmA, box[0], box[1], tmB, pp, tiles, stream)
+               : launch_pairs<PAIR_FORWARD>(h, tmA, box[0], box[1], tmB, pp, tiles, stream);
 }
 
 kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const kapyb_tensor2d *grad,
@@ -513,14 +514,14 @@ kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, 
   gp.wait_limit_us = h->wait_limit_us;
   const long long tiles = static_cast<long long>(groups) * gp.n_tiles * gp.k_tiles;
   if (tiles >= (1ll << 31)) return KAPYB_OK;
-  CUtensorMap tmA, tmA8, tmA1;
-  const uint64_t ld = grad->size0 > 1 ? grad->stride0 : (grad->size1 + 7) / 8 * 8;
-  TRY(make_row_tmap(h, &tmA, elem_ptr(grad), grad->dtype, grad->size1, grad->size0, ld, 64));
-  TRY(make_row_tmap(h, &tmA8, elem_ptr(grad), grad->dtype, grad->size1, grad->size0, ld, 8));
-  TRY(make_row_tmap(h, &tmA1, elem_ptr(grad), grad->dtype, grad->size1, grad->size0, ld, 1));
+  CUtensorMap tmA;
+  TRY(make_row_tmap(h, &tmA, elem_ptr(grad), grad->dtype, grad->size1, grad->size0,
+                    grad->size0 > 1 ? grad->stride0 : (grad->size1 + 7) / 8 * 8, 64));
   *taken = true;
-  const PairParams pp = pair_params(gp, lhs, true, 256);
-  return launch_pairs<PAIR_GRADIENT>(h, tmA, tmA, tmA8, tmA1, pp, tiles, stream);
+  PairParams pp = pair_params(gp, lhs, true, 256);
+  pp.grad = static_cast<const uint8_t *>(elem_ptr(grad));
+  pp.grad_pitch = grad->stride0 * 2ll;
+  return launch_pairs<PAIR_GRADIENT>(h, tmA, tmA, tmA, tmA, pp, tiles, stream);
 }
 
 // What the two grouped products check alike.
@@ -1045,7 +1046,7 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
   gp.group_scale = c.scale;
   gp.status = h->status;
   gp.wait_limit_us = h->wait_limit_us;
-  CUtensorMap tmD, tmW, tmU, tmL;
+  CUtensorMap tmD, tmW, tmU, tmL, tmR;
   TRY(make_tmap(h, &tmD, elem_ptr(c.down), c.down->dtype, d_unit, d_other, c.groups, d_ld, c.down_stride, 64,
                 d_mn ? 64 : 128));
   // narrow tiles while a wave of pairs holds them all
@@ -1079,8 +1080,9 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
   TRY(make_tmap(h, &tmW, elem_ptr(c.rhs), c.rhs->dtype, w_unit, w_other, 1, w_ld, 0, 64, w_mn ? 64 : 128));
   TRY(make_tmap(h, &tmU, elem_ptr(c.up), c.up->dtype, u_unit, u_other, c.groups, u_ld, c.up_stride, 64,
                 u_mn ? 64 : 128));
-  TRY(make_row_tmap(h, &tmL, scratch + sc.low, c.lhs->dtype, rank, 2ull * positions, low_pitch, 16));
-  return launch_pairs<PAIR_ADAPTERS>(h, tmW, tmW, tmU, tmL, pp, (positions / 256 + 1ll) * n_tiles, stream);
+  TRY(make_row_tmap(h, &tmL, scratch + sc.low, c.lhs->dtype, rank, 2ull * positions, low_pitch, PairCfg::BT / 2));
+  TRY(make_row_tmap(h, &tmR, scratch + sc.low, c.lhs->dtype, rank, 2ull * positions, low_pitch, 16));
+  return launch_pairs<PAIR_ADAPTERS>(h, tmW, tmL, tmR, tmU, pp, (positions / 256 + 1ll) * n_tiles, stream);
 }
 
 }  // namespace
