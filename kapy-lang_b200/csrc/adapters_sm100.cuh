@@ -1,8 +1,9 @@
-// A shared projection with low-rank adapters beside it, for few rows (a decode step):
+// A shared projection with low-rank adapters beside it, for few rows (a decode step of up
+// to 256 sequences):
 //   out[t] = act(alpha x[t] . W + bias + low[t] . up[i(t)]),   low[t] = scale[i] x[t] . down[i]
 //
 // What such a call costs is reading W once, so the kernel is a weight stream: 128 columns
-// of W fill the M side of the MMA, the at most 64 rows of x its N side, and a cluster of
+// of W fill the M side of the MMA, the at most 256 rows of x its N side, and a cluster of
 // CTAs shares a column block by cutting K into pieces, so that every SM streams even when
 // there are few column blocks.  The CTAs' partial sums meet in distributed shared memory,
 // each CTA finishing its share of the rows, added in CTA order: no scratch in global
@@ -25,8 +26,9 @@
 
 namespace kapyb {
 
-constexpr int kDecodeMaxRows = 64;
+constexpr int kDecodeMaxRows = 256;
 constexpr int kLowThreads = 512;
+constexpr int kLowMaxSplit = 4;
 
 struct LowParams {
   const uint16_t *x;
@@ -37,39 +39,53 @@ struct LowParams {
   const int32_t *index;
   const float *scale;
   float *low;                // [rows, rank]
+  int split;                 // CTAs of a cluster that share a row's K
 };
+
+__device__ __forceinline__ float ld_shared_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 
 template <bool BF>
 __device__ __forceinline__ float widen16(uint16_t h) {
   return cvt_16_to_f32(h, BF ? KAPYB_BF16 : KAPYB_F16);
 }
 
-// low[t]: one block per row.  KMAJOR: down has its unit stride on K, a warp per column of
-// it; otherwise unit stride on the rank, a thread per eight columns and K residue.  Sums in
-// f32 in a fixed order.  Rows of down and x start on 16 bytes and rank is a multiple of 8
+// low[t]: a cluster of `split` blocks per row, each a run of K; the first one adds up.
+// KMAJOR: down has its unit stride on K, a warp per column of it; otherwise unit stride on
+// the rank, a thread per eight columns and K residue.  Sums in f32 in a fixed order.  Rows of down and x start on 16 bytes and rank is a multiple of 8
 // (!KMAJOR).
 template <bool BF, bool KMAJOR>
 __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(const LowParams p) {
   ptx::griddep_launch();
   constexpr int DT = BF ? KAPYB_BF16 : KAPYB_F16;
   __shared__ float part[kLowThreads / 32][128];
-  const long long t = blockIdx.x;
+  __shared__ float mine[128];
+  const long long t = blockIdx.x / p.split;
+  const int rank = blockIdx.x % p.split;
   const int i = p.index[t];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  if (i < 0 || i >= p.groups) {
-    for (int j = threadIdx.x; j < p.rank; j += kLowThreads) p.low[t * p.rank + j] = 0.0f;
+  if (i < 0 || i >= p.groups) {  // the whole cluster
+    if (rank == 0)
+      for (int j = threadIdx.x; j < p.rank; j += kLowThreads) p.low[t * p.rank + j] = 0.0f;
     return;
   }
   const float scale = p.scale ? p.scale[i] : 1.0f;
   const uint16_t *x = p.x + t * p.x_s0;
   const uint16_t *down = p.down + i * p.d_group;
+  // this block's run of K, in whole 16-byte pieces but for the last one's end
+  const int pieces = (p.K + 7) / 8;
+  const int first_k = static_cast<int>(static_cast<long long>(rank) * pieces / p.split) * 8;
+  const int last_k = min(p.K, static_cast<int>(static_cast<long long>(rank + 1) * pieces / p.split) * 8);
   if constexpr (KMAJOR) {
     for (int j = w; j < p.rank; j += kLowThreads / 32) {
       const uint16_t *col = down + j * p.d_s1;
       float acc = 0.0f;
-      const int whole = p.K / 8;
+      const int whole = last_k / 8;
       constexpr int U = 4;
-      for (int v = lane; v < whole; v += 32 * U) {
+      for (int v = first_k / 8 + lane; v < whole; v += 32 * U) {
         uint4 a[U], b[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -91,10 +107,10 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(const LowParam
           }
         }
       }
-      for (int k = whole * 8 + lane; k < p.K; k += 32) acc = fmaf(widen16<BF>(x[k]), widen16<BF>(col[k]), acc);
+      for (int k = max(first_k, whole * 8) + lane; k < last_k; k += 32) acc = fmaf(widen16<BF>(x[k]), widen16<BF>(col[k]), acc);
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-      if (lane == 0) p.low[t * p.rank + j] = acc * scale;
+      if (lane == 0) mine[j] = acc;
     }
   } else {
     const int chunks = p.rank / 8;
@@ -106,14 +122,14 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(const LowParam
     for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
     if (chunk < chunks) {
       constexpr int U = 8;
-      for (int k = k0; k < p.K; k += step * U) {
+      for (int k = first_k + k0; k < last_k; k += step * U) {
         uint4 a[U];
         float xv[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           a[u] = make_uint4(0u, 0u, 0u, 0u);
           xv[u] = 0.0f;
-          if (k + step * u < p.K) {
+          if (k + step * u < last_k) {
             a[u] = __ldg(reinterpret_cast<const uint4 *>(down + (k + step * u) * p.d_s0) + chunk);
             xv[u] = widen16<BF>(__ldg(x + k + step * u));
           }
@@ -144,9 +160,21 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(const LowParam
     for (int j = threadIdx.x; j < p.rank; j += kLowThreads) {
       float s = 0.0f;
       for (int k = 0; k < kLowThreads / 32; ++k) s += part[k][j];
+      mine[j] = s;
+    }
+  }
+  __syncthreads();
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  if (rank == 0) {
+    for (int j = threadIdx.x; j < p.rank; j += kLowThreads) {
+      float s = 0.0f;
+      for (int c = 0; c < p.split; ++c) s += ld_shared_cluster(ptx::mapa(ptx::smem_u32(&mine[j]), c));
       p.low[t * p.rank + j] = s * scale;
     }
   }
+  ptx::cluster_arrive();  // nobody leaves while the first one may read
+  ptx::cluster_wait();
 }
 
 struct DecodeParams {
@@ -171,17 +199,10 @@ struct DecodeParams {
   uint32_t wait_limit_us;
 };
 
-__device__ __forceinline__ float ld_shared_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 // low[t] . up[a] for columns n0 .. n0 + 127 into dst[128]; one warp.
 template <bool BF>
-__device__ __forceinline__ void adapter_delta(const DecodeParams &p, int t, int n0, float *dst, int lane) {
+__device__ __forceinline__ void adapter_delta(const DecodeParams &p, int t, int a, int n0, float *dst, int lane) {
   constexpr int DT = BF ? KAPYB_BF16 : KAPYB_F16;
-  const int a = p.index[t];
   const bool on = a >= 0 && a < p.groups;
   const float *low = p.low + static_cast<long long>(t) * p.rank;
   const uint16_t *up = p.up + (on ? a * p.u_group : 0ll);
@@ -372,7 +393,16 @@ __global__ void __launch_bounds__(192) adapter_decode_kernel(const __grid_consta
   } else {
     ptx::griddep_wait();  // low
     const int q = warp & 3;
-    for (int r = r0 + q; r < r1; r += 4) adapter_delta<BF>(p, r, n0, delta + (r - r0) * 128, lane);
+    // row r of this CTA's belongs to warp r % 4; lane l looks up its l-th one's adapter
+    for (int base = r0 + q; base < r1; base += 4 * 32) {
+      const int look = base + 4 * lane < r1 ? p.index[base + 4 * lane] : -1;
+#pragma unroll 2
+      for (int i = 0; i < 32; ++i) {
+        const int r = base + 4 * i;
+        if (r >= r1) break;
+        adapter_delta<BF>(p, r, __shfl_sync(0xffffffffu, look, i), n0, delta + (r - r0) * 128, lane);
+      }
+    }
     const bool ok = __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&done_bar), 0u, abort_flag));
     ptx::tc_fence_after();
     if (ok) {
@@ -396,14 +426,26 @@ __global__ void __launch_bounds__(192) adapter_decode_kernel(const __grid_consta
     const int n = n0 + q * 32 + lane;
     if (n < p.cols) {
       const float bias_col = p.bias != nullptr && p.bias_axis == 1 ? load_as_f32(p.bias, p.bias_dtype, n) : 0.0f;
-      for (int r = r0; r < r1; ++r) {
-        const uint32_t at = ptx::smem_u32(partial + r * 128 + q * 32 + lane);
-        float v = 0.0f;
-        for (int c = 0; c < split; ++c) v += ld_shared_cluster(ptx::mapa(at, c));
-        v = v * p.alpha + bias_col;
-        if (p.bias != nullptr && p.bias_axis == 0) v += load_as_f32(p.bias, p.bias_dtype, r);
-        v += delta[(r - r0) * 128 + q * 32 + lane];
-        store_from_f32(p.out, p.out_dtype, r * p.out_s0 + n * p.out_s1, apply_activation(p.activation, v), p.rounding);
+      constexpr int U = 8;  // rows whose remote loads overlap
+      for (int r = r0; r < r1; r += U) {
+        float v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = 0.0f;
+        for (int c = 0; c < split; ++c) {
+          const uint32_t at = ptx::mapa(ptx::smem_u32(partial + r * 128 + q * 32 + lane), c);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (r + u < r1) v[u] += ld_shared_cluster(at + u * 512u);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (r + u >= r1) break;
+          float o = v[u] * p.alpha + bias_col;
+          if (p.bias != nullptr && p.bias_axis == 0) o += load_as_f32(p.bias, p.bias_dtype, r + u);
+          o += delta[(r + u - r0) * 128 + q * 32 + lane];
+          store_from_f32(p.out, p.out_dtype, (r + u) * p.out_s0 + n * p.out_s1, apply_activation(p.activation, o),
+                         p.rounding);
+        }
       }
     }
   }

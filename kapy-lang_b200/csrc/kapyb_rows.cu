@@ -867,7 +867,7 @@ bool stack_tma_ok(const kapyb_tensor2d *t, int groups, int64_t stride, bool &mn,
   return tma_ok(elem_ptr(t), t->dtype, unit, other, ld, groups, stride);
 }
 
-// At most 64 rows: the weight stream with the adapters' part beside it.
+// At most 256 rows: the weight stream with the adapters' part beside it.
 kapyb_status adapters_decode(kapyb_handle h, const AdapterCall &c, cudaStream_t stream, bool *taken) {
   *taken = false;
   bool mn;
@@ -879,19 +879,60 @@ kapyb_status adapters_decode(kapyb_handle h, const AdapterCall &c, cudaStream_t 
   float *low = static_cast<float *>(c.scratch);
   const bool bf = c.lhs->dtype == KAPYB_BF16;
 
+  const int wide = (rows + 15) / 16 * 16, num_kb = (c.lhs->size1 + 63) / 64;
+  // CTAs per column block.  Up to 64 rows two CTAs fit an SM (the ring is kept below half
+  // of its shared memory), so that one streams while the other starts or ends, and a CTA
+  // by itself streams some 50 GB/s at most.  The share of those places that is used, over
+  // whole waves, decides; more CTAs must gain a fifth.  Each keeps at least four K blocks.
+  const int tiles = (c.out->size1 + 127) / 128;
+  const int per_sm = wide <= 64 ? 2 : 1;
+  const int places = h->sm_count * per_sm;
+  int split = 1;
+  double best = 0.0;
+  for (int s = 1; s <= 8 && s * 4 <= std::max(4, num_kb); s *= 2) {
+    const long long units = static_cast<long long>(tiles) * s;
+    const long long waves = (units + places - 1) / places;
+    const double used = static_cast<double>(units) / (waves * places);
+    if (used > best * 1.2) {
+      best = used;
+      split = s;
+    }
+  }
+  const int stage_bytes = 16384 + wide * 128;
+  int delta = 0, stages = 0;
+  for (;; split *= 2) {  // rows of a CTA's share of the output, in f32, beside the ring
+    delta = (rows + split - 1) / split * 512;
+    const int budget = 232448 / per_sm - 3072 - delta;
+    stages = std::min(8, budget / stage_bytes);
+    // the ring also takes the partial sums
+    if (stages >= 3 && stages * stage_bytes >= wide * 512) break;
+    if (split >= 8 || 2 * split > num_kb) return KAPYB_OK;
+  }
+  const int smem = 1024 + stages * stage_bytes + delta;
+
   // low = scale * x . down
   const bool d_aligned = aligned16(down) && c.down_stride % 8 == 0;
   const bool d_k = c.down->stride0 == 1 && c.down->stride1 % 8 == 0 && d_aligned;
   const bool d_r = c.down->stride1 == 1 && c.down->stride0 % 8 == 0 && d_aligned && rank % 8 == 0;
   if (d_k || d_r) {
     const LowParams lp{static_cast<const uint16_t *>(elem_ptr(c.lhs)), c.lhs->stride0, down, c.down->stride0,
-                       c.down->stride1, c.down_stride, bf, c.groups, rows, c.lhs->size1, rank, c.index, c.scale, low};
-    if (d_r)
-      bf ? adapter_low_kernel<true, false><<<rows, kLowThreads, 0, stream>>>(lp)
-         : adapter_low_kernel<false, false><<<rows, kLowThreads, 0, stream>>>(lp);
-    else
-      bf ? adapter_low_kernel<true, true><<<rows, kLowThreads, 0, stream>>>(lp)
-         : adapter_low_kernel<false, true><<<rows, kLowThreads, 0, stream>>>(lp);
+                       c.down->stride1, c.down_stride, bf, c.groups, rows, c.lhs->size1, rank, c.index, c.scale, low,
+                       // few rows share their K between CTAs: two blocks of 512 threads an SM at most
+                       rows <= h->sm_count / 2 ? kLowMaxSplit : rows <= h->sm_count ? 2 : 1};
+    auto kern = d_r ? (bf ? adapter_low_kernel<true, false> : adapter_low_kernel<false, false>)
+                    : (bf ? adapter_low_kernel<true, true> : adapter_low_kernel<false, true>);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(static_cast<unsigned>(rows) * lp.split, 1, 1);
+    cfg.blockDim = dim3(kLowThreads, 1, 1);
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = lp.split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CUDA_TRY(h, cudaLaunchKernelEx(&cfg, kern, lp));
   } else {
     AdapterSimtParams sp{};
     sp.x = elem_ptr(c.lhs);
@@ -915,12 +956,15 @@ kapyb_status adapters_decode(kapyb_handle h, const AdapterCall &c, cudaStream_t 
 
   DecodeParams p{};
   p.rows = rows;
-  p.wide = (rows + 15) / 16 * 16;
+  p.wide = wide;
   p.cols = c.out->size1;
-  p.num_kb = (c.lhs->size1 + 63) / 64;
+  p.num_kb = num_kb;
+  p.stages = stages;
+  p.stage_bytes = stage_bytes;
   p.w_mn_major = mn;
   p.bf16 = bf;
-  p.tmem_cols = p.wide <= 32 ? 32 : 64;
+  p.tmem_cols = 32;
+  while (static_cast<int>(p.tmem_cols) < p.wide) p.tmem_cols *= 2;
   p.low = low;
   p.index = c.index;
   p.groups = c.groups;
@@ -945,27 +989,6 @@ kapyb_status adapters_decode(kapyb_handle h, const AdapterCall &c, cudaStream_t 
   p.rounding = c.ep.rounding;
   p.status = h->status;
   p.wait_limit_us = h->wait_limit_us;
-  // CTAs per column block: the share of the SMs' time that is used, units over whole
-  // waves, decides; more CTAs must gain a tenth.  Each keeps at least four K blocks.
-  const int tiles = (p.cols + 127) / 128;
-  int split = 1;
-  double best = 0.0;
-  for (int s = 1; s <= 8 && s * 4 <= std::max(4, p.num_kb); s *= 2) {
-    const long long units = static_cast<long long>(tiles) * s;
-    const long long waves = (units + h->sm_count - 1) / h->sm_count;
-    const double used = static_cast<double>(units) / (waves * h->sm_count);
-    if (used > best * 1.1) {
-      best = used;
-      split = s;
-    }
-  }
-  const int delta = (rows + split - 1) / split * 512;
-  p.stage_bytes = 16384 + p.wide * 128;
-  const int budget = 232448 - 2048 - delta;
-  p.stages = std::min(8, budget / p.stage_bytes);
-  // the ring also takes the partial sums
-  const int ring = std::max(p.stages * p.stage_bytes, p.wide * 512);
-  const int smem = 1024 + ring + delta;
   CUtensorMap tmW, tmX;
   TRY(make_tmap(h, &tmW, elem_ptr(c.rhs), c.rhs->dtype, unit, other, 1, ld, 0, 64, mn ? 64 : 128));
   TRY(make_row_tmap(h, &tmX, elem_ptr(c.lhs), c.lhs->dtype, c.lhs->size1, rows,

@@ -605,7 +605,8 @@ ADAPTERS = [  # T, G, K, N, r, how the rows choose
     (1, 1, 64, 64, 8, "one"), (1, 4, 256, 136, 16, "none"), (3, 4, 72, 128, 1, "each"), (16, 8, 256, 256, 16, "each"),
     (64, 30, 512, 200, 16, "each"), (65, 5, 128, 264, 32, "each"), (130, 3, 264, 128, 64, "runs"),
     (300, 7, 192, 384, 16, "runs"), (513, 40, 128, 130, 8, "each"), (700, 2, 320, 256, 128, "runs"),
-    (260, 6, 136, 72, 20, "runs")]
+    (260, 6, 136, 72, 20, "runs"), (200, 3, 64, 72, 8, "each"), (256, 9, 640, 264, 16, "each"),
+    (257, 4, 64, 256, 8, "each"), (90, 5, 1160, 136, 40, "each")]
 
 
 def make_adapters(case, dt, up_layout="rn", seed=0):
