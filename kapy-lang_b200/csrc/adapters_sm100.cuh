@@ -465,4 +465,243 @@ __global__ void __launch_bounds__(192) adapter_decode_kernel(const __grid_consta
   }
 }
 
+// ---------------------------------------------------------------- many rows
+//
+// low[p] = scale[g] x[row(p)] . down[g] for the positions of a padded plan, as two 16-bit
+// halves (the value rounded, and what that left, so that the pair kernel's product with
+// `up` is exact to 16 bits and more).  A tile is up to 64 positions of one adapter: the
+// rank fills the M side of the MMA (lanes beyond it hold what the stage happened to hold
+// and are not stored), the positions its N side.  There are few tiles and K is long, so a
+// cluster shares K as in the kernel above.  Rows are gathered by cp.async (see
+// grouped_sm100.cuh); down comes by TMA.
+
+struct LowTileParams {
+  const int32_t *offsets, *order;  // the padded plan; groups of `groups` adapters
+  int groups, positions;
+  const uint8_t *x;
+  long long x_pitch;     // bytes
+  int src_rows, K, rank, split;
+  int d_mn_major, bf16;
+  int a_bytes;           // of down in a stage: 8192 up to rank 64, else 16384
+  const float *scale;
+  float alpha;           // 1 / the epilogue's scale
+  uint16_t *high, *low;  // [positions][pitch]
+  int pitch;
+  uint32_t *status;
+  uint32_t wait_limit_us;
+};
+
+constexpr int kLowTile = 64, kLowStages = 4;
+constexpr int kLowTileThreads = 224;
+constexpr int kLowStageBytes = 16384 + kLowTile * 128;
+constexpr int kLowTileSmem = 1024 + kLowStages * kLowStageBytes + (3 * kGroupedMaxGroups + 8) * 4;
+
+// tmD: down, 3-D, in boxes of 64 x 64 (unit stride on the rank, or rank <= 64) or 64 x 128.
+template <bool BF>
+__global__ void __launch_bounds__(kLowTileThreads) adapter_low_tile_kernel(const __grid_constant__ CUtensorMap tmD,
+                                                                           const LowTileParams p) {
+  ptx::griddep_launch();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                              ~static_cast<uintptr_t>(1023));
+  __shared__ uint64_t full_bar[kLowStages], empty_bar[kLowStages], rows_bar[kLowStages], done_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t abort_words[2];
+  volatile uint32_t *abort_flag = abort_words;
+  int *table_mem = reinterpret_cast<int *>(smem + kLowStages * kLowStageBytes);
+  GroupedTable table{table_mem, table_mem + kGroupedMaxGroups + 2, table_mem + 2 * kGroupedMaxGroups + 4};
+  float *partial = reinterpret_cast<float *>(smem);  // [kLowTile][128], over the ring
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x) % p.split;  // in the cluster
+  const int want = static_cast<int>(blockIdx.x) / p.split;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kLowStages; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&full_bar[s]), 2);  // down's bytes, the rows
+      ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&rows_bar[s]), 128);
+    }
+    ptx::mbar_init(ptx::smem_u32(&done_bar), 1);
+    abort_flag[0] = 0u;
+    abort_flag[1] = p.wait_limit_us;
+    ptx::fence_barrier_init();
+    ptx::prefetch_tensormap(&tmD);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc<1>(ptx::smem_u32(&tmem_slot), 64);
+    ptx::tmem_relinquish<1>();
+  }
+  if (warp == 0) build_tile_table(p.offsets, p.groups, p.positions, kLowTile, table, lane);
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  // this cluster's tile; clusters behind the last one only keep the barriers company
+  const bool mine = want < table.first[p.groups];
+  const int g = find_group(table, p.groups, want);
+  const int at = (want - table.first[g]) * kLowTile;
+  const int p0 = table.begin[g] + at, rows = mine ? min(kLowTile, table.count[g] - at) : 0;
+  const int num_kb = (p.K + 63) / 64;
+  const int kb0 = mine ? static_cast<int>(static_cast<long long>(rank) * num_kb / p.split) : 0;
+  const int kb1 = mine ? static_cast<int>(static_cast<long long>(rank + 1) * num_kb / p.split) : 0;
+  const int wide = round16(rows);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) break;
+        const uint32_t fb = ptx::smem_u32(&full_bar[stage]);
+        const uint32_t dst = ptx::smem_u32(smem) + stage * kLowStageBytes;
+        ptx::mbar_arrive_expect_tx(fb, p.a_bytes);
+        if (p.d_mn_major) {
+          ptx::tma_load_3d(dst, &tmD, fb, 0, kb * 64, g);
+          if (p.a_bytes > 8192) ptx::tma_load_3d(dst + 8192, &tmD, fb, 64, kb * 64, g);
+        } else {
+          ptx::tma_load_3d(dst, &tmD, fb, kb * 64, 0, g);
+        }
+        if (++stage == kLowStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t idesc = ptx::make_idesc_f16(p.bf16, p.d_mn_major, 0, 128, mine ? wide : 16);
+    const uint32_t a_lo_c = ((p.d_mn_major ? 8192u : 16u) >> 4) << 16;
+    const uint32_t a_step = (p.d_mn_major ? 2048u : 32u) >> 4;
+    constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&full_bar[stage]), phase, abort_flag))) {
+        ok = false;
+        break;
+      }
+      ptx::tc_fence_after();
+      if (ptx::elect_one()) {
+        const uint32_t base = (ptx::smem_u32(smem) + stage * kLowStageBytes) & 0x3ffffu;  // see adapter_decode_kernel
+        const uint32_t a_lo = a_lo_c | (base >> 4), b_lo = (1u << 16) | ((base + 16384u) >> 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          ptx::umma_k<1, 0>(tmem, (static_cast<uint64_t>(hi) << 32) | (a_lo + k * a_step),
+                            (static_cast<uint64_t>(hi) << 32) | (b_lo + k * 2u), idesc, (kb != kb0 || k != 0) ? 1u : 0u);
+        ptx::umma_commit<1>(ptx::smem_u32(&empty_bar[stage]));
+      }
+      if (++stage == kLowStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    if (ok && mine && ptx::elect_one()) ptx::umma_commit<1>(ptx::smem_u32(&done_bar));
+  } else if (warp == 6) {
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&rows_bar[stage]), phase, abort_flag))) break;
+      ptx::fence_proxy_async_smem();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&full_bar[stage]));
+      if (++stage == kLowStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+  } else {
+    const int tid = threadIdx.x - 64, piece = tid & 7, row0 = tid >> 3;  // 16 rows a pass
+    const uint8_t *row[kLowTile / 16];
+#pragma unroll
+    for (int i = 0; i < kLowTile / 16; ++i) {
+      row[i] = nullptr;
+      if (row0 + 16 * i < rows) {
+        const long long from = source_row(p.order, 1, p.src_rows, p0 + row0 + 16 * i);
+        if (from >= 0) row[i] = p.x + from * p.x_pitch;
+      }
+    }
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag))) {
+        ok = false;
+        break;
+      }
+      const int k = kb * 64 + piece * 8;
+      const uint32_t bytes = static_cast<uint32_t>(max(0, min(16, (p.K - k) * 2)));
+      const uint32_t dst = ptx::smem_u32(smem) + stage * kLowStageBytes + 16384u + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
+      const long long off = bytes ? k * 2ll : 0ll;
+#pragma unroll
+      for (int i = 0; i < kLowTile / 16; ++i)
+        if (row0 + 16 * i < wide) cp_async16(dst + i * 2048, row[i] ? row[i] + off : p.x, row[i] ? bytes : 0u);
+      cp_async_arrive(ptx::smem_u32(&rows_bar[stage]));
+      if (++stage == kLowStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    cp_async_wait_all();
+    if (mine) ok = ok && ptx::mbar_wait(ptx::smem_u32(&done_bar), 0u, abort_flag);
+    ok = __all_sync(0xffffffffu, ok) != 0;
+    ptx::tc_fence_after();
+    if (ok && mine) {
+      const int q = warp & 3;
+      for (int c = 0; c < rows; c += 16) {
+        uint32_t v[16];
+        ptx::tmem_ld_32x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + c, v);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) partial[(c + i) * 128 + q * 32 + lane] = __uint_as_float(v[i]);
+      }
+      ptx::tc_fence_before();
+    }
+  }
+  __syncthreads();
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  if (mine && warp >= 2 && warp < 6 && *abort_flag == 0u) {
+    const int j = (warp & 3) * 32 + lane;
+    const int r0 = rank * rows / p.split, r1 = (rank + 1) * rows / p.split;
+    if (j < p.rank) {
+      const float alpha = p.alpha * (p.scale ? p.scale[g] : 1.0f);
+      constexpr int DT = BF ? KAPYB_BF16 : KAPYB_F16;
+      constexpr int U = 8;
+      for (int r = r0; r < r1; r += U) {
+        float v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = 0.0f;
+        for (int c = 0; c < p.split; ++c) {
+          const uint32_t from = ptx::mapa(ptx::smem_u32(partial + r * 128 + j), c);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (r + u < r1) v[u] += ld_shared_cluster(from + u * 512u);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (r + u >= r1) break;
+          const float f = v[u] * alpha;
+          const uint16_t high = cvt_f32_to_16(f, DT, 1);
+          const long long to = static_cast<long long>(p0 + r + u) * p.pitch + j;
+          p.high[to] = high;
+          p.low[to] = cvt_f32_to_16(f - cvt_16_to_f32(high, DT), DT, 1);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (*abort_flag != 0u) {
+    if (threadIdx.x == 0) atomicExch(p.status, kStatusTimeout);
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 200000ull) {
+    }
+  }
+  ptx::cluster_arrive();
+  ptx::cluster_wait();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<1>(tmem, 64);
+  }
+}
+
 }  // namespace kapyb

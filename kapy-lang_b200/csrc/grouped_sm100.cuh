@@ -74,10 +74,6 @@ struct GroupedParams {
   float alpha;
   const void *bias;      // [groups, bias_cols]; adapters: [cols], or [source rows] with bias_axis 0
   int bias_dtype, bias_cols, bias_axis, activation, rounding;
-  // pairs, forward: the result as two 16-bit halves, v rounded and what that left, the
-  // second array lo_bytes behind the first (0: off); scaled by alpha * group_scale[g]
-  long long lo_bytes;
-  const float *group_scale;
   uint32_t *status;
   uint32_t wait_limit_us;
 };
@@ -133,6 +129,43 @@ struct GroupedTable {
   int *first, *begin, *count;
 };
 
+// Builds the table from the plan's offsets; one warp.
+__device__ __forceinline__ void build_tile_table(const int32_t *offsets, int groups, int rows, int tile_rows,
+                                                 const GroupedTable &table, int lane) {
+  int before = 0;
+  for (int g0 = 0; g0 < groups; g0 += 32) {
+    const int g = g0 + lane;
+    int b = 0, e = 0;
+    if (g < groups) group_range(offsets, g, rows, b, e);
+    const int cnt = max(0, e - b);
+    const int tiles = (cnt + tile_rows - 1) / tile_rows;
+    int scan = tiles;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, scan, off);
+      if (lane >= off) scan += o;
+    }
+    if (g < groups) {
+      table.first[g] = before + scan - tiles;
+      table.begin[g] = b;
+      table.count[g] = cnt;
+    }
+    before += __shfl_sync(0xffffffffu, scan, 31);
+  }
+  if (lane == 0) table.first[groups] = before;
+}
+
+// The group that row tile q belongs to.
+__device__ __forceinline__ int find_group(const GroupedTable &t, int groups, int q) {
+  int lo = 0, hi = groups;  // first[lo] <= q < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.first[mid] <= q) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
 template <int BT, bool GRAD>
 __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams &p, const GroupedTable &t, int idx) {
   GroupedTile r;
@@ -151,12 +184,7 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams &p, cons
     r.num_kb = (t.count[r.g] + 63) >> 6;
   } else {
     const int q = idx / p.n_tiles;
-    int lo = 0, hi = p.groups;  // the group g with first[g] <= q < first[g + 1]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (t.first[mid] <= q) lo = mid;
-      else hi = mid;
-    }
+    const int lo = find_group(t, p.groups, q);
     r.g = lo;
     const int tiles = t.first[lo + 1] - t.first[lo];
     const int in = idx - t.first[lo] * p.n_tiles;
@@ -369,29 +397,7 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     ptx::tmem_alloc<1>(ptx::smem_u32(tmem_slot), Cfg::TMEM_COLS);
     ptx::tmem_relinquish<1>();
   }
-  if (warp == 0) {
-    int before = 0;
-    for (int g0 = 0; g0 < p.groups; g0 += 32) {
-      const int g = g0 + lane;
-      int b = 0, e = 0;
-      if (g < p.groups) group_range(p.offsets, g, p.rows, b, e);
-      const int cnt = max(0, e - b);
-      const int tiles = GRAD ? 0 : (cnt + BT - 1) / BT;
-      int scan = tiles;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, scan, off);
-        if (lane >= off) scan += o;
-      }
-      if (g < p.groups) {
-        table.first[g] = before + scan - tiles;
-        table.begin[g] = b;
-        table.count[g] = cnt;
-      }
-      before += __shfl_sync(0xffffffffu, scan, 31);
-    }
-    if (lane == 0) table.first[p.groups] = before;
-  }
+  if (warp == 0) build_tile_table(p.offsets, p.groups, p.rows, BT, table, lane);
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
@@ -639,7 +645,10 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 // (gaps and rows without an adapter included), and the tile's main loop over the shared
 // weights is followed by more K blocks, for each adapter that has rows in the tile: its
 // `up` block times the rows' low-rank products (scale x . down, computed before), into
-// exactly the accumulator columns those rows own.  The products come in two 16-bit
+// exactly the accumulator columns those rows own.  (The kernel is launched with
+// programmatic serialization behind the one that computes the products and only waits for
+// it there: the plan and everything else it reads were complete when that one started.)
+// The products come in two 16-bit
 // halves, so the second factor is exact to 16 bits and more.  Nothing is added twice to
 // memory and one rounding remains; what a broken adapter produces stays in its own rows.
 
@@ -659,7 +668,6 @@ struct PairParams {
   const uint8_t *grad;   // gradient: the same of grad
   long long grad_pitch;
   FastDiv div_fan;
-  int tile_rows;         // forward: most rows of a tile, at most BT and a multiple of 32
   // adapters: g.groups = adapters + 1 (the last group: rows without one)
   int rank, up_mn_major;
   int low_rows;          // rows of one half of the low-rank products
@@ -731,12 +739,7 @@ __device__ __forceinline__ GroupedTile pair_tile(const GroupedParams &p, const G
     r.num_kb = (t.count[r.g] + 63) >> 6;
   } else {
     const int q = idx / p.n_tiles;
-    int lo = 0, hi = p.groups;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (t.first[mid] <= q) lo = mid;
-      else hi = mid;
-    }
+    const int lo = find_group(t, p.groups, q);
     r.g = lo;
     const int tiles = t.first[lo + 1] - t.first[lo];
     const int in = idx - t.first[lo] * p.n_tiles;
@@ -846,27 +849,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       }
     }
   } else if (warp == 0) {
-    int before = 0;
-    for (int g0 = 0; g0 < p.groups; g0 += 32) {
-      const int g = g0 + lane;
-      int b = 0, e = 0;
-      if (g < p.groups) group_range(p.offsets, g, p.rows, b, e);
-      const int cnt = max(0, e - b);
-      const int tiles = GRAD ? 0 : (cnt + pp.tile_rows - 1) / pp.tile_rows;
-      int scan = tiles;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, scan, off);
-        if (lane >= off) scan += o;
-      }
-      if (g < p.groups) {
-        table.first[g] = before + scan - tiles;
-        table.begin[g] = b;
-        table.count[g] = cnt;
-      }
-      before += __shfl_sync(0xffffffffu, scan, 31);
-    }
-    if (lane == 0) table.first[p.groups] = before;
+    build_tile_table(p.offsets, p.groups, p.rows, BT, table, lane);
   }
   ptx::tc_fence_before();
   __syncthreads();
@@ -946,6 +929,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
         if constexpr (ADAPT) {
           if (!ok) break;
+          if (idx == unit) ptx::griddep_wait();  // the low-rank products, of the kernel ahead
           ok = each_adapter(table, p.groups - 1, t.r0, t.r0 + t.rows, [&](int g, int s0, int s1) {
             const int mine = (s1 - s0) >> 1;  // rows this CTA fetches: a multiple of 16
             for (int b = 0; b < 2 * low_blocks; ++b) {
@@ -1099,7 +1083,6 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const long long at = (ADAPT ? 0ll : static_cast<long long>(t.g) * p.bias_cols) + n;
         bias = load_as_f32(p.bias, p.bias_dtype, GATED && q >= 2 ? at + p.cols : at);
       }
-      const float alpha = !ADAPT && p.group_scale != nullptr ? p.alpha * p.group_scale[t.g] : p.alpha;
       if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc]), acc_phase, abort_flag))) break;
       ptx::tc_fence_after();
       const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BT);
@@ -1131,16 +1114,16 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           if (p.bias != nullptr && p.bias_axis == 0) {
             const float row_bias = to >= 0 ? load_as_f32(p.bias, p.bias_dtype, to) : 0.0f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = f[j] * alpha + __shfl_sync(0xffffffffu, row_bias, j);
+            for (int j = 0; j < 32; ++j) f[j] = f[j] * p.alpha + __shfl_sync(0xffffffffu, row_bias, j);
             grouped_activation(p.activation, f);
           } else {
-            grouped_finish32<1>(p, alpha, f, nullptr, bias, 0.0f);
+            grouped_finish32<1>(p, p.alpha, f, nullptr, bias, 0.0f);
           }
           grouped_scatter32(p, static_cast<char *>(p.out) + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll), f, to, lane,
                             mine, both);
         } else if constexpr (GATED) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) f[j] = f[j] * alpha + bias;
+          for (int j = 0; j < 32; ++j) f[j] = f[j] * p.alpha + bias;
           // the gate's warp hands over its rows 16 .. 31 and finishes 0 .. 15, the up
           // columns' warp the other way round; two buffers take turns
           const bool up_side = q >= 2;
@@ -1168,14 +1151,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           const int first = c + (up_side ? 16 : 0);
           grouped_store(p, out + static_cast<long long>(first) * p.row_pitch, g, t.rows - first, lane, mine, both);
         } else {
-          grouped_finish32<1>(p, alpha, f, nullptr, bias, 0.0f);
+          grouped_finish32<1>(p, p.alpha, f, nullptr, bias, 0.0f);
           char *at = out + static_cast<long long>(c) * p.row_pitch;
           grouped_store(p, at, f, t.rows - c, lane, mine, both);
-          if (MODE == PAIR_FORWARD && p.lo_bytes != 0) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] -= cvt_16_to_f32(cvt_f32_to_16(f[j], p.out_dtype, 1), p.out_dtype);
-            grouped_store(p, at + p.lo_bytes, f, t.rows - c, lane, mine, both);
-          }
         }
       }
       if (!alive) break;

@@ -365,14 +365,13 @@ kapyb_status launch_grouped(kapyb_handle h, const CUtensorMap &tmA, const CUtens
   return launched(h, GRAD ? "grouped_grad_tcgen05" : "grouped_tcgen05");
 }
 
-PairParams pair_params(const GroupedParams &gp, const kapyb_tensor2d *lhs, bool gather, int tile_rows) {
+PairParams pair_params(const GroupedParams &gp, const kapyb_tensor2d *lhs, bool gather) {
   PairParams pp{};
   pp.g = gp;
   pp.gather = gather;
   pp.lhs = static_cast<const uint8_t *>(elem_ptr(lhs));
   pp.lhs_pitch = lhs->stride0 * 2ll;
   pp.div_fan = FastDiv::make(static_cast<uint32_t>(gp.fan));
-  pp.tile_rows = tile_rows;
   return pp;
 }
 
@@ -384,7 +383,9 @@ kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensor
   using Cfg = PairCfg;
   auto kern = grouped_pair_kernel<MODE>;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // adapters: see grouped_sm100.cuh
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.blockDim = dim3(kPairThreads, 1, 1);
   cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
   cfg.stream = stream;
@@ -407,6 +408,7 @@ kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensor
     resident[h->device].store(pairs);
   }
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min<long long>(tiles, pairs)), 1, 1);
+  if (MODE == PAIR_ADAPTERS) cfg.numAttrs = 2;
   CUDA_TRY(h, cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmR, tmU, pp));
   return launched(h, MODE == PAIR_GRADIENT ? "grouped_grad_pair" : MODE == PAIR_ADAPTERS ? "adapters_pair" : "grouped_pair");
 }
@@ -473,7 +475,7 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
   if (narrow)
     return gated ? launch_grouped<64, 2, false>(h, tmA, tmB, gp, tiles, stream)
                  : launch_grouped<64, 1, false>(h, tmA, tmB, gp, tiles, stream);
-  const PairParams pp = pair_params(gp, lhs, order != nullptr, bt);
+  const PairParams pp = pair_params(gp, lhs, order != nullptr);
   CUtensorMap box[2];
   for (int i = 0; i < 2; ++i)
     TRY(make_row_tmap(h, &box[i], elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
@@ -518,7 +520,7 @@ kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, 
   TRY(make_row_tmap(h, &tmA, elem_ptr(grad), grad->dtype, grad->size1, grad->size0,
                     grad->size0 > 1 ? grad->stride0 : (grad->size1 + 7) / 8 * 8, 64));
   *taken = true;
-  PairParams pp = pair_params(gp, lhs, true, 256);
+  PairParams pp = pair_params(gp, lhs, true);
   pp.grad = static_cast<const uint8_t *>(elem_ptr(grad));
   pp.grad_pitch = grad->stride0 * 2ll;
   return launch_pairs<PAIR_GRADIENT>(h, tmA, tmA, tmA, tmA, pp, tiles, stream);
@@ -1044,42 +1046,64 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
   TRY(launch_plan(h, PlanParams{c.index, rows, c.groups + 1, order, offsets, nullptr, positions, 32, 1}, stream));
 
   // the rows' products with their adapter's down, in two halves
+  CUtensorMap tmD, tmW, tmU, tmL, tmR;
+  LowTileParams lp{};
+  lp.offsets = offsets;
+  lp.order = order;
+  lp.groups = c.groups;
+  lp.positions = positions;
+  lp.x = static_cast<const uint8_t *>(elem_ptr(c.lhs));
+  lp.x_pitch = c.lhs->stride0 * 2ll;
+  lp.src_rows = rows;
+  lp.K = K;
+  lp.rank = rank;
+  lp.d_mn_major = d_mn;
+  lp.bf16 = c.lhs->dtype == KAPYB_BF16;
+  lp.a_bytes = rank <= 64 ? 8192 : 16384;
+  lp.scale = c.scale;
+  lp.alpha = 1.0f / c.ep.alpha;
+  lp.high = reinterpret_cast<uint16_t *>(scratch + sc.low);
+  lp.low = lp.high + static_cast<size_t>(positions) * low_pitch;
+  lp.pitch = low_pitch;
+  lp.status = h->status;
+  lp.wait_limit_us = h->wait_limit_us;
+  TRY(make_tmap(h, &tmD, elem_ptr(c.down), c.down->dtype, d_unit, d_other, c.groups, d_ld, c.down_stride, 64,
+                d_mn || rank <= 64 ? 64 : 128));
+  // tiles at most; CTAs per tile until two an SM are busy, each keeping four K blocks
+  const long long low_tiles = (positions + kLowTile - 1ll) / kLowTile + std::min(c.groups, rows);
+  const int num_kb = (K + 63) / 64;
+  lp.split = 1;
+  while (lp.split < 8 && low_tiles * lp.split < 2 * h->sm_count && lp.split * 8 <= num_kb) lp.split *= 2;
+  {
+    auto kern = lp.bf16 ? adapter_low_tile_kernel<true> : adapter_low_tile_kernel<false>;
+    CUDA_TRY(h, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLowTileSmem));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(static_cast<unsigned>(low_tiles) * lp.split, 1, 1);
+    cfg.blockDim = dim3(kLowTileThreads, 1, 1);
+    cfg.dynamicSmemBytes = kLowTileSmem;
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = lp.split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CUDA_TRY(h, cudaLaunchKernelEx(&cfg, kern, tmD, lp));
+    TRY(launched(h, "adapter_low_tile"));
+  }
+
   GroupedParams gp{};
-  gp.groups = c.groups;
   gp.rows = positions;
-  gp.cols = rank;
   gp.K = K;
-  gp.n_tiles = 1;
-  gp.num_kb = (K + 63) / 64;
+  gp.num_kb = num_kb;
   gp.offsets = offsets;
   gp.order = order;
   gp.fan = 1;
   gp.src_rows = rows;
-  gp.a_mn_major = d_mn;
-  gp.bf16 = c.lhs->dtype == KAPYB_BF16;
-  gp.out = scratch + sc.low;
-  gp.row_pitch = static_cast<uint32_t>(low_pitch) * 2u;
-  gp.out_dtype = c.lhs->dtype;
-  gp.pair_stores = 1;
-  gp.alpha = 1.0f / c.ep.alpha;
-  gp.bias_axis = 1;
-  gp.activation = KAPYB_ACT_NONE;
-  gp.rounding = KAPYB_RN;
-  gp.lo_bytes = static_cast<long long>(positions) * low_pitch * 2;
-  gp.group_scale = c.scale;
+  gp.bf16 = lp.bf16;
   gp.status = h->status;
   gp.wait_limit_us = h->wait_limit_us;
-  CUtensorMap tmD, tmW, tmU, tmL, tmR;
-  TRY(make_tmap(h, &tmD, elem_ptr(c.down), c.down->dtype, d_unit, d_other, c.groups, d_ld, c.down_stride, 64,
-                d_mn ? 64 : 128));
-  // narrow tiles while a wave of pairs holds them all
-  const int pairs = h->sm_count / 2;
-  int tile_rows = 64;
-  while (tile_rows < 256 && (positions + tile_rows - 1) / tile_rows > pairs) tile_rows *= 2;
-  PairParams pp = pair_params(gp, c.lhs, true, tile_rows);
-  TRY((launch_pairs<PAIR_FORWARD>(h, tmD, tmD, tmD, tmD, pp, (positions + tile_rows - 1ll) / tile_rows + c.groups,
-                                          stream)));
-
   gp.groups = c.groups + 1;
   gp.cols = c.out->size1;
   gp.n_tiles = n_tiles;
@@ -1094,9 +1118,7 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
   gp.bias_axis = c.ep.bias_axis;
   gp.activation = c.ep.activation;
   gp.rounding = c.ep.rounding;
-  gp.lo_bytes = 0;
-  gp.group_scale = nullptr;
-  pp = pair_params(gp, c.lhs, true, 256);
+  PairParams pp = pair_params(gp, c.lhs, true);
   pp.rank = rank;
   pp.up_mn_major = u_mn;
   pp.low_rows = positions;
