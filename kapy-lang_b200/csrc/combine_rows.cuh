@@ -8,6 +8,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "reduce.cuh"
 
 namespace kapyb {
 
@@ -56,37 +57,63 @@ __device__ __forceinline__ uint4 pack16B(const float (&f)[DT == KAPYB_F32 ? 4 : 
   return q;
 }
 
-// Rows and output of one type, 16-byte pieces throughout: a thread owns one piece of
-// one token and has all its rows' loads in flight (up to eight) before it adds.
+// 32 bytes of a row (16 of a 16-bit type, 8 of f32).
 template <int DT>
+__device__ __forceinline__ void fma32B(const Vec32B &v, float w, float (&acc)[DT == KAPYB_F32 ? 8 : 16]) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    if constexpr (DT == KAPYB_F32) {
+      acc[t] = fmaf(w, __uint_as_float(v.w[t]), acc[t]);
+    } else {
+      float lo, hi;
+      unpack2_16<DT>(v.w[t], lo, hi);
+      acc[2 * t] = fmaf(w, lo, acc[2 * t]);
+      acc[2 * t + 1] = fmaf(w, hi, acc[2 * t + 1]);
+    }
+  }
+}
+
+// Rows and output of one type, in pieces of 32 bytes (WIDE) or 16: a thread owns one
+// piece of one token and has the loads of four rows in flight before it adds them.
+// A row's rows lie anywhere, but a warp reads 1 KB runs of each.
+template <int DT, bool WIDE>
 __global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p, uint32_t pieces) {
-  constexpr int E = DT == KAPYB_F32 ? 4 : 8;
+  constexpr int esz = DT == KAPYB_F32 ? 4 : 2;
+  constexpr int BYTES = WIDE ? 32 : 16, E = BYTES / esz, U = 4;
   const unsigned long long id = static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x;
   const long long t = id / pieces;
   if (t >= p.tokens) return;
   const long long col = static_cast<long long>(id - t * static_cast<unsigned long long>(pieces)) * E;
-  constexpr int esz = DT == KAPYB_F32 ? 4 : 2;
   const char *base = static_cast<const char *>(p.rows) + col * esz;
+  const long long pitch = p.rows_s0 * esz;
   float acc[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.0f;
-  for (int j0 = 0; j0 < p.k; j0 += 8) {
-    uint4 q[8];
-    float w[8];
-    bool on[8];
+  for (int j0 = 0; j0 < p.k; j0 += U) {
+    Vec32B v[WIDE ? U : 1];
+    uint4 q[WIDE ? 1 : U];
+    float w[U];
+    bool on[U];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
+    for (int u = 0; u < U; ++u) {
       on[u] = false;
       if (j0 + u < p.k) {
         const int s = __ldg(p.slots + t * p.k + j0 + u);
         on[u] = s >= 0 && s < p.n_rows;
         w[u] = p.weights ? __ldg(p.weights + t * p.k + j0 + u) : 1.0f;
-        if (on[u]) q[u] = __ldg(reinterpret_cast<const uint4 *>(base + s * p.rows_s0 * esz));
+        if constexpr (WIDE) {
+          if (on[u]) v[u] = ld_nc_v8(base + s * pitch);
+        } else {
+          if (on[u]) q[u] = __ldg(reinterpret_cast<const uint4 *>(base + s * pitch));
+        }
       }
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (on[u]) {
+    for (int u = 0; u < U; ++u) {
+      if (!on[u]) continue;
+      if constexpr (WIDE) {
+        fma32B<DT>(v[u], w[u], acc);
+      } else {
         float f[E];
         unpack16B<DT>(q[u], f);
 #pragma unroll
@@ -94,7 +121,14 @@ __global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p,
       }
     }
   }
-  __stcs(reinterpret_cast<uint4 *>(static_cast<char *>(p.out) + (t * p.out_s0 + col) * esz), pack16B<DT>(acc));
+  uint4 *out = reinterpret_cast<uint4 *>(static_cast<char *>(p.out) + (t * p.out_s0 + col) * esz);
+#pragma unroll
+  for (int h = 0; h < BYTES / 16; ++h) {
+    float f[16 / esz];
+#pragma unroll
+    for (int i = 0; i < 16 / esz; ++i) f[i] = acc[h * (16 / esz) + i];
+    __stcs(out + h, pack16B<DT>(f));
+  }
 }
 
 // Any strides, types and alignment: one element per thread.

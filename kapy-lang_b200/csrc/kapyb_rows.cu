@@ -685,10 +685,17 @@ extern "C" KAPYB_API kapyb_status kapyb_matmul_grouped_grad(kapyb_handle h, cons
 
 namespace {
 
-// 16-byte pieces: unit column stride, 16-byte aligned base and row pitch
-bool pieces_ok(const kapyb_tensor2d *t) {
+// Whole pieces of `bytes`: unit column stride, base and row pitch aligned to them
+bool pieces_ok(const kapyb_tensor2d *t, int bytes) {
   const int64_t esz = dtype_size(t->dtype);
-  return t->stride1 == 1 && aligned16(elem_ptr(t)) && (t->stride0 * esz) % 16 == 0 && (t->size1 * esz) % 16 == 0;
+  return t->stride1 == 1 && reinterpret_cast<uintptr_t>(elem_ptr(t)) % bytes == 0 && (t->stride0 * esz) % bytes == 0 &&
+         (t->size1 * esz) % bytes == 0;
+}
+
+template <int DT>
+void launch_combine_vec(const CombineParams &p, bool wide, uint32_t per_row, int grid, cudaStream_t s) {
+  if (wide) combine_vec_kernel<DT, true><<<grid, 256, 0, s>>>(p, per_row);
+  else combine_vec_kernel<DT, false><<<grid, 256, 0, s>>>(p, per_row);
 }
 
 kapyb_status check_slots(kapyb_handle h, const char *call, const int32_t *slots, int k, const float *weights) {
@@ -737,8 +744,10 @@ extern "C" KAPYB_API kapyb_status kapyb_combine_rows(kapyb_handle h, const kapyb
   p.out_dtype = out->dtype;
   p.rounding = KAPYB_RN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool vec = rows->dtype == out->dtype && pieces_ok(rows) && pieces_ok(out);
-  const uint32_t per_row = vec ? static_cast<uint32_t>(p.cols * dtype_size(rows->dtype) / 16) : p.cols;
+  const bool vec = rows->dtype == out->dtype && pieces_ok(rows, 16) && pieces_ok(out, 16);
+  const bool wide = vec && pieces_ok(rows, 32);
+  const uint32_t per_row =
+      vec ? static_cast<uint32_t>(static_cast<int64_t>(p.cols) * dtype_size(rows->dtype) / (wide ? 32 : 16)) : p.cols;
   const unsigned long long threads = static_cast<unsigned long long>(p.tokens) * per_row;
   const unsigned long long blocks = (threads + 255) / 256;
   if (blocks > 0x7fffffffull) return fail(h, KAPYB_UNSUPPORTED, "%s: output too large", call);
@@ -746,11 +755,11 @@ extern "C" KAPYB_API kapyb_status kapyb_combine_rows(kapyb_handle h, const kapyb
   if (!vec)
     combine_any_kernel<<<grid, 256, 0, s>>>(p);
   else if (rows->dtype == KAPYB_F32)
-    combine_vec_kernel<KAPYB_F32><<<grid, 256, 0, s>>>(p, per_row);
+    launch_combine_vec<KAPYB_F32>(p, wide, per_row, grid, s);
   else if (rows->dtype == KAPYB_BF16)
-    combine_vec_kernel<KAPYB_BF16><<<grid, 256, 0, s>>>(p, per_row);
+    launch_combine_vec<KAPYB_BF16>(p, wide, per_row, grid, s);
   else
-    combine_vec_kernel<KAPYB_F16><<<grid, 256, 0, s>>>(p, per_row);
+    launch_combine_vec<KAPYB_F16>(p, wide, per_row, grid, s);
   return launched(h, vec ? "combine_vec" : "combine_any");
 }
 
@@ -809,8 +818,8 @@ extern "C" KAPYB_API kapyb_status kapyb_combine_rows_backward(kapyb_handle h, co
   }
   p.grad_weights = grad_weights;
   const int dt = grad_out->dtype;
-  const bool vec = pieces_ok(grad_out) && (!rows || (rows->dtype == dt && pieces_ok(rows))) &&
-                   (!grad_rows || (grad_rows->dtype == dt && pieces_ok(grad_rows)));
+  const bool vec = pieces_ok(grad_out, 16) && (!rows || (rows->dtype == dt && pieces_ok(rows, 16))) &&
+                   (!grad_rows || (grad_rows->dtype == dt && pieces_ok(grad_rows, 16)));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const long long units = vec ? static_cast<long long>(p.cols) * dtype_size(dt) / 16 : p.cols;
   const int threads = static_cast<int>(std::min(256ll, std::max(32ll, (units + 31) / 32 * 32)));

@@ -14,11 +14,14 @@
 // Without a bias the order of the scores is the order of the logits, so the logits
 // themselves are the keys, which is exact.  With a bias (or with groups ranked by a sum
 // of two scores) c is formed in 32 bits with a bound on its error, and a row in which
-// two neighbours of the ranking lie within that bound of one another is decided again
-// in 64 bits (choose_f64), about one row in a thousand on normally distributed logits.
+// two neighbours of the ranking lie within that bound of one another is put in order
+// again with the candidates' scores in 64 bits, one per lane; a row whose choice of
+// groups is that close, or with more than 32 candidates, is decided afresh (choose_f64).
+// On normally distributed logits that is one row in some thousand and ten thousand.
 // The bound for a sigmoid: with e = ex2.approx of a rounded product the relative error
 // of e is (|x| + 4) 2^-24, so s = 1 / (1 + e) is off by s (1 - s) (|x| + 4) 2^-24 for e
-// and 4 s 2^-24 for the sum and the reciprocal, below 6 2^-24 in all; 16 2^-24 is used.
+// and 4 s 2^-24 for the sum and the reciprocal: s (1 - s) |x| is below 0.23 and s (1 - s) 4
+// at most 1, so 6 2^-24 covers it.
 // For a softmax: s = e / z, e off by (d + 4) 2^-24 relative, d = max - x; z by the mean of
 // that over the row, at most ln(1024) + 4, and 37 roundings of its sum; s is at most 1 / z
 // and (d + 4) exp(-d) at most 4, so 64 2^-24 / z covers it.  The sum with the bias adds one
@@ -176,8 +179,52 @@ __device__ __forceinline__ uint32_t keep_groups(const RouteParams &p, Key key, i
   return kept;
 }
 
+// One expert's selection score in 64 bits; top and z as for 32 bits, in 64.
+__device__ __forceinline__ double score_f64(const RouteParams &p, float x, int e, double top, double z) {
+  const double xd = x;
+  double c = p.sigmoid ? 1.0 / (1.0 + exp(-xd)) : exp(xd - top) / z;
+  if (p.bias) c += static_cast<double>(p.bias[e]);
+  return c;
+}
+
+// A row's largest logit and the sum of its exponentials, in 64 bits.
+__device__ __forceinline__ void normaliser_f64(const RouteParams &p, long long row, int lane, double &top, double &z) {
+  float m = -INFINITY;
+  for (int e = lane; e < p.experts; e += 32) m = fmaxf(m, route_logit(p, row, e));
+  top = warp_max(m);
+  double s = 0.0;
+#pragma unroll 1
+  for (int e = lane; e < p.experts; e += 32) {
+    const float x = route_logit(p, row, e);
+    if (x != -INFINITY) s += exp(static_cast<double>(x) - top);
+  }
+  z = warp_sum64(s);
+}
+
+// Candidates of a row, lane j < n holding the j-th, in the order of their scores in 64
+// bits: lane j gets the j-th of them.
+__device__ __noinline__ int reorder_f64(const RouteParams &p, long long row, int n, int pick) {
+  const int lane = threadIdx.x & 31;
+  double top = 0.0, z = 1.0;
+  if (!p.sigmoid) normaliser_f64(p, row, lane, top, z);
+  unsigned long long key = 0ull;
+  if (lane < n) key = rank_key64(score_f64(p, route_logit(p, row, pick), pick, top, z));
+  int ahead = 0;
+  for (int i = 0; i < n; ++i) {
+    const unsigned long long k = __shfl_sync(0xffffffffu, key, i);
+    const int e = __shfl_sync(0xffffffffu, pick, i);
+    ahead += k > key || (k == key && e < pick);
+  }
+  int out = -1;
+  for (int i = 0; i < n; ++i) {
+    const int place = __shfl_sync(0xffffffffu, ahead, i), e = __shfl_sync(0xffffffffu, pick, i);
+    if (place == lane) out = e;
+  }
+  return out;
+}
+
 // One row's choice with every score in 64 bits: lane j < top_k returns the j-th choice, or
-// -1.  Every score is formed once, a lane's in parallel.
+// -1.  Rare, so its code is kept short: a lane's scores are formed one after the other.
 template <int VPT>
 __device__ __noinline__ int choose_f64(const RouteParams &p, long long row) {
   const int lane = threadIdx.x & 31;
@@ -185,26 +232,11 @@ __device__ __noinline__ int choose_f64(const RouteParams &p, long long row) {
   unsigned long long key[VPT];  // rank of expert e0 + i, 0 when it is masked
   {
     double top = 0.0, z = 1.0;
-    if (!p.sigmoid) {
-      float m = -INFINITY;
-      for (int i = 0; i < VPT; ++i)
-        if (e0 + i < p.experts) m = fmaxf(m, route_logit(p, row, e0 + i));
-      top = warp_max(m);
-      double s = 0.0;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const float x = e0 + i < p.experts ? route_logit(p, row, e0 + i) : -INFINITY;
-        if (x != -INFINITY) s += exp(static_cast<double>(x) - top);
-      }
-      z = warp_sum64(s);
-    }
-#pragma unroll
+    if (!p.sigmoid) normaliser_f64(p, row, lane, top, z);
+#pragma unroll 1
     for (int i = 0; i < VPT; ++i) {
       const float x = e0 + i < p.experts ? route_logit(p, row, e0 + i) : -INFINITY;
-      const double xd = x;
-      double c = p.sigmoid ? 1.0 / (1.0 + exp(-xd)) : exp(xd - top) / z;
-      if (p.bias && e0 + i < p.experts) c += static_cast<double>(p.bias[e0 + i]);
-      key[i] = x == -INFINITY ? 0ull : rank_key64(c);
+      key[i] = x == -INFINITY ? 0ull : rank_key64(score_f64(p, x, e0 + i, top, z));
     }
   }
   auto value_of = [](unsigned long long k) -> double {
@@ -216,7 +248,7 @@ __device__ __noinline__ int choose_f64(const RouteParams &p, long long row) {
     for (int q = 0; q < p.n_groups; ++q) {
       const int lo = q * p.group_size, hi = lo + p.group_size;
       unsigned long long k1 = 0ull, k2 = 0ull;  // this lane's two best of the group
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < VPT; ++i) {
         const unsigned long long k = e0 + i >= lo && e0 + i < hi ? key[i] : 0ull;
         k2 = k > k1 ? k1 : k > k2 ? k : k2;
@@ -232,7 +264,7 @@ __device__ __noinline__ int choose_f64(const RouteParams &p, long long row) {
       if (lane == q) mine = gk;
     }
     const uint32_t kept = keep_groups(p, mine, lane);
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < VPT; ++i)
       if (e0 + i < p.experts && !((kept >> ((e0 + i) / p.group_size)) & 1u)) key[i] = 0ull;
   }
@@ -240,7 +272,7 @@ __device__ __noinline__ int choose_f64(const RouteParams &p, long long row) {
   for (int j = 0; j < p.top_k; ++j) {
     unsigned long long best = 0ull;
     int at = -1;
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < VPT; ++i)
       if (key[i] > best) {
         best = key[i];
@@ -251,26 +283,22 @@ __device__ __noinline__ int choose_f64(const RouteParams &p, long long row) {
     const int w = __ffs(__ballot_sync(0xffffffffu, best == g)) - 1;
     const int i_w = __shfl_sync(0xffffffffu, at, w);
     if (lane == j) pick = w * VPT + i_w;
-    if (lane == w) {
-#pragma unroll
-      for (int i = 0; i < VPT; ++i)
-        if (i == at) key[i] = 0ull;
-    }
+    if (lane == w) key[at] = 0ull;
   }
   return pick;
 }
 
-// A lane's two best of what is behind (bound, index) in the ranking.
+// A lane's two best of what is behind (bound, index) in the ranking (ALL: of everything).
 struct LaneBest {
   uint32_t k1, k2;
   int i1, i2;
 };
-template <int VPT>
-__device__ __forceinline__ LaneBest two_best(const uint32_t (&key)[VPT], uint32_t bound, int behind) {
+template <int VPT, bool ALL>
+__device__ __forceinline__ LaneBest two_best(const uint32_t (&key)[VPT], uint32_t bound = 0u, int behind = 0) {
   LaneBest b{0u, 0u, 0, 0};
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const uint32_t k = key[i] < bound || (key[i] == bound && i > behind) ? key[i] : 0u;
+    const uint32_t k = ALL || key[i] < bound || (key[i] == bound && i > behind) ? key[i] : 0u;
     const bool first = k > b.k1, second = k > b.k2;
     b.k2 = first ? b.k1 : second ? k : b.k2;
     b.i2 = first ? b.i1 : second ? i : b.i2;
@@ -309,7 +337,7 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
       z = warp_sum(s);
     }
     if constexpr (SCORED) {
-      err = (p.sigmoid ? 16.0f : 64.0f / z) * 5.9604645e-8f + 1e-37f;
+      err = (p.sigmoid ? 6.0f : 64.0f / z) * 5.9604645e-8f + 1e-37f;
       const float rz = 1.0f / z;
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
@@ -323,7 +351,7 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
     }
   }
   bool unsure = false;
-  LaneBest b = two_best<VPT>(key, 0xffffffffu, VPT);
+  LaneBest b = two_best<VPT, true>(key);
   if (p.n_groups > 1) {
     uint32_t mine = 0u;
     float slack = 0.0f;  // error of this lane's group
@@ -340,7 +368,8 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
       }
     };
     const int lanes = p.group_size / VPT;  // lanes per group, when groups are whole lanes
-    if (lanes * VPT == p.group_size && (lanes & (lanes - 1)) == 0 && lanes <= 32) {
+    const bool whole = lanes * VPT == p.group_size && (lanes & (lanes - 1)) == 0 && lanes <= 32;
+    if (whole) {
       // every lane's two best belong to one group: join them over its lanes
       uint32_t k1 = b.k1, k2 = b.k2;
       for (int off = 1; off < lanes; off <<= 1) {
@@ -388,36 +417,53 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
       const uint32_t high = __reduce_max_sync(0xffffffffu, in ? 0u : mine);
       if (kept != 0u && high != 0u) unsure = !(key_value(low) - key_value(high) > 2.0f * warp_max(slack));
     }
-    int q = e0 / p.group_size, next = (q + 1) * p.group_size - e0;  // group of expert e0 + i
+    if (whole) {
+      // all of a lane's experts are kept or none
+      if (e0 < p.experts && !((kept >> (lane / lanes)) & 1u)) {
+        b = LaneBest{0u, 0u, 0, 0};
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      while (i >= next) {
-        ++q;
-        next += p.group_size;
+        for (int i = 0; i < VPT; ++i) key[i] = 0u;
       }
-      if (q < 32 && !((kept >> q) & 1u)) key[i] = 0u;
+    } else {
+      int q = e0 / p.group_size, next = (q + 1) * p.group_size - e0;  // group of expert e0 + i
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        while (i >= next) {
+          ++q;
+          next += p.group_size;
+        }
+        if (q < 32 && !((kept >> q) & 1u)) key[i] = 0u;
+      }
+      b = two_best<VPT, true>(key);
     }
-    b = two_best<VPT>(key, 0xffffffffu, VPT);
   }
   int pick = -1;
-  float prev = 0.0f;
+  float prev = 0.0f, last = 0.0f;  // scores: of the pick before, and of the top_k-th
   bool spent = false;  // this lane's second best is its candidate already
-  // with scores as keys one more rank is looked at: the best expert left out
-  const int steps = SCORED ? p.top_k + 1 : p.top_k;
-  for (int j = 0; j < steps && !unsure; ++j) {
+  bool close = false;  // two neighbours are within the error of one another
+  int found = 0;
+  // with scores as keys the candidates go on until one is clearly behind the top_k-th
+  for (int j = 0; j < (SCORED ? 32 : p.top_k) && !unsure; ++j) {
     const uint32_t g = __reduce_max_sync(0xffffffffu, b.k1);
     if (g == 0u) break;
     const int w = __ffs(__ballot_sync(0xffffffffu, b.k1 == g)) - 1;
     const int i_w = __shfl_sync(0xffffffffu, b.i1, w);
     if constexpr (SCORED) {
       const float c = key_value(g);
-      if (j > 0 && !(prev - c > 2.0f * err + (fabsf(prev) + fabsf(c)) * 1.1920929e-7f)) unsure = true;
+      const auto apart = [&](float above) {
+        return above - c > 2.0f * err + (fabsf(above) + fabsf(c)) * 1.1920929e-7f;
+      };
+      if (j >= p.top_k && apart(last)) break;
+      if (j > 0 && !apart(prev)) close = true;
+      if (j == 31 && p.top_k <= 31) unsure = true;  // more candidates than lanes
       prev = c;
+      if (j < p.top_k) last = c;
     }
-    if (lane == j && j < p.top_k) pick = w * VPT + i_w;
+    if (lane == j) pick = w * VPT + i_w;
+    found = j + 1;
     if (lane == w) {
       if (spent) {
-        b = two_best<VPT>(key, g, i_w);
+        b = two_best<VPT, false>(key, g, i_w);
         spent = false;
       } else {
         b.k1 = b.k2;
@@ -428,7 +474,14 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
     __syncwarp();
   }
   if constexpr (SCORED) {
+    // 32 picks of a top 32: the one left out has not been looked at
+    if (p.top_k == 32 && found == 32) {
+      const uint32_t g = __reduce_max_sync(0xffffffffu, b.k1);
+      const float c = key_value(g);
+      if (g != 0u && !(last - c > 2.0f * err + (fabsf(last) + fabsf(c)) * 1.1920929e-7f)) unsure = true;
+    }
     if (unsure) pick = choose_f64<VPT>(p, row);
+    else if (close) pick = reorder_f64(p, row, found, pick);
   }
 
   // weights of the choices, lane j the j-th
