@@ -51,6 +51,23 @@ class OnDevice {
   OnDevice on_device_(h);  \
   CUDA_TRY(h, on_device_.error())
 
+#define TRY(expr)                          \
+  do {                                     \
+    const kapyb_status st_ = (expr);       \
+    if (st_ != KAPYB_OK) return st_;       \
+  } while (0)
+
+// Lets a kernel use `bytes` of dynamic shared memory, once per device.
+template <auto Kernel>
+kapyb_status allow_smem(kapyb_handle h, int bytes) {
+  static std::atomic<bool> done[kMaxDevices];
+  if (!done[h->device].load()) {
+    CUDA_TRY(h, cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done[h->device].store(true);
+  }
+  return KAPYB_OK;
+}
+
 kapyb_status launched(kapyb_handle h, const char *name, int kernels = 1) {
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(h, KAPYB_CUDA_ERROR, "%s: launch failed: %s", name, cudaGetErrorString(e));
@@ -117,12 +134,6 @@ kapyb_status check_epilogue(kapyb_handle h, const char *call, const kapyb_epilog
 }
 
 const kapyb_epilogue kPlainEpilogue = {1.0f, nullptr, KAPYB_F32, 1, KAPYB_ACT_NONE, KAPYB_RN};
-
-#define TRY(expr)                          \
-  do {                                     \
-    const kapyb_status st_ = (expr);       \
-    if (st_ != KAPYB_OK) return st_;       \
-  } while (0)
 
 // ------------------------------------------------------------------- routing
 
@@ -276,8 +287,7 @@ namespace {
 
 kapyb_status launch_plan(kapyb_handle h, const PlanParams &p, cudaStream_t stream) {
   const size_t smem = plan_smem_bytes(p.groups);
-  CUDA_TRY(h, cudaFuncSetAttribute(plan_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   static_cast<int>(plan_smem_bytes(kPlanMaxGroups + 1))));
+  TRY(allow_smem<plan_rows_kernel>(h, static_cast<int>(plan_smem_bytes(kPlanMaxGroups + 1))));
   // A warp's piece is a whole number of 32-entry steps.  One CTA takes up to two steps a
   // warp; beyond that the work is spread over the cluster.
   int ctas = 1;
@@ -358,8 +368,8 @@ template <int BT, int MSETS, bool GRAD>
 kapyb_status launch_grouped(kapyb_handle h, const CUtensorMap &tmA, const CUtensorMap &tmB, const GroupedParams &gp,
                             long long tiles, cudaStream_t stream) {
   using Cfg = GroupedCfg<BT, MSETS>;
-  auto kern = grouped_tcgen05_kernel<BT, MSETS, GRAD>;
-  CUDA_TRY(h, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+  constexpr auto kern = grouped_tcgen05_kernel<BT, MSETS, GRAD>;
+  TRY(allow_smem<kern>(h, Cfg::SMEM_BYTES));
   const int grid = static_cast<int>(std::min<long long>(tiles, h->sm_count));
   kern<<<grid, kGroupedThreads, Cfg::SMEM_BYTES, stream>>>(tmA, tmB, gp);
   return launched(h, GRAD ? "grouped_grad_tcgen05" : "grouped_tcgen05");
@@ -1005,7 +1015,8 @@ kapyb_status adapters_decode(kapyb_handle h, const AdapterCall &c, cudaStream_t 
   TRY(make_row_tmap(h, &tmX, elem_ptr(c.lhs), c.lhs->dtype, c.lhs->size1, rows,
                     rows > 1 ? c.lhs->stride0 : (c.lhs->size1 + 7) / 8 * 8, p.wide));
   auto kern = bf ? adapter_decode_kernel<true> : adapter_decode_kernel<false>;
-  CUDA_TRY(h, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448 - 512));
+  TRY(bf ? allow_smem<adapter_decode_kernel<true>>(h, 232448 - 512)
+         : allow_smem<adapter_decode_kernel<false>>(h, 232448 - 512));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(static_cast<unsigned>(tiles) * split, 1, 1);
@@ -1085,7 +1096,8 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
   while (lp.split < 8 && low_tiles * lp.split < 2 * h->sm_count && lp.split * 8 <= num_kb) lp.split *= 2;
   {
     auto kern = lp.bf16 ? adapter_low_tile_kernel<true> : adapter_low_tile_kernel<false>;
-    CUDA_TRY(h, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLowTileSmem));
+    TRY(lp.bf16 ? allow_smem<adapter_low_tile_kernel<true>>(h, kLowTileSmem)
+                : allow_smem<adapter_low_tile_kernel<false>>(h, kLowTileSmem));
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     cfg.gridDim = dim3(static_cast<unsigned>(low_tiles) * lp.split, 1, 1);

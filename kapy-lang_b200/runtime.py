@@ -10,7 +10,6 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-from contextlib import nullcontext
 from typing import Optional, Sequence
 
 from . import _abi as abi
@@ -31,7 +30,25 @@ def _torch():
     return torch
 
 
+_I32 = 2 ** 31 - 1
+_codes: dict = {}
+
+
+def _current_stream(device: int) -> int:
+    """torch's current stream on `device`, without the Stream object where torch can."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def dtype_code(dt) -> int:
+    code = _codes.get(dt)
+    if code is None:
+        code = _codes[dt] = _dtype_code(dt)
+    return code
+
+
+def _dtype_code(dt) -> int:
     torch = _torch()
     if dt == torch.float16:
         return abi.F16
@@ -189,6 +206,7 @@ class Handle:
             msg = self._lib.kapyb_last_error_string(None).decode()
             raise KapybError(st, msg)
         self.device = int(device)
+        self._torch_device = _torch().device("cuda", self.device)
 
     def close(self):
         if getattr(self, "_h", None) is not None and self._h:
@@ -437,54 +455,60 @@ class Handle:
         return out
 
     # ------------------------------------------- rows that pick their weights
+    # These calls are often shorter than the host code in front of them, so that code
+    # looks at each tensor once and builds nothing it does not pass on.
     def _launch_stream(self, stream):
-        """(ctypes stream, context in which tensors the call allocates belong to it)."""
+        """(stream as an integer, context in which tensors the call allocates belong to it;
+        None: the current stream, no context needed)."""
         torch = _torch()
         if stream is None:
-            return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream), nullcontext()
+            return _current_stream(self.device), None
         if not hasattr(stream, "cuda_stream"):
             stream = torch.cuda.ExternalStream(int(stream), device=self.device)
-        return C.c_void_p(stream.cuda_stream), torch.cuda.stream(stream)
+        return stream.cuda_stream, torch.cuda.stream(stream)
 
-    def _on_device(self, **tensors):
-        for name, t in tensors.items():
-            if t is None:
-                continue
+    def _new(self, where, shape, dtype, zero=False):
+        torch = _torch()
+        make = torch.zeros if zero else torch.empty
+        if where is None:  # sizes one by one: a tuple of them costs torch 0.8 us more
+            return make(*shape, dtype=dtype, device=self._torch_device)
+        with where:
+            return make(*shape, dtype=dtype, device=self._torch_device)
+
+    def _here(self, name, t):
+        """The tensor's address, once it is known to be on the handle's GPU."""
+        if t.get_device() != self.device:
             if not t.is_cuda:
                 raise ValueError(f"{name} must be a CUDA tensor")
-            if t.device.index != self.device:
-                raise ValueError(f"{name} is on {t.device}, the handle on cuda:{self.device}")
+            raise ValueError(f"{name} is on {t.device}, the handle on cuda:{self.device}")
+        return t.data_ptr()
 
-    def _dense(self, dtype, **tensors):
-        """Plain device arrays: right element type, contiguous, on the handle's GPU."""
-        self._on_device(**tensors)
-        for name, t in tensors.items():
-            if t is None:
-                continue
-            if t.dtype != dtype:
-                raise ValueError(f"{name} must have element type {dtype}, not {t.dtype}")
-            if not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous")
+    def _dense(self, name, t, dtype):
+        """Address of a plain device array: right element type, contiguous, on the GPU."""
+        if t.dtype is not dtype:
+            raise ValueError(f"{name} must have element type {dtype}, not {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        return self._here(name, t)
 
-    @staticmethod
-    def _ptr(t):
-        return None if t is None else C.c_void_p(t.data_ptr())
+    def _matrix(self, name, t):
+        """Descriptor of a 2-D tensor on the handle's GPU."""
+        if t.dim() != 2:
+            raise ValueError("kapy tensors are rank 2")
+        (rows, cols), (s0, s1) = t.shape, t.stride()
+        if rows > _I32 or cols > _I32 or s0 > _I32 or s1 > _I32:
+            raise ValueError("sizes and strides must fit i32")
+        return abi.Tensor2d(self._here(name, t), 0, rows, cols, s0, s1, dtype_code(t.dtype), 0, 0, 0)
 
-    @staticmethod
-    def _grouped2d(t, name):
-        """Descriptor of the first matrix of [groups, rows, cols] and the group stride."""
+    def _stack(self, name, t):
+        """Descriptor of the first matrix of [groups, rows, columns] and the group stride."""
         if t.dim() != 3:
             raise ValueError(f"{name} must be [groups, rows, columns]")
-        d = abi.Tensor2d(t.data_ptr(), 0, t.shape[1], t.shape[2], t.stride(1), t.stride(2),
-                         dtype_code(t.dtype), abi.PAD_ZERO, 0, 0)
-        for v in (t.shape[1], t.shape[2], t.stride(1), t.stride(2)):
-            if v >= 2 ** 31:
-                raise ValueError("sizes and strides must fit i32")
-        return d, t.stride(0)
-
-    def _routing(self, top_k, score, groups, top_groups, group_best, renormalize, scale):
-        return abi.Routing(int(score), int(top_k), int(groups), int(top_groups), int(group_best),
-                           1 if renormalize else 0, float(scale))
+        (_, rows, cols), (stride, s0, s1) = t.shape, t.stride()
+        if rows > _I32 or cols > _I32 or s0 > _I32 or s1 > _I32:
+            raise ValueError("sizes and strides must fit i32")
+        return abi.Tensor2d(self._here(name, t), 0, rows, cols, s0, s1, dtype_code(t.dtype), 0, 0,
+                            0), stride
 
     def route(self, logits, top_k: int, *, bias=None, score: int = abi.SCORE_SOFTMAX,
               groups: int = 1, top_groups: Optional[int] = None, group_best: int = 1,
@@ -493,27 +517,29 @@ class Handle:
         """Routing of rows to experts (kapyb_route): (weights f32 [T, k], experts int32
         [T, k]) of logits [T, E]; the bias (f32 [E]) takes part in the choice only."""
         torch = _torch()
-        self._on_device(logits=logits)
-        self._dense(torch.float32, bias=bias, weights=weights)
-        self._dense(torch.int32, experts=experts)
-        tl = tensor2d(logits)
-        shape = (logits.shape[0], int(top_k))
-        if bias is not None and tuple(bias.shape) != (logits.shape[1],):
-            raise ValueError("bias must have one value per expert")
-        for name, t in (("weights", weights), ("experts", experts)):
-            if t is not None and tuple(t.shape) != shape:
-                raise ValueError(f"{name} must have shape {shape}")
-        r = self._routing(top_k, score, groups, groups if top_groups is None else top_groups,
-                          group_best, renormalize, scale)
+        tl = self._matrix("logits", logits)
+        shape = (tl.size0, int(top_k))
+        at_bias = None
+        if bias is not None:
+            if bias.shape != (tl.size1,):
+                raise ValueError("bias must have one value per expert")
+            at_bias = self._dense("bias", bias, torch.float32)
+        r = abi.Routing(int(score), shape[1], int(groups),
+                        int(groups if top_groups is None else top_groups), int(group_best),
+                        1 if renormalize else 0, float(scale))
         s, where = self._launch_stream(stream)
-        with where:
-            if weights is None:
-                weights = torch.empty(max(0, shape[0]), max(0, shape[1]), device=logits.device)
-            if experts is None:
-                experts = torch.empty(max(0, shape[0]), max(0, shape[1]), device=logits.device,
-                                      dtype=torch.int32)
-        st = self._lib.kapyb_route(self._h, C.byref(tl), self._ptr(bias), C.byref(r),
-                                   self._ptr(weights), self._ptr(experts), s)
+        held = (shape[0], max(0, shape[1]))  # a refused top_k is refused by the call itself
+        if weights is None:
+            weights = self._new(where, held, torch.float32)
+        elif weights.shape != shape:
+            raise ValueError(f"weights must have shape {shape}")
+        if experts is None:
+            experts = self._new(where, held, torch.int32)
+        elif experts.shape != shape:
+            raise ValueError(f"experts must have shape {shape}")
+        st = self._lib.kapyb_route(self._h, tl, at_bias, r,
+                                   self._dense("weights", weights, torch.float32),
+                                   self._dense("experts", experts, torch.int32), s)
         if st != abi.OK:
             self._raise(st)
         return weights, experts
@@ -523,21 +549,17 @@ class Handle:
         """Gradient of the logits (kapyb_route_backward) from the gradient of route's
         weights; `experts`, score, renormalize and scale as in the forward call."""
         torch = _torch()
-        self._on_device(logits=logits, out=out)
-        self._dense(torch.int32, experts=experts)
-        self._dense(torch.float32, grad_weights=grad_weights)
-        if experts.dim() != 2 or experts.shape[0] != logits.shape[0] or \
+        tl = self._matrix("logits", logits)
+        if experts.dim() != 2 or experts.shape[0] != tl.size0 or \
                 grad_weights.shape != experts.shape:
             raise ValueError("experts and grad_weights must be [rows of logits, k]")
-        tl = tensor2d(logits)
-        r = self._routing(experts.shape[1], score, 1, 1, 1, renormalize, scale)
+        r = abi.Routing(int(score), experts.shape[1], 1, 1, 1, 1 if renormalize else 0, float(scale))
         s, where = self._launch_stream(stream)
         if out is None:
-            with where:
-                out = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        to = tensor2d(out)
-        st = self._lib.kapyb_route_backward(self._h, C.byref(tl), C.byref(r), self._ptr(experts),
-                                            self._ptr(grad_weights), C.byref(to), s)
+            out = self._new(where, logits.shape, logits.dtype)
+        st = self._lib.kapyb_route_backward(
+            self._h, tl, r, self._dense("experts", experts, torch.int32),
+            self._dense("grad_weights", grad_weights, torch.float32), self._matrix("out", out), s)
         if st != abi.OK:
             self._raise(st)
         return out
@@ -546,33 +568,41 @@ class Handle:
         """Stable counting sort of an int32 index (any shape) into groups
         (kapyb_plan_rows): (order [n], offsets [groups + 1], slots of index's shape)."""
         torch = _torch()
-        self._dense(torch.int32, index=index, order=order, offsets=offsets, slots=slots)
-        n = index.numel()
-        for name, t, want in (("order", order, n), ("offsets", offsets, int(groups) + 1),
-                              ("slots", slots, n)):
-            if t is not None and t.numel() != want:
-                raise ValueError(f"{name} must have {want} elements")
+        n, groups = index.numel(), int(groups)
         s, where = self._launch_stream(stream)
-        with where:
-            new = lambda *shape: torch.empty(*shape, device=index.device, dtype=torch.int32)
-            order = new(n) if order is None else order
-            offsets = new(max(0, int(groups)) + 1) if offsets is None else offsets
-            slots = new(index.shape) if slots is None else slots
-        st = self._lib.kapyb_plan_rows(self._h, self._ptr(index), n, int(groups),
-                                       self._ptr(order), self._ptr(offsets), self._ptr(slots), s)
+        if order is None:
+            order = self._new(where, (n,), torch.int32)
+        elif order.numel() != n:
+            raise ValueError(f"order must have {n} elements")
+        if offsets is None:
+            offsets = self._new(where, (max(0, groups) + 1,), torch.int32)
+        elif offsets.numel() != groups + 1:
+            raise ValueError(f"offsets must have {groups + 1} elements")
+        if slots is None:
+            slots = self._new(where, index.shape or (1,), torch.int32)
+        elif slots.numel() != n:
+            raise ValueError(f"slots must have {n} elements")
+        st = self._lib.kapyb_plan_rows(
+            self._h, self._dense("index", index, torch.int32), n, groups,
+            self._dense("order", order, torch.int32), self._dense("offsets", offsets, torch.int32),
+            self._dense("slots", slots, torch.int32), s)
         if st != abi.OK:
             self._raise(st)
         return order, offsets, slots
 
-    def _check_plan(self, offsets, order, fan, groups, rows):
+    def _plan(self, offsets, order, fan, groups, rows):
+        """Addresses of a plan's offsets and order."""
         torch = _torch()
-        self._dense(torch.int32, offsets=offsets, order=order)
         if offsets.numel() != groups + 1:
             raise ValueError(f"offsets must have {groups + 1} elements")
-        if order is not None and order.numel() != rows:
+        at = self._dense("offsets", offsets, torch.int32)
+        if order is None:
+            return at, None
+        if order.numel() != rows:
             raise ValueError(f"order must have {rows} elements")
-        if order is not None and int(fan) < 1:
+        if int(fan) < 1:
             raise ValueError("fan must be at least 1")
+        return at, self._dense("order", order, torch.int32)
 
     def matmul_grouped(self, lhs, rhs, offsets, out=None, *, order=None, fan: int = 1,
                        alpha: float = 1.0, bias=None, activation: int = abi.ACT_NONE,
@@ -581,25 +611,24 @@ class Handle:
         (kapyb_matmul_grouped): row = order[p] // fan, or p without an order.  rhs is
         [groups, K, N]; gated: [groups, K, 2 N], gate columns then up columns, out =
         activation(gate) * up.  bias: [groups, columns of rhs]."""
-        torch = _torch()
-        self._on_device(lhs=lhs, rhs=rhs, out=out, bias=bias)
-        tr, stride = self._grouped2d(rhs, "rhs")
-        rows = order.numel() if order is not None else lhs.shape[0]
-        self._check_plan(offsets, order, fan, rhs.shape[0], rows)
-        if bias is not None and tuple(bias.shape) != (rhs.shape[0], rhs.shape[2]):
-            raise ValueError("bias must be [groups, columns of rhs]")
-        if out is not None and out.shape[0] != rows:
-            raise ValueError(f"out must have {rows} rows")
+        tl = self._matrix("lhs", lhs)
+        tr, group_stride = self._stack("rhs", rhs)
+        groups = rhs.shape[0]
+        rows = order.numel() if order is not None else tl.size0
+        at_offsets, at_order = self._plan(offsets, order, fan, groups, rows)
+        if bias is not None:
+            if bias.shape != (groups, tr.size1):
+                raise ValueError("bias must be [groups, columns of rhs]")
+            self._here("bias", bias)
         s, where = self._launch_stream(stream)
         if out is None:
-            with where:
-                out = torch.empty(rows, rhs.shape[2] // 2 if gated else rhs.shape[2],
-                                  device=lhs.device, dtype=out_dtype or lhs.dtype)
-        tl, to = tensor2d(lhs), tensor2d(out)
+            out = self._new(where, (rows, tr.size1 // 2 if gated else tr.size1), out_dtype or lhs.dtype)
+        elif out.shape[0] != rows:
+            raise ValueError(f"out must have {rows} rows")
         ep = self._epilogue(alpha, bias, 1, activation, rounding)
-        st = self._lib.kapyb_matmul_grouped(self._h, C.byref(tl), C.byref(tr), rhs.shape[0], stride,
-                                            self._ptr(offsets), self._ptr(order), int(fan),
-                                            C.byref(to), C.byref(ep), 1 if gated else 0, s)
+        st = self._lib.kapyb_matmul_grouped(self._h, tl, tr, groups, group_stride, at_offsets,
+                                            at_order, int(fan), self._matrix("out", out), ep,
+                                            1 if gated else 0, s)
         if st != abi.OK:
             self._raise(st)
         return out
@@ -609,22 +638,18 @@ class Handle:
                             stream=None):
         """Gradient of matmul_grouped's weights (kapyb_matmul_grouped_grad): [groups, K, N]
         from lhs, the gradient of the products [positions, N] and the plan they ran on."""
-        torch = _torch()
-        self._on_device(lhs=lhs, grad=grad, out=out)
+        tl, tg = self._matrix("lhs", lhs), self._matrix("grad", grad)
         groups = offsets.numel() - 1
-        self._check_plan(offsets, order, fan, groups, grad.shape[0])
+        at_offsets, at_order = self._plan(offsets, order, fan, groups, tg.size0)
         s, where = self._launch_stream(stream)
         if out is None:
-            with where:
-                out = torch.empty(groups, lhs.shape[1], grad.shape[1], device=lhs.device,
-                                  dtype=out_dtype or lhs.dtype)
-        if out.shape[0] != groups:
+            out = self._new(where, (groups, tl.size1, tg.size1), out_dtype or lhs.dtype)
+        elif out.shape[0] != groups:
             raise ValueError(f"out must have {groups} groups")
-        tl, tg = tensor2d(lhs), tensor2d(grad)
-        to, stride = self._grouped2d(out, "out")
-        st = self._lib.kapyb_matmul_grouped_grad(self._h, C.byref(tl), C.byref(tg), groups,
-                                                 self._ptr(offsets), self._ptr(order), int(fan),
-                                                 C.byref(to), stride, float(alpha), int(rounding), s)
+        to, group_stride = self._stack("out", out)
+        st = self._lib.kapyb_matmul_grouped_grad(self._h, tl, tg, groups, at_offsets, at_order,
+                                                 int(fan), to, group_stride, float(alpha),
+                                                 int(rounding), s)
         if st != abi.OK:
             self._raise(st)
         return out
@@ -632,21 +657,19 @@ class Handle:
     def combine_rows(self, rows, slots, out=None, *, weights=None, out_dtype=None, stream=None):
         """out[t] = sum_j weights[t, j] * rows[slots[t, j]] (kapyb_combine_rows)."""
         torch = _torch()
-        self._on_device(rows=rows, out=out)
-        self._dense(torch.int32, slots=slots)
-        self._dense(torch.float32, weights=weights)
+        tr = self._matrix("rows", rows)
         if slots.dim() != 2 or (weights is not None and weights.shape != slots.shape):
             raise ValueError("slots and weights must be [tokens, k]")
+        tokens, k = slots.shape
         s, where = self._launch_stream(stream)
         if out is None:
-            with where:
-                out = torch.empty(slots.shape[0], rows.shape[1], device=rows.device,
-                                  dtype=out_dtype or rows.dtype)
-        if out.shape[0] != slots.shape[0]:
+            out = self._new(where, (tokens, tr.size1), out_dtype or rows.dtype)
+        elif out.shape[0] != tokens:
             raise ValueError("out must have a row per token")
-        tr, to = tensor2d(rows), tensor2d(out)
-        st = self._lib.kapyb_combine_rows(self._h, C.byref(tr), self._ptr(slots), slots.shape[1],
-                                          self._ptr(weights), C.byref(to), s)
+        st = self._lib.kapyb_combine_rows(
+            self._h, tr, self._dense("slots", slots, torch.int32), k,
+            None if weights is None else self._dense("weights", weights, torch.float32),
+            self._matrix("out", out), s)
         if st != abi.OK:
             self._raise(st)
         return out
@@ -657,22 +680,21 @@ class Handle:
         grad_weights); the latter is None for a sum without weights.  A given grad_rows
         keeps the rows no slot names; an allocated one starts as zeros."""
         torch = _torch()
-        self._on_device(rows=rows, grad_out=grad_out, grad_rows=grad_rows)
-        self._dense(torch.int32, slots=slots)
-        self._dense(torch.float32, weights=weights, grad_weights=grad_weights)
-        if slots.dim() != 2 or grad_out.shape[0] != slots.shape[0] or \
+        tr, tg = self._matrix("rows", rows), self._matrix("grad_out", grad_out)
+        if slots.dim() != 2 or tg.size0 != slots.shape[0] or \
                 any(t is not None and t.shape != slots.shape for t in (weights, grad_weights)):
             raise ValueError("slots, weights and grad_weights must be [rows of grad_out, k]")
         s, where = self._launch_stream(stream)
-        with where:
-            if grad_rows is None:
-                grad_rows = torch.zeros(rows.shape, device=rows.device, dtype=rows.dtype)
-            if grad_weights is None and weights is not None:
-                grad_weights = torch.empty(slots.shape, device=rows.device, dtype=torch.float32)
-        tr, tg, td = tensor2d(rows), tensor2d(grad_out), tensor2d(grad_rows)
+        if grad_rows is None:
+            grad_rows = self._new(where, rows.shape, rows.dtype, zero=True)
+        if grad_weights is None and weights is not None:
+            grad_weights = self._new(where, slots.shape, torch.float32)
         st = self._lib.kapyb_combine_rows_backward(
-            self._h, C.byref(tr), self._ptr(slots), slots.shape[1], self._ptr(weights),
-            C.byref(tg), C.byref(td), self._ptr(grad_weights), s)
+            self._h, tr, self._dense("slots", slots, torch.int32), slots.shape[1],
+            None if weights is None else self._dense("weights", weights, torch.float32), tg,
+            self._matrix("grad_rows", grad_rows),
+            None if grad_weights is None else self._dense("grad_weights", grad_weights, torch.float32),
+            s)
         if st != abi.OK:
             self._raise(st)
         return grad_rows, grad_weights
@@ -685,35 +707,32 @@ class Handle:
         row t adds scale[i] * (lhs[t] . down[i]) . up[i], i = index[t]; an index outside
         the adapters adds nothing.  down [groups, K, rank], up [groups, rank, N]."""
         torch = _torch()
-        self._on_device(lhs=lhs, rhs=rhs, down=down, up=up, out=out, bias=bias)
-        self._dense(torch.int32, index=index)
-        self._dense(torch.float32, scale=scale)
-        td, d_stride = self._grouped2d(down, "down")
-        tu, u_stride = self._grouped2d(up, "up")
+        tl, tr = self._matrix("lhs", lhs), self._matrix("rhs", rhs)
+        td, down_stride = self._stack("down", down)
+        tu, up_stride = self._stack("up", up)
         groups = down.shape[0]
         if up.shape[0] != groups or (scale is not None and scale.numel() != groups):
             raise ValueError("down, up and scale must have as many adapters")
-        if index.numel() != lhs.shape[0]:
+        if index.numel() != tl.size0:
             raise ValueError("index must have an element per row of lhs")
-        if bias is not None and bias.numel() != (rhs.shape[1] if bias_axis == 1 else lhs.shape[0]):
-            raise ValueError("bias must have a value per column (bias_axis 1) or row (0)")
+        if bias is not None:
+            if bias.numel() != (tr.size1 if bias_axis == 1 else tl.size0):
+                raise ValueError("bias must have a value per column (bias_axis 1) or row (0)")
+            self._here("bias", bias)
         s, where = self._launch_stream(stream)
-        nbytes = int(self._lib.kapyb_matmul_adapters_scratch(lhs.shape[0], groups, down.shape[2]))
-        with where:
-            scratch = torch.empty(nbytes, device=lhs.device, dtype=torch.uint8)
-            if out is None:
-                out = torch.empty(lhs.shape[0], rhs.shape[1], device=lhs.device,
-                                  dtype=out_dtype or lhs.dtype)
-        tl, tr, to = tensor2d(lhs), tensor2d(rhs), tensor2d(out)
+        nbytes = self._lib.kapyb_matmul_adapters_scratch(tl.size0, groups, td.size1)
+        scratch = self._new(where, (nbytes,), torch.uint8)
+        if out is None:
+            out = self._new(where, (tl.size0, tr.size1), out_dtype or lhs.dtype)
         ep = self._epilogue(alpha, bias, bias_axis, activation, rounding)
         st = self._lib.kapyb_matmul_adapters(
-            self._h, C.byref(tl), C.byref(tr), groups, C.byref(td), d_stride, C.byref(tu), u_stride,
-            self._ptr(index), self._ptr(scale), C.byref(to), C.byref(ep), self._ptr(scratch), nbytes,
-            s)
+            self._h, tl, tr, groups, td, down_stride, tu, up_stride,
+            self._dense("index", index, torch.int32),
+            None if scale is None else self._dense("scale", scale, torch.float32),
+            self._matrix("out", out), ep, scratch.data_ptr(), nbytes, s)
         if st != abi.OK:
             self._raise(st)
         return out
-
 
 def shard_range(total: int, parts: int, rank: int, align: int = 1):
     """[begin, end) of `total` units owned by `rank` (blocks of `align`)."""
