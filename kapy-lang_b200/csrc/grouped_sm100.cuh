@@ -70,7 +70,8 @@ struct GroupedParams {
   void *out;
   uint32_t row_pitch;           // bytes between output rows, below 2^26; unit stride on n
   long long group_bytes;        // gradient: bytes between groups
-  int out_dtype, pair_stores;   // pair_stores: two 16-bit columns may be stored as one word
+  int out_dtype, wide_stores;   // wide_stores: two 16-bit columns may be stored as one word,
+                                // or four f32 ones added to as 16 bytes
   float alpha;
   const void *bias;      // [groups, bias_cols]; adapters: [cols], or [source rows] with bias_axis 0
   int bias_dtype, bias_cols, bias_axis, activation, rounding;
@@ -277,6 +278,44 @@ __device__ __forceinline__ void store_rows16(char *at, uint32_t pitch, const flo
   }
 }
 
+// Four rows of four neighbouring lanes' columns: lane l (of four) goes from rows 0..3 of its
+// own column to all four columns of row l.  Two exchanges, two values each.
+__device__ __forceinline__ float4 transpose4(float a0, float a1, float a2, float a3, int lane) {
+  const bool odd = lane & 1, high = lane & 2;
+  const float s0 = __shfl_xor_sync(0xffffffffu, odd ? a0 : a1, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? a2 : a3, 1);
+  // rows 0 and 2 in even lanes, 1 and 3 in odd ones, columns (even, odd) of the pair
+  const float lo0 = odd ? s0 : a0, hi0 = odd ? a1 : s0, lo1 = odd ? s1 : a2, hi1 = odd ? a3 : s1;
+  const float t0 = __shfl_xor_sync(0xffffffffu, high ? lo0 : lo1, 2), t1 = __shfl_xor_sync(0xffffffffu, high ? hi0 : hi1, 2);
+  return high ? make_float4(t0, t1, lo1, hi1) : make_float4(lo0, hi0, t0, t1);
+}
+
+// f32 rows added to memory, in 16-byte pieces where addresses and columns allow.  One
+// thread alone adds to an element, and its additions to one address keep their order, so
+// the sum is the same bits on every run.
+__device__ __forceinline__ void add_rows32(char *at, uint32_t pitch, const float (&f)[32], int left, int lane,
+                                           bool mine, bool pieces) {
+  if (pieces && __all_sync(0xffffffffu, mine)) {
+    char *base = at - (lane & 3) * 4 + (lane & 3) * static_cast<unsigned long long>(pitch);
+    uint32_t off = 0u;
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 v = transpose4(f[j], f[j + 1], f[j + 2], f[j + 3], lane);
+      if (j + (lane & 3) < left)
+        asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(base + off), "f"(v.x),
+                     "f"(v.y), "f"(v.z), "f"(v.w)
+                     : "memory");
+      off += 4u * pitch;
+    }
+  } else if (mine) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left)
+        asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(at + static_cast<unsigned long long>(j) * pitch),
+                     "f"(f[j])
+                     : "memory");
+  }
+}
+
 // p.row_pitch (bytes) is below 2^26, so 32 rows span less than 2^31.
 template <int R>
 __device__ __forceinline__ void grouped_store(const GroupedParams &p, char *at, const float (&f)[R], int left,
@@ -297,7 +336,7 @@ __device__ __forceinline__ void grouped_store(const GroupedParams &p, char *at, 
     }
     return;
   }
-  const bool pairs = p.pair_stores != 0;
+  const bool pairs = p.wide_stores != 0;
   if (p.out_dtype == KAPYB_BF16) {
     if (p.rounding) store_rows16<KAPYB_BF16, 1>(at, pitch, f, left, lane, mine, both, pairs);
     else store_rows16<KAPYB_BF16, 0>(at, pitch, f, left, lane, mine, both, pairs);
@@ -338,7 +377,7 @@ __device__ __forceinline__ void scatter_rows16(char *col, uint32_t pitch, const 
 __device__ __forceinline__ void grouped_scatter32(const GroupedParams &p, char *col, const float (&f)[32], int to,
                                                   int lane, bool mine, bool both) {
   const uint32_t pitch = p.row_pitch;
-  const bool pairs = p.pair_stores != 0;
+  const bool pairs = p.wide_stores != 0;
   if (p.out_dtype == KAPYB_F32) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
@@ -640,6 +679,14 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
 // In the gradient the rows are the contraction: lhs is always gathered (zeros behind
 // the group's end); grad lies in plan order and comes by TMA, but for the block that
 // holds the group's end, which the gathering warps bring as well, with zeros behind it.
+// The tensor core's f32 additions truncate: a sum loses about 1e-9 of itself per row (9e-6
+// over 8192 rows, measured; rounded sums 2e-7).  So an f32 gradient is accumulated 1024
+// rows at a time (1e-6 at any length): the epilogue joins two such pieces, one from each
+// accumulator slot, rounded to nearest, and adds further pairs to what it has stored.  That
+// addition is what it costs: reductions in L2 run at 1.8 TB/s, so 8192 rows of 4096 x 4096
+// take 289 us and not 205; reading, adding and storing took 408.  A group of up to
+// 2048 rows needs none of it.  What is rounded to 16 bits in the end stays in one
+// accumulator.
 
 // Adapters: the rows are a plan sorted by adapter whose groups start at multiples of 32
 // (gaps and rows without an adapter included), and the tile's main loop over the shared
@@ -667,6 +714,7 @@ struct PairParams {
   long long lhs_pitch;   // bytes between rows
   const uint8_t *grad;   // gradient: the same of grad
   long long grad_pitch;
+  int piece_kb;          // gradient: K blocks to an accumulator
   FastDiv div_fan;
   // adapters: g.groups = adapters + 1 (the last group: rows without one)
   int rank, up_mn_major;
@@ -1001,13 +1049,31 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
+    // the accumulator goes to the epilogue warps of both CTAs
+    auto publish = [&]() {
+      if (ptx::elect_one()) {
+        ptx::umma_commit<2>(ptx::smem_u32(&tfull_bar[acc]));
+        ptx::umma_commit<2>(ptx::mapa(ptx::smem_u32(&tfull_bar[acc]), 1));
+      }
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    };
     for (int idx = unit; ok && idx < total; idx += units) {
       const GroupedTile t = pair_tile<MODE>(p, table, idx);
       const uint32_t idesc = ptx::make_idesc_f16(p.bf16, a_mn, b_mn, 256, t.wide);
-      if (!wait_all(ptx::smem_u32(&tempty_bar[acc]), acc_phase ^ 1u)) break;
+      // gradient: one accumulator after the other, all but the last published in between
+      const int pieces = GRAD ? max(1, (t.num_kb + pp.piece_kb - 1) / pp.piece_kb) : 1;
+      uint32_t d = 0u;
+      for (int piece = 0; ok && piece < pieces; ++piece) {
+      const int kb_end = GRAD ? min(t.num_kb, (piece + 1) * pp.piece_kb) : t.num_kb;
+      if (!wait_all(ptx::smem_u32(&tempty_bar[acc]), acc_phase ^ 1u)) {
+        ok = false;
+        break;
+      }
       ptx::tc_fence_after();
-      const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BT);
-      for (int kb = 0; kb < t.num_kb; ++kb) {
+      d = tmem_base + static_cast<uint32_t>(acc * BT);
+      const int kb_begin = GRAD ? piece * pp.piece_kb : 0;
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
         if (!wait_all(ptx::smem_u32(&full_bar[stage]), phase)) {
           ok = false;
           break;
@@ -1020,7 +1086,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           for (int k = 0; k < 4; ++k) {
             const uint64_t ad = (static_cast<uint64_t>(hi) << 32) | (a_lo + k * a_step);
             const uint64_t bd = (static_cast<uint64_t>(hi) << 32) | (b_lo + k * b_step);
-            ptx::umma_k<2, 0>(d, ad, bd, idesc, (kb | k) != 0 ? 1u : 0u);
+            ptx::umma_k<2, 0>(d, ad, bd, idesc, kb != kb_begin || k != 0 ? 1u : 0u);
           }
           ptx::umma_commit<2>(ptx::smem_u32(&empty_bar[stage]));
           ptx::umma_commit<2>(ptx::mapa(ptx::smem_u32(&empty_bar[stage]), 1));
@@ -1029,6 +1095,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           stage = 0;
           phase ^= 1u;
         }
+      }
+      if constexpr (GRAD) {
+        if (ok && piece + 1 < pieces) publish();
+      }
       }
       if constexpr (ADAPT) {
         if (!ok) break;
@@ -1058,12 +1128,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         });
       }
       if (!ok) break;
-      if (ptx::elect_one()) {
-        ptx::umma_commit<2>(ptx::smem_u32(&tfull_bar[acc]));
-        ptx::umma_commit<2>(ptx::mapa(ptx::smem_u32(&tfull_bar[acc]), 1));
-      }
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
+      publish();
     }
   } else if (warp >= 2 && warp < 6) {
     // ------------------------------------------------------------ epilogue
@@ -1083,7 +1148,17 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const long long at = (ADAPT ? 0ll : static_cast<long long>(t.g) * p.bias_cols) + n;
         bias = load_as_f32(p.bias, p.bias_dtype, GATED && q >= 2 ? at + p.cols : at);
       }
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc]), acc_phase, abort_flag))) break;
+      const int pieces = GRAD ? max(1, (t.num_kb + pp.piece_kb - 1) / pp.piece_kb) : 1;
+      for (int piece = 0; piece < pieces; piece += 2) {
+      // two pieces: from this slot and the other one, which is a phase on when this is slot 1
+      const bool two = GRAD && piece + 1 < pieces;
+      if (!__all_sync(0xffffffffu,
+                      ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc]), acc_phase, abort_flag) &&
+                          (!two || ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc ^ 1]),
+                                                  acc == 0 ? acc_phase : acc_phase ^ 1u, abort_flag)))) {
+        alive = false;
+        break;
+      }
       ptx::tc_fence_after();
       const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BT);
       const uint32_t tempty = leader(&tempty_bar[acc]);
@@ -1098,6 +1173,12 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           ptx::tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+          if (GRAD && two) {
+            ptx::tmem_ld_32x32(src + (acc == 0 ? BT : -BT) + c, v);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] += __uint_as_float(v[i]);
+          }
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) f[i] = 0.0f;
@@ -1105,7 +1186,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (c + 32 >= t.rows) {
           ptx::tc_fence_before();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive_cluster(tempty);
+          if (lane == 0) {
+            ptx::mbar_arrive_cluster(tempty);
+            if (two) ptx::mbar_arrive_cluster(leader(&tempty_bar[acc ^ 1]));
+          }
         }
         if constexpr (ADAPT) {
           // rows go where the plan took them from; lane l holds row c + l's number
@@ -1153,17 +1237,30 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         } else {
           grouped_finish32<1>(p, p.alpha, f, nullptr, bias, 0.0f);
           char *at = out + static_cast<long long>(c) * p.row_pitch;
-          grouped_store(p, at, f, t.rows - c, lane, mine, both);
+          if (GRAD && piece > 0) {  // f32: to what the pieces before have left there
+            add_rows32(at, p.row_pitch, f, t.rows - c, lane, mine, p.wide_stores);
+          } else {
+            grouped_store(p, at, f, t.rows - c, lane, mine, both);
+          }
         }
       }
       if (!alive) break;
       if (!warp_has) {
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive_cluster(tempty);
+        if (lane == 0) {
+          ptx::mbar_arrive_cluster(tempty);
+          if (two) ptx::mbar_arrive_cluster(leader(&tempty_bar[acc ^ 1]));
+        }
       }
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
+      if (two) {
+        acc_phase ^= 1u;  // both slots are done with: the same slot, a phase on
+      } else {
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+      }
+      if (!alive) break;
     }
   } else if (warp == 14 && gather) {
     // ------------------------- finished copies of this CTA -> the leader's barrier

@@ -359,9 +359,11 @@ bool half_type(int dtype) { return dtype == KAPYB_F16 || dtype == KAPYB_BF16; }
 
 constexpr int64_t kMaxRowPitch = 1 << 26;  // bytes between output rows on the tcgen05 paths
 
-// Two neighbouring 16-bit columns of the output may be written as one aligned word.
-bool pair_stores_ok(const void *out, int dtype, int64_t s0, int64_t group) {
-  return half_type(dtype) && reinterpret_cast<uintptr_t>(out) % 4 == 0 && s0 % 2 == 0 && group % 2 == 0;
+// Two neighbouring 16-bit columns of the output may be written as one aligned word, four
+// f32 ones as 16 bytes.
+bool wide_stores_ok(const void *out, int dtype, int64_t s0, int64_t group) {
+  const int64_t n = half_type(dtype) ? 2 : 4;
+  return reinterpret_cast<uintptr_t>(out) % (n * dtype_size(dtype)) == 0 && s0 % n == 0 && group % n == 0;
 }
 
 template <int BT, int MSETS, bool GRAD>
@@ -461,7 +463,7 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
   gp.out = const_cast<void *>(elem_ptr(out));
   gp.row_pitch = static_cast<uint32_t>(pitch);
   gp.out_dtype = out->dtype;
-  gp.pair_stores = pair_stores_ok(gp.out, out->dtype, out->stride0, 0);
+  gp.wide_stores = wide_stores_ok(gp.out, out->dtype, out->stride0, 0);
   gp.alpha = ep.alpha;
   gp.bias = ep.bias;
   gp.bias_dtype = ep.bias_dtype;
@@ -518,7 +520,7 @@ kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, 
   gp.row_pitch = static_cast<uint32_t>(pitch);
   gp.group_bytes = groups > 1 ? out_group_stride * dtype_size(out->dtype) : 0;
   gp.out_dtype = out->dtype;
-  gp.pair_stores = pair_stores_ok(gp.out, out->dtype, out->stride0, groups > 1 ? out_group_stride : 0);
+  gp.wide_stores = wide_stores_ok(gp.out, out->dtype, out->stride0, groups > 1 ? out_group_stride : 0);
   gp.alpha = alpha;
   gp.activation = KAPYB_ACT_NONE;
   gp.rounding = rounding;
@@ -533,6 +535,7 @@ kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, 
   PairParams pp = pair_params(gp, lhs, true);
   pp.grad = static_cast<const uint8_t *>(elem_ptr(grad));
   pp.grad_pitch = grad->stride0 * 2ll;
+  pp.piece_kb = out->dtype == KAPYB_F32 ? 16 : 1 << 30;
   return launch_pairs<PAIR_GRADIENT>(h, tmA, tmA, tmA, tmA, pp, tiles, stream);
 }
 
@@ -1132,7 +1135,7 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
   gp.out = const_cast<void *>(elem_ptr(c.out));
   gp.row_pitch = static_cast<uint32_t>(pitch);
   gp.out_dtype = c.out->dtype;
-  gp.pair_stores = pair_stores_ok(gp.out, c.out->dtype, c.out->stride0, 0);
+  gp.wide_stores = wide_stores_ok(gp.out, c.out->dtype, c.out->stride0, 0);
   gp.alpha = c.ep.alpha;
   gp.bias = c.ep.bias;
   gp.bias_dtype = c.ep.bias_dtype;

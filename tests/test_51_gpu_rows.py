@@ -497,6 +497,29 @@ def test_matmul_grouped_gradients(handle, case, dt):
         within(dw, want, slack + U[out_dt] * (want.abs() + slack) + TINY[out_dt])
 
 
+def test_matmul_grouped_grad_of_long_groups(handle):
+    """An f32 gradient over thousands of rows keeps the precision of rounded sums: it is
+    accumulated 1024 rows at a time.  A sum of R random terms in which each of the R / 16
+    additions loses at most 2^-23 of the running sum is off by at most R / 16 2^-23 of it;
+    pieces of 1024 rows lose 64 2^-23, and joining them half a step each."""
+    R = [5000, 0, 1024, 1025, 2049, 3100, 7]
+    K, N = 264, 392
+    off = torch.tensor([0] + R).cumsum(0).to(torch.int32).to(DEV)
+    x, dy = randn(1, sum(R), K, dtype=torch.bfloat16), randn(2, sum(R), N, dtype=torch.bfloat16)
+    for out_dt in (torch.float32, torch.bfloat16):
+        big = torch.full((len(R), K, N + 4), 3.0, device=DEV, dtype=out_dt)
+        d = handle.matmul_grouped_grad(x, dy, off, big[:, :, :N])
+        handle.check()
+        assert (big[:, :, N:] == 3.0).all()
+        assert torch.equal(d, handle.matmul_grouped_grad(x, dy, off, out_dtype=out_dt))
+        ends = off.tolist()
+        for g, r in enumerate(R):
+            ref = x[ends[g]:ends[g + 1]].double().t() @ dy[ends[g]:ends[g + 1]].double()
+            err = (d[g].double() - ref).norm().item()
+            limit = (64 * 2.0 ** -23 + 8 * 2.0 ** -24) if out_dt == torch.float32 else r / 16 * 2.0 ** -23 + 2.0 ** -8
+            assert err <= limit * ref.norm().item(), (g, err / ref.norm().item())
+
+
 def test_matmul_grouped_grad_ignores_other_rows(handle):
     """Rows behind the plan and rows of other groups hold NaN and infinities."""
     T, E, K, N = 100, 4, 72, 136
