@@ -188,7 +188,10 @@ bool row_vec_ok(const RouteParams &p) {
          (p.x_s0 * esz) % align == 0;
 }
 template <int VPT>
-void launch_route(const RouteParams &p, int grid, cudaStream_t s) {
+void launch_route(RouteParams p, int grid, cudaStream_t s) {
+  const int lanes = p.group_size / VPT;
+  p.group_lanes = lanes * VPT == p.group_size && (lanes & (lanes - 1)) == 0 && lanes <= 32 ? lanes : 0;
+  p.bias_pieces = VPT % 4 == 0 && aligned16(p.bias);
   const bool scored = p.bias != nullptr || (p.n_groups > 1 && p.group_best > 1);
   const bool vec = row_vec_ok<VPT>(p);
   if (scored && vec) route_kernel<VPT, true, true><<<grid, 256, 0, s>>>(p);

@@ -42,7 +42,9 @@ struct RouteParams {
   int x_dtype;
   int rows, experts;
   const float *bias;  // [experts] or nullptr
+  int bias_pieces;    // bias starts on 16 bytes
   int sigmoid, top_k, n_groups, group_size, top_groups, group_best, renormalize;
+  int group_lanes;    // lanes a group's experts fill, 0 unless whole lanes and a power of two
   float scale;
   float *weights;  // [rows, top_k]
   int32_t *chosen;  // [rows, top_k]
@@ -308,8 +310,30 @@ __device__ __forceinline__ LaneBest two_best(const uint32_t (&key)[VPT], uint32_
   return b;
 }
 
+// Approximations for the 32-bit selection scores only (their error is bounded above, and
+// results below 2^-126, which they flush, are covered by its smallest term).
+__device__ __forceinline__ float exp_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fmul_rn(x, 1.4426950408889634f)));
+  return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// rank_key of a number that is not NaN.
+__device__ __forceinline__ uint32_t number_key(float c) {
+  const int b = __float_as_int(c + 0.0f);
+  return static_cast<uint32_t>(b ^ ((b >> 31) | static_cast<int>(0x80000000u)));
+}
+
 // Weights from full-precision expf and division, f32 throughout.  SCORED: experts (or
-// groups) are ranked by their scores, not by their logits.
+// groups) are ranked by their scores, not by their logits.  The kernel is bound by the
+// instructions it issues (some 1450 a row of 256 experts in eight groups before, 70 % of
+// the issue slots): rows without a mask, NaN or infinity take the short forms of the keys,
+// the bias comes in 16-byte pieces, and a logit that served as key is its own copy.
 template <int VPT, bool SCORED, bool VEC>
 __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
   const int lane = threadIdx.x & 31;
@@ -318,14 +342,21 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
   const int e0 = lane * VPT;
   uint32_t key[VPT];
   float top = 0.0f, z = 1.0f, err = 0.0f;
-  bool bad;  // a NaN or +inf among the logits: softmax weights are NaN
+  bool bad = false;  // a NaN or +inf among the logits: softmax weights are NaN
   {
     float x[VPT];
     load_row<VPT, VEC>(p, row, lane, x);
-    bool off = false;
+    float odd = 0.0f;  // NaN as soon as one of the logits is not finite
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) off |= !(x[i] < INFINITY);
-    bad = __any_sync(0xffffffffu, off);
+    for (int i = 0; i < VPT; ++i) odd = fmaf(x[i], 0.0f, odd);
+    // (experts that do not exist read as masked, so a short last lane counts as odd)
+    const bool plain = __all_sync(0xffffffffu, odd == odd);
+    if (!plain) {
+      bool off = false;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) off |= !(x[i] < INFINITY);
+      bad = __any_sync(0xffffffffu, off);
+    }
     if (!p.sigmoid && (SCORED || !p.renormalize)) {
       float m = x[0];
 #pragma unroll
@@ -338,16 +369,50 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
     }
     if constexpr (SCORED) {
       err = (p.sigmoid ? 6.0f : 64.0f / z) * 5.9604645e-8f + 1e-37f;
-      const float rz = 1.0f / z;
+      float bias[VPT];
+      if (p.bias != nullptr && VEC && p.bias_pieces) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const float s = p.sigmoid ? __fdividef(1.0f, 1.0f + kapy_exp(-x[i])) : kapy_exp(x[i] - top) * rz;
-        const float c = p.bias != nullptr && e0 + i < p.experts ? s + __ldg(p.bias + e0 + i) : s;
-        key[i] = x[i] == -INFINITY ? 0u : rank_key(c);
+        for (int i = 0; i < VPT; i += 4) {
+          const float4 v = e0 < p.experts ? __ldg(reinterpret_cast<const float4 *>(p.bias + e0 + i))
+                                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          bias[i] = v.x;
+          bias[i + 1] = v.y;
+          if (VPT > 2) {
+            bias[(i + 2) % VPT] = v.z;
+            bias[(i + 3) % VPT] = v.w;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) bias[i] = p.bias != nullptr && e0 + i < p.experts ? __ldg(p.bias + e0 + i) : 0.0f;
+      }
+      float c[VPT];
+      if (p.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) c[i] = rcp_fast(1.0f + exp_fast(-x[i])) + bias[i];
+      } else {
+        const float rz = 1.0f / z;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) c[i] = fmaf(exp_fast(x[i] - top), rz, bias[i]);
+      }
+      float nan = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) nan = fmaf(c[i], 0.0f, nan);
+      if (plain && __all_sync(0xffffffffu, nan == nan)) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) key[i] = number_key(c[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) key[i] = x[i] == -INFINITY ? 0u : rank_key(c[i]);
       }
     } else {
+      if (plain) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) key[i] = x[i] == -INFINITY ? 0u : rank_key(x[i]);
+        for (int i = 0; i < VPT; ++i) key[i] = number_key(x[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) key[i] = x[i] == -INFINITY ? 0u : rank_key(x[i]);
+      }
     }
   }
   bool unsure = false;
@@ -367,9 +432,9 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
         }
       }
     };
-    const int lanes = p.group_size / VPT;  // lanes per group, when groups are whole lanes
-    const bool whole = lanes * VPT == p.group_size && (lanes & (lanes - 1)) == 0 && lanes <= 32;
-    if (whole) {
+    // lanes per group, when every lane's experts belong to one group
+    const int lanes = p.group_lanes;
+    if (lanes) {
       // every lane's two best belong to one group: join them over its lanes
       uint32_t k1 = b.k1, k2 = b.k2;
       for (int off = 1; off < lanes; off <<= 1) {
@@ -394,7 +459,7 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
           const uint32_t k = i >= lo && i < hi ? key[i] : 0u;
-          k2 = k > k1 ? k1 : max(k2, k);
+          k2 = max(min(k, k1), k2);
           k1 = max(k1, k);
         }
         const uint32_t g1 = __reduce_max_sync(0xffffffffu, k1);
@@ -415,11 +480,13 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
       const bool in = (kept >> lane) & 1u;
       const uint32_t low = __reduce_min_sync(0xffffffffu, in ? mine : 0xffffffffu);
       const uint32_t high = __reduce_max_sync(0xffffffffu, in ? 0u : mine);
-      if (kept != 0u && high != 0u) unsure = !(key_value(low) - key_value(high) > 2.0f * warp_max(slack));
+      // (errors are not negative, so their bits order like they do; a NaN is the largest)
+      const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(slack) & 0x7fffffffu));
+      if (kept != 0u && high != 0u) unsure = !(key_value(low) - key_value(high) > 2.0f * most);
     }
-    if (whole) {
+    if (lanes) {
       // all of a lane's experts are kept or none
-      if (e0 < p.experts && !((kept >> (lane / lanes)) & 1u)) {
+      if (e0 < p.experts && !((kept >> (e0 / p.group_size)) & 1u)) {
         b = LaneBest{0u, 0u, 0, 0};
 #pragma unroll
         for (int i = 0; i < VPT; ++i) key[i] = 0u;
@@ -438,10 +505,15 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
     }
   }
   int pick = -1;
+  uint32_t pick_key = 0u;
   float prev = 0.0f, last = 0.0f;  // scores: of the pick before, and of the top_k-th
   bool spent = false;  // this lane's second best is its candidate already
   bool close = false;  // two neighbours are within the error of one another
   int found = 0;
+  // c is clearly behind `above`: by more than both errors, 2 err + (|above| + |c|) 2^-23,
+  // where |above| is at most |c| and the difference
+  const float err2 = 2.1f * err;
+  const auto apart = [&](float above, float c) { return above - c > fmaf(fabsf(c), 2.5e-7f, err2); };
   // with scores as keys the candidates go on until one is clearly behind the top_k-th
   for (int j = 0; j < (SCORED ? 32 : p.top_k) && !unsure; ++j) {
     const uint32_t g = __reduce_max_sync(0xffffffffu, b.k1);
@@ -450,17 +522,17 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
     const int i_w = __shfl_sync(0xffffffffu, b.i1, w);
     if constexpr (SCORED) {
       const float c = key_value(g);
-      const auto apart = [&](float above) {
-        return above - c > 2.0f * err + (fabsf(above) + fabsf(c)) * 1.1920929e-7f;
-      };
-      if (j >= p.top_k && apart(last)) break;
-      if (j > 0 && !apart(prev)) close = true;
+      if (j >= p.top_k && apart(last, c)) break;
+      if (j > 0 && !apart(prev, c)) close = true;
       if (j == 31 && p.top_k <= 31) unsure = true;  // more candidates than lanes
       prev = c;
       if (j < p.top_k) last = c;
+      found = j + 1;
     }
-    if (lane == j) pick = w * VPT + i_w;
-    found = j + 1;
+    if (lane == j) {
+      pick = w * VPT + i_w;
+      pick_key = g;
+    }
     if (lane == w) {
       if (spent) {
         b = two_best<VPT, false>(key, g, i_w);
@@ -477,8 +549,7 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
     // 32 picks of a top 32: the one left out has not been looked at
     if (p.top_k == 32 && found == 32) {
       const uint32_t g = __reduce_max_sync(0xffffffffu, b.k1);
-      const float c = key_value(g);
-      if (g != 0u && !(last - c > 2.0f * err + (fabsf(last) + fabsf(c)) * 1.1920929e-7f)) unsure = true;
+      if (g != 0u && !apart(last, key_value(g))) unsure = true;
     }
     if (unsure) pick = choose_f64<VPT>(p, row);
     else if (close) pick = reorder_f64(p, row, found, pick);
@@ -486,7 +557,8 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
 
   // weights of the choices, lane j the j-th
   const bool on = lane < p.top_k && pick >= 0;
-  const float xv = on ? route_logit(p, row, pick) : -INFINITY;
+  float xv = -INFINITY;
+  if (on) xv = SCORED ? route_logit(p, row, pick) : key_value(pick_key);
   float w = 0.0f;
   if (p.renormalize) {
     // only ratios matter, so both scores are divided by e^shift, which keeps the sum away

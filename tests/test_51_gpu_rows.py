@@ -123,6 +123,28 @@ def test_route_ties_and_borders(handle, pkg):
 
 
 @pytest.mark.parametrize("sig", [0, 1])
+@pytest.mark.parametrize("groups, tg, best", [(1, 1, 1), (8, 3, 2), (5, 2, 2)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_route_many_rows_of_near_ties(handle, sig, groups, tg, best, dt):
+    """Coarse logits and a coarse bias make equal and nearly equal scores common; the
+    choice is still that of the scores in 64 bits, ties by index."""
+    T, E, k = 700, 40 if groups == 5 else 64, 6
+    x = (torch.randn(T, E, generator=gen(E)) * 8).round().div(8).to(dt).to(DEV)
+    if dt == torch.float32:  # and scores that differ by less than 32 bits can tell
+        x = x + (torch.randint(0, 3, (T, E), generator=gen(1)) * 2.0 ** -27).to(DEV)
+    x[5::17, ::3] = -math.inf
+    b = (torch.randn(E, generator=gen(2)) * 4).round().div(16).to(DEV)
+    w, e = handle.route(x, k, bias=b, score=sig, groups=groups, top_groups=tg, group_best=best)
+    handle.check()
+    W, I = route_ref(x, k, b, sig, groups, tg, best, 1, 1.0)
+    # torch's and the kernel's 64-bit exponentials may differ in the last bit, which can
+    # only show where two sums are that close without being equal: allow for it by value
+    same = (e == I).all(1)
+    assert same.float().mean() > 0.999
+    within(w[same], W[same], 64 * 2.0 ** -24 * W[same].abs())
+
+
+@pytest.mark.parametrize("sig", [0, 1])
 def test_route_far_logits(handle, pkg, sig):
     # chosen scores far below what f32 can hold: the ratios are still those of the scores
     x = torch.tensor([[-300.0, -301.0, -400.0, -302.0]], device=DEV)
