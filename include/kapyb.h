@@ -522,7 +522,9 @@ KAPYB_API kapyb_status kapyb_reduce(kapyb_handle h, const kapyb_tensor2d *src,
  * device, whichever device is current.  Indices, orders and offsets are read on the
  * device and may hold anything: one that leads outside its tensor names no group /
  * a row of zeros, and no memory outside the tensors is touched.  Outputs must not
- * overlap inputs (KAPYB_INVALID_ARG where the descriptors show it). */
+ * overlap inputs (KAPYB_INVALID_ARG where the descriptors show it).  Operands are padded
+ * with zeros; cache hints are checked and otherwise ignored.  The arguments are checked
+ * before the handle is looked at. */
 
 typedef enum {
   KAPYB_SCORE_SOFTMAX = 0,
@@ -595,7 +597,8 @@ KAPYB_API kapyb_status kapyb_plan_rows(kapyb_handle h, const int32_t *index, int
  * as f32), out f16 / bf16 / f32; sums in f32.  16-bit operands with 16-byte aligned
  * bases, leading dimensions and group stride, lhs with unit stride on K, run on
  * tcgen05; any other strides run on CUDA cores.  Up to 1024 groups.  The same bits on
- * every run. */
+ * every run.  (The tensor cores' f32 additions truncate: a sum of K terms is off by about
+ * K * 1e-9 of itself, as in kapyb_matmul.) */
 KAPYB_API kapyb_status kapyb_matmul_grouped(kapyb_handle h, const kapyb_tensor2d *lhs,
                                             const kapyb_tensor2d *rhs, int32_t groups,
                                             int64_t group_stride, const int32_t *offsets,
@@ -607,8 +610,10 @@ KAPYB_API kapyb_status kapyb_matmul_grouped(kapyb_handle h, const kapyb_tensor2d
 /* Gradient of the groups' weights: out[g] = alpha * sum over group g's positions p of
  * lhs[row(p)]^T grad[p], [K, N] per group (g * out_group_stride elements apart), zeros
  * for a group without rows.  lhs [source rows, K], grad [positions, N] (f16, bf16 or
- * f32, of one type), offsets / order / fan as in kapyb_matmul_grouped; a position whose
- * row does not exist adds nothing.  Sums in f32, rounded once to out's type. */
+ * f32, of one type), offsets / order / fan as in kapyb_matmul_grouped; a row that does not
+ * exist counts as zeros.  Groups of out must not overlap (out_group_stride at least one
+ * group's extent).  Sums in f32, for an f32 out 1024 positions at a time so that long
+ * groups keep f32's precision, rounded once to out's type.  The same bits on every run. */
 KAPYB_API kapyb_status kapyb_matmul_grouped_grad(kapyb_handle h, const kapyb_tensor2d *lhs,
                                                  const kapyb_tensor2d *grad, int32_t groups,
                                                  const int32_t *offsets, const int32_t *order,
@@ -642,9 +647,14 @@ KAPYB_API kapyb_status kapyb_combine_rows_backward(kapyb_handle h, const kapyb_t
  * and [rank, N], the next ones down_stride / up_stride elements later; scale f32
  * [groups] or NULL (1).  rank 1 .. 128.  alpha and bias apply to the shared part, as
  * in kapyb_matmul.  lhs, rhs, down, up: all f16, all bf16 or all f32; out f16 / bf16 /
- * f32.  The inner product lhs . down is kept to at least 16 bits of precision and the
- * whole sum is formed in f32.  An inference operator: it has no gradient here (rhs,
- * down and up of a training step are ordinary kapyb_matmul problems).
+ * f32.  The inner product scale * (lhs . down) is kept to at least 16 bits of precision
+ * (in two values of the operands' type from 257 rows on, so with f16 operands it must stay
+ * below 65504 there) and the whole sum is formed in f32.  What a row's own adapter or
+ * values hold, NaN and infinities included, reaches no other row.  16-bit operands TMA can
+ * describe (as in kapyb_matmul_grouped; up to 256 rows only lhs and rhs, and any alpha;
+ * beyond, all four and an alpha of magnitude 1/256 .. 256) run on tcgen05, the rest on CUDA
+ * cores.  The same bits on every run.  An inference operator: it has no gradient here
+ * (rhs, down and up of a training step are ordinary kapyb_matmul problems).
  * scratch: device memory of kapyb_matmul_adapters_scratch() bytes, 256-byte aligned,
  * the call's own until it has run on `stream`. */
 KAPYB_API kapyb_status kapyb_matmul_adapters(kapyb_handle h, const kapyb_tensor2d *lhs,
@@ -696,8 +706,10 @@ KAPYB_API kapyb_status kapyb_matmul_plan(kapyb_handle h, int32_t sm_count,
 KAPYB_API kapyb_status kapyb_tuning_load(const char *file, int32_t *n_entries);
 KAPYB_API kapyb_status kapyb_tuning_clear(void);
 
-/* Name of the kernel family the last matmul on `h` dispatched to
- * ("tcgen05_1cta", "tcgen05_2cta", "tcgen05_skinny", "simt"). */
+/* Name of the kernel family the last call on `h` dispatched to ("tcgen05_1cta",
+ * "tcgen05_2cta", "tcgen05_skinny", "simt"; the rows calls: "grouped_tcgen05",
+ * "grouped_pair", "grouped_grad_pair", "adapters_decode", "adapters_pair", the "_simt"
+ * ones on CUDA cores, ...). */
 KAPYB_API const char *kapyb_last_kernel(kapyb_handle h);
 
 /* Number of kernels this handle has launched since creation. */

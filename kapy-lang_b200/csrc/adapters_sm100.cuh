@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(192) adapter_decode_kernel(const __grid_consta
         phase ^= 1u;
       }
     }
-    if (ok && ptx::elect_one()) ptx::umma_commit<1>(ptx::smem_u32(&done_bar));
+    if (ok && kb1 > kb0 && ptx::elect_one()) ptx::umma_commit<1>(ptx::smem_u32(&done_bar));
   } else {
     ptx::griddep_wait();  // low
     const int q = warp & 3;
@@ -403,9 +403,13 @@ __global__ void __launch_bounds__(192) adapter_decode_kernel(const __grid_consta
         adapter_delta<BF>(p, r, __shfl_sync(0xffffffffu, look, i), n0, delta + (r - r0) * 128, lane);
       }
     }
-    const bool ok = __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&done_bar), 0u, abort_flag));
+    // (a K shorter than the cluster leaves some of its CTAs without a block)
+    const bool some = kb1 > kb0;
+    const bool ok = !some || __all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&done_bar), 0u, abort_flag));
     ptx::tc_fence_after();
-    if (ok) {
+    if (!some) {
+      for (int c = 0; c < p.rows; ++c) partial[c * 128 + q * 32 + lane] = 0.0f;
+    } else if (ok) {
       // every MMA is done, so every stage has been read: the ring takes the partial sums
       const uint32_t src = tmem + (static_cast<uint32_t>(q * 32) << 16);
       for (int c = 0; c < p.rows; c += 16) {

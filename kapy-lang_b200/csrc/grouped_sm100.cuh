@@ -1,6 +1,7 @@
 // Products of rows that pick their weights, on tcgen05:
 //   forward   out[p, n]    = epilogue( sum_k lhs[row(p), k] * rhs[g(p)][k, n] )
 //   gradient  out[g][k, n] = alpha * sum over p of group g  lhs[row(p), k] * grad[p, n]
+//   adapters  out[t, n]    = epilogue( lhs[t] . rhs ) + low[t] . up[i(t)]
 //
 // The output columns n always fill the 128-row side of the MMA (TMEM lanes) and the
 // output rows its N side:  D[n, r] = sum A[n, .] B[r, .].  The N side of a tcgen05.mma
@@ -167,39 +168,24 @@ __device__ __forceinline__ int find_group(const GroupedTable &t, int groups, int
   return lo;
 }
 
-template <int BT, bool GRAD>
+template <int BT>
 __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams &p, const GroupedTable &t, int idx) {
   GroupedTile r;
-  if constexpr (GRAD) {
-    // group by group; row tiles of one column block next to one another
-    const int per = p.n_tiles * p.k_tiles;
-    r.g = idx / per;
-    const int in = idx - r.g * per;
-    const int n = in / p.k_tiles;
-    r.r0 = (in - n * p.k_tiles) * BT;
-    r.n0 = n * 128;
-    r.rows = min(BT, p.K - r.r0);
-    r.wide = round16(r.rows);
-    r.p0 = t.begin[r.g];
-    r.p1 = r.p0 + t.count[r.g];
-    r.num_kb = (t.count[r.g] + 63) >> 6;
-  } else {
-    const int q = idx / p.n_tiles;
-    const int lo = find_group(t, p.groups, q);
-    r.g = lo;
-    const int tiles = t.first[lo + 1] - t.first[lo];
-    const int in = idx - t.first[lo] * p.n_tiles;
-    int m, n;
-    raster(in, tiles, p.n_tiles, m, n);
-    const int cnt = t.count[lo];
-    const int each = round16((cnt + tiles - 1) / tiles);
-    r.n0 = n * 128;
-    r.r0 = t.begin[lo] + m * each;
-    r.rows = min(each, cnt - m * each);
-    r.wide = round16(r.rows);
-    r.num_kb = p.num_kb;
-    r.p0 = r.p1 = 0;
-  }
+  const int q = idx / p.n_tiles;
+  const int lo = find_group(t, p.groups, q);
+  r.g = lo;
+  const int tiles = t.first[lo + 1] - t.first[lo];
+  const int in = idx - t.first[lo] * p.n_tiles;
+  int m, n;
+  raster(in, tiles, p.n_tiles, m, n);
+  const int cnt = t.count[lo];
+  const int each = round16((cnt + tiles - 1) / tiles);
+  r.n0 = n * 128;
+  r.r0 = t.begin[lo] + m * each;
+  r.rows = min(each, cnt - m * each);
+  r.wide = round16(r.rows);
+  r.num_kb = p.num_kb;
+  r.p0 = r.p1 = 0;
   return r;
 }
 
@@ -397,7 +383,7 @@ __device__ __forceinline__ void grouped_scatter32(const GroupedParams &p, char *
 // 64 x 64 (MN-major); gradient: grad [positions, cols], one-row boxes of 64 columns.
 // tmB: lhs [source rows, K]: one-row boxes of 64 columns (gathered, and the gradient),
 // or 64 x 32 boxes (rows already in plan order).
-template <int BT, int MSETS, bool GRAD>
+template <int BT, int MSETS>
 __global__ void __launch_bounds__(kGroupedThreads, 1)
 grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const GroupedParams p) {
@@ -441,7 +427,7 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int total = GRAD ? p.groups * p.n_tiles * p.k_tiles : table.first[p.groups] * p.n_tiles;
+  const int total = table.first[p.groups] * p.n_tiles;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -454,24 +440,21 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
       const long long r = source_row(p.order, p.fan, p.src_rows, q);
       return r < 0 ? p.src_rows : static_cast<int>(r);
     };
-    const bool gather = GRAD || p.order != nullptr;
+    const bool gather = p.order != nullptr;
     for (int idx = blockIdx.x; ok && idx < total; idx += gridDim.x) {
-      const GroupedTile t = grouped_tile<BT, GRAD>(p, table, idx);
-      // forward: this lane's rows of the tile, four per gather instruction
-      constexpr int kMine = GRAD ? 1 : BT / 128 > 0 ? BT / 128 : 1;
-      int rows4[kMine][4];
-      if (!GRAD && gather) {
+      const GroupedTile t = grouped_tile<BT>(p, table, idx);
+      // this lane's four rows of the tile: one gather instruction
+      static_assert(BT <= 128, "one gather instruction a lane");
+      int rows4[4];
+      if (gather) {
 #pragma unroll
-        for (int i = 0; i < kMine; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = (i * 32 + lane) * 4 + j;
-            rows4[i][j] = r < t.wide ? row_of(t.r0 + r, t.r0 + t.rows) : p.src_rows;
-          }
+        for (int j = 0; j < 4; ++j) {
+          const int r = lane * 4 + j;
+          rows4[j] = r < t.wide ? row_of(t.r0 + r, t.r0 + t.rows) : p.src_rows;
+        }
       }
-      const int boxes = gather ? t.wide / 4 : (t.wide + 31) / 32;  // forward, token side
-      const uint32_t b_bytes = GRAD ? static_cast<uint32_t>((t.rows + 63) / 64) * 8192u
-                                    : static_cast<uint32_t>(boxes) * (gather ? 512u : 4096u);
+      const int boxes = gather ? t.wide / 4 : (t.wide + 31) / 32;
+      const uint32_t b_bytes = static_cast<uint32_t>(boxes) * (gather ? 512u : 4096u);
       for (int kb = 0; kb < t.num_kb; ++kb) {
         const bool got = ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag);
         if (!__all_sync(0xffffffffu, got)) {
@@ -483,40 +466,17 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
         const uint32_t b_dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES);
         if (lane == 0) ptx::mbar_arrive_expect_tx(fb, Cfg::A_BYTES + b_bytes);
         __syncwarp();
-        if constexpr (GRAD) {
-          // 64 positions: 16 groups of four rows; lane l fetches rows 4 (l % 16) .. + 3
-          // of every other 64-column chunk
-          const int q = t.p0 + kb * 64 + (lane & 15) * 4;
-          int src[4], own[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            src[j] = row_of(q + j, t.p1);
-            own[j] = src[j] < p.src_rows ? q + j : p.rows;  // zeros on both sides
-          }
-          const uint32_t off = static_cast<uint32_t>(lane & 15) * 512u;
-          const int c0 = lane >> 4;
-          tma_gather4(a_dst + c0 * 8192 + off, &tmA, fb, t.n0 + c0 * 64, own[0], own[1], own[2], own[3]);
-#pragma unroll
-          for (int c = c0; c < BT / 64; c += 2)
-            if (c * 64 < t.rows)
-              tma_gather4(b_dst + c * 8192 + off, &tmB, fb, t.r0 + c * 64, src[0], src[1], src[2], src[3]);
+        const int k0 = kb * 64;
+        if (p.a_mn_major) {
+          if (lane < 2 * MSETS)
+            ptx::tma_load_3d(a_dst + lane * 8192, &tmA, fb, t.n0 + (lane & 1) * 64 + (lane >> 1) * p.cols, k0, t.g);
         } else {
-          const int k0 = kb * 64;
-          if (p.a_mn_major) {
-            if (lane < 2 * MSETS)
-              ptx::tma_load_3d(a_dst + lane * 8192, &tmA, fb, t.n0 + (lane & 1) * 64 + (lane >> 1) * p.cols, k0, t.g);
-          } else {
-            if (lane < MSETS) ptx::tma_load_3d(a_dst + lane * 16384, &tmA, fb, k0, t.n0 + lane * p.cols, t.g);
-          }
-          if (gather) {
-#pragma unroll
-            for (int i = 0; i < kMine; ++i)
-              if (i * 32 + lane < boxes)
-                tma_gather4(b_dst + (i * 32 + lane) * 512, &tmB, fb, k0, rows4[i][0], rows4[i][1], rows4[i][2],
-                            rows4[i][3]);
-          } else if (lane < boxes) {
-            tma_load_2d(b_dst + lane * 4096, &tmB, fb, k0, t.r0 + lane * 32);
-          }
+          if (lane < MSETS) ptx::tma_load_3d(a_dst + lane * 16384, &tmA, fb, k0, t.n0 + lane * p.cols, t.g);
+        }
+        if (gather) {
+          if (lane < boxes) tma_gather4(b_dst + lane * 512, &tmB, fb, k0, rows4[0], rows4[1], rows4[2], rows4[3]);
+        } else if (lane < boxes) {
+          tma_load_2d(b_dst + lane * 4096, &tmB, fb, k0, t.r0 + lane * 32);
         }
         if (++stage == STAGES) {
           stage = 0;
@@ -531,18 +491,17 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     };
     // K-major tile: 128-byte rows, 8-row groups 1024 bytes apart, a K step is 32 bytes.
     // MN-major tile: 64-column chunks 8192 bytes apart, a K step is 16 rows of 128 bytes.
-    const bool a_mn = GRAD || p.a_mn_major;
-    constexpr bool b_mn = GRAD;
+    const bool a_mn = p.a_mn_major;
     const uint32_t a_lo0 = ((a_mn ? 8192u : 16u) >> 4) << 16 | (ptx::smem_u32(sA) >> 4);
-    const uint32_t b_lo0 = ((b_mn ? 8192u : 16u) >> 4) << 16 | (ptx::smem_u32(sB) >> 4);
+    const uint32_t b_lo0 = 1u << 16 | (ptx::smem_u32(sB) >> 4);
     constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    const uint32_t a_step = (a_mn ? 2048u : 32u) >> 4, b_step = (b_mn ? 2048u : 32u) >> 4;
+    const uint32_t a_step = (a_mn ? 2048u : 32u) >> 4;
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
     for (int idx = blockIdx.x; ok && idx < total; idx += gridDim.x) {
-      const GroupedTile t = grouped_tile<BT, GRAD>(p, table, idx);
-      const uint32_t idesc = ptx::make_idesc_f16(p.bf16, a_mn, b_mn, 128, t.wide);
+      const GroupedTile t = grouped_tile<BT>(p, table, idx);
+      const uint32_t idesc = ptx::make_idesc_f16(p.bf16, a_mn, 0, 128, t.wide);
       if (!wait_all(ptx::smem_u32(&tempty_bar[acc]), acc_phase ^ 1u)) break;
       ptx::tc_fence_after();
       const uint32_t d = tmem_base + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
@@ -557,7 +516,7 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
           const uint32_t b_lo = b_lo0 + static_cast<uint32_t>(stage) * (Cfg::B_BYTES >> 4);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint64_t bd = (static_cast<uint64_t>(hi) << 32) | (b_lo + k * b_step);
+            const uint64_t bd = (static_cast<uint64_t>(hi) << 32) | (b_lo + k * 2u);
 #pragma unroll
             for (int s = 0; s < MSETS; ++s) {
               const uint64_t ad = (static_cast<uint64_t>(hi) << 32) | (a_lo + s * (16384u >> 4) + k * a_step);
@@ -582,7 +541,7 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int idx = blockIdx.x; idx < total; idx += gridDim.x) {
-      const GroupedTile t = grouped_tile<BT, GRAD>(p, table, idx);
+      const GroupedTile t = grouped_tile<BT>(p, table, idx);
       const int n = t.n0 + q * 32 + lane;
       const bool mine = n < p.cols, both = (n | 1) < p.cols;
       float bias = 0.0f, bias_up = 0.0f;
@@ -595,29 +554,23 @@ grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_con
       ptx::tc_fence_after();
       const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
       const bool warp_has = t.n0 + q * 32 < p.cols;
-      char *out = static_cast<char *>(p.out) + (GRAD ? t.g * p.group_bytes : 0ll) +
+      char *out = static_cast<char *>(p.out) +
                   static_cast<long long>(t.r0) * p.row_pitch + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll);
       for (int c = 0; c < t.rows && warp_has; c += 32) {
         float f[32], u[MSETS == 2 ? 32 : 1];
-        if (!GRAD || t.num_kb > 0) {
-          uint32_t v[32];
-          ptx::tmem_ld_32x32(src + c, v);
-          if constexpr (MSETS == 2) {
-            uint32_t w[32];
-            ptx::tmem_ld_32x32(src + BT + c, w);
-            ptx::tmem_ld_wait();
+        uint32_t v[32];
+        ptx::tmem_ld_32x32(src + c, v);
+        if constexpr (MSETS == 2) {
+          uint32_t w[32];
+          ptx::tmem_ld_32x32(src + BT + c, w);
+          ptx::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(w[i]);
-          } else {
-            ptx::tmem_ld_wait();
-          }
-#pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+          for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(w[i]);
         } else {
-          // a group without rows: no MMA has written the accumulator
-#pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+          ptx::tmem_ld_wait();
         }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
         if (c + 32 >= t.rows) {
           // the accumulator has been read: the slot is the MMA warp's again
           ptx::tc_fence_before();
@@ -1065,40 +1018,40 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       const int pieces = GRAD ? max(1, (t.num_kb + pp.piece_kb - 1) / pp.piece_kb) : 1;
       uint32_t d = 0u;
       for (int piece = 0; ok && piece < pieces; ++piece) {
-      const int kb_end = GRAD ? min(t.num_kb, (piece + 1) * pp.piece_kb) : t.num_kb;
-      if (!wait_all(ptx::smem_u32(&tempty_bar[acc]), acc_phase ^ 1u)) {
-        ok = false;
-        break;
-      }
-      ptx::tc_fence_after();
-      d = tmem_base + static_cast<uint32_t>(acc * BT);
-      const int kb_begin = GRAD ? piece * pp.piece_kb : 0;
-      for (int kb = kb_begin; kb < kb_end; ++kb) {
-        if (!wait_all(ptx::smem_u32(&full_bar[stage]), phase)) {
+        const int kb_end = GRAD ? min(t.num_kb, (piece + 1) * pp.piece_kb) : t.num_kb;
+        if (!wait_all(ptx::smem_u32(&tempty_bar[acc]), acc_phase ^ 1u)) {
           ok = false;
           break;
         }
         ptx::tc_fence_after();
-        if (ptx::elect_one()) {
-          const uint32_t a_lo = a_lo0 + static_cast<uint32_t>(stage) * (Cfg::A_BYTES >> 4);
-          const uint32_t b_lo = b_lo0 + static_cast<uint32_t>(stage) * (Cfg::B_BYTES >> 4);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint64_t ad = (static_cast<uint64_t>(hi) << 32) | (a_lo + k * a_step);
-            const uint64_t bd = (static_cast<uint64_t>(hi) << 32) | (b_lo + k * b_step);
-            ptx::umma_k<2, 0>(d, ad, bd, idesc, kb != kb_begin || k != 0 ? 1u : 0u);
+        d = tmem_base + static_cast<uint32_t>(acc * BT);
+        const int kb_begin = GRAD ? piece * pp.piece_kb : 0;
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
+          if (!wait_all(ptx::smem_u32(&full_bar[stage]), phase)) {
+            ok = false;
+            break;
           }
-          ptx::umma_commit<2>(ptx::smem_u32(&empty_bar[stage]));
-          ptx::umma_commit<2>(ptx::mapa(ptx::smem_u32(&empty_bar[stage]), 1));
+          ptx::tc_fence_after();
+          if (ptx::elect_one()) {
+            const uint32_t a_lo = a_lo0 + static_cast<uint32_t>(stage) * (Cfg::A_BYTES >> 4);
+            const uint32_t b_lo = b_lo0 + static_cast<uint32_t>(stage) * (Cfg::B_BYTES >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint64_t ad = (static_cast<uint64_t>(hi) << 32) | (a_lo + k * a_step);
+              const uint64_t bd = (static_cast<uint64_t>(hi) << 32) | (b_lo + k * b_step);
+              ptx::umma_k<2, 0>(d, ad, bd, idesc, kb != kb_begin || k != 0 ? 1u : 0u);
+            }
+            ptx::umma_commit<2>(ptx::smem_u32(&empty_bar[stage]));
+            ptx::umma_commit<2>(ptx::mapa(ptx::smem_u32(&empty_bar[stage]), 1));
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
+        if constexpr (GRAD) {
+          if (ok && piece + 1 < pieces) publish();
         }
-      }
-      if constexpr (GRAD) {
-        if (ok && piece + 1 < pieces) publish();
-      }
       }
       if constexpr (ADAPT) {
         if (!ok) break;
@@ -1150,40 +1103,102 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       }
       const int pieces = GRAD ? max(1, (t.num_kb + pp.piece_kb - 1) / pp.piece_kb) : 1;
       for (int piece = 0; piece < pieces; piece += 2) {
-      // two pieces: from this slot and the other one, which is a phase on when this is slot 1
-      const bool two = GRAD && piece + 1 < pieces;
-      if (!__all_sync(0xffffffffu,
-                      ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc]), acc_phase, abort_flag) &&
-                          (!two || ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc ^ 1]),
-                                                  acc == 0 ? acc_phase : acc_phase ^ 1u, abort_flag)))) {
-        alive = false;
-        break;
-      }
-      ptx::tc_fence_after();
-      const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BT);
-      const uint32_t tempty = leader(&tempty_bar[acc]);
-      const bool warp_has = warp_n < p.cols;
-      char *out = static_cast<char *>(p.out) + (GRAD ? t.g * p.group_bytes : 0ll) +
-                  static_cast<long long>(t.r0) * p.row_pitch + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll);
-      for (int c = 0; c < t.rows && warp_has; c += 32) {
-        float f[32];
-        if (!GRAD || t.num_kb > 0) {
-          uint32_t v[32];
-          ptx::tmem_ld_32x32(src + c, v);
-          ptx::tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
-          if (GRAD && two) {
-            ptx::tmem_ld_32x32(src + (acc == 0 ? BT : -BT) + c, v);
+        // two pieces: from this slot and the other one, which is a phase on when this is slot 1
+        const bool two = GRAD && piece + 1 < pieces;
+        if (!__all_sync(0xffffffffu,
+                        ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc]), acc_phase, abort_flag) &&
+                            (!two || ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc ^ 1]),
+                                                    acc == 0 ? acc_phase : acc_phase ^ 1u, abort_flag)))) {
+          alive = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BT);
+        const uint32_t tempty = leader(&tempty_bar[acc]);
+        const bool warp_has = warp_n < p.cols;
+        char *out = static_cast<char *>(p.out) + (GRAD ? t.g * p.group_bytes : 0ll) +
+                    static_cast<long long>(t.r0) * p.row_pitch + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll);
+        for (int c = 0; c < t.rows && warp_has; c += 32) {
+          float f[32];
+          if (!GRAD || t.num_kb > 0) {
+            uint32_t v[32];
+            ptx::tmem_ld_32x32(src + c, v);
             ptx::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] += __uint_as_float(v[i]);
-          }
-        } else {
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+            if (GRAD && two) {
+              ptx::tmem_ld_32x32(src + (acc == 0 ? BT : -BT) + c, v);
+              ptx::tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+              for (int i = 0; i < 32; ++i) f[i] += __uint_as_float(v[i]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+          }
+          if (c + 32 >= t.rows) {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              ptx::mbar_arrive_cluster(tempty);
+              if (two) ptx::mbar_arrive_cluster(leader(&tempty_bar[acc ^ 1]));
+            }
+          }
+          if constexpr (ADAPT) {
+            // rows go where the plan took them from; lane l holds row c + l's number
+            int to = c + lane < t.rows ? p.order[t.r0 + c + lane] : -1;
+            if (to >= p.src_rows) to = -1;
+            if (p.bias != nullptr && p.bias_axis == 0) {
+              const float row_bias = to >= 0 ? load_as_f32(p.bias, p.bias_dtype, to) : 0.0f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[j] = f[j] * p.alpha + __shfl_sync(0xffffffffu, row_bias, j);
+              grouped_activation(p.activation, f);
+            } else {
+              grouped_finish32<1>(p, p.alpha, f, nullptr, bias, 0.0f);
+            }
+            grouped_scatter32(p, static_cast<char *>(p.out) + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll), f, to, lane,
+                              mine, both);
+          } else if constexpr (GATED) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = f[j] * p.alpha + bias;
+            // the gate's warp hands over its rows 16 .. 31 and finishes 0 .. 15, the up
+            // columns' warp the other way round; two buffers take turns
+            const bool up_side = q >= 2;
+            float *box = swap_mem + ((q & 1) * 2 + (swaps & 1)) * 1024;
+            float g[16], u[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) (up_side ? box : box + 512)[j * 32 + lane] = up_side ? f[j] : f[16 + j];
+            __syncwarp();
+            const uint32_t bar = ptx::smem_u32(&swap_bar[(q & 1) * 2 + (swaps & 1)]);
+            if (lane == 0) ptx::mbar_arrive(bar);
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar, (swaps >> 1) & 1, abort_flag))) {
+              alive = false;
+              break;
+            }
+            ++swaps;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float other = (up_side ? box + 512 : box)[j * 32 + lane];
+              g[j] = up_side ? other : f[j];
+              u[j] = up_side ? f[16 + j] : other;
+            }
+            grouped_activation(p.activation, g);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) g[j] *= u[j];
+            const int first = c + (up_side ? 16 : 0);
+            grouped_store(p, out + static_cast<long long>(first) * p.row_pitch, g, t.rows - first, lane, mine, both);
+          } else {
+            grouped_finish32<1>(p, p.alpha, f, nullptr, bias, 0.0f);
+            char *at = out + static_cast<long long>(c) * p.row_pitch;
+            if (GRAD && piece > 0) {  // f32: to what the pieces before have left there
+              add_rows32(at, p.row_pitch, f, t.rows - c, lane, mine, p.wide_stores);
+            } else {
+              grouped_store(p, at, f, t.rows - c, lane, mine, both);
+            }
+          }
         }
-        if (c + 32 >= t.rows) {
+        if (!alive) break;
+        if (!warp_has) {
           ptx::tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -1191,74 +1206,12 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             if (two) ptx::mbar_arrive_cluster(leader(&tempty_bar[acc ^ 1]));
           }
         }
-        if constexpr (ADAPT) {
-          // rows go where the plan took them from; lane l holds row c + l's number
-          int to = c + lane < t.rows ? p.order[t.r0 + c + lane] : -1;
-          if (to >= p.src_rows) to = -1;
-          if (p.bias != nullptr && p.bias_axis == 0) {
-            const float row_bias = to >= 0 ? load_as_f32(p.bias, p.bias_dtype, to) : 0.0f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = f[j] * p.alpha + __shfl_sync(0xffffffffu, row_bias, j);
-            grouped_activation(p.activation, f);
-          } else {
-            grouped_finish32<1>(p, p.alpha, f, nullptr, bias, 0.0f);
-          }
-          grouped_scatter32(p, static_cast<char *>(p.out) + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll), f, to, lane,
-                            mine, both);
-        } else if constexpr (GATED) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) f[j] = f[j] * p.alpha + bias;
-          // the gate's warp hands over its rows 16 .. 31 and finishes 0 .. 15, the up
-          // columns' warp the other way round; two buffers take turns
-          const bool up_side = q >= 2;
-          float *box = swap_mem + ((q & 1) * 2 + (swaps & 1)) * 1024;
-          float g[16], u[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) (up_side ? box : box + 512)[j * 32 + lane] = up_side ? f[j] : f[16 + j];
-          __syncwarp();
-          const uint32_t bar = ptx::smem_u32(&swap_bar[(q & 1) * 2 + (swaps & 1)]);
-          if (lane == 0) ptx::mbar_arrive(bar);
-          if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar, (swaps >> 1) & 1, abort_flag))) {
-            alive = false;
-            break;
-          }
-          ++swaps;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float other = (up_side ? box + 512 : box)[j * 32 + lane];
-            g[j] = up_side ? other : f[j];
-            u[j] = up_side ? f[16 + j] : other;
-          }
-          grouped_activation(p.activation, g);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) g[j] *= u[j];
-          const int first = c + (up_side ? 16 : 0);
-          grouped_store(p, out + static_cast<long long>(first) * p.row_pitch, g, t.rows - first, lane, mine, both);
+        if (two) {
+          acc_phase ^= 1u;  // both slots are done with: the same slot, a phase on
         } else {
-          grouped_finish32<1>(p, p.alpha, f, nullptr, bias, 0.0f);
-          char *at = out + static_cast<long long>(c) * p.row_pitch;
-          if (GRAD && piece > 0) {  // f32: to what the pieces before have left there
-            add_rows32(at, p.row_pitch, f, t.rows - c, lane, mine, p.wide_stores);
-          } else {
-            grouped_store(p, at, f, t.rows - c, lane, mine, both);
-          }
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1u;
         }
-      }
-      if (!alive) break;
-      if (!warp_has) {
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          ptx::mbar_arrive_cluster(tempty);
-          if (two) ptx::mbar_arrive_cluster(leader(&tempty_bar[acc ^ 1]));
-        }
-      }
-      if (two) {
-        acc_phase ^= 1u;  // both slots are done with: the same slot, a phase on
-      } else {
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1u;
-      }
       }
       if (!alive) break;
     }

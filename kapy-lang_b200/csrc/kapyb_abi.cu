@@ -29,7 +29,7 @@
 
 using namespace kapyb;
 
-extern "C" KAPYB_API int kapyb_version(void) { return 110; }
+extern "C" KAPYB_API int kapyb_version(void) { return 120; }
 
 extern "C" KAPYB_API kapyb_status kapyb_create(kapyb_handle *out, int device) {
   if (!out) return fail(nullptr, KAPYB_INVALID_ARG, "kapyb_create: out is NULL");

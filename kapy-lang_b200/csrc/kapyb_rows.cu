@@ -369,15 +369,15 @@ bool wide_stores_ok(const void *out, int dtype, int64_t s0, int64_t group) {
   return reinterpret_cast<uintptr_t>(out) % (n * dtype_size(dtype)) == 0 && s0 % n == 0 && group % n == 0;
 }
 
-template <int BT, int MSETS, bool GRAD>
+template <int BT, int MSETS>
 kapyb_status launch_grouped(kapyb_handle h, const CUtensorMap &tmA, const CUtensorMap &tmB, const GroupedParams &gp,
                             long long tiles, cudaStream_t stream) {
   using Cfg = GroupedCfg<BT, MSETS>;
-  constexpr auto kern = grouped_tcgen05_kernel<BT, MSETS, GRAD>;
+  constexpr auto kern = grouped_tcgen05_kernel<BT, MSETS>;
   TRY(allow_smem<kern>(h, Cfg::SMEM_BYTES));
   const int grid = static_cast<int>(std::min<long long>(tiles, h->sm_count));
   kern<<<grid, kGroupedThreads, Cfg::SMEM_BYTES, stream>>>(tmA, tmB, gp);
-  return launched(h, GRAD ? "grouped_grad_tcgen05" : "grouped_tcgen05");
+  return launched(h, "grouped_tcgen05");
 }
 
 PairParams pair_params(const GroupedParams &gp, const kapyb_tensor2d *lhs, bool gather) {
@@ -488,8 +488,8 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
                     lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, order && narrow ? 1 : 32));
   *taken = true;
   if (narrow)
-    return gated ? launch_grouped<64, 2, false>(h, tmA, tmB, gp, tiles, stream)
-                 : launch_grouped<64, 1, false>(h, tmA, tmB, gp, tiles, stream);
+    return gated ? launch_grouped<64, 2>(h, tmA, tmB, gp, tiles, stream)
+                 : launch_grouped<64, 1>(h, tmA, tmB, gp, tiles, stream);
   const PairParams pp = pair_params(gp, lhs, order != nullptr);
   CUtensorMap box[2];
   for (int i = 0; i < 2; ++i)
@@ -933,7 +933,7 @@ kapyb_status adapters_decode(kapyb_handle h, const AdapterCall &c, cudaStream_t 
     stages = std::min(8, budget / stage_bytes);
     // the ring also takes the partial sums
     if (stages >= 3 && stages * stage_bytes >= wide * 512) break;
-    if (split >= 8 || 2 * split > num_kb) return KAPYB_OK;
+    if (split >= 8) return KAPYB_OK;
   }
   const int smem = 1024 + stages * stage_bytes + delta;
 
@@ -1224,7 +1224,7 @@ extern "C" KAPYB_API kapyb_status kapyb_matmul_adapters(kapyb_handle h, const ka
     bool taken = false;
     kapyb_status st = adapters_decode(h, c, s, &taken);
     if (st != KAPYB_OK || taken) return st;
-    if (lhs->size0 > kDecodeMaxRows) st = adapters_pairs(h, c, s, &taken);
+    st = adapters_pairs(h, c, s, &taken);
     if (st != KAPYB_OK || taken) return st;
   }
   AdapterSimtParams p{};

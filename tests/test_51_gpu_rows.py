@@ -422,6 +422,54 @@ def test_matmul_grouped_epilogue(handle, act, out_dt, gated):
         within(y[:val.shape[0]], val, tol)
 
 
+def test_which_kernels_run(handle):
+    """16-bit operands TMA can describe run on the tensor cores, the rest on CUDA cores."""
+    ran = lambda call: (call(), handle.last_kernel)[1]
+    for dt, few, many, grad in [(torch.bfloat16, "grouped_tcgen05", "grouped_pair", "grouped_grad_pair"),
+                                (torch.float32, "grouped_simt", "grouped_simt", "grouped_grad_simt")]:
+        w = randn(1, 4, 64, 128, dtype=dt)
+        for T, want in ((40, few), (400, many)):
+            order, offsets, _ = plan_of(handle, 3, T, 4, 1)
+            x = randn(2, T, 64, dtype=dt)
+            assert ran(lambda: handle.matmul_grouped(x, w, offsets, order=order)) == want
+            assert ran(lambda: handle.matmul_grouped(x, w, offsets, gated=True)) == want
+        assert ran(lambda: handle.matmul_grouped_grad(x, x, offsets)) == grad
+        for T, want in ((256, "adapters_decode"), (257, "adapters_pair")):
+            x, wo, a, b, index = make_adapters((T, 2, 64, 64, 8, "each"), dt)
+            assert ran(lambda: handle.matmul_adapters(x, wo, a, b, index)) == (
+                want if dt == torch.bfloat16 else "adapter_simt")
+    # a row pitch that is not a multiple of 16 bytes
+    x = randn(2, 400, 67, dtype=torch.bfloat16)[:, :64]
+    assert ran(lambda: handle.matmul_grouped(x, randn(1, 4, 64, 128, dtype=torch.bfloat16), offsets)) == "grouped_simt"
+
+
+def test_rows_beyond_two_to_the_31_elements(handle):
+    """A source, and rows to combine, whose last rows lie behind 2^31 elements."""
+    R, K = 550_000, 4096
+    x = torch.zeros(R, K, device=DEV, dtype=torch.bfloat16)
+    pick = torch.tensor([R - 1, 3, 524_289, R - 2], device=DEV)
+    x[pick] = randn(1, 4, K, dtype=torch.bfloat16)
+    w = randn(2, 2, K, 64, dtype=torch.bfloat16, std=0.02)
+    for P in (4, 300):
+        order = pick[torch.arange(P, device=DEV) % 4].to(torch.int32)
+        offsets = torch.tensor([0, P // 2, P], dtype=torch.int32, device=DEV)
+        y = handle.matmul_grouped(x, w, offsets, order=order)
+        handle.check()
+        val, tol = products_ref(x, w, offsets, order, 1, False, 0, 1.0, None, torch.bfloat16, K)
+        within(y, val, tol)
+    d = handle.matmul_grouped_grad(x, randn(3, P, 64, dtype=torch.bfloat16), offsets, order=order)
+    e = handle.matmul_grouped_grad(x[order.long()], randn(3, P, 64, dtype=torch.bfloat16), offsets)
+    assert torch.equal(d, e)
+    slots = pick.to(torch.int32).view(2, 2)
+    assert torch.equal(handle.combine_rows(x, slots, out_dtype=torch.float32),
+                       x[pick].float().view(2, 2, K).sum(1))
+    g = randn(4, 2, K, dtype=torch.bfloat16)
+    other = torch.empty_like(x)
+    handle.combine_rows_backward(x, slots, g, grad_rows=other)
+    handle.check()
+    assert torch.equal(other[pick], g.repeat_interleave(2, 0))
+
+
 def test_matmul_grouped_strides(handle):
     """Operands and outputs that are views: row pitches, a column offset, weights inside a
     larger tensor, and layouts the tensor cores cannot be fed from."""
