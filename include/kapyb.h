@@ -707,7 +707,7 @@ KAPYB_API kapyb_status kapyb_tuning_load(const char *file, int32_t *n_entries);
 KAPYB_API kapyb_status kapyb_tuning_clear(void);
 
 /* Name of the kernel family the last call on `h` dispatched to ("tcgen05_1cta",
- * "tcgen05_2cta", "tcgen05_skinny", "simt"; the rows calls: "grouped_tcgen05",
+ * "tcgen05_2cta", "tcgen05_skinny", "simt"; the rows calls:
  * "grouped_pair", "grouped_grad_pair", "adapters_decode", "adapters_pair", the "_simt"
  * ones on CUDA cores, ...). */
 KAPYB_API const char *kapyb_last_kernel(kapyb_handle h);

@@ -26,6 +26,8 @@
 
 namespace kapyb {
 
+__device__ __forceinline__ int round16(int v) { return (v + 15) & ~15; }
+
 constexpr int kDecodeMaxRows = 256;
 constexpr int kLowThreads = 512;
 constexpr int kLowMaxSplit = 4;

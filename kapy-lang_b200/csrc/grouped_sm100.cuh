@@ -3,25 +3,27 @@
 //   gradient  out[g][k, n] = alpha * sum over p of group g  lhs[row(p), k] * grad[p, n]
 //   adapters  out[t, n]    = epilogue( lhs[t] . rhs ) + low[t] . up[i(t)]
 //
-// The output columns n always fill the 128-row side of the MMA (TMEM lanes) and the
-// output rows its N side:  D[n, r] = sum A[n, .] B[r, .].  The N side of a tcgen05.mma
-// is any multiple of 16 up to 256, so a group of three rows costs a 16-wide MMA and
-// not a 128-row tile, and one kernel serves a decode step (a few rows per group,
-// bound by streaming the weights) and a prompt (hundreds of rows, bound by the tensor
-// cores).  A group's rows are dealt out in equal tiles of at most BT.
+// Two CTAs of a cluster share a tile of 256 output columns and up to 256 rows through
+// tcgen05.mma.cta_group::2.  The output columns n always fill the M side of the MMA (TMEM
+// lanes, 128 in each CTA) and the output rows its N side:  D[n, r] = sum A[n, .] B[r, .].
+// The N side of a pair's MMA is any multiple of 32 up to 256, so a group of three rows
+// costs a 32-wide MMA and not a tile of 256 rows, and one kernel serves a decode step (a
+// few rows per group, bound by streaming the weights) and a prompt (hundreds of rows,
+// bound by the tensor cores).  A group's rows are dealt out in equal tiles.
+// (A kernel of single CTAs with tiles of 64 rows, for few rows a group, was 2% quicker at
+// best, 301 us against 308 for 8 groups of 4 rows, 4096 x 14336 gated.  64 groups of 2048 x
+// 2048 took it 115 us against 103 at 8 rows a group, 168 against 104 at 32.)
 //
-// Rows named by a plan are fetched by TMA where they lie (tile::gather4: four row
-// numbers per instruction, one lane each), so no permuted copy of lhs is written.
+// Rows named by a plan are fetched where they lie, so no permuted copy of lhs is written.
 // Rows outside lhs, and the K tail of both operands, arrive as zeros.  A tile's rows
 // behind the end of its group may be those of the next group: they only reach output
 // rows that are not stored.  In the gradient the rows are the contraction, so there
 // everything behind a group's end is fetched as zeros on both sides (a zero on one
 // side alone would still let a NaN through).
 //
-// Persistent CTAs; warp 0 produces (the whole warp, one TMA instruction per lane),
-// warp 1 issues the MMAs, warps 2..5 drain: two accumulator slots in TMEM let the
-// drain of one tile run under the next one's main loop.  MSETS = 2 multiplies the
-// same rows with two column blocks, gate and up, and joins them in the drain.
+// Persistent CTAs; warp 0 fetches columns, warp 1 issues the MMAs, warps 2..5 drain: two
+// accumulator slots in TMEM let the drain of one tile run under the next one's main loop.
+// The other warps fetch rows (below).
 //
 // The table of tiles depends on the plan, which only the device knows: every CTA
 // builds it in shared memory from the offsets (a scan over at most 1024 groups).
@@ -36,19 +38,6 @@
 
 namespace kapyb {
 
-// Four rows of a 2-D tensor (map with a box one row high), named one by one: they land
-// behind one another in shared memory, under the map's swizzle.  Rows outside the
-// tensor are filled with zeros.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const void *tmap, uint32_t bar, int x, int r0,
-                                            int r1, int r2, int r3) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-      :
-      : "r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2),
-        "r"(r3)
-      : "memory");
-}
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *tmap, uint32_t bar, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -61,7 +50,7 @@ struct GroupedParams {
   int groups, rows;      // rows: positions of the plan
   int cols;              // output columns (of one group)
   int K;                 // forward: contraction length; gradient: output rows of one group
-  int n_tiles;           // ceil(cols / 128)
+  int n_tiles;           // column blocks of 256 (gated: 128)
   int k_tiles;           // gradient: ceil(K / BT)
   int num_kb;            // forward: ceil(K / 64)
   const int32_t *offsets, *order;
@@ -80,25 +69,7 @@ struct GroupedParams {
   uint32_t wait_limit_us;
 };
 
-constexpr int kGroupedThreads = 192;
 constexpr int kGroupedMaxGroups = 1024;
-
-template <int BT, int MSETS>
-struct GroupedCfg {
-  static constexpr int A_BYTES = MSETS * 128 * 128;  // 128 columns x 64 of the contraction, 16-bit
-  static constexpr int B_BYTES = BT * 128;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int CTRL_BYTES = 1024;
-  static constexpr int TABLE_BYTES = (3 * kGroupedMaxGroups + 8) * 4;
-  static constexpr int SMEM_LIMIT = 232448;
-  static constexpr int STAGES_RAW = (SMEM_LIMIT - 1024 - CTRL_BYTES - TABLE_BYTES) / STAGE_BYTES;
-  static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + CTRL_BYTES + TABLE_BYTES;
-  static constexpr int SLOT_COLS = BT * MSETS;
-  static constexpr int TMEM_COLS = 2 * SLOT_COLS;
-  static_assert(BT % 32 == 0 && BT <= 256 && TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "tile");
-  static_assert(STAGES >= 3, "pipeline too shallow");
-};
 
 // One output tile.
 struct GroupedTile {
@@ -122,8 +93,6 @@ __device__ __forceinline__ void raster(int in, int tiles, int n_tiles, int &m, i
   n = r / high;
   m = first + r - n * high;
 }
-
-__device__ __forceinline__ int round16(int v) { return (v + 15) & ~15; }
 
 // The tile table in shared memory: first[g] = tiles of output rows in front of group
 // g, begin[g] / count[g] its positions.
@@ -168,27 +137,6 @@ __device__ __forceinline__ int find_group(const GroupedTable &t, int groups, int
   return lo;
 }
 
-template <int BT>
-__device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams &p, const GroupedTable &t, int idx) {
-  GroupedTile r;
-  const int q = idx / p.n_tiles;
-  const int lo = find_group(t, p.groups, q);
-  r.g = lo;
-  const int tiles = t.first[lo + 1] - t.first[lo];
-  const int in = idx - t.first[lo] * p.n_tiles;
-  int m, n;
-  raster(in, tiles, p.n_tiles, m, n);
-  const int cnt = t.count[lo];
-  const int each = round16((cnt + tiles - 1) / tiles);
-  r.n0 = n * 128;
-  r.r0 = t.begin[lo] + m * each;
-  r.rows = min(each, cnt - m * each);
-  r.wide = round16(r.rows);
-  r.num_kb = p.num_kb;
-  r.p0 = r.p1 = 0;
-  return r;
-}
-
 template <int R>
 __device__ __forceinline__ void grouped_activation(int activation, float (&f)[R]) {
   switch (activation) {
@@ -209,16 +157,10 @@ __device__ __forceinline__ void grouped_activation(int activation, float (&f)[R]
 }
 
 // Scale, bias and activation of 32 values of one output column.
-template <int MSETS>
-__device__ __forceinline__ void grouped_finish32(const GroupedParams &p, float alpha, float (&f)[32], const float *up,
-                                                 float bias, float bias_up) {
+__device__ __forceinline__ void grouped_finish32(const GroupedParams &p, float (&f)[32], float bias) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = f[i] * alpha + bias;
+  for (int i = 0; i < 32; ++i) f[i] = f[i] * p.alpha + bias;
   grouped_activation(p.activation, f);
-  if constexpr (MSETS == 2) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] *= up[i] * alpha + bias_up;
-  }
 }
 
 // R output rows of one column per lane -> memory.  `at` points at (first row, column n),
@@ -379,241 +321,11 @@ __device__ __forceinline__ void grouped_scatter32(const GroupedParams &p, char *
   }
 }
 
-// tmA: forward: rhs, 3-D (unit axis, other axis, group), boxes of 64 x 128 (K-major) or
-// 64 x 64 (MN-major); gradient: grad [positions, cols], one-row boxes of 64 columns.
-// tmB: lhs [source rows, K]: one-row boxes of 64 columns (gathered, and the gradient),
-// or 64 x 32 boxes (rows already in plan order).
-template <int BT, int MSETS>
-__global__ void __launch_bounds__(kGroupedThreads, 1)
-grouped_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                       const GroupedParams p) {
-  using Cfg = GroupedCfg<BT, MSETS>;
-  constexpr int STAGES = Cfg::STAGES;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                              ~static_cast<uintptr_t>(1023));
-  uint8_t *sA = smem;
-  uint8_t *sB = sA + STAGES * Cfg::A_BYTES;
-  uint64_t *bars = reinterpret_cast<uint64_t *>(sB + STAGES * Cfg::B_BYTES);
-  uint64_t *full_bar = bars, *empty_bar = bars + STAGES, *tfull_bar = bars + 2 * STAGES, *tempty_bar = tfull_bar + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tempty_bar + 2);
-  volatile uint32_t *abort_flag = tmem_slot + 1;  // two words
-  int *table_mem = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(bars) + Cfg::CTRL_BYTES);
-  GroupedTable table{table_mem, table_mem + kGroupedMaxGroups + 1, table_mem + 2 * kGroupedMaxGroups + 1};
-
-  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
-  const int lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      ptx::mbar_init(ptx::smem_u32(&full_bar[s]), 1);
-      ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), 1);
-    }
-    for (int a = 0; a < 2; ++a) {
-      ptx::mbar_init(ptx::smem_u32(&tfull_bar[a]), 1);
-      ptx::mbar_init(ptx::smem_u32(&tempty_bar[a]), 4);
-    }
-    abort_flag[0] = 0u;
-    abort_flag[1] = p.wait_limit_us;
-    ptx::fence_barrier_init();
-    ptx::prefetch_tensormap(&tmA);
-    ptx::prefetch_tensormap(&tmB);
-  }
-  if (warp == 1) {
-    ptx::tmem_alloc<1>(ptx::smem_u32(tmem_slot), Cfg::TMEM_COLS);
-    ptx::tmem_relinquish<1>();
-  }
-  if (warp == 0) build_tile_table(p.offsets, p.groups, p.rows, BT, table, lane);
-  ptx::tc_fence_before();
-  __syncthreads();
-  ptx::tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  const int total = table.first[p.groups] * p.n_tiles;
-
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    // the source row of position q, src_rows (a row of zeros) where there is none
-    auto row_of = [&](int q, int end) -> int {
-      if (q >= end) return p.src_rows;
-      const long long r = source_row(p.order, p.fan, p.src_rows, q);
-      return r < 0 ? p.src_rows : static_cast<int>(r);
-    };
-    const bool gather = p.order != nullptr;
-    for (int idx = blockIdx.x; ok && idx < total; idx += gridDim.x) {
-      const GroupedTile t = grouped_tile<BT>(p, table, idx);
-      // this lane's four rows of the tile: one gather instruction
-      static_assert(BT <= 128, "one gather instruction a lane");
-      int rows4[4];
-      if (gather) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = lane * 4 + j;
-          rows4[j] = r < t.wide ? row_of(t.r0 + r, t.r0 + t.rows) : p.src_rows;
-        }
-      }
-      const int boxes = gather ? t.wide / 4 : (t.wide + 31) / 32;
-      const uint32_t b_bytes = static_cast<uint32_t>(boxes) * (gather ? 512u : 4096u);
-      for (int kb = 0; kb < t.num_kb; ++kb) {
-        const bool got = ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag);
-        if (!__all_sync(0xffffffffu, got)) {
-          ok = false;
-          break;
-        }
-        const uint32_t fb = ptx::smem_u32(&full_bar[stage]);
-        const uint32_t a_dst = ptx::smem_u32(sA + stage * Cfg::A_BYTES);
-        const uint32_t b_dst = ptx::smem_u32(sB + stage * Cfg::B_BYTES);
-        if (lane == 0) ptx::mbar_arrive_expect_tx(fb, Cfg::A_BYTES + b_bytes);
-        __syncwarp();
-        const int k0 = kb * 64;
-        if (p.a_mn_major) {
-          if (lane < 2 * MSETS)
-            ptx::tma_load_3d(a_dst + lane * 8192, &tmA, fb, t.n0 + (lane & 1) * 64 + (lane >> 1) * p.cols, k0, t.g);
-        } else {
-          if (lane < MSETS) ptx::tma_load_3d(a_dst + lane * 16384, &tmA, fb, k0, t.n0 + lane * p.cols, t.g);
-        }
-        if (gather) {
-          if (lane < boxes) tma_gather4(b_dst + lane * 512, &tmB, fb, k0, rows4[0], rows4[1], rows4[2], rows4[3]);
-        } else if (lane < boxes) {
-          tma_load_2d(b_dst + lane * 4096, &tmB, fb, k0, t.r0 + lane * 32);
-        }
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------- MMA issuer
-    auto wait_all = [&](uint32_t bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort_flag)) != 0;
-    };
-    // K-major tile: 128-byte rows, 8-row groups 1024 bytes apart, a K step is 32 bytes.
-    // MN-major tile: 64-column chunks 8192 bytes apart, a K step is 16 rows of 128 bytes.
-    const bool a_mn = p.a_mn_major;
-    const uint32_t a_lo0 = ((a_mn ? 8192u : 16u) >> 4) << 16 | (ptx::smem_u32(sA) >> 4);
-    const uint32_t b_lo0 = 1u << 16 | (ptx::smem_u32(sB) >> 4);
-    constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    const uint32_t a_step = (a_mn ? 2048u : 32u) >> 4;
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    bool ok = true;
-    for (int idx = blockIdx.x; ok && idx < total; idx += gridDim.x) {
-      const GroupedTile t = grouped_tile<BT>(p, table, idx);
-      const uint32_t idesc = ptx::make_idesc_f16(p.bf16, a_mn, 0, 128, t.wide);
-      if (!wait_all(ptx::smem_u32(&tempty_bar[acc]), acc_phase ^ 1u)) break;
-      ptx::tc_fence_after();
-      const uint32_t d = tmem_base + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
-      for (int kb = 0; kb < t.num_kb; ++kb) {
-        if (!wait_all(ptx::smem_u32(&full_bar[stage]), phase)) {
-          ok = false;
-          break;
-        }
-        ptx::tc_fence_after();
-        if (ptx::elect_one()) {
-          const uint32_t a_lo = a_lo0 + static_cast<uint32_t>(stage) * (Cfg::A_BYTES >> 4);
-          const uint32_t b_lo = b_lo0 + static_cast<uint32_t>(stage) * (Cfg::B_BYTES >> 4);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint64_t bd = (static_cast<uint64_t>(hi) << 32) | (b_lo + k * 2u);
-#pragma unroll
-            for (int s = 0; s < MSETS; ++s) {
-              const uint64_t ad = (static_cast<uint64_t>(hi) << 32) | (a_lo + s * (16384u >> 4) + k * a_step);
-              ptx::umma_k<1, 0>(d + s * BT, ad, bd, idesc, (kb | k) != 0 ? 1u : 0u);
-            }
-          }
-          ptx::umma_commit<1>(ptx::smem_u32(&empty_bar[stage]));
-        }
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-      if (!ok) break;
-      if (ptx::elect_one()) ptx::umma_commit<1>(ptx::smem_u32(&tfull_bar[acc]));
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
-    }
-  } else {
-    // ------------------------------------------------------------ epilogue
-    const int q = warp & 3;  // TMEM lane quarter this warp may touch
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    for (int idx = blockIdx.x; idx < total; idx += gridDim.x) {
-      const GroupedTile t = grouped_tile<BT>(p, table, idx);
-      const int n = t.n0 + q * 32 + lane;
-      const bool mine = n < p.cols, both = (n | 1) < p.cols;
-      float bias = 0.0f, bias_up = 0.0f;
-      if (p.bias != nullptr && mine) {
-        const long long at = static_cast<long long>(t.g) * p.bias_cols + n;
-        bias = load_as_f32(p.bias, p.bias_dtype, at);
-        if constexpr (MSETS == 2) bias_up = load_as_f32(p.bias, p.bias_dtype, at + p.cols);
-      }
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&tfull_bar[acc]), acc_phase, abort_flag))) break;
-      ptx::tc_fence_after();
-      const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * Cfg::SLOT_COLS);
-      const bool warp_has = t.n0 + q * 32 < p.cols;
-      char *out = static_cast<char *>(p.out) +
-                  static_cast<long long>(t.r0) * p.row_pitch + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll);
-      for (int c = 0; c < t.rows && warp_has; c += 32) {
-        float f[32], u[MSETS == 2 ? 32 : 1];
-        uint32_t v[32];
-        ptx::tmem_ld_32x32(src + c, v);
-        if constexpr (MSETS == 2) {
-          uint32_t w[32];
-          ptx::tmem_ld_32x32(src + BT + c, w);
-          ptx::tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) u[i] = __uint_as_float(w[i]);
-        } else {
-          ptx::tmem_ld_wait();
-        }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
-        if (c + 32 >= t.rows) {
-          // the accumulator has been read: the slot is the MMA warp's again
-          ptx::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&tempty_bar[acc]));
-        }
-        grouped_finish32<MSETS>(p, p.alpha, f, u, bias, bias_up);
-        grouped_store(p, out + static_cast<long long>(c) * p.row_pitch, f, t.rows - c, lane, mine, both);
-      }
-      if (!warp_has) {
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&tempty_bar[acc]));
-      }
-      acc ^= 1;
-      if (acc == 0) acc_phase ^= 1u;
-    }
-  }
-
-  // ---------------------------------------------------------------- teardown
-  ptx::tc_fence_before();
-  __syncthreads();
-  if (*abort_flag != 0u) {
-    if (threadIdx.x == 0) atomicExch(p.status, kStatusTimeout);
-    // loads in flight land before the shared memory they target is released
-    const uint64_t t0 = ptx::globaltimer_ns();
-    while (ptx::globaltimer_ns() - t0 < 200000ull) {
-    }
-    __syncthreads();
-  }
-  if (warp == 1) {
-    ptx::tc_fence_after();
-    ptx::tmem_dealloc<1>(tmem_base, Cfg::TMEM_COLS);
-  }
-}
-
 // ------------------------------------------------------------------- CTA pairs
 //
-// The kernel for many rows per group: two CTAs of a cluster share one tile through
-// tcgen05.mma.cta_group::2.  Each holds 128 of the tile's 256 output columns (its M
-// half) and fetches half of its rows (its half of the N side), so a row is pulled
-// from L2 once per 256 columns and an SM reads a third fewer operand bytes from
-// shared memory per flop than alone.
+// Each CTA holds 128 of the tile's 256 output columns (its M half) and fetches half of
+// its rows (its half of the N side), so a row is pulled from L2 once per 256 columns and
+// an SM reads a third fewer operand bytes from shared memory per flop than alone.
 //
 // Gathered rows.  tile::gather4 costs about 70 clocks per four rows here (measured:
 // 37 ns with every lane of a warp issuing), four times the MMA time of the tile they
@@ -710,8 +422,7 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void *tmap,
 
 __device__ __forceinline__ int round32(int v) { return (v + 31) & ~31; }
 
-// The tile of a pair: as grouped_tile, for blocks of 256 columns (128 gated ones), rows
-// rounded to 32 (the N side of a pair's MMA is a multiple of 32).
+// Tile number idx.
 template <int MODE>
 __device__ __forceinline__ GroupedTile pair_tile(const GroupedParams &p, const GroupedTable &t, int idx) {
   constexpr int BT = PairCfg::BT;
@@ -775,7 +486,8 @@ __device__ __forceinline__ bool each_adapter(const GroupedTable &t, int adapters
   return true;
 }
 
-// tmA: forward: rhs as in grouped_tcgen05_kernel; gradient: grad in boxes of 64 x 64.
+// tmA: forward: rhs, 3-D (unit axis, other axis, group), boxes of 64 x 128 (K-major) or
+// 64 x 64 (MN-major, gated); gradient: grad [positions, cols] in boxes of 64 x 64.
 // Rows that come by TMA: lhs in plan order in boxes of 64 x 128 (tmB), 64 x 64 (tmR) and
 // 64 x 32 (tmU); adapters: the low-rank products, both halves behind one another, in boxes
 // of 64 x 128 (tmB) and 64 x 16 (tmR), and tmU up, 3-D as rhs.
@@ -1154,7 +866,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
               for (int j = 0; j < 32; ++j) f[j] = f[j] * p.alpha + __shfl_sync(0xffffffffu, row_bias, j);
               grouped_activation(p.activation, f);
             } else {
-              grouped_finish32<1>(p, p.alpha, f, nullptr, bias, 0.0f);
+              grouped_finish32(p, f, bias);
             }
             grouped_scatter32(p, static_cast<char *>(p.out) + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll), f, to, lane,
                               mine, both);
@@ -1188,7 +900,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             const int first = c + (up_side ? 16 : 0);
             grouped_store(p, out + static_cast<long long>(first) * p.row_pitch, g, t.rows - first, lane, mine, both);
           } else {
-            grouped_finish32<1>(p, p.alpha, f, nullptr, bias, 0.0f);
+            grouped_finish32(p, f, bias);
             char *at = out + static_cast<long long>(c) * p.row_pitch;
             if (GRAD && piece > 0) {  // f32: to what the pieces before have left there
               add_rows32(at, p.row_pitch, f, t.rows - c, lane, mine, p.wide_stores);

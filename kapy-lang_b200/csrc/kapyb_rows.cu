@@ -369,17 +369,6 @@ bool wide_stores_ok(const void *out, int dtype, int64_t s0, int64_t group) {
   return reinterpret_cast<uintptr_t>(out) % (n * dtype_size(dtype)) == 0 && s0 % n == 0 && group % n == 0;
 }
 
-template <int BT, int MSETS>
-kapyb_status launch_grouped(kapyb_handle h, const CUtensorMap &tmA, const CUtensorMap &tmB, const GroupedParams &gp,
-                            long long tiles, cudaStream_t stream) {
-  using Cfg = GroupedCfg<BT, MSETS>;
-  constexpr auto kern = grouped_tcgen05_kernel<BT, MSETS>;
-  TRY(allow_smem<kern>(h, Cfg::SMEM_BYTES));
-  const int grid = static_cast<int>(std::min<long long>(tiles, h->sm_count));
-  kern<<<grid, kGroupedThreads, Cfg::SMEM_BYTES, stream>>>(tmA, tmB, gp);
-  return launched(h, "grouped_tcgen05");
-}
-
 PairParams pair_params(const GroupedParams &gp, const kapyb_tensor2d *lhs, bool gather) {
   PairParams pp{};
   pp.g = gp;
@@ -455,7 +444,7 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
   gp.rows = out->size0;
   gp.cols = out->size1;
   gp.K = lhs->size1;
-  gp.n_tiles = (gp.cols + 127) / 128;
+  gp.n_tiles = gated ? (gp.cols + 127) / 128 : (gp.cols + 255) / 256;
   gp.num_kb = (gp.K + 63) / 64;
   gp.offsets = offsets;
   gp.order = order;
@@ -476,27 +465,17 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
   gp.status = h->status;
   gp.wait_limit_us = h->wait_limit_us;
   const long long busy = std::min(groups, gp.rows);
-  const bool narrow = gp.rows <= 32 * busy;  // rows per group that has any, at most
-  const int bt = narrow ? 64 : PairCfg::BT;
-  if (!narrow) gp.n_tiles = gated ? (gp.cols + 127) / 128 : (gp.cols + 255) / 256;
-  const long long tiles = ((gp.rows + bt - 1ll) / bt + busy) * gp.n_tiles;
+  const long long tiles = ((gp.rows + PairCfg::BT - 1ll) / PairCfg::BT + busy) * gp.n_tiles;
   if (tiles >= (1ll << 31)) return KAPYB_OK;
-  CUtensorMap tmA, tmB;
-  TRY(make_tmap(h, &tmA, elem_ptr(rhs), rhs->dtype, unit, other, groups, ld, group_stride, 64,
-                mn || (gated && !narrow) ? 64 : 128));
-  TRY(make_row_tmap(h, &tmB, elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
-                    lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, order && narrow ? 1 : 32));
+  const int64_t lhs_ld = lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8;
+  CUtensorMap tmA, box[3];  // rows in plan order come in boxes of 128, 64 and 32
+  TRY(make_tmap(h, &tmA, elem_ptr(rhs), rhs->dtype, unit, other, groups, ld, group_stride, 64, mn || gated ? 64 : 128));
+  for (int i = 0; i < 3; ++i)
+    TRY(make_row_tmap(h, &box[i], elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0, lhs_ld, 128 >> i));
   *taken = true;
-  if (narrow)
-    return gated ? launch_grouped<64, 2>(h, tmA, tmB, gp, tiles, stream)
-                 : launch_grouped<64, 1>(h, tmA, tmB, gp, tiles, stream);
   const PairParams pp = pair_params(gp, lhs, order != nullptr);
-  CUtensorMap box[2];
-  for (int i = 0; i < 2; ++i)
-    TRY(make_row_tmap(h, &box[i], elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0,
-                      lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8, i == 0 ? 128 : 64));
-  return gated ? launch_pairs<PAIR_GATED>(h, tmA, box[0], box[1], tmB, pp, tiles, stream)
-               : launch_pairs<PAIR_FORWARD>(h, tmA, box[0], box[1], tmB, pp, tiles, stream);
+  return gated ? launch_pairs<PAIR_GATED>(h, tmA, box[0], box[1], box[2], pp, tiles, stream)
+               : launch_pairs<PAIR_FORWARD>(h, tmA, box[0], box[1], box[2], pp, tiles, stream);
 }
 
 kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const kapyb_tensor2d *grad,

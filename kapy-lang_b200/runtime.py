@@ -734,6 +734,7 @@ class Handle:
             self._raise(st)
         return out
 
+
 def shard_range(total: int, parts: int, rank: int, align: int = 1):
     """[begin, end) of `total` units owned by `rank` (blocks of `align`)."""
     lib = abi.load()

@@ -425,19 +425,19 @@ def test_matmul_grouped_epilogue(handle, act, out_dt, gated):
 def test_which_kernels_run(handle):
     """16-bit operands TMA can describe run on the tensor cores, the rest on CUDA cores."""
     ran = lambda call: (call(), handle.last_kernel)[1]
-    for dt, few, many, grad in [(torch.bfloat16, "grouped_tcgen05", "grouped_pair", "grouped_grad_pair"),
-                                (torch.float32, "grouped_simt", "grouped_simt", "grouped_grad_simt")]:
+    for dt, want, grad in [(torch.bfloat16, "grouped_pair", "grouped_grad_pair"),
+                           (torch.float32, "grouped_simt", "grouped_grad_simt")]:
         w = randn(1, 4, 64, 128, dtype=dt)
-        for T, want in ((40, few), (400, many)):
+        for T in (40, 400):
             order, offsets, _ = plan_of(handle, 3, T, 4, 1)
             x = randn(2, T, 64, dtype=dt)
             assert ran(lambda: handle.matmul_grouped(x, w, offsets, order=order)) == want
             assert ran(lambda: handle.matmul_grouped(x, w, offsets, gated=True)) == want
         assert ran(lambda: handle.matmul_grouped_grad(x, x, offsets)) == grad
-        for T, want in ((256, "adapters_decode"), (257, "adapters_pair")):
+        for T, fast in ((256, "adapters_decode"), (257, "adapters_pair")):
             x, wo, a, b, index = make_adapters((T, 2, 64, 64, 8, "each"), dt)
             assert ran(lambda: handle.matmul_adapters(x, wo, a, b, index)) == (
-                want if dt == torch.bfloat16 else "adapter_simt")
+                fast if dt == torch.bfloat16 else "adapter_simt")
     # a row pitch that is not a multiple of 16 bytes
     x = randn(2, 400, 67, dtype=torch.bfloat16)[:, :64]
     assert ran(lambda: handle.matmul_grouped(x, randn(1, 4, 64, 128, dtype=torch.bfloat16), offsets)) == "grouped_simt"
