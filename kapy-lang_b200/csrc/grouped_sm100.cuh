@@ -21,9 +21,12 @@
 // everything behind a group's end is fetched as zeros on both sides (a zero on one
 // side alone would still let a NaN through).
 //
-// Persistent CTAs; warp 0 fetches columns, warp 1 issues the MMAs, warps 2..5 drain: two
-// accumulator slots in TMEM let the drain of one tile run under the next one's main loop.
-// The other warps fetch rows (below).
+// Persistent CTAs; warp 0 fetches columns, warp 1 issues the MMAs, warps 6..14 fetch rows
+// (below), warps 2..5 and 15..18 drain: two accumulator slots in TMEM let the drain of one
+// tile run under the next one's main loop.  A drain is bound by latency, some 700 clocks
+// for 32 rows of 32 columns, twice that with gate and up; with four warps it took longer
+// than 16 K blocks of MMAs (64 gradients of 2048 x 2048 from 64 rows each: 251 us, with
+// eight 188; K of 256, gated, 16384 x 4096: 122 and 89).
 //
 // The table of tiles depends on the plan, which only the device knows: every CTA
 // builds it in shared memory from the offsets (a scan over at most 1024 groups).
@@ -163,25 +166,41 @@ __device__ __forceinline__ void grouped_finish32(const GroupedParams &p, float (
   grouped_activation(p.activation, f);
 }
 
+// 16-bit values of one column per lane (rows 2i, 2i + 1 in w[i]) -> words of two adjacent
+// columns: of every four rows the even lane of two neighbours gets the first two and the
+// odd lane the others, one exchange for four stores.
+template <int WORDS>
+__device__ __forceinline__ void join_columns16(uint32_t (&w)[WORDS], int lane) {
+  const bool odd = lane & 1;
+  const uint32_t first = odd ? 0x1054u : 0x5410u, second = odd ? 0x3276u : 0x7632u;
+#pragma unroll
+  for (int i = 0; i < WORDS; i += 2) {
+    const uint32_t keep = odd ? w[i + 1] : w[i];
+    const uint32_t take = __shfl_xor_sync(0xffffffffu, odd ? w[i] : w[i + 1], 1);
+    w[i] = __byte_perm(keep, take, first);
+    w[i + 1] = __byte_perm(keep, take, second);
+  }
+}
+
 // R output rows of one column per lane -> memory.  `at` points at (first row, column n),
 // rows are `pitch` bytes apart, `left` of them exist (ALL: all of them).
-// Neighbouring lanes swap half of their 16-bit values so that each stores two adjacent
-// columns of every other row as one word: half the store instructions of one value
-// each.  The common case (32 rows, 32 columns) carries no conditions and 32-bit row
-// offsets: the drain of a short main loop is bound by the instructions of this loop.
+// The common case (32 rows, 32 columns) carries no conditions and 32-bit row offsets: the
+// drain of a short main loop is bound by the latency of this loop, one warp a scheduler.
 template <int DT, int RN, bool ALL, int R>
 __device__ __forceinline__ void store_pairs16(char *at, uint32_t pitch, const float (&f)[R], int left, int lane,
                                               bool both) {
-  const bool odd = lane & 1;
-  char *base = odd ? at - 2 + pitch : at;  // (first row + odd, even column)
+  uint32_t w[R / 2];
+#pragma unroll
+  for (int i = 0; i < R / 2; ++i) w[i] = cvt_pack2_t<DT, RN>(f[2 * i], f[2 * i + 1]);
+  join_columns16(w, lane);
+  const int skip = lane & 1 ? 2 : 0;
+  char *base = lane & 1 ? at - 2 + 2 * pitch : at;  // (first row + skip, even column)
   uint32_t off = 0u;
 #pragma unroll
-  for (int j = 0; j < R; j += 2) {
-    const float give = odd ? f[j] : f[j + 1];
-    const float take = __shfl_xor_sync(0xffffffffu, give, 1);
-    const uint32_t w = odd ? cvt_pack2_t<DT, RN>(take, f[j + 1]) : cvt_pack2_t<DT, RN>(f[j], take);
-    if (ALL || (both && j + (odd ? 1 : 0) < left)) *reinterpret_cast<uint32_t *>(base + off) = w;
-    off += 2u * pitch;
+  for (int i = 0; i < R / 2; i += 2) {
+    if (ALL || (both && 2 * i + skip < left)) *reinterpret_cast<uint32_t *>(base + off) = w[i];
+    if (ALL || (both && 2 * i + skip + 1 < left)) *reinterpret_cast<uint32_t *>(base + off + pitch) = w[i + 1];
+    off += 4u * pitch;
   }
 }
 template <int DT, int RN, int R>
@@ -279,17 +298,16 @@ __device__ __forceinline__ void grouped_store(const GroupedParams &p, char *at, 
 template <int DT, int RN>
 __device__ __forceinline__ void scatter_rows16(char *col, uint32_t pitch, const float (&f)[32], int to, int lane,
                                                bool mine, bool both, bool pairs) {
-  const bool odd = lane & 1;
   if (pairs) {
+    uint32_t w[16];
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      const float give = odd ? f[j] : f[j + 1];
-      const float take = __shfl_xor_sync(0xffffffffu, give, 1);
-      const uint32_t w = odd ? cvt_pack2_t<DT, RN>(take, f[j + 1]) : cvt_pack2_t<DT, RN>(f[j], take);
-      const int even_row = __shfl_sync(0xffffffffu, to, j), odd_row = __shfl_sync(0xffffffffu, to, j + 1);
-      const int row = odd ? odd_row : even_row;
-      char *at = col + static_cast<long long>(row) * pitch;
-      if (both && row >= 0) *reinterpret_cast<uint32_t *>(odd ? at - 2 : at) = w;
+    for (int i = 0; i < 16; ++i) w[i] = cvt_pack2_t<DT, RN>(f[2 * i], f[2 * i + 1]);
+    join_columns16(w, lane);
+    char *even = lane & 1 ? col - 2 : col;  // the even column of the two
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int row = __shfl_sync(0xffffffffu, to, (i & ~1) * 2 + (i & 1) + (lane & 1) * 2);
+      if (both && row >= 0) *reinterpret_cast<uint32_t *>(even + static_cast<long long>(row) * pitch) = w[i];
     }
     if (!__any_sync(0xffffffffu, mine && !both)) return;
   }
@@ -386,7 +404,7 @@ struct PairParams {
   int low_rows;          // rows of one half of the low-rank products
 };
 
-constexpr int kPairThreads = 192 + 256 + 32;
+constexpr int kPairThreads = 192 + 256 + 32 + 128;
 
 struct PairCfg {
   static constexpr int BT = 256;             // rows of a tile
@@ -395,7 +413,7 @@ struct PairCfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int CTRL_BYTES = 1024;
   static constexpr int TABLE_BYTES = (3 * kGroupedMaxGroups + 8) * 4;
-  static constexpr int SWAP_BYTES = 2 * 2 * 2 * 16 * 32 * 4;  // warp pairs, buffers, directions x 16 rows x 32 lanes
+  static constexpr int SWAP_BYTES = 4 * 2 * 16 * 32 * 4;  // warp pairs, directions x 16 rows x 32 lanes
   static constexpr int SMEM_LIMIT = 232448;
   static constexpr int STAGES = (SMEM_LIMIT - 1024 - CTRL_BYTES - TABLE_BYTES - SWAP_BYTES) / STAGE_BYTES;
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + CTRL_BYTES + TABLE_BYTES + SWAP_BYTES;
@@ -508,8 +526,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   uint64_t *bars = reinterpret_cast<uint64_t *>(sB + STAGES * Cfg::B_BYTES);
   uint64_t *full_bar = bars, *empty_bar = bars + STAGES, *tfull_bar = bars + 2 * STAGES, *tempty_bar = tfull_bar + 2;
   uint64_t *rows_bar = tempty_bar + 2;
-  uint64_t *swap_bar = rows_bar + STAGES;  // [warp pair][buffer]
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(swap_bar + 4);
+  uint64_t *swap_bar = rows_bar + STAGES;  // [warp pair][written, read]
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(swap_bar + 8);
   volatile uint32_t *abort_flag = tmem_slot + 1;  // two words
   int *table_mem = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(bars) + Cfg::CTRL_BYTES);
   GroupedTable table{table_mem, table_mem + kGroupedMaxGroups + 2, table_mem + 2 * kGroupedMaxGroups + 4};
@@ -531,9 +549,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     for (int a = 0; a < 2; ++a) {
       ptx::mbar_init(ptx::smem_u32(&tfull_bar[a]), 1);
-      ptx::mbar_init(ptx::smem_u32(&tempty_bar[a]), 8);  // four epilogue warps of each CTA
+      ptx::mbar_init(ptx::smem_u32(&tempty_bar[a]), 16);  // eight epilogue warps of each CTA
     }
-    for (int i = 0; i < 4; ++i) ptx::mbar_init(ptx::smem_u32(&swap_bar[i]), 2);  // both warps
+    for (int i = 0; i < 8; ++i) ptx::mbar_init(ptx::smem_u32(&swap_bar[i]), 2);  // both warps
     abort_flag[0] = 0u;
     abort_flag[1] = p.wait_limit_us;
     ptx::fence_barrier_init();
@@ -795,8 +813,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       if (!ok) break;
       publish();
     }
-  } else if (warp >= 2 && warp < 6) {
+  } else if ((warp >= 2 && warp < 6) || warp >= 15) {
     // ------------------------------------------------------------ epilogue
+    // Two teams of four warps, one warp to each quarter of TMEM's lanes: they take the
+    // tile's chunks of 32 rows in turn.
+    const int team = warp >= 15 ? 1 : 0;
     const int q = warp & 3;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -827,10 +848,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         ptx::tc_fence_after();
         const uint32_t src = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BT);
         const uint32_t tempty = leader(&tempty_bar[acc]);
-        const bool warp_has = warp_n < p.cols;
+        const bool warp_has = warp_n < p.cols && team * 32 < t.rows;
         char *out = static_cast<char *>(p.out) + (GRAD ? t.g * p.group_bytes : 0ll) +
                     static_cast<long long>(t.r0) * p.row_pitch + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll);
-        for (int c = 0; c < t.rows && warp_has; c += 32) {
+        for (int c = team * 32; c < t.rows && warp_has; c += 64) {
           float f[32];
           if (!GRAD || t.num_kb > 0) {
             uint32_t v[32];
@@ -848,7 +869,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
             for (int i = 0; i < 32; ++i) f[i] = 0.0f;
           }
-          if (c + 32 >= t.rows) {
+          if (c + 64 >= t.rows) {  // this warp's last
             ptx::tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -874,16 +895,20 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] = f[j] * p.alpha + bias;
             // the gate's warp hands over its rows 16 .. 31 and finishes 0 .. 15, the up
-            // columns' warp the other way round; two buffers take turns
+            // columns' warp the other way round
             const bool up_side = q >= 2;
-            float *box = swap_mem + ((q & 1) * 2 + (swaps & 1)) * 1024;
+            float *box = swap_mem + (team * 2 + (q & 1)) * 1024;
+            const uint32_t written = ptx::smem_u32(&swap_bar[(team * 2 + (q & 1)) * 2]), read = written + 8u;
             float g[16], u[16];
+            if (swaps > 0 && !__all_sync(0xffffffffu, ptx::mbar_wait(read, (swaps - 1) & 1, abort_flag))) {
+              alive = false;
+              break;
+            }
 #pragma unroll
             for (int j = 0; j < 16; ++j) (up_side ? box : box + 512)[j * 32 + lane] = up_side ? f[j] : f[16 + j];
             __syncwarp();
-            const uint32_t bar = ptx::smem_u32(&swap_bar[(q & 1) * 2 + (swaps & 1)]);
-            if (lane == 0) ptx::mbar_arrive(bar);
-            if (!__all_sync(0xffffffffu, ptx::mbar_wait(bar, (swaps >> 1) & 1, abort_flag))) {
+            if (lane == 0) ptx::mbar_arrive(written);
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait(written, swaps & 1, abort_flag))) {
               alive = false;
               break;
             }
@@ -894,6 +919,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
               g[j] = up_side ? other : f[j];
               u[j] = up_side ? f[16 + j] : other;
             }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(read);
             grouped_activation(p.activation, g);
 #pragma unroll
             for (int j = 0; j < 16; ++j) g[j] *= u[j];
@@ -948,7 +975,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
       }
     }
-  } else if (warp >= 6 && gather) {
+  } else if (warp >= 6 && warp < 14 && gather) {
     // -------------------------------------------------------------- gather
     // Two teams of four warps take stages in turn, so that one waits and reports while
     // the other keeps the copies coming: the copies alone take 460 clocks of a 512-clock
