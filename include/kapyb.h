@@ -516,8 +516,9 @@ KAPYB_API kapyb_status kapyb_reduce(kapyb_handle h, const kapyb_tensor2d *src,
  * the weights), kapyb_combine_rows without weights (sum over a token's rows) and
  * kapyb_route_backward.  A plan serves every product of the step.
  *
- * Integer and f32 arrays passed as plain pointers are dense device arrays aligned
- * to their element size.  The calls keep no state between them, use no handle
+ * Tensors have up to 2^30 rows and columns (elements lie anywhere in 64 bits).  Integer
+ * and f32 arrays passed as plain pointers are dense device arrays aligned to their
+ * element size.  The calls keep no state between them, use no handle
  * workspace and may be captured into a graph; `stream` must belong to the handle's
  * device, whichever device is current.  Indices, orders and offsets are read on the
  * device and may hold anything: one that leads outside its tensor names no group /
@@ -583,7 +584,7 @@ KAPYB_API kapyb_status kapyb_plan_rows(kapyb_handle h, const int32_t *index, int
 
 /* out[p] = epilogue(lhs[row(p)] . rhs of p's group) for the planned positions p:
  * group g holds positions offsets[g] .. offsets[g+1]-1 (device, int32 [groups+1], not
- * decreasing, at most out->size0), row(p) = order[p] / fan, or p itself when order is
+ * decreasing, at most out->size0; a smaller one counts as the one before it), row(p) = order[p] / fan, or p itself when order is
  * NULL (then fan is ignored).  fan = rows of the plan per row of lhs (the k of a top-k
  * routing whose index has k entries per token).  A row of lhs that does not exist
  * counts as zeros.  Rows of out behind the last planned position keep what they hold.
@@ -612,8 +613,8 @@ KAPYB_API kapyb_status kapyb_matmul_grouped(kapyb_handle h, const kapyb_tensor2d
  * for a group without rows.  lhs [source rows, K], grad [positions, N] (f16, bf16 or
  * f32, of one type), offsets / order / fan as in kapyb_matmul_grouped; a row that does not
  * exist counts as zeros.  Groups of out must not overlap (out_group_stride at least one
- * group's extent).  Sums in f32, for an f32 out 1024 positions at a time so that long
- * groups keep f32's precision, rounded once to out's type.  The same bits on every run. */
+ * group's extent).  Sums in f32 (on the tensor cores, for an f32 out, 1024 positions at a
+ * time, so that long groups keep f32's precision), rounded once to out's type.  The same bits on every run. */
 KAPYB_API kapyb_status kapyb_matmul_grouped_grad(kapyb_handle h, const kapyb_tensor2d *lhs,
                                                  const kapyb_tensor2d *grad, int32_t groups,
                                                  const int32_t *offsets, const int32_t *order,

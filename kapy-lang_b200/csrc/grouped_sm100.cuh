@@ -103,14 +103,23 @@ struct GroupedTable {
   int *first, *begin, *count;
 };
 
-// Builds the table from the plan's offsets; one warp.
+// Builds the table from the plan's offsets; one warp.  An offset below one in front of it
+// counts as that one, so that groups never overlap, whatever the memory holds: the number
+// of tiles stays below the bound the host has checked.
 __device__ __forceinline__ void build_tile_table(const int32_t *offsets, int groups, int rows, int tile_rows,
                                                  const GroupedTable &table, int lane) {
-  int before = 0;
+  int before = 0, high = 0;
   for (int g0 = 0; g0 < groups; g0 += 32) {
     const int g = g0 + lane;
     int b = 0, e = 0;
     if (g < groups) group_range(offsets, g, rows, b, e);
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, b, off);
+      if (lane >= off) b = max(b, o);
+    }
+    b = max(b, high);
+    high = __shfl_sync(0xffffffffu, b, 31);
     const int cnt = max(0, e - b);
     const int tiles = (cnt + tile_rows - 1) / tile_rows;
     int scan = tiles;
@@ -563,7 +572,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     ptx::tmem_relinquish<2>();
   }
   if constexpr (ADAPT) {
-    // group starts only, made ascending whatever the memory holds
+    // group starts only, made ascending as in build_tile_table
     if (warp == 0) {
       int high = 0;
       for (int g0 = 0; g0 <= p.groups; g0 += 32) {

@@ -76,12 +76,16 @@ kapyb_status launched(kapyb_handle h, const char *name, int kernels = 1) {
   return KAPYB_OK;
 }
 
+constexpr int32_t kMaxSize = 1 << 30;  // rows and columns: the kernels' index arithmetic adds to them
+
 bool empty(const kapyb_tensor2d *t) { return t->size0 == 0 || t->size1 == 0; }
 
 kapyb_status check_tensor(kapyb_handle h, const char *call, const char *what, const kapyb_tensor2d *t) {
   if (!t) return fail(h, KAPYB_INVALID_ARG, "%s: %s is NULL", call, what);
   if (t->size0 < 0 || t->size1 < 0 || t->stride0 < 0 || t->stride1 < 0 || t->offset_elems < 0)
     return fail(h, KAPYB_INVALID_ARG, "%s: %s has a negative size, stride or offset", call, what);
+  if (t->size0 > kMaxSize || t->size1 > kMaxSize)
+    return fail(h, KAPYB_UNSUPPORTED, "%s: %s has more than 2^30 rows or columns", call, what);
   if (!valid_dtype(t->dtype))
     return fail(h, KAPYB_INVALID_ARG, "%s: %s must have f16, bf16 or f32 element type", call, what);
   if (!t->ptr && !empty(t)) return fail(h, KAPYB_INVALID_ARG, "%s: %s has no data pointer", call, what);
@@ -466,7 +470,7 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
   gp.wait_limit_us = h->wait_limit_us;
   const long long busy = std::min(groups, gp.rows);
   const long long tiles = ((gp.rows + PairCfg::BT - 1ll) / PairCfg::BT + busy) * gp.n_tiles;
-  if (tiles >= (1ll << 31)) return KAPYB_OK;
+  if (tiles >= (1ll << 30)) return KAPYB_OK;
   const int64_t lhs_ld = lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8;
   CUtensorMap tmA, box[3];  // rows in plan order come in boxes of 128, 64 and 32
   TRY(make_tmap(h, &tmA, elem_ptr(rhs), rhs->dtype, unit, other, groups, ld, group_stride, 64, mn || gated ? 64 : 128));
@@ -509,7 +513,7 @@ kapyb_status grouped_grad_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, 
   gp.status = h->status;
   gp.wait_limit_us = h->wait_limit_us;
   const long long tiles = static_cast<long long>(groups) * gp.n_tiles * gp.k_tiles;
-  if (tiles >= (1ll << 31)) return KAPYB_OK;
+  if (tiles >= (1ll << 30)) return KAPYB_OK;
   CUtensorMap tmA;
   TRY(make_row_tmap(h, &tmA, elem_ptr(grad), grad->dtype, grad->size1, grad->size0,
                     grad->size0 > 1 ? grad->stride0 : (grad->size1 + 7) / 8 * 8, 64));
@@ -1040,7 +1044,7 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
   if (!(size >= 0.00390625f && size <= 256.0f)) return KAPYB_OK;
   const AdapterScratch sc(rows, c.groups, rank);
   const int n_tiles = (c.out->size1 + 255) / 256;
-  if (sc.positions >= (1ll << 30) || (sc.positions / 256 + 1) * n_tiles >= (1ll << 31)) return KAPYB_OK;
+  if (sc.positions >= (1ll << 30) || (sc.positions / 256 + 1) * n_tiles >= (1ll << 30)) return KAPYB_OK;
   char *scratch = static_cast<char *>(c.scratch);
   int32_t *order = reinterpret_cast<int32_t *>(scratch + sc.order);
   int32_t *offsets = reinterpret_cast<int32_t *>(scratch + sc.offsets);

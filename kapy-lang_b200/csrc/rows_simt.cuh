@@ -56,11 +56,12 @@ __global__ void __launch_bounds__(256) rows_simt_kernel(const RowsSimtParams p) 
   const int n0 = blockIdx.x * 32;
   for (int want = blockIdx.y;; want += gridDim.y) {
     if (threadIdx.x == 0) {
-      int left = want;
+      int left = want, high = 0;
       sg = -1;
       for (int g = 0; g < p.groups; ++g) {
         int b, e;
         group_range(p.offsets, g, p.rows, b, e);
+        high = b = max(b, high);  // as in the tensor-core kernels, groups never overlap
         const int blocks = e > b ? (e - b + 31) / 32 : 0;
         if (left < blocks) {
           sg = g;

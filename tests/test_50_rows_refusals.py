@@ -124,6 +124,19 @@ def test_grouped_arguments(pkg):
     d("overlaps", x, gr, 2, P(6), None, 1, t2(a, 16, 24, at=2), 384, 1.0, 1)
 
 
+def test_sizes_beyond_the_index_arithmetic(pkg):
+    a, big = pkg.abi, (1 << 30) + 1
+    no = lambda name, *args: refuse(pkg, "2^30", name, *args, status=a.UNSUPPORTED)
+    no("kapyb_route", t2(a, big, 16), None, routing(a), P(3), P(4))
+    no("kapyb_matmul_grouped", t2(a, 8, big), t2(a, big, 24, at=3), 1, 0, P(6), None, 1, t2(a, 8, 24, at=2), None, 0)
+    no("kapyb_matmul_grouped_grad", t2(a, big, 16), t2(a, big, 24, at=2), 1, P(6), None, 1, t2(a, 16, 24, at=3), 0,
+       1.0, 1)
+    no("kapyb_combine_rows", t2(a, 8, big), P(3), 2, None, t2(a, 4, big, at=2))
+    no("kapyb_combine_rows_backward", None, P(3), 2, None, t2(a, 4, big), t2(a, 8, big, at=2), None)
+    no("kapyb_matmul_adapters", t2(a, big, 16), t2(a, 16, 24, at=3), 1, t2(a, 16, 4, at=4), 0, t2(a, 4, 24, at=5), 0,
+       P(6), None, t2(a, big, 24, at=2), None, P(7), 1 << 19)
+
+
 def test_combine_arguments(pkg):
     a = pkg.abi
     rows, out = t2(a, 8, 16), t2(a, 4, 16, at=2)

@@ -531,6 +531,13 @@ def test_matmul_grouped_broken_plans(handle):
     handle.matmul_grouped(x, w, wild, out[:6], order=order)
     handle.check()
     assert (out[6:] == 2).all()
+    for dt in (torch.bfloat16, torch.float32):  # groups that seem to overlap: the first one has the rows
+        big, v = randn(4, 700, 64, dtype=dt), randn(5, 40, 64, 64, dtype=dt, std=0.125)
+        over = torch.tensor([0] + [700, 0] * 20, dtype=torch.int32, device=DEV)
+        got = handle.matmul_grouped(big, v, over)
+        handle.check()
+        val, tol = products_ref(big, v, torch.tensor([0] + [700] * 40), None, 1, False, 0, 1.0, None, dt, 64)
+        within(got, val, tol)
     d = handle.matmul_grouped_grad(x, randn(3, 6, 64, dtype=torch.bfloat16), wild, order=order)
     handle.check()
     assert d.shape == (3, 64, 64)
@@ -877,6 +884,47 @@ def test_experts_layer_in_a_graph_on_another_stream(handle, pkg, dt):
     got = layer(*held[1], stream=s.cuda_stream)
     s.synchronize()
     assert torch.equal(got, layer(*held[1]))
+
+
+def test_training_step_in_a_graph(handle, pkg):
+    """Forward and backward calls, long groups in pieces and adapters of many rows, captured
+    once and replayed on new inputs: the bits of eager calls."""
+    T, E, k, H, N = 1500, 2, 2, 128, 264
+    dt = torch.bfloat16
+    w = randn(3, E, H, N, dtype=dt, std=H ** -0.5)
+    wo, a, b = randn(5, H, N, dtype=dt, std=H ** -0.5), randn(6, 4, H, 24, dtype=dt), randn(7, 4, 24, N, dtype=dt)
+
+    def step(x, logits, g, who):
+        wts, e = handle.route(logits, k)
+        order, offsets, slots = handle.plan_rows(e, E)
+        y = handle.matmul_grouped(x, w, offsets, order=order, fan=k)
+        out = handle.combine_rows(y, slots, weights=wts)
+        dy, dwts = handle.combine_rows_backward(y, slots, g, weights=wts)
+        dw = handle.matmul_grouped_grad(x, dy, offsets, order=order, fan=k, out_dtype=torch.float32)
+        dx = handle.combine_rows(handle.matmul_grouped(dy, w.transpose(1, 2), offsets), slots)
+        dl = handle.route_backward(logits, e, dwts)
+        return out, dw, dx, dl, handle.matmul_adapters(x, wo, a, b, who)
+
+    def inputs(seed):
+        return (randn(seed, T, H, dtype=dt), randn(seed + 1, T, E), randn(seed + 2, T, N, dtype=dt),
+                torch.randint(-1, 4, (T,), generator=gen(seed), dtype=torch.int32).to(DEV))
+
+    held = inputs(50)
+    step(*held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*held)
+    for turn in range(3):
+        fresh = inputs(100 + 10 * turn)
+        for dst, src in zip(held, fresh):
+            dst.copy_(src)
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, (u, v) in enumerate(zip(got, step(*fresh))):
+            assert torch.equal(u, v), (turn, i)
+    handle.check()
 
 
 def test_python_refusals(handle, pkg):
