@@ -131,29 +131,88 @@ __global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p,
   }
 }
 
-// Any strides, types and alignment: one element per thread.
-__global__ void __launch_bounds__(256) combine_any_kernel(const CombineParams p) {
-  const unsigned long long id = static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x;
-  const long long t = id / static_cast<unsigned>(p.cols);
+// An element as it lies in memory, zero where it is not wanted.  What bounds the kernels of
+// single elements is the latency of their loads, so those of four rows are issued before
+// the first is widened, in an order the compiler keeps (four of 8192 tokens' rows of 2047
+// f16: 53 us, backward 84; an element at a time 117 and 129; rows of 2048 by pieces 39 and 59).
+template <int DT>
+struct RawOf {
+  using type = uint16_t;
+};
+template <>
+struct RawOf<KAPYB_F32> {
+  using type = uint32_t;
+};
+template <int DT>
+__device__ __forceinline__ typename RawOf<DT>::type raw_at(const char *at, bool wanted) {
+  typename RawOf<DT>::type v;
+  if constexpr (DT == KAPYB_F32)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.nc.u32 %0, [%1];\n\t}"
+                 : "=r"(v)
+                 : "l"(at), "r"(static_cast<int>(wanted)));
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %2, 0;\n\tmov.b16 %0, 0;\n\t@p ld.global.nc.u16 %0, [%1];\n\t}"
+                 : "=h"(v)
+                 : "l"(at), "r"(static_cast<int>(wanted)));
+  return v;
+}
+template <int DT>
+__device__ __forceinline__ float raw_to_f32(typename RawOf<DT>::type v) {
+  if constexpr (DT == KAPYB_F32) return __uint_as_float(v);
+  else return cvt_16_to_f32(v, DT);
+}
+
+// Any strides and alignment, the output in any type: a warp owns 32 * COLS columns of one
+// token, a lane every 32nd of them, with four rows' loads in flight.  UNIT: the rows'
+// columns are adjacent (offsets known to the compiler: the loop is bound by instructions).
+template <int DT, int COLS, bool UNIT>
+__global__ void __launch_bounds__(256) combine_any_kernel(const CombineParams p, uint32_t chunks) {
+  constexpr int U = 4;
+  const unsigned long long id = blockIdx.x * 8ull + (threadIdx.x >> 5);
+  const long long t = id / chunks;
   if (t >= p.tokens) return;
-  const long long col = id - t * static_cast<unsigned long long>(p.cols);
-  float acc = 0.0f;
-  for (int j = 0; j < p.k; ++j) {
-    const int s = p.slots[t * p.k + j];
-    if (s < 0 || s >= p.n_rows) continue;
-    const float w = p.weights ? p.weights[t * p.k + j] : 1.0f;
-    acc = fmaf(w, load_as_f32(p.rows, p.rows_dtype, s * p.rows_s0 + col * p.rows_s1), acc);
+  const int c0 = static_cast<int>(id - t * static_cast<unsigned long long>(chunks)) * (32 * COLS) + (threadIdx.x & 31);
+  constexpr int esz = DT == KAPYB_F32 ? 4 : 2;
+  const int out_esz = p.out_dtype == KAPYB_F32 ? 4 : 2;
+  const char *base = static_cast<const char *>(p.rows) + c0 * (UNIT ? 1ll : p.rows_s1) * esz;
+  char *out = static_cast<char *>(p.out) + (t * p.out_s0 + c0 * p.out_s1) * out_esz;
+  const long long pitch = p.rows_s0 * esz, step = (UNIT ? 32ll : 32 * p.rows_s1) * esz, out_step = 32 * p.out_s1 * out_esz;
+  float acc[COLS];
+#pragma unroll
+  for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;
+  for (int j0 = 0; j0 < p.k; j0 += U) {
+    typename RawOf<DT>::type raw[U][COLS];
+    float w[U];
+    bool on[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = j0 + u < p.k ? __ldg(p.slots + t * p.k + j0 + u) : -1;
+      on[u] = s >= 0 && s < p.n_rows;
+      w[u] = p.weights && j0 + u < p.k ? __ldg(p.weights + t * p.k + j0 + u) : 1.0f;
+      const char *row = base + s * pitch;
+#pragma unroll
+      for (int i = 0; i < COLS; ++i) raw[u][i] = raw_at<DT>(row + i * step, on[u] && c0 + 32 * i < p.cols);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!on[u]) continue;
+#pragma unroll
+      for (int i = 0; i < COLS; ++i) acc[i] = fmaf(w[u], raw_to_f32<DT>(raw[u][i]), acc[i]);
+    }
   }
-  store_from_f32(p.out, p.out_dtype, t * p.out_s0 + col * p.out_s1, acc, p.rounding);
+#pragma unroll
+  for (int i = 0; i < COLS; ++i)
+    if (c0 + 32 * i < p.cols) store_from_f32(out + i * out_step, p.out_dtype, 0, acc[i], p.rounding);
 }
 
 // Backward: one block per token.  A thread keeps its pieces of the output's gradient
 // only for the row at hand; the k inner products meet in a warp tree and then in
 // warp order, so a result is the same bits every time.
-// VEC: 16-byte pieces of one type everywhere; otherwise element by element.
+// VEC: 16-byte pieces of one type everywhere; otherwise a thread's elements lie a block
+// apart, all of type DT or (DT negative) each tensor's own.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256) combine_backward_kernel(const CombineParams p) {
-  constexpr int E = VEC ? (DT == KAPYB_F32 ? 4 : 8) : 1;
+  constexpr int E = VEC && DT != KAPYB_F32 ? 8 : 4;
   constexpr int esz = DT == KAPYB_F32 ? 4 : 2;
   constexpr int U = 4;  // rows in flight
   __shared__ float part[8][U];
@@ -173,13 +232,31 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const CombinePara
         if (p.weights) w[u] = p.weights[t * p.k + j0 + u];
       }
     }
-    for (int c = threadIdx.x * E; c < p.cols; c += blockDim.x * E) {
+    for (int c = threadIdx.x * (VEC ? E : 1); c < p.cols; c += blockDim.x * E) {
       float g[E];
+      // !VEC: element i of this thread, of a row at element `first`, stride s1
+      auto in_row = [&](int i) { return c + i * static_cast<int>(blockDim.x) < p.cols; };
+      auto type = [](int own) { return DT < 0 ? own : DT; };
+      auto bytes_at = [&](long long first, long long s1, int own) {
+        return (first + c * s1) * (type(own) == KAPYB_F32 ? 4 : 2);
+      };
+      auto step_of = [&](long long s1, int own) { return blockDim.x * s1 * (type(own) == KAPYB_F32 ? 4 : 2); };
       if constexpr (VEC) {
         unpack16B<DT>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const char *>(p.grad_out) +
                                                             (t * p.go_s0 + c) * esz)), g);
       } else {
-        g[0] = load_as_f32(p.grad_out, p.go_dtype, t * p.go_s0 + c * p.go_s1);
+        const char *src = static_cast<const char *>(p.grad_out) + bytes_at(t * p.go_s0, p.go_s1, p.go_dtype);
+        const long long step = step_of(p.go_s1, p.go_dtype);
+        if constexpr (DT >= 0) {
+          typename RawOf<DT>::type raw[E];
+#pragma unroll
+          for (int i = 0; i < E; ++i) raw[i] = raw_at<DT>(src + i * step, in_row(i));
+#pragma unroll
+          for (int i = 0; i < E; ++i) g[i] = raw_to_f32<DT>(raw[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < E; ++i) g[i] = in_row(i) ? load_as_f32(src + i * step, p.go_dtype, 0) : 0.0f;
+        }
       }
       if (p.grad_weights) {
         float f[U][E];
@@ -195,9 +272,27 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const CombinePara
 #pragma unroll
           for (int u = 0; u < U; ++u) unpack16B<DT>(q[u], f[u]);
         } else {
+          const long long step = step_of(p.rows_s1, p.rows_dtype);
+          auto row = [&](int u) {
+            return static_cast<const char *>(p.rows) + bytes_at(s[u] * p.rows_s0, p.rows_s1, p.rows_dtype);
+          };
+          if constexpr (DT >= 0) {
+            typename RawOf<DT>::type raw[U][E];
 #pragma unroll
-          for (int u = 0; u < U; ++u)
-            f[u][0] = s[u] >= 0 ? load_as_f32(p.rows, p.rows_dtype, s[u] * p.rows_s0 + c * p.rows_s1) : 0.0f;
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+              for (int i = 0; i < E; ++i) raw[u][i] = raw_at<DT>(row(u) + i * step, s[u] >= 0 && in_row(i));
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+              for (int i = 0; i < E; ++i) f[u][i] = raw_to_f32<DT>(raw[u][i]);
+          } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+              for (int i = 0; i < E; ++i)
+                f[u][i] = s[u] >= 0 && in_row(i) ? load_as_f32(row(u) + i * step, p.rows_dtype, 0) : 0.0f;
+          }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -217,7 +312,11 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const CombinePara
             __stcs(reinterpret_cast<uint4 *>(static_cast<char *>(p.grad_rows) + (s[u] * p.gr_s0 + c) * esz),
                    pack16B<DT>(o));
           } else {
-            store_from_f32(p.grad_rows, p.gr_dtype, s[u] * p.gr_s0 + c * p.gr_s1, w[u] * g[0], p.rounding);
+            char *dst = static_cast<char *>(p.grad_rows) + bytes_at(s[u] * p.gr_s0, p.gr_s1, p.gr_dtype);
+            const long long step = step_of(p.gr_s1, p.gr_dtype);
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+              if (in_row(i)) store_from_f32(dst + i * step, type(p.gr_dtype), 0, w[u] * g[i], p.rounding);
           }
         }
       }

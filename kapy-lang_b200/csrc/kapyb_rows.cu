@@ -697,6 +697,15 @@ void launch_combine_vec(const CombineParams &p, bool wide, uint32_t per_row, int
   else combine_vec_kernel<DT, false><<<grid, 256, 0, s>>>(p, per_row);
 }
 
+template <int DT>
+void launch_combine_any(const CombineParams &p, bool wide, uint32_t chunks, int grid, cudaStream_t s) {
+  const bool unit = p.rows_s1 == 1;
+  if (wide && unit) combine_any_kernel<DT, 8, true><<<grid, 256, 0, s>>>(p, chunks);
+  else if (wide) combine_any_kernel<DT, 8, false><<<grid, 256, 0, s>>>(p, chunks);
+  else if (unit) combine_any_kernel<DT, 2, true><<<grid, 256, 0, s>>>(p, chunks);
+  else combine_any_kernel<DT, 2, false><<<grid, 256, 0, s>>>(p, chunks);
+}
+
 kapyb_status check_slots(kapyb_handle h, const char *call, const int32_t *slots, int k, const float *weights) {
   if (k < 1 || k > kCombineMaxK)
     return fail(h, KAPYB_INVALID_ARG, "%s: k must be 1 to %d (got %d)", call, kCombineMaxK, k);
@@ -744,15 +753,22 @@ extern "C" KAPYB_API kapyb_status kapyb_combine_rows(kapyb_handle h, const kapyb
   p.rounding = KAPYB_RN;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool vec = rows->dtype == out->dtype && pieces_ok(rows, 16) && pieces_ok(out, 16);
-  const bool wide = vec && pieces_ok(rows, 32);
+  const bool wide = vec ? pieces_ok(rows, 32) : p.cols > 128;
+  // threads of a token: one per piece, or whole warps of 8 (few columns: 2) elements a lane
+  const int any = wide ? 256 : 64;
   const uint32_t per_row =
-      vec ? static_cast<uint32_t>(static_cast<int64_t>(p.cols) * dtype_size(rows->dtype) / (wide ? 32 : 16)) : p.cols;
-  const unsigned long long threads = static_cast<unsigned long long>(p.tokens) * per_row;
+      vec ? static_cast<uint32_t>(static_cast<int64_t>(p.cols) * dtype_size(rows->dtype) / (wide ? 32 : 16))
+          : (p.cols + any - 1) / any;
+  const unsigned long long threads = static_cast<unsigned long long>(p.tokens) * per_row * (vec ? 1 : 32);
   const unsigned long long blocks = (threads + 255) / 256;
   if (blocks > 0x7fffffffull) return fail(h, KAPYB_UNSUPPORTED, "%s: output too large", call);
   const int grid = static_cast<int>(blocks);
-  if (!vec)
-    combine_any_kernel<<<grid, 256, 0, s>>>(p);
+  if (!vec && rows->dtype == KAPYB_F32)
+    launch_combine_any<KAPYB_F32>(p, wide, per_row, grid, s);
+  else if (!vec && rows->dtype == KAPYB_BF16)
+    launch_combine_any<KAPYB_BF16>(p, wide, per_row, grid, s);
+  else if (!vec)
+    launch_combine_any<KAPYB_F16>(p, wide, per_row, grid, s);
   else if (rows->dtype == KAPYB_F32)
     launch_combine_vec<KAPYB_F32>(p, wide, per_row, grid, s);
   else if (rows->dtype == KAPYB_BF16)
@@ -817,13 +833,20 @@ extern "C" KAPYB_API kapyb_status kapyb_combine_rows_backward(kapyb_handle h, co
   }
   p.grad_weights = grad_weights;
   const int dt = grad_out->dtype;
-  const bool vec = pieces_ok(grad_out, 16) && (!rows || (rows->dtype == dt && pieces_ok(rows, 16))) &&
-                   (!grad_rows || (grad_rows->dtype == dt && pieces_ok(grad_rows, 16)));
+  const bool same = (!rows || rows->dtype == dt) && (!grad_rows || grad_rows->dtype == dt);
+  const bool vec = same && pieces_ok(grad_out, 16) && (!rows || pieces_ok(rows, 16)) &&
+                   (!grad_rows || pieces_ok(grad_rows, 16));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const long long units = vec ? static_cast<long long>(p.cols) * dtype_size(dt) / 16 : p.cols;
+  const long long units = vec ? static_cast<long long>(p.cols) * dtype_size(dt) / 16 : (p.cols + 3ll) / 4;
   const int threads = static_cast<int>(std::min(256ll, std::max(32ll, (units + 31) / 32 * 32)));
-  if (!vec)
+  if (!same)
+    combine_backward_kernel<-1, false><<<p.tokens, threads, 0, s>>>(p);
+  else if (!vec && dt == KAPYB_F32)
     combine_backward_kernel<KAPYB_F32, false><<<p.tokens, threads, 0, s>>>(p);
+  else if (!vec && dt == KAPYB_BF16)
+    combine_backward_kernel<KAPYB_BF16, false><<<p.tokens, threads, 0, s>>>(p);
+  else if (!vec)
+    combine_backward_kernel<KAPYB_F16, false><<<p.tokens, threads, 0, s>>>(p);
   else if (dt == KAPYB_F32)
     combine_backward_kernel<KAPYB_F32, true><<<p.tokens, threads, 0, s>>>(p);
   else if (dt == KAPYB_BF16)

@@ -671,6 +671,47 @@ def test_combine_rows_views(handle):
     assert handle.combine_rows(rows, torch.empty(0, 4, dtype=torch.int32, device=DEV)).shape == (0, 64)
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("N", [127, 129, 300, 1301])
+@pytest.mark.parametrize("layout", ["odd", "spread", "columns", "types"])
+def test_combine_rows_any_layout(handle, dt, N, layout):
+    """Rows that start anywhere, columns apart, rows behind one another column by column, and
+    tensors of three types: forward and backward."""
+    T, k, other = 11, 5, {torch.bfloat16: torch.float32, torch.float16: torch.bfloat16, torch.float32: torch.float16}
+
+    def view(seed, rows, dt):
+        if layout == "spread":
+            return randn(seed, rows, 2 * N + 1, dtype=dt)[:, 1::2]
+        if layout == "columns":
+            return randn(seed, N, rows, dtype=dt).t()
+        return randn(seed, rows, N, dtype=dt)
+
+    rows, dout = view(1, T * k, dt), view(2, T, other[dt] if layout == "types" else dt)
+    drows = view(3, T * k, other[other[dt]] if layout == "types" else dt)
+    slots = torch.randperm(T * k, generator=gen(4)).to(torch.int32).view(T, k).to(DEV)
+    slots[3, 2] = -1
+    kept = torch.ones(T * k, dtype=torch.bool, device=DEV)
+    kept[slots[slots >= 0].long()] = False
+    before = drows.clone()
+    w = randn(5, T, k)
+    out = torch.zeros_like(dout)
+    handle.combine_rows(rows, slots, out, weights=w)
+    _, dw = handle.combine_rows_backward(rows, slots, dout, weights=w, grad_rows=drows)
+    handle.check()
+    live = (slots >= 0).unsqueeze(2)
+    pick = torch.where(live, rows[slots.clamp(min=0).long()].double(), 0.0)
+    ww, g = w.double().unsqueeze(2), dout.double().unsqueeze(1)
+    val, slack = (pick * ww).sum(1), 2 * k * 2.0 ** -24 * (pick * ww).abs().sum(1)
+    within(out, val, slack + U[out.dtype] * (val.abs() + slack) + TINY[out.dtype])
+    want = torch.where(live, ww * g, 0.0)
+    got = drows[slots.clamp(min=0).long()]
+    within(torch.where(live, got, 0.0), want,
+           2.0 ** -24 * want.abs() + U[drows.dtype] * (1 + 2.0 ** -23) * want.abs() + TINY[drows.dtype])
+    assert torch.equal(drows[kept], before[kept])
+    wd = (pick * g).sum(2)
+    within(dw, wd, 2 * N * 2.0 ** -24 * (pick * g).abs().sum(2) + 2.0 ** -24 * wd.abs())
+
+
 # ------------------------------------------------------------------------ adapters
 
 def adapters_ref(x, w, a, b, index, scale, alpha, bias, bias_axis, act, out_dt):
