@@ -75,12 +75,9 @@ __device__ __forceinline__ float key_value(uint32_t key) {
 }
 
 __device__ __forceinline__ unsigned long long warp_max64(unsigned long long v) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const unsigned long long o = __shfl_xor_sync(0xffffffffu, v, off);
-    v = o > v ? o : v;
-  }
-  return v;
+  const uint32_t high = static_cast<uint32_t>(v >> 32), top = __reduce_max_sync(0xffffffffu, high);
+  const uint32_t low = __reduce_max_sync(0xffffffffu, high == top ? static_cast<uint32_t>(v) : 0u);
+  return static_cast<unsigned long long>(top) << 32 | low;
 }
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
