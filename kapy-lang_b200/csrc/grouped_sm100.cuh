@@ -571,6 +571,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     ptx::tmem_alloc<2>(ptx::smem_u32(tmem_slot), Cfg::TMEM_COLS);
     ptx::tmem_relinquish<2>();
   }
+  if constexpr (!ADAPT) {
+    // the set-up above ran under the end of the kernel in front; what follows reads its results
+    ptx::griddep_wait();
+    ptx::griddep_launch();
+  }
   if constexpr (ADAPT) {
     // group starts only, made ascending as in build_tile_table
     if (warp == 0) {

@@ -416,7 +416,7 @@ kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensor
     resident[h->device].store(pairs);
   }
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min<long long>(tiles, pairs)), 1, 1);
-  if (MODE == PAIR_ADAPTERS) cfg.numAttrs = 2;
+  cfg.numAttrs = 2;
   CUDA_TRY(h, cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmR, tmU, pp));
   return launched(h, MODE == PAIR_GRADIENT ? "grouped_grad_pair" : MODE == PAIR_ADAPTERS ? "adapters_pair" : "grouped_pair");
 }

@@ -16,6 +16,7 @@
 #include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "ptx_sm100.cuh"
 
 namespace kapyb {
 
@@ -47,6 +48,7 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ int32_t plan_smem[];
   __shared__ int scan_part[kPlanWarps];
+  ptx::griddep_launch();  // the product that reads the plan sets up meanwhile
   const int G = p.groups;
   const int pitch = plan_pitch(G);
   int32_t *count = plan_smem;                       // [kPlanWarps][pitch]
