@@ -8,6 +8,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "ptx_sm100.cuh"
 #include "reduce.cuh"
 
 namespace kapyb {
@@ -80,6 +81,7 @@ template <int DT, bool WIDE>
 __global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p, uint32_t pieces) {
   constexpr int esz = DT == KAPYB_F32 ? 4 : 2;
   constexpr int BYTES = WIDE ? 32 : 16, E = BYTES / esz, U = 4;
+  ptx::griddep_wait();
   const unsigned long long id = static_cast<unsigned long long>(blockIdx.x) * 256 + threadIdx.x;
   const long long t = id / pieces;
   if (t >= p.tokens) return;

@@ -139,6 +139,14 @@ kapyb_status check_epilogue(kapyb_handle h, const char *call, const kapyb_epilog
 
 const kapyb_epilogue kPlainEpilogue = {1.0f, nullptr, KAPYB_F32, 1, KAPYB_ACT_NONE, KAPYB_RN};
 
+// Launches.  A step is a chain of short kernels, so plan, products, weighted sums and the
+// adapters' second kernels are launched with programmatic serialization: they are set up
+// while the kernel in front ends, and every one of them waits for its end
+// (griddepcontrol.wait) before it reads or writes what another kernel may hold.  Each such
+// kernel has a thread that waits, so one that has ended vouches for all in front of it.
+// (Plan and product of 5331 rows 36.5 -> 31.4 us; a layer of 64 tokens x 2 of 8 experts in a
+// graph 35.3 -> 33.8 us, 512 x 2 of 16 68.6 -> 65.5; the smallest, one token, 29.2 -> 30.7.)
+
 // ------------------------------------------------------------------- routing
 
 kapyb_status check_routing(kapyb_handle h, const char *call, const kapyb_tensor2d *logits, const kapyb_routing *r) {
@@ -302,7 +310,7 @@ kapyb_status launch_plan(kapyb_handle h, const PlanParams &p, cudaStream_t strea
   if (ctas > 8)
     CUDA_TRY(h, cudaFuncSetAttribute(plan_rows_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(ctas, 1, 1);
   cfg.blockDim = dim3(kPlanWarps * 32, 1, 1);
   cfg.dynamicSmemBytes = smem;
@@ -311,8 +319,10 @@ kapyb_status launch_plan(kapyb_handle h, const PlanParams &p, cudaStream_t strea
   attr[0].val.clusterDim.x = ctas;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   CUDA_TRY(h, cudaLaunchKernelEx(&cfg, plan_rows_kernel, p));
   return launched(h, "plan_rows");
 }
@@ -392,7 +402,7 @@ kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensor
   auto kern = grouped_pair_kernel<MODE>;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // adapters: see grouped_sm100.cuh
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see "Launches" above
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.blockDim = dim3(kPairThreads, 1, 1);
   cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
@@ -693,8 +703,17 @@ bool pieces_ok(const kapyb_tensor2d *t, int bytes) {
 
 template <int DT>
 void launch_combine_vec(const CombineParams &p, bool wide, uint32_t per_row, int grid, cudaStream_t s) {
-  if (wide) combine_vec_kernel<DT, true><<<grid, 256, 0, s>>>(p, per_row);
-  else combine_vec_kernel<DT, false><<<grid, 256, 0, s>>>(p, per_row);
+  auto kern = wide ? combine_vec_kernel<DT, true> : combine_vec_kernel<DT, false>;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = s;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, p, per_row);
 }
 
 template <int DT>

@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ int32_t plan_smem[];
   __shared__ int scan_part[kPlanWarps];
-  ptx::griddep_launch();  // the product that reads the plan sets up meanwhile
+  ptx::griddep_launch();  // the product that reads the plan sets up meanwhile, as this does here
   const int G = p.groups;
   const int pitch = plan_pitch(G);
   int32_t *count = plan_smem;                       // [kPlanWarps][pitch]
@@ -62,6 +62,7 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
   const long long hi = min(static_cast<long long>(p.n), lo + step);
 
   for (int i = threadIdx.x; i < kPlanWarps * pitch; i += blockDim.x) count[i] = 0;
+  ptx::griddep_wait();
   __syncthreads();
   int32_t *mine = count + w * pitch;
   // walks this warp's piece, kPlanBatch steps of 32 entries at a time so that their loads

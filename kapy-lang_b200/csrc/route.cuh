@@ -29,6 +29,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "ptx_sm100.cuh"
 
 namespace kapyb {
 
@@ -333,6 +334,7 @@ __device__ __forceinline__ uint32_t number_key(float c) {
 // the bias comes in 16-byte pieces, and a logit that served as key is its own copy.
 template <int VPT, bool SCORED, bool VEC>
 __global__ void __launch_bounds__(256) route_kernel(const RouteParams p) {
+  ptx::griddep_launch();
   const int lane = threadIdx.x & 31;
   const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (row >= p.rows) return;
