@@ -482,9 +482,10 @@ kapyb_status grouped_on_tcgen05(kapyb_handle h, const kapyb_tensor2d *lhs, const
   const long long tiles = ((gp.rows + PairCfg::BT - 1ll) / PairCfg::BT + busy) * gp.n_tiles;
   if (tiles >= (1ll << 30)) return KAPYB_OK;
   const int64_t lhs_ld = lhs->size0 > 1 ? lhs->stride0 : (lhs->size1 + 7) / 8 * 8;
-  CUtensorMap tmA, box[3];  // rows in plan order come in boxes of 128, 64 and 32
+  CUtensorMap tmA;
   TRY(make_tmap(h, &tmA, elem_ptr(rhs), rhs->dtype, unit, other, groups, ld, group_stride, 64, mn || gated ? 64 : 128));
-  for (int i = 0; i < 3; ++i)
+  CUtensorMap box[3] = {tmA, tmA, tmA};  // rows in plan order come in boxes of 128, 64 and 32, others without
+  for (int i = 0; i < 3 && !order; ++i)
     TRY(make_row_tmap(h, &box[i], elem_ptr(lhs), lhs->dtype, lhs->size1, lhs->size0, lhs_ld, 128 >> i));
   *taken = true;
   const PairParams pp = pair_params(gp, lhs, order != nullptr);
