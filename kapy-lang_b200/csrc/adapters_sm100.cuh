@@ -57,8 +57,8 @@ __device__ __forceinline__ float widen16(uint16_t h) {
 
 // low[t]: a cluster of `split` blocks per row, each a run of K; the first one adds up.
 // KMAJOR: down has its unit stride on K, a warp per column of it; otherwise unit stride on
-// the rank, a thread per eight columns and K residue.  Sums in f32 in a fixed order.  Rows of down and x start on 16 bytes and rank is a multiple of 8
-// (!KMAJOR).
+// the rank, a thread per eight columns and K residue.  Sums in f32 in a fixed order.  Rows
+// of down and x start on 16 bytes and rank is a multiple of 8 (!KMAJOR).
 template <bool BF, bool KMAJOR>
 __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(const LowParams p) {
   ptx::griddep_launch();
@@ -109,7 +109,8 @@ __global__ void __launch_bounds__(kLowThreads) adapter_low_kernel(const LowParam
           }
         }
       }
-      for (int k = max(first_k, whole * 8) + lane; k < last_k; k += 32) acc = fmaf(widen16<BF>(x[k]), widen16<BF>(col[k]), acc);
+      for (int k = max(first_k, whole * 8) + lane; k < last_k; k += 32)
+        acc = fmaf(widen16<BF>(x[k]), widen16<BF>(col[k]), acc);
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
       if (lane == 0) mine[j] = acc;
@@ -636,7 +637,8 @@ __global__ void __launch_bounds__(kLowTileThreads) adapter_low_tile_kernel(const
       }
       const int k = kb * 64 + piece * 8;
       const uint32_t bytes = static_cast<uint32_t>(max(0, min(16, (p.K - k) * 2)));
-      const uint32_t dst = ptx::smem_u32(smem) + stage * kLowStageBytes + 16384u + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
+      const uint32_t dst =
+          ptx::smem_u32(smem) + stage * kLowStageBytes + 16384u + row0 * 128 + ((piece ^ (row0 & 7)) << 4);
       const long long off = bytes ? k * 2ll : 0ll;
 #pragma unroll
       for (int i = 0; i < kLowTile / 16; ++i)

@@ -100,9 +100,9 @@ __global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p,
     for (int u = 0; u < U; ++u) {
       on[u] = false;
       if (j0 + u < p.k) {
-        const int s = __ldg(p.slots + t * p.k + j0 + u);
+        const int s = p.slots[t * p.k + j0 + u];  // an ordinary load stays behind the wait
         on[u] = s >= 0 && s < p.n_rows;
-        w[u] = p.weights ? __ldg(p.weights + t * p.k + j0 + u) : 1.0f;
+        w[u] = p.weights ? p.weights[t * p.k + j0 + u] : 1.0f;
         if constexpr (WIDE) {
           if (on[u]) v[u] = ld_nc_v8(base + s * pitch);
         } else {
@@ -178,7 +178,8 @@ __global__ void __launch_bounds__(256) combine_any_kernel(const CombineParams p,
   const int out_esz = p.out_dtype == KAPYB_F32 ? 4 : 2;
   const char *base = static_cast<const char *>(p.rows) + c0 * (UNIT ? 1ll : p.rows_s1) * esz;
   char *out = static_cast<char *>(p.out) + (t * p.out_s0 + c0 * p.out_s1) * out_esz;
-  const long long pitch = p.rows_s0 * esz, step = (UNIT ? 32ll : 32 * p.rows_s1) * esz, out_step = 32 * p.out_s1 * out_esz;
+  const long long pitch = p.rows_s0 * esz, step = (UNIT ? 32ll : 32 * p.rows_s1) * esz;
+  const long long out_step = 32 * p.out_s1 * out_esz;
   float acc[COLS];
 #pragma unroll
   for (int i = 0; i < COLS; ++i) acc[i] = 0.0f;

@@ -241,7 +241,8 @@ __device__ __forceinline__ float4 transpose4(float a0, float a1, float a2, float
   const float s0 = __shfl_xor_sync(0xffffffffu, odd ? a0 : a1, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? a2 : a3, 1);
   // rows 0 and 2 in even lanes, 1 and 3 in odd ones, columns (even, odd) of the pair
   const float lo0 = odd ? s0 : a0, hi0 = odd ? a1 : s0, lo1 = odd ? s1 : a2, hi1 = odd ? a3 : s1;
-  const float t0 = __shfl_xor_sync(0xffffffffu, high ? lo0 : lo1, 2), t1 = __shfl_xor_sync(0xffffffffu, high ? hi0 : hi1, 2);
+  const float t0 = __shfl_xor_sync(0xffffffffu, high ? lo0 : lo1, 2);
+  const float t1 = __shfl_xor_sync(0xffffffffu, high ? hi0 : hi1, 2);
   return high ? make_float4(t0, t1, lo1, hi1) : make_float4(lo0, hi0, t0, t1);
 }
 
@@ -573,6 +574,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
   if constexpr (!ADAPT) {
     // the set-up above ran under the end of the kernel in front; what follows reads its results
+    // (with ordinary loads: the compiler may move those marked read-only across the wait)
     ptx::griddep_wait();
     ptx::griddep_launch();
   }
@@ -1036,7 +1038,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int q = t.p0 + kb * 64 + row0 + 16 * i;
-            entry[i] = q >= t.p1 ? -1 : p.order ? __ldg(p.order + q) : q;
+            entry[i] = q >= t.p1 ? -1 : p.order ? p.order[q] : q;
           }
         };
         fetch((turn & 1u) == static_cast<uint32_t>(team) ? 0 : 1);
@@ -1084,7 +1086,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
           const int r = rank * half + row0 + 16 * i;  // row of the tile
-          entry[i] = row0 + 16 * i < half && r < t.rows ? p.order ? __ldg(p.order + t.r0 + r) : t.r0 + r : -1;
+          entry[i] = row0 + 16 * i < half && r < t.rows ? p.order ? p.order[t.r0 + r] : t.r0 + r : -1;
         }
       };
       fetch(unit);

@@ -145,7 +145,7 @@ const kapyb_epilogue kPlainEpilogue = {1.0f, nullptr, KAPYB_F32, 1, KAPYB_ACT_NO
 // (griddepcontrol.wait) before it reads or writes what another kernel may hold.  Each such
 // kernel has a thread that waits, so one that has ended vouches for all in front of it.
 // (Plan and product of 5331 rows 36.5 -> 31.4 us; a layer of 64 tokens x 2 of 8 experts in a
-// graph 35.3 -> 33.8 us, 512 x 2 of 16 68.6 -> 65.5; the smallest, one token, 29.2 -> 30.7.)
+// graph 35.3 -> 33.8 us, 512 x 2 of 16 68.6 -> 65.3; one token 29.2 -> 29.0.)
 
 // ------------------------------------------------------------------- routing
 
@@ -428,7 +428,9 @@ kapyb_status launch_pairs(kapyb_handle h, const CUtensorMap &tmA, const CUtensor
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min<long long>(tiles, pairs)), 1, 1);
   cfg.numAttrs = 2;
   CUDA_TRY(h, cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmR, tmU, pp));
-  return launched(h, MODE == PAIR_GRADIENT ? "grouped_grad_pair" : MODE == PAIR_ADAPTERS ? "adapters_pair" : "grouped_pair");
+  return launched(h, MODE == PAIR_GRADIENT   ? "grouped_grad_pair"
+                     : MODE == PAIR_ADAPTERS ? "adapters_pair"
+                                             : "grouped_pair");
 }
 
 // Rows of lhs as TMA can fetch them: 16-bit, unit stride along K, 16-byte rows.
@@ -955,7 +957,7 @@ kapyb_status adapters_decode(kapyb_handle h, const AdapterCall &c, cudaStream_t 
   int delta = 0, stages = 0;
   for (;; split *= 2) {  // rows of a CTA's share of the output, in f32, beside the ring
     delta = (rows + split - 1) / split * 512;
-    const int budget = 232448 / per_sm - 3072 - delta;
+    const int budget = 232448 / per_sm - 3 * 1024 - delta;
     stages = std::min(8, budget / stage_bytes);
     // the ring also takes the partial sums
     if (stages >= 3 && stages * stage_bytes >= wide * 512) break;

@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kPlanWarps * 32) plan_rows_kernel(const PlanPa
 #pragma unroll
       for (int u = 0; u < kPlanBatch; ++u) {
         const long long i = i0 + 32 * u + lane;
-        g[u] = i < hi ? __ldg(p.index + i) : -1;
+        g[u] = i < hi ? p.index[i] : -1;
       }
 #pragma unroll
       for (int u = 0; u < kPlanBatch; ++u)
