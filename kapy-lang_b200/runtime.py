@@ -32,6 +32,7 @@ def _torch():
 
 _I32 = 2 ** 31 - 1
 _codes: dict = {}
+_Tensor2d = abi.Tensor2d  # what a constructor leaves out is zero
 
 
 def _current_stream(device: int) -> int:
@@ -206,7 +207,8 @@ class Handle:
             msg = self._lib.kapyb_last_error_string(None).decode()
             raise KapybError(st, msg)
         self.device = int(device)
-        self._torch_device = _torch().device("cuda", self.device)
+        self._t = _torch()
+        self._torch_device = self._t.device("cuda", self.device)
 
     def close(self):
         if getattr(self, "_h", None) is not None and self._h:
@@ -460,16 +462,15 @@ class Handle:
     def _launch_stream(self, stream):
         """(stream as an integer, context in which tensors the call allocates belong to it;
         None: the current stream, no context needed)."""
-        torch = _torch()
         if stream is None:
             return _current_stream(self.device), None
+        torch = self._t
         if not hasattr(stream, "cuda_stream"):
             stream = torch.cuda.ExternalStream(int(stream), device=self.device)
         return stream.cuda_stream, torch.cuda.stream(stream)
 
     def _new(self, where, shape, dtype, zero=False):
-        torch = _torch()
-        make = torch.zeros if zero else torch.empty
+        make = self._t.zeros if zero else self._t.empty
         if where is None:  # sizes one by one: a tuple of them costs torch 0.8 us more
             return make(*shape, dtype=dtype, device=self._torch_device)
         with where:
@@ -489,7 +490,7 @@ class Handle:
             raise ValueError(f"{name} must have element type {dtype}, not {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
-        return self._here(name, t)
+        return t.data_ptr() if t.get_device() == self.device else self._here(name, t)
 
     def _matrix(self, name, t):
         """Descriptor of a 2-D tensor on the handle's GPU."""
@@ -498,7 +499,8 @@ class Handle:
         (rows, cols), (s0, s1) = t.shape, t.stride()
         if rows > _I32 or cols > _I32 or s0 > _I32 or s1 > _I32:
             raise ValueError("sizes and strides must fit i32")
-        return abi.Tensor2d(self._here(name, t), 0, rows, cols, s0, s1, dtype_code(t.dtype), 0, 0, 0)
+        at = t.data_ptr() if t.get_device() == self.device else self._here(name, t)
+        return _Tensor2d(at, 0, rows, cols, s0, s1, _codes.get(t.dtype) or dtype_code(t.dtype))
 
     def _stack(self, name, t):
         """Descriptor of the first matrix of [groups, rows, columns] and the group stride."""
@@ -507,8 +509,8 @@ class Handle:
         (_, rows, cols), (stride, s0, s1) = t.shape, t.stride()
         if rows > _I32 or cols > _I32 or s0 > _I32 or s1 > _I32:
             raise ValueError("sizes and strides must fit i32")
-        return abi.Tensor2d(self._here(name, t), 0, rows, cols, s0, s1, dtype_code(t.dtype), 0, 0,
-                            0), stride
+        at = t.data_ptr() if t.get_device() == self.device else self._here(name, t)
+        return _Tensor2d(at, 0, rows, cols, s0, s1, _codes.get(t.dtype) or dtype_code(t.dtype)), stride
 
     def route(self, logits, top_k: int, *, bias=None, score: int = abi.SCORE_SOFTMAX,
               groups: int = 1, top_groups: Optional[int] = None, group_best: int = 1,
@@ -516,7 +518,7 @@ class Handle:
               stream=None):
         """Routing of rows to experts (kapyb_route): (weights f32 [T, k], experts int32
         [T, k]) of logits [T, E]; the bias (f32 [E]) takes part in the choice only."""
-        torch = _torch()
+        torch = self._t
         tl = self._matrix("logits", logits)
         shape = (tl.size0, int(top_k))
         at_bias = None
@@ -548,7 +550,7 @@ class Handle:
                        renormalize: bool = True, scale: float = 1.0, out=None, stream=None):
         """Gradient of the logits (kapyb_route_backward) from the gradient of route's
         weights; `experts`, score, renormalize and scale as in the forward call."""
-        torch = _torch()
+        torch = self._t
         tl = self._matrix("logits", logits)
         if experts.dim() != 2 or experts.shape[0] != tl.size0 or \
                 grad_weights.shape != experts.shape:
@@ -567,7 +569,7 @@ class Handle:
     def plan_rows(self, index, groups: int, *, order=None, offsets=None, slots=None, stream=None):
         """Stable counting sort of an int32 index (any shape) into groups
         (kapyb_plan_rows): (order [n], offsets [groups + 1], slots of index's shape)."""
-        torch = _torch()
+        torch = self._t
         n, groups = index.numel(), int(groups)
         s, where = self._launch_stream(stream)
         if order is None:
@@ -592,7 +594,7 @@ class Handle:
 
     def _plan(self, offsets, order, fan, groups, rows):
         """Addresses of a plan's offsets and order."""
-        torch = _torch()
+        torch = self._t
         if offsets.numel() != groups + 1:
             raise ValueError(f"offsets must have {groups + 1} elements")
         at = self._dense("offsets", offsets, torch.int32)
@@ -625,7 +627,9 @@ class Handle:
             out = self._new(where, (rows, tr.size1 // 2 if gated else tr.size1), out_dtype or lhs.dtype)
         elif out.shape[0] != rows:
             raise ValueError(f"out must have {rows} rows")
-        ep = self._epilogue(alpha, bias, 1, activation, rounding)
+        ep = None  # nothing to apply: the call's default
+        if bias is not None or activation or alpha != 1.0 or rounding != abi.RN:
+            ep = self._epilogue(alpha, bias, 1, activation, rounding)
         st = self._lib.kapyb_matmul_grouped(self._h, tl, tr, groups, group_stride, at_offsets,
                                             at_order, int(fan), self._matrix("out", out), ep,
                                             1 if gated else 0, s)
@@ -656,7 +660,7 @@ class Handle:
 
     def combine_rows(self, rows, slots, out=None, *, weights=None, out_dtype=None, stream=None):
         """out[t] = sum_j weights[t, j] * rows[slots[t, j]] (kapyb_combine_rows)."""
-        torch = _torch()
+        torch = self._t
         tr = self._matrix("rows", rows)
         if slots.dim() != 2 or (weights is not None and weights.shape != slots.shape):
             raise ValueError("slots and weights must be [tokens, k]")
@@ -679,7 +683,7 @@ class Handle:
         """Gradients of combine_rows (kapyb_combine_rows_backward): (grad_rows,
         grad_weights); the latter is None for a sum without weights.  A given grad_rows
         keeps the rows no slot names; an allocated one starts as zeros."""
-        torch = _torch()
+        torch = self._t
         tr, tg = self._matrix("rows", rows), self._matrix("grad_out", grad_out)
         if slots.dim() != 2 or tg.size0 != slots.shape[0] or \
                 any(t is not None and t.shape != slots.shape for t in (weights, grad_weights)):
@@ -706,7 +710,7 @@ class Handle:
         """lhs . rhs with every row's low-rank adapter beside it (kapyb_matmul_adapters):
         row t adds scale[i] * (lhs[t] . down[i]) . up[i], i = index[t]; an index outside
         the adapters adds nothing.  down [groups, K, rank], up [groups, rank, N]."""
-        torch = _torch()
+        torch = self._t
         tl, tr = self._matrix("lhs", lhs), self._matrix("rhs", rhs)
         td, down_stride = self._stack("down", down)
         tu, up_stride = self._stack("up", up)
@@ -724,7 +728,9 @@ class Handle:
         scratch = self._new(where, (nbytes,), torch.uint8)
         if out is None:
             out = self._new(where, (tl.size0, tr.size1), out_dtype or lhs.dtype)
-        ep = self._epilogue(alpha, bias, bias_axis, activation, rounding)
+        ep = None  # nothing to apply: the call's default
+        if bias is not None or activation or alpha != 1.0 or rounding != abi.RN or bias_axis != 1:
+            ep = self._epilogue(alpha, bias, bias_axis, activation, rounding)
         st = self._lib.kapyb_matmul_adapters(
             self._h, tl, tr, groups, td, down_stride, tu, up_stride,
             self._dense("index", index, torch.int32),
