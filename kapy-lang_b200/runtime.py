@@ -476,6 +476,11 @@ class Handle:
         with where:
             return make(*shape, dtype=dtype, device=self._torch_device)
 
+    def _fresh(self, where, rows, cols, dtype):
+        """A new matrix and its descriptor."""
+        t = self._new(where, (rows, cols), dtype)
+        return t, _Tensor2d(t.data_ptr(), 0, rows, cols, max(1, cols), 1, _codes.get(dtype) or dtype_code(dtype))
+
     def _here(self, name, t):
         """The tensor's address, once it is known to be on the handle's GPU."""
         if t.get_device() != self.device:
@@ -533,15 +538,19 @@ class Handle:
         held = (shape[0], max(0, shape[1]))  # a refused top_k is refused by the call itself
         if weights is None:
             weights = self._new(where, held, torch.float32)
+            at_weights = weights.data_ptr()
         elif weights.shape != shape:
             raise ValueError(f"weights must have shape {shape}")
+        else:
+            at_weights = self._dense("weights", weights, torch.float32)
         if experts is None:
             experts = self._new(where, held, torch.int32)
+            at_experts = experts.data_ptr()
         elif experts.shape != shape:
             raise ValueError(f"experts must have shape {shape}")
-        st = self._lib.kapyb_route(self._h, tl, at_bias, r,
-                                   self._dense("weights", weights, torch.float32),
-                                   self._dense("experts", experts, torch.int32), s)
+        else:
+            at_experts = self._dense("experts", experts, torch.int32)
+        st = self._lib.kapyb_route(self._h, tl, at_bias, r, at_weights, at_experts, s)
         if st != abi.OK:
             self._raise(st)
         return weights, experts
@@ -572,22 +581,19 @@ class Handle:
         torch = self._t
         n, groups = index.numel(), int(groups)
         s, where = self._launch_stream(stream)
-        if order is None:
-            order = self._new(where, (n,), torch.int32)
-        elif order.numel() != n:
-            raise ValueError(f"order must have {n} elements")
-        if offsets is None:
-            offsets = self._new(where, (max(0, groups) + 1,), torch.int32)
-        elif offsets.numel() != groups + 1:
-            raise ValueError(f"offsets must have {groups + 1} elements")
-        if slots is None:
-            slots = self._new(where, index.shape or (1,), torch.int32)
-        elif slots.numel() != n:
-            raise ValueError(f"slots must have {n} elements")
-        st = self._lib.kapyb_plan_rows(
-            self._h, self._dense("index", index, torch.int32), n, groups,
-            self._dense("order", order, torch.int32), self._dense("offsets", offsets, torch.int32),
-            self._dense("slots", slots, torch.int32), s)
+        def place(name, t, shape, count):
+            if t is None:
+                t = self._new(where, shape, torch.int32)
+                return t, t.data_ptr()
+            if t.numel() != count:
+                raise ValueError(f"{name} must have {count} elements")
+            return t, self._dense(name, t, torch.int32)
+
+        order, at_order = place("order", order, (n,), n)
+        offsets, at_offsets = place("offsets", offsets, (max(0, groups) + 1,), groups + 1)
+        slots, at_slots = place("slots", slots, index.shape or (1,), n)
+        st = self._lib.kapyb_plan_rows(self._h, self._dense("index", index, torch.int32), n, groups,
+                                       at_order, at_offsets, at_slots, s)
         if st != abi.OK:
             self._raise(st)
         return order, offsets, slots
@@ -624,15 +630,16 @@ class Handle:
             self._here("bias", bias)
         s, where = self._launch_stream(stream)
         if out is None:
-            out = self._new(where, (rows, tr.size1 // 2 if gated else tr.size1), out_dtype or lhs.dtype)
+            out, to = self._fresh(where, rows, tr.size1 // 2 if gated else tr.size1, out_dtype or lhs.dtype)
         elif out.shape[0] != rows:
             raise ValueError(f"out must have {rows} rows")
+        else:
+            to = self._matrix("out", out)
         ep = None  # nothing to apply: the call's default
         if bias is not None or activation or alpha != 1.0 or rounding != abi.RN:
             ep = self._epilogue(alpha, bias, 1, activation, rounding)
         st = self._lib.kapyb_matmul_grouped(self._h, tl, tr, groups, group_stride, at_offsets,
-                                            at_order, int(fan), self._matrix("out", out), ep,
-                                            1 if gated else 0, s)
+                                            at_order, int(fan), to, ep, 1 if gated else 0, s)
         if st != abi.OK:
             self._raise(st)
         return out
@@ -667,13 +674,14 @@ class Handle:
         tokens, k = slots.shape
         s, where = self._launch_stream(stream)
         if out is None:
-            out = self._new(where, (tokens, tr.size1), out_dtype or rows.dtype)
+            out, to = self._fresh(where, tokens, tr.size1, out_dtype or rows.dtype)
         elif out.shape[0] != tokens:
             raise ValueError("out must have a row per token")
+        else:
+            to = self._matrix("out", out)
         st = self._lib.kapyb_combine_rows(
             self._h, tr, self._dense("slots", slots, torch.int32), k,
-            None if weights is None else self._dense("weights", weights, torch.float32),
-            self._matrix("out", out), s)
+            None if weights is None else self._dense("weights", weights, torch.float32), to, s)
         if st != abi.OK:
             self._raise(st)
         return out
@@ -727,7 +735,9 @@ class Handle:
         nbytes = self._lib.kapyb_matmul_adapters_scratch(tl.size0, groups, td.size1)
         scratch = self._new(where, (nbytes,), torch.uint8)
         if out is None:
-            out = self._new(where, (tl.size0, tr.size1), out_dtype or lhs.dtype)
+            out, to = self._fresh(where, tl.size0, tr.size1, out_dtype or lhs.dtype)
+        else:
+            to = self._matrix("out", out)
         ep = None  # nothing to apply: the call's default
         if bias is not None or activation or alpha != 1.0 or rounding != abi.RN or bias_axis != 1:
             ep = self._epilogue(alpha, bias, bias_axis, activation, rounding)
@@ -735,7 +745,7 @@ class Handle:
             self._h, tl, tr, groups, td, down_stride, tu, up_stride,
             self._dense("index", index, torch.int32),
             None if scale is None else self._dense("scale", scale, torch.float32),
-            self._matrix("out", out), ep, scratch.data_ptr(), nbytes, s)
+            to, ep, scratch.data_ptr(), nbytes, s)
         if st != abi.OK:
             self._raise(st)
         return out
