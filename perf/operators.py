@@ -369,10 +369,10 @@ def run(st):
         if c["train"]:
             dx = h.matmul_grouped(st["dy"], st["w"].transpose(1, 2), offsets, st["dx"])
             dw = h.matmul_grouped_grad(st["x"], st["dy"], offsets, out_dtype=torch.float32, **via)
-            return order, offsets, slots.reshape(-1), dx, dw
+            return order, offsets, slots, dx, dw
         y = h.matmul_grouped(st["x"], st["w"], offsets, st["y"], gated=c["gated"],
                              activation=st["activation"], **via)
-        return order, offsets, slots.reshape(-1), y
+        return order, offsets, slots, y
     if c["op"] == "combine":
         out = h.combine_rows(st["rows"], st["slots"], weights=st["w"])
         if not c["train"]:
