@@ -19,7 +19,13 @@ def _library():
     if _handle is None:
         import __graft_entry__
         _package = __graft_entry__.load_package()
-        _handle = _package.Handle(0)
+
+        class Handle(_package.Handle):
+            def plan_rows(self, index, groups):
+                # slots have the shape of the index: a flat one, as the plain form's
+                return super().plan_rows(index.reshape(-1), groups)
+
+        _handle = Handle(0)
     return _package.abi, _handle
 
 
