@@ -648,13 +648,14 @@ KAPYB_API kapyb_status kapyb_combine_rows_backward(kapyb_handle h, const kapyb_t
  * and [rank, N], the next ones down_stride / up_stride elements later; scale f32
  * [groups] or NULL (1).  rank 1 .. 128.  alpha and bias apply to the shared part, as
  * in kapyb_matmul.  lhs, rhs, down, up: all f16, all bf16 or all f32; out f16 / bf16 /
- * f32.  The inner product scale * (lhs . down) is kept to at least 16 bits of precision
- * (in two values of the operands' type from 257 rows on, so with f16 operands it must stay
- * below 65504 there) and the whole sum is formed in f32.  What a row's own adapter or
- * values hold, NaN and infinities included, reaches no other row.  16-bit operands TMA can
- * describe (as in kapyb_matmul_grouped; up to 256 rows only lhs and rhs, and any alpha;
- * beyond, all four and an alpha of magnitude 1/256 .. 256) run on tcgen05, the rest on CUDA
- * cores.  The same bits on every run.  An inference operator: it has no gradient here
+ * f32.  The whole sum is formed in f32.  The inner product scale * (lhs . down) is an f32
+ * up to 256 rows and on CUDA cores.  From 257 rows on it is held in two values of the
+ * operands' type, which keep 16 bits of it; with f16 operands it must stay below 65504 there
+ * and is off by up to 2^-24 as well (|alpha| 2^-25 where that is more).  What a row's own
+ * adapter or values hold, NaN and infinities included, reaches no other row.  16-bit
+ * operands TMA can describe (as in kapyb_matmul_grouped; up to 256 rows only lhs and rhs, and
+ * any alpha; beyond, all four and an alpha of magnitude 1/256 .. 256) run on tcgen05, the
+ * rest on CUDA cores.  The same bits on every run.  An inference operator: it has no gradient here
  * (rhs, down and up of a training step are ordinary kapyb_matmul problems).
  * scratch: device memory of kapyb_matmul_adapters_scratch() bytes, 256-byte aligned,
  * the call's own until it has run on `stream`. */

@@ -491,7 +491,7 @@ struct LowTileParams {
   int d_mn_major, bf16;
   int a_bytes;           // of down in a stage: 8192 up to rank 64, else 16384
   const float *scale;
-  float alpha;           // 1 / the epilogue's scale
+  float alpha;           // 1 / what rows with an adapter are multiplied by at the end
   uint16_t *high, *low;  // [positions][pitch]
   int pitch;
   uint32_t *status;

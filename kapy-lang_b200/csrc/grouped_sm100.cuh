@@ -169,9 +169,9 @@ __device__ __forceinline__ void grouped_activation(int activation, float (&f)[R]
 }
 
 // Scale, bias and activation of 32 values of one output column.
-__device__ __forceinline__ void grouped_finish32(const GroupedParams &p, float (&f)[32], float bias) {
+__device__ __forceinline__ void grouped_finish32(const GroupedParams &p, float (&f)[32], float alpha, float bias) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = f[i] * p.alpha + bias;
+  for (int i = 0; i < 32; ++i) f[i] = f[i] * alpha + bias;
   grouped_activation(p.activation, f);
 }
 
@@ -391,6 +391,13 @@ __device__ __forceinline__ void grouped_scatter32(const GroupedParams &p, char *
 // The products come in two 16-bit
 // halves, so the second factor is exact to 16 bits and more.  Nothing is added twice to
 // memory and one rounding remains; what a broken adapter produces stays in its own rows.
+//
+// The accumulator is scaled as a whole at the end, so the products are divided by that
+// scale when they are stored.  f16 has no room for a quotient larger than the product, so a
+// scale of m 2^-s with 1 <= m < 2 and s > 0 is applied in two steps: the first MMA of an
+// adapter's blocks takes 2^-s of what its rows have accumulated (exact), the products are
+// divided by m only, and the end multiplies by m.  Rows without an adapter take the whole
+// scale at the end; a chunk of 32 rows has the one or the other.
 
 // Gated products: the 128 columns a CTA holds are 64 gate columns and the 64 up columns
 // that go with them, so the tile keeps its 256-wide MMA (two sets of columns beside one
@@ -412,6 +419,8 @@ struct PairParams {
   // adapters: g.groups = adapters + 1 (the last group: rows without one)
   int rank, up_mn_major;
   int low_rows;          // rows of one half of the low-rank products
+  float adapter_alpha;   // what rows with an adapter are multiplied by at the end,
+  int adapter_shift;     // and how often their shared part is halved before
 };
 
 constexpr int kPairThreads = 192 + 256 + 32 + 128;
@@ -812,9 +821,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             if (ptx::elect_one()) {
               const uint32_t a_lo = u_lo0 + static_cast<uint32_t>(stage) * (Cfg::A_BYTES >> 4);
               const uint32_t b_lo = b_lo0 + static_cast<uint32_t>(stage) * (Cfg::B_BYTES >> 4);
-              for (int k = 0; k < steps; ++k)
-                ptx::umma_k<2, 0>(d + (s0 - t.r0), (static_cast<uint64_t>(hi) << 32) | (a_lo + k * u_step),
-                                  (static_cast<uint64_t>(hi) << 32) | (b_lo + k * 2u), idesc_s, 1u);
+              for (int k = 0; k < steps; ++k) {
+                const uint64_t ad = (static_cast<uint64_t>(hi) << 32) | (a_lo + k * u_step);
+                const uint64_t bd = (static_cast<uint64_t>(hi) << 32) | (b_lo + k * 2u);
+                if (b == 0 && k == 0 && pp.adapter_shift > 0)
+                  ptx::umma_pair_f16_scaled(pp.adapter_shift, d + (s0 - t.r0), ad, bd, idesc_s);
+                else
+                  ptx::umma_k<2, 0>(d + (s0 - t.r0), ad, bd, idesc_s, 1u);
+              }
               ptx::umma_commit<2>(ptx::smem_u32(&empty_bar[stage]));
               ptx::umma_commit<2>(ptx::mapa(ptx::smem_u32(&empty_bar[stage]), 1));
             }
@@ -897,13 +911,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             // rows go where the plan took them from; lane l holds row c + l's number
             int to = c + lane < t.rows ? p.order[t.r0 + c + lane] : -1;
             if (to >= p.src_rows) to = -1;
+            const float alpha = t.r0 + c < table.begin[p.groups - 1] ? pp.adapter_alpha : p.alpha;
             if (p.bias != nullptr && p.bias_axis == 0) {
               const float row_bias = to >= 0 ? load_as_f32(p.bias, p.bias_dtype, to) : 0.0f;
 #pragma unroll
-              for (int j = 0; j < 32; ++j) f[j] = f[j] * p.alpha + __shfl_sync(0xffffffffu, row_bias, j);
+              for (int j = 0; j < 32; ++j) f[j] = f[j] * alpha + __shfl_sync(0xffffffffu, row_bias, j);
               grouped_activation(p.activation, f);
             } else {
-              grouped_finish32(p, f, bias);
+              grouped_finish32(p, f, alpha, bias);
             }
             grouped_scatter32(p, static_cast<char *>(p.out) + n * (p.out_dtype == KAPYB_F32 ? 4ll : 2ll), f, to, lane,
                               mine, both);
@@ -943,7 +958,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             const int first = c + (up_side ? 16 : 0);
             grouped_store(p, out + static_cast<long long>(first) * p.row_pitch, g, t.rows - first, lane, mine, both);
           } else {
-            grouped_finish32(p, f, bias);
+            grouped_finish32(p, f, p.alpha, bias);
             char *at = out + static_cast<long long>(c) * p.row_pitch;
             if (GRAD && piece > 0) {  // f32: to what the pieces before have left there
               add_rows32(at, p.row_pitch, f, t.rows - c, lane, mine, p.wide_stores);

@@ -1083,10 +1083,17 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
       !stack_tma_ok(c.down, c.groups, c.down_stride, d_mn, d_unit, d_other, d_ld) ||
       !stack_tma_ok(c.up, c.groups, c.up_stride, u_mn, u_unit, u_other, u_ld))
     return KAPYB_OK;
-  // the accumulator is scaled as a whole: the adapters' part is divided by alpha first,
-  // which needs an alpha that division does not push out of the 16-bit types' ranges
+  // the adapters' part is divided by alpha (or, in f16, by its mantissa), which needs an
+  // alpha that division does not push out of the 16-bit types' ranges
   const float size = std::fabs(c.ep.alpha);
   if (!(size >= 0.00390625f && size <= 256.0f)) return KAPYB_OK;
+  // f16: alpha = adapter_alpha 2^-shift, see grouped_sm100.cuh
+  int shift = 0;
+  if (c.lhs->dtype == KAPYB_F16 && size < 1.0f) {
+    std::frexp(size, &shift);  // size = fraction 2^shift, fraction in [1/2, 1)
+    shift = 1 - shift;
+  }
+  const float adapter_alpha = std::ldexp(c.ep.alpha, shift);
   const AdapterScratch sc(rows, c.groups, rank);
   const int n_tiles = (c.out->size1 + 255) / 256;
   if (sc.positions >= (1ll << 30) || (sc.positions / 256 + 1) * n_tiles >= (1ll << 30)) return KAPYB_OK;
@@ -1115,7 +1122,7 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
   lp.bf16 = c.lhs->dtype == KAPYB_BF16;
   lp.a_bytes = rank <= 64 ? 8192 : 16384;
   lp.scale = c.scale;
-  lp.alpha = 1.0f / c.ep.alpha;
+  lp.alpha = 1.0f / adapter_alpha;
   lp.high = reinterpret_cast<uint16_t *>(scratch + sc.low);
   lp.low = lp.high + static_cast<size_t>(positions) * low_pitch;
   lp.pitch = low_pitch;
@@ -1177,6 +1184,8 @@ kapyb_status adapters_pairs(kapyb_handle h, const AdapterCall &c, cudaStream_t s
   pp.rank = rank;
   pp.up_mn_major = u_mn;
   pp.low_rows = positions;
+  pp.adapter_alpha = adapter_alpha;
+  pp.adapter_shift = shift;
   TRY(make_tmap(h, &tmW, elem_ptr(c.rhs), c.rhs->dtype, w_unit, w_other, 1, w_ld, 0, 64, w_mn ? 64 : 128));
   TRY(make_tmap(h, &tmU, elem_ptr(c.up), c.up->dtype, u_unit, u_other, c.groups, u_ld, c.up_stride, 64,
                 u_mn ? 64 : 128));

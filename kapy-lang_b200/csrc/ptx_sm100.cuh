@@ -356,6 +356,35 @@ __device__ __forceinline__ void umma_k(uint32_t d_tmem, uint64_t a_desc, uint64_
   }
 }
 
+// A pair's kind::f16 MMA that adds to 2^-SCALE of what the accumulator holds.
+template <int SCALE>
+__device__ __forceinline__ void umma_pair_f16_scaled(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                     uint32_t idesc) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, 1, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p, %4;\n\t"
+      "}\n"
+      :
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "n"(SCALE)
+      : "memory");
+}
+// The same for a SCALE of 1 .. 8 known at run time.
+__device__ __forceinline__ void umma_pair_f16_scaled(int scale, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                     uint32_t idesc) {
+  switch (scale) {
+  case 1: return umma_pair_f16_scaled<1>(d_tmem, a_desc, b_desc, idesc);
+  case 2: return umma_pair_f16_scaled<2>(d_tmem, a_desc, b_desc, idesc);
+  case 3: return umma_pair_f16_scaled<3>(d_tmem, a_desc, b_desc, idesc);
+  case 4: return umma_pair_f16_scaled<4>(d_tmem, a_desc, b_desc, idesc);
+  case 5: return umma_pair_f16_scaled<5>(d_tmem, a_desc, b_desc, idesc);
+  case 6: return umma_pair_f16_scaled<6>(d_tmem, a_desc, b_desc, idesc);
+  case 7: return umma_pair_f16_scaled<7>(d_tmem, a_desc, b_desc, idesc);
+  default: return umma_pair_f16_scaled<8>(d_tmem, a_desc, b_desc, idesc);
+  }
+}
+
 template <int CTAS>
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                          uint32_t idesc, uint32_t accumulate) {

@@ -1,0 +1,86 @@
+"""Rows that pick their weights, at the ends of what the calls are documented to take.
+
+Tolerances as in test_51_gpu_rows.  Beyond 256 rows the low-rank part is 2 r more terms
+(two halves of each inner product) in the sum of the shared part, so all of it is one sum of
+K + 2 r terms.  The inner product is divided by d before it is stored as two 16-bit values and
+multiplied by d at the end (bf16: d = alpha; f16: alpha, or below 1 its mantissa, 1 <= d < 2).
+The second value is half a step off what the first one left: in bf16 2^-8 of 2^-8 of the
+product, in f16 2^-11 of 2^-11, but at least half of f16's smallest step, 2^-25 of what was
+stored, d 2^-25 of the product: below 2^-24 for d < 2, else |alpha| 2^-25."""
+import pytest
+import torch
+
+from test_51_gpu_rows import DEV, TINY, U, act_ref, make_adapters, randn, within
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------ adapters
+
+def adapters_want(x, w, a, b, index, scale, alpha, bias, bias_axis, act, out_dt):
+    """(value, tolerance) in 64 bits."""
+    K, r = a.shape[1], a.shape[2]
+    eps = 2.0 * (K + 2 * r + 16) * 2.0 ** -24
+    xd, wd, ad, bd = (t.double() for t in (x, w, a, b))
+    v = alpha * (xd @ wd)
+    size = abs(alpha) * (xd.abs() @ wd.abs())
+    low_err = torch.zeros_like(v)
+    if bias is not None:
+        bb = bias.double() if bias_axis == 1 else bias.double().unsqueeze(1)
+        v, size = v + bb, size + bb.abs()
+    for i in range(a.shape[0]):
+        rows = (index == i).nonzero().flatten()
+        s = 1.0 if scale is None else scale[i].double()
+        low = s * (xd[rows] @ ad[i])
+        e = 2.0 * (K + 8) * 2.0 ** -24 * abs(s) * (xd[rows].abs() @ ad[i].abs()) + \
+            2.0 ** -16 * low.abs() + max(2.0 ** -24, abs(alpha) * 2.0 ** -25)
+        v[rows] += low @ bd[i]
+        size[rows] += low.abs() @ bd[i].abs()
+        low_err[rows] += e @ bd[i].abs()
+    e = eps * size + low_err + 2.0 ** -22 * v.abs()
+    o = act_ref(v, act)
+    e = 1.15 * e + ((v.abs() + 8) * 2.0 ** -22 * o.abs() if act >= 2 else 0)
+    return o, e + U[out_dt] * (o.abs() + e) + TINY[out_dt]
+
+
+@pytest.mark.parametrize("T", [256, 257, 700])
+@pytest.mark.parametrize("alpha", [1 / 256, -0.5, 1.0, -2.0, 256.0, 1000.0])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_matmul_adapters_any_alpha(handle, T, alpha, dt):
+    """Inner products of some 300 beside any scale of the shared part, and one row more or
+    less does not change what a call can take."""
+    x, w, a, b, index = make_adapters((T, 4, 192, 144, 16, "each"), dt)
+    scale = torch.tensor([300.0, 1.0, 2.0 ** -10, 30.0], device=DEV)
+    out = handle.matmul_adapters(x, w, a, b, index, scale=scale, alpha=alpha, out_dtype=torch.float32)
+    handle.check()
+    val, tol = adapters_want(x, w, a, b, index, scale, alpha, None, 1, 0, torch.float32)
+    within(out, val, tol)
+
+
+@pytest.mark.parametrize("T", [200, 300])
+@pytest.mark.parametrize("alpha", [1 / 256, 1.0, 2.0, 16.0, 256.0])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_matmul_adapters_small_products(handle, T, alpha, dt):
+    """Inner products of 2^-10 and less with nothing else in the sum."""
+    x, w, a, b, index = make_adapters((T, 3, 128, 72, 16, "each"), dt)
+    scale = torch.tensor([2.0 ** -10, 2.0 ** -14, 1.0], device=DEV)
+    w = torch.zeros_like(w)
+    out = handle.matmul_adapters(x, w, a, b, index, scale=scale, alpha=alpha, out_dtype=torch.float32)
+    handle.check()
+    val, tol = adapters_want(x, w, a, b, index, scale, alpha, None, 1, 0, torch.float32)
+    within(out, val, tol)
+
+
+@pytest.mark.parametrize("alpha", [1 / 256, 0.3, 0.5, 0.999, -0.0625])
+@pytest.mark.parametrize("axis", [0, 1])
+def test_matmul_adapters_f16_scales_below_one(handle, alpha, axis):
+    """Rows with an adapter are scaled in two steps, rows without one at once."""
+    x, w, a, b, index = make_adapters((600, 4, 128, 144, 16, "each"), torch.float16)
+    bias = randn(8, 600 if axis == 0 else 144, dtype=torch.float16)
+    out = torch.full((600, 150), 3.0, device=DEV, dtype=torch.float16)
+    handle.matmul_adapters(x, w, a, b, index, out[:, 3:147], alpha=alpha, bias=bias, bias_axis=axis, activation=1)
+    handle.check()
+    assert handle.last_kernel == "adapters_pair"
+    val, tol = adapters_want(x, w, a, b, index, None, alpha, bias, axis, 1, torch.float16)
+    within(out[:, 3:147], val, tol)
+    assert (out[:, :3] == 3.0).all() and (out[:, 147:] == 3.0).all()
