@@ -651,8 +651,9 @@ KAPYB_API kapyb_status kapyb_combine_rows_backward(kapyb_handle h, const kapyb_t
  * f32.  The whole sum is formed in f32.  The inner product scale * (lhs . down) is an f32
  * up to 256 rows and on CUDA cores.  From 257 rows on it is held in two values of the
  * operands' type, which keep 16 bits of it; with f16 operands it must stay below 65504 there
- * and is off by up to 2^-24 as well (|alpha| 2^-25 where that is more).  What a row's own
- * adapter or values hold, NaN and infinities included, reaches no other row.  16-bit
+ * (beyond, it counts as infinite) and is off by up to 2^-24 as well (|alpha| 2^-25 where that
+ * is more); where `up` itself holds an infinity the row may be NaN and not infinite.  What a
+ * row's own adapter or values hold, NaN and infinities included, reaches no other row.  16-bit
  * operands TMA can describe (as in kapyb_matmul_grouped; up to 256 rows only lhs and rhs, and
  * any alpha; beyond, all four and an alpha of magnitude 1/256 .. 256) run on tcgen05, the
  * rest on CUDA cores.  The same bits on every run.  An inference operator: it has no gradient here

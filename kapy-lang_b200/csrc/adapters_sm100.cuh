@@ -692,7 +692,9 @@ __global__ void __launch_bounds__(kLowTileThreads) adapter_low_tile_kernel(const
           const uint16_t high = cvt_f32_to_16(f, DT, 1);
           const long long to = static_cast<long long>(p0 + r + u) * p.pitch + j;
           p.high[to] = high;
-          p.low[to] = cvt_f32_to_16(f - cvt_16_to_f32(high, DT), DT, 1);
+          // an infinite product leaves nothing (inf - inf would make a NaN of it)
+          const float held = cvt_16_to_f32(high, DT);
+          p.low[to] = cvt_f32_to_16(isinf(held) ? 0.0f : f - held, DT, 1);
         }
       }
     }

@@ -7,6 +7,8 @@ multiplied by d at the end (bf16: d = alpha; f16: alpha, or below 1 its mantissa
 The second value is half a step off what the first one left: in bf16 2^-8 of 2^-8 of the
 product, in f16 2^-11 of 2^-11, but at least half of f16's smallest step, 2^-25 of what was
 stored, d 2^-25 of the product: below 2^-24 for d < 2, else |alpha| 2^-25."""
+import math
+
 import pytest
 import torch
 
@@ -84,3 +86,19 @@ def test_matmul_adapters_f16_scales_below_one(handle, alpha, axis):
     val, tol = adapters_want(x, w, a, b, index, None, alpha, bias, axis, 1, torch.float16)
     within(out[:, 3:147], val, tol)
     assert (out[:, :3] == 3.0).all() and (out[:, 147:] == 3.0).all()
+
+
+@pytest.mark.parametrize("T", [200, 300])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_matmul_adapters_infinite_product(handle, T, dt):
+    """An inner product of +inf meets positive factors: +inf, and no other row changes."""
+    x, w, a, b, index = make_adapters((T, 3, 128, 72, 8, "each"), dt)
+    x[:, 0], b[1] = 1.0, b[1].abs() + 0.125
+    clean = handle.matmul_adapters(x, w, a, b, index)
+    a2 = a.clone()
+    a2[1, 0, 3] = math.inf
+    out = handle.matmul_adapters(x, w, a2, b, index)
+    handle.check()
+    hit = index == 1
+    assert hit.any() and (out[hit] == math.inf).all()
+    assert torch.equal(out[~hit], clean[~hit])
