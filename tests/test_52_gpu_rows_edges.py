@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from test_51_gpu_rows import DEV, TINY, U, act_ref, make_adapters, randn, within
+from test_51_gpu_rows import DEV, TINY, U, act_ref, gen, make_adapters, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +102,65 @@ def test_matmul_adapters_infinite_product(handle, T, dt):
     hit = index == 1
     assert hit.any() and (out[hit] == math.inf).all()
     assert torch.equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("T", [300, 700])
+@pytest.mark.parametrize("act", [0, 1, 2, 3])
+@pytest.mark.parametrize("axis", [0, 1, None])
+@pytest.mark.parametrize("dt, alpha", [(torch.bfloat16, 0.5), (torch.bfloat16, -2.0), (torch.float16, 1.5)])
+def test_matmul_adapters_epilogue_of_many_rows(handle, T, act, axis, dt, alpha):
+    x, w, a, b, index = make_adapters((T, 4, 128, 144, 16, "each"), dt)
+    for out_dt in (torch.float32, torch.bfloat16, torch.float16):
+        bias = None if axis is None else randn(8, 144 if axis == 1 else T, dtype=out_dt)
+        out = handle.matmul_adapters(x, w, a, b, index, alpha=alpha, bias=bias, bias_axis=axis or 0, activation=act,
+                                     out_dtype=out_dt)
+        handle.check()
+        assert handle.last_kernel == "adapters_pair"
+        val, tol = adapters_want(x, w, a, b, index, None, alpha, bias, axis, act, out_dt)
+        within(out, val, tol)
+
+
+@pytest.mark.parametrize("T", [300, 700])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_matmul_adapters_keep_many_requests_apart(handle, T, dt):
+    x, w, a, b, index = make_adapters((T, 4, 128, 128, 16, "each"), dt)
+    clean = handle.matmul_adapters(x, w, a, b, index)
+    a2, b2, x2 = a.clone(), b.clone(), x.clone()
+    a2[1], b2[2] = math.nan, math.inf
+    x2[0], x2[T - 1] = math.nan, math.inf
+    out = handle.matmul_adapters(x2, w, a2, b2, index)
+    handle.check()
+    assert handle.last_kernel == "adapters_pair"
+    hit = (index == 1) | (index == 2)
+    hit[0] = hit[T - 1] = True
+    assert torch.equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("T", [300, 513])
+@pytest.mark.parametrize("out_dt", [torch.bfloat16, torch.float32])
+def test_matmul_adapters_strides_of_many_rows(handle, T, out_dt):
+    """Views TMA can describe, outputs that start anywhere, an odd number of columns (weights
+    and up stored the other way round), and views it cannot."""
+    G, K, r = 3, 96, 16
+    for N in (112, 131):
+        bx = randn(1, T, K + 24, dtype=torch.bfloat16)
+        bw = randn(2, K + 3, 136, dtype=torch.bfloat16, std=0.1)
+        bt = randn(6, 136, K + 8, dtype=torch.bfloat16, std=0.1)
+        ba = randn(3, G + 1, K, r + 8, dtype=torch.bfloat16, std=0.1)
+        bb = randn(4, G, r + 1, 136, dtype=torch.bfloat16)
+        bu = randn(7, G, 136, r + 8, dtype=torch.bfloat16)
+        index = torch.randint(-1, G, (T,), generator=gen(5), dtype=torch.int32).to(DEV)
+        o = torch.full((T, N + 5), 3.0, device=DEV, dtype=out_dt)
+        straight = [(bx[:, 8:8 + K], bw[3:, :N], ba[1:, :, 8:], bb[:, 1:, :N], N % 8 == 0 or "adapters_pair"),
+                    (bx[:, :K], bt[:N, 8:].t(), ba[:G, :, :r], bu[:, :N, 8:].transpose(1, 2), "adapters_pair"),
+                    (bx[:, 1:1 + K], bw[:K, 1:1 + N], ba[:G, :, 1:1 + r], bb[:, :r, 3:3 + N], "adapter_simt")]
+        for x, w, a, b, kernel in straight:
+            for out in (o[:, :N], o[:, 5:], o[:, 4:4 + N]):
+                o.fill_(3.0)
+                handle.matmul_adapters(x, w, a, b, index, out)
+                handle.check()
+                assert kernel is True or handle.last_kernel == kernel
+                val, tol = adapters_want(x, w, a, b, index, None, 1.0, None, 1, 0, out_dt)
+                within(out, val, tol)
+                out.fill_(3.0)
+                assert (o == 3.0).all()
