@@ -136,6 +136,10 @@ __global__ void __launch_bounds__(256) rows_grad_simt_kernel(const RowsSimtParam
   for (int g = blockIdx.z; g < p.groups; g += gridDim.z) {
     int b, e;
     group_range(p.offsets, g, p.rows, b, e);
+    // an offset below one in front of it counts as that one: as in the other kernels, groups
+    // never overlap
+    for (int i = tx; i < g; i += 32) b = max(b, min(p.offsets[i], p.rows));
+    b = __reduce_max_sync(0xffffffffu, b);
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int q0 = b; q0 < e; q0 += 32) {
 #pragma unroll

@@ -164,3 +164,41 @@ def test_matmul_adapters_strides_of_many_rows(handle, T, out_dt):
                 within(out, val, tol)
                 out.fill_(3.0)
                 assert (o == 3.0).all()
+
+
+# ----------------------------------------------------------------- weight gradients
+
+def gradient_want(x, dy, offsets, order, fan, out_dt):
+    """(value, tolerance): offsets clamped to the positions and made ascending, positions
+    whose source does not exist left out on both sides."""
+    P, src = dy.shape[0], x.shape[0]
+    high, starts, ends = 0, [], []
+    raw = [min(max(o, 0), P) for o in offsets.tolist()]
+    for g in range(len(raw) - 1):
+        high = max(high, raw[g])
+        starts.append(high)
+        ends.append(max(high, raw[g + 1]))
+    val = torch.zeros(len(starts), x.shape[1], dy.shape[1], dtype=torch.float64, device=DEV)
+    tol = torch.zeros_like(val)
+    rows = torch.arange(P, device=DEV) if order is None else \
+        torch.where(order < 0, -1, torch.div(order.long(), fan, rounding_mode="floor"))
+    there = (rows >= 0) & (rows < src)
+    for g, (a, b) in enumerate(zip(starts, ends)):
+        on = there[a:b].nonzero().flatten() + a
+        xr, d = x[rows[on]].double(), dy[on].double()
+        val[g] = xr.t() @ d
+        tol[g] = 2.0 * (b - a + 4) * 2.0 ** -24 * (xr.abs().t() @ d.abs())
+    return val, tol + U[out_dt] * (val.abs() + tol) + TINY[out_dt]
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offsets", [[0, 10, 5, 20], [0] + [700, 0] * 20, [-7, 2, 900, 1], [30, 20, 10, 700],
+                                     [0, 300, 100, 400, 200, 700]])
+def test_matmul_grouped_grad_of_falling_offsets(handle, dt, offsets):
+    """An offset below the one before it counts as that one: no row in two groups."""
+    x, dy = randn(1, 700, 40, dtype=dt), randn(2, 700, 72, dtype=dt)
+    off = torch.tensor(offsets, dtype=torch.int32, device=DEV)
+    d = handle.matmul_grouped_grad(x, dy, off, out_dtype=torch.float32)
+    handle.check()
+    val, tol = gradient_want(x, dy, off, None, 1, torch.float32)
+    within(d, val, tol)
