@@ -18,8 +18,8 @@
 // Rows outside lhs, and the K tail of both operands, arrive as zeros.  A tile's rows
 // behind the end of its group may be those of the next group: they only reach output
 // rows that are not stored.  In the gradient the rows are the contraction, so there
-// everything behind a group's end is fetched as zeros on both sides (a zero on one
-// side alone would still let a NaN through).
+// everything behind a group's end, and every position whose entry names no row, is fetched
+// as zeros on both sides (a zero on one side alone would still let a NaN through).
 //
 // Persistent CTAs; warp 0 fetches columns, warp 1 issues the MMAs, warps 6..14 fetch rows
 // (below), warps 2..5 and 15..18 drain: two accumulator slots in TMEM let the drain of one
@@ -370,8 +370,9 @@ __device__ __forceinline__ void grouped_scatter32(const GroupedParams &p, char *
 // 4096 as one group: 259 us); eight nearly keep up.
 //
 // In the gradient the rows are the contraction: lhs is always gathered (zeros behind
-// the group's end); grad lies in plan order and comes by TMA, but for the block that
-// holds the group's end, which the gathering warps bring as well, with zeros behind it.
+// the group's end and for entries that name no row); grad lies in plan order and comes by
+// TMA, but for blocks of 64 positions that have such a place: those the gathering warps
+// bring as well, with zeros where lhs has them.  Both roles look at the block's entries.
 // The tensor core's f32 additions truncate: a sum loses about 1e-9 of itself per row (9e-6
 // over 8192 rows, measured; rounded sums 2e-7).  So an f32 gradient is accumulated 1024
 // rows at a time (1e-6 at any length): the epilogue joins two such pieces, one from each
@@ -416,6 +417,7 @@ struct PairParams {
   long long grad_pitch;
   int piece_kb;          // gradient: K blocks to an accumulator
   FastDiv div_fan;
+  uint32_t entries;      // entries of the plan below this name a row of lhs
   // adapters: g.groups = adapters + 1 (the last group: rows without one)
   int rank, up_mn_major;
   int low_rows;          // rows of one half of the low-rank products
@@ -630,7 +632,60 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const uint32_t full0 = ptx::mapa(ptx::smem_u32(full_bar), 0);  // the leader's barriers
   auto leader = [](const void *bar) { return ptx::mapa(ptx::smem_u32(bar), 0); };
 
-  if (warp == 0) {
+  // whether a plan entry (a position, without an order) names a row of lhs
+  auto names_row = [&](int entry) { return static_cast<uint32_t>(entry) < pp.entries; };
+
+  if (GRAD && warp == 0) {
+    // ---------------------------------------------- TMA: the columns' side, gradient
+    // The warp loads the entries of four blocks while those in front are fetched.
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int idx = unit; ok && idx < total; idx += units) {
+      const GroupedTile t = pair_tile<MODE>(p, table, idx);
+      const int n0 = t.n0 + rank * 128;
+      int entry[8];
+      auto fetch = [&](int kb) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int q = t.p0 + kb * 64 + 32 * u + lane;
+          entry[u] = q >= t.p1 ? -1 : p.order ? p.order[q] : q;
+        }
+      };
+      fetch(0);
+      for (int kb0 = 0; ok && kb0 < t.num_kb; kb0 += 4) {
+        uint32_t holes = 0u;  // of these four blocks: a position without a row
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (__any_sync(0xffffffffu, !names_row(entry[u]))) holes |= 1u << (u >> 1);
+        fetch(kb0 + 4);
+        if (lane == 0) {
+          for (int kb = kb0; kb < min(kb0 + 4, t.num_kb); ++kb) {
+            if (!ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) {
+              ok = false;
+              break;
+            }
+            const bool whole = !((holes >> (kb - kb0)) & 1u);
+            if (rank == 0) {
+              if (whole) ptx::mbar_arrive_expect_tx(ptx::smem_u32(&full_bar[stage]), 2u * Cfg::A_BYTES);
+              else ptx::mbar_arrive(ptx::smem_u32(&full_bar[stage]));
+            }
+            if (whole) {
+              const uint32_t fb = full0 + stage * 8u;
+              const uint32_t a_dst = ptx::smem_u32(sA) + stage * Cfg::A_BYTES;
+              tma_load_2d_pair(a_dst, &tmA, fb, n0, t.p0 + kb * 64);
+              tma_load_2d_pair(a_dst + 8192, &tmA, fb, n0 + 64, t.p0 + kb * 64);
+            }
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0) != 0;
+      }
+    }
+  } else if (!GRAD && warp == 0) {
     // -------------------------------------------------- TMA: the columns' side
     // One lane walks the loop: a load issued by several lanes at once is serialised with
     // its operands moved to uniform registers lane by lane, some 150 clocks each, and at
@@ -642,10 +697,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       // a free stage, its barrier told to expect `bytes` from both CTAs together
       auto open = [&](uint32_t bytes) -> bool {
         if (!ptx::mbar_wait(ptx::smem_u32(&empty_bar[stage]), phase ^ 1u, abort_flag)) return false;
-        if (rank == 0) {
-          if (bytes) ptx::mbar_arrive_expect_tx(ptx::smem_u32(&full_bar[stage]), bytes);
-          else ptx::mbar_arrive(ptx::smem_u32(&full_bar[stage]));
-        }
+        if (rank == 0) ptx::mbar_arrive_expect_tx(ptx::smem_u32(&full_bar[stage]), bytes);
         return true;
       };
       auto advance = [&]() {
@@ -659,20 +711,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const int n0 = t.n0 + rank * (GATED ? 64 : 128);
         const int second = GATED ? p.cols : 64;  // from the first 64 columns to the other 64
         for (int kb = 0; kb < t.num_kb; ++kb) {
-          const int q = t.p0 + kb * 64;
-          const bool tail = GRAD && t.p1 - q < 64;  // the gathering warps bring grad's rows as well
-          if (!open(tail ? 0u : 2u * Cfg::A_BYTES)) {
+          if (!open(2u * Cfg::A_BYTES)) {
             ok = false;
             break;
           }
           const uint32_t fb = full0 + stage * 8u;
           const uint32_t a_dst = ptx::smem_u32(sA) + stage * Cfg::A_BYTES;
-          if constexpr (GRAD) {
-            if (!tail) {
-              tma_load_2d_pair(a_dst, &tmA, fb, n0, q);
-              tma_load_2d_pair(a_dst + 8192, &tmA, fb, n0 + 64, q);
-            }
-          } else if (p.a_mn_major) {
+          if (p.a_mn_major) {
             ptx::tma_load_3d_pair(a_dst, &tmA, fb, n0, kb * 64, t.g);
             ptx::tma_load_3d_pair(a_dst + 8192, &tmA, fb, n0 + second, kb * 64, t.g);
           } else if (GATED) {
@@ -1028,9 +1073,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     };
     // source row of a plan entry, -1 for none
     auto row_of = [&](int entry) -> int {
-      if (entry < 0) return -1;
-      const int r = p.order ? pp.div_fan.div(entry) : entry;
-      return r < p.src_rows ? r : -1;
+      if (!names_row(entry)) return -1;
+      return p.order ? pp.div_fan.div(entry) : entry;
     };
     if constexpr (GRAD) {
       for (int idx = unit; ok && idx < total; idx += units) {
@@ -1046,14 +1090,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const bool need[2] = {piece * 8 < half, 64 + piece * 8 < half};
         const uint8_t *base = pp.lhs + (bytes[0] ? col * 2ll : 0ll);
         const uint32_t next_chunk = bytes[1] ? 128u : 0u;
-        // the plan's entries of this team's next block are loaded as soon as it has issued
-        // one, and only turned into row numbers when they are needed
-        int entry[4];
+        // the plan's entries of this team's next block (all 64, two a lane) are loaded as soon
+        // as it has issued one, and only turned into row numbers when they are needed
+        int entry[2];
         auto fetch = [&](int kb) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int q = t.p0 + kb * 64 + row0 + 16 * i;
-            entry[i] = q >= t.p1 ? -1 : p.order ? p.order[q] : q;
+          for (int u = 0; u < 2; ++u) {
+            const int q = t.p0 + kb * 64 + 32 * u + lane;
+            entry[u] = q >= t.p1 ? -1 : p.order ? p.order[q] : q;
           }
         };
         fetch((turn & 1u) == static_cast<uint32_t>(team) ? 0 : 1);
@@ -1065,22 +1109,23 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           }
           const uint32_t off = row0 * 128 + ((piece ^ (row0 & 7)) << 4);
           const uint32_t dst = ptx::smem_u32(sB) + stage * Cfg::B_BYTES + off;
+          int from[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) from[i] = row_of(__shfl_sync(0xffffffffu, entry[i >> 1], row0 + 16 * (i & 1)));
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int from = row_of(entry[i]);
-            const uint8_t *src = base + (from >= 0 ? from * pp.lhs_pitch : 0ll);
-            if (need[0]) cp_async16(dst + i * 2048, src, from >= 0 ? bytes[0] : 0u);
-            if (need[1]) cp_async16(dst + 8192 + i * 2048, src + next_chunk, from >= 0 ? bytes[1] : 0u);
+            const uint8_t *src = base + (from[i] >= 0 ? from[i] * pp.lhs_pitch : 0ll);
+            if (need[0]) cp_async16(dst + i * 2048, src, from[i] >= 0 ? bytes[0] : 0u);
+            if (need[1]) cp_async16(dst + 8192 + i * 2048, src + next_chunk, from[i] >= 0 ? bytes[1] : 0u);
           }
-          const int q0 = t.p0 + kb * 64;
-          if (t.p1 - q0 < 64) {  // grad's rows of the block with the group's end
+          if (__any_sync(0xffffffffu, !names_row(entry[0]) || !names_row(entry[1]))) {  // grad's, which TMA leaves out
             const uint32_t a_dst = ptx::smem_u32(sA) + stage * Cfg::A_BYTES + off;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int q = q0 + row0 + 16 * i;
+              const int q = t.p0 + kb * 64 + row0 + 16 * i;
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                const uint32_t have = q < t.p1 ? n_bytes[c] : 0u;
+                const uint32_t have = from[i] >= 0 ? n_bytes[c] : 0u;
                 cp_async16(a_dst + c * 8192 + i * 2048,
                            pp.grad + (have ? q * pp.grad_pitch + (n + c * 64) * 2ll : 0ll), have);
               }

@@ -390,6 +390,7 @@ PairParams pair_params(const GroupedParams &gp, const kapyb_tensor2d *lhs, bool 
   pp.lhs = static_cast<const uint8_t *>(elem_ptr(lhs));
   pp.lhs_pitch = lhs->stride0 * 2ll;
   pp.div_fan = FastDiv::make(static_cast<uint32_t>(gp.fan));
+  pp.entries = static_cast<uint32_t>(std::min<int64_t>(static_cast<int64_t>(gp.src_rows) * gp.fan, 1ll << 31));
   return pp;
 }
 

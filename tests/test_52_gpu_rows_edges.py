@@ -202,3 +202,32 @@ def test_matmul_grouped_grad_of_falling_offsets(handle, dt, offsets):
     handle.check()
     val, tol = gradient_want(x, dy, off, None, 1, torch.float32)
     within(d, val, tol)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("out_dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("fan", [1, 3])
+def test_matmul_grouped_grad_of_missing_rows(handle, dt, out_dt, fan):
+    """A position whose order names no row counts as zeros, whatever its gradient holds."""
+    src, P, E, K, N = 900, 2600, 4, 72, 264
+    x = randn(1, src, K, dtype=dt)
+    order = torch.randint(0, src * fan, (P,), generator=gen(3), dtype=torch.int32)
+    holes = torch.tensor([0, 63, 64, 130, 131, 199, 1000, 1500, 1501, 2400, 2599])
+    order[holes] = torch.tensor([-1, src * fan, 2 ** 31 - 1, -2 ** 31, src * fan + 1, -5, -1, -1, src * fan, -3, -1],
+                                dtype=torch.int32)
+    order = order.to(DEV)
+    offsets = torch.tensor([0, 200, 200, 2500, 2600], dtype=torch.int32, device=DEV)
+    dy = randn(2, P, N, dtype=dt)
+    clean = handle.matmul_grouped_grad(x, dy, offsets, order=order, fan=fan, out_dtype=out_dt)
+    val, tol = gradient_want(x, dy, offsets, order, fan, out_dt)
+    within(clean, val, tol)
+    dy[holes.to(DEV)] = math.nan
+    dy[holes[3].item()] = math.inf
+    d = handle.matmul_grouped_grad(x, dy, offsets, order=order, fan=fan, out_dtype=out_dt)
+    handle.check()
+    assert torch.equal(d, clean)
+    # a plan without holes is not affected, and a group of holes only has a gradient of zeros
+    order[200:2500] = -1
+    d = handle.matmul_grouped_grad(x, dy, offsets, order=order, fan=fan, out_dtype=out_dt)
+    handle.check()
+    assert (d[2] == 0).all() and torch.equal(d[[0, 3]], clean[[0, 3]])
