@@ -74,6 +74,27 @@ __device__ __forceinline__ void fma32B(const Vec32B &v, float w, float (&acc)[DT
   }
 }
 
+// 32 or 16 bytes of a row that the kernel in front may still be writing when this one is
+// set up: ordinary loads (the .nc ones are for memory nothing writes while a kernel lives),
+// kept behind the wait.
+__device__ __forceinline__ Vec32B ld_behind_v8(const void *p) {
+  Vec32B v;
+  asm volatile("ld.global.L1::no_allocate.v8.u32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]),
+                 "=r"(v.w[7])
+               : "l"(p)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 ld_behind_v4(const void *p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
 // Rows and output of one type, in pieces of 32 bytes (WIDE) or 16: a thread owns one
 // piece of one token and has the loads of four rows in flight before it adds them.
 // A row's rows lie anywhere, but a warp reads 1 KB runs of each.
@@ -104,9 +125,9 @@ __global__ void __launch_bounds__(256) combine_vec_kernel(const CombineParams p,
         on[u] = s >= 0 && s < p.n_rows;
         w[u] = p.weights ? p.weights[t * p.k + j0 + u] : 1.0f;
         if constexpr (WIDE) {
-          if (on[u]) v[u] = ld_nc_v8(base + s * pitch);
+          if (on[u]) v[u] = ld_behind_v8(base + s * pitch);
         } else {
-          if (on[u]) q[u] = __ldg(reinterpret_cast<const uint4 *>(base + s * pitch));
+          if (on[u]) q[u] = ld_behind_v4(base + s * pitch);
         }
       }
     }

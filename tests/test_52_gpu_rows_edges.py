@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from test_51_gpu_rows import DEV, TINY, U, act_ref, gen, make_adapters, randn, within
+from test_51_gpu_rows import DEV, TINY, U, act_ref, gen, make_adapters, plan_of, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -231,3 +231,33 @@ def test_matmul_grouped_grad_of_missing_rows(handle, dt, out_dt, fan):
     d = handle.matmul_grouped_grad(x, dy, offsets, order=order, fan=fan, out_dtype=out_dt)
     handle.check()
     assert (d[2] == 0).all() and torch.equal(d[[0, 3]], clean[[0, 3]])
+
+
+# ------------------------------------------------------------------ chains of calls
+
+@pytest.mark.parametrize("N", [2048, 1032])
+def test_weighted_sum_right_behind_the_product(handle, N):
+    """The sum is set up while the product in front still writes its rows: it reads what the
+    product has written, never what was there before."""
+    T, E, k, K = 512, 8, 4, 256
+    order, offsets, slots = plan_of(handle, 3, T, E, k)
+    w = randn(2, E, K, N, dtype=torch.bfloat16, std=K ** -0.5)
+    weights = randn(4, T, k)
+    y = torch.zeros(T * k, N, device=DEV, dtype=torch.bfloat16)
+    out, xs = torch.empty(T, N, device=DEV, dtype=torch.bfloat16), [randn(10 + i, T, K, dtype=torch.bfloat16)
+                                                                     for i in range(4)]
+    want = []
+    for x in xs:
+        handle.matmul_grouped(x, w, offsets, y, order=order, fan=k)
+        torch.cuda.synchronize()
+        want.append(handle.combine_rows(y, slots, weights=weights))
+        torch.cuda.synchronize()
+    for turn in range(40):
+        got = []
+        for x in xs:
+            handle.matmul_grouped(x, w, offsets, y, order=order, fan=k)
+            handle.combine_rows(y, slots, out, weights=weights)
+            got.append(out.clone())
+        for i, (u, v) in enumerate(zip(got, want)):
+            assert torch.equal(u, v), (turn, i)
+    handle.check()
