@@ -548,9 +548,8 @@ typedef struct {
  * who is chosen and is not part of the weights).  experts[t][j] is the expert with
  * the j-th largest c of row t among the kept groups, ties (of experts and of
  * groups) go to the lower index, and weights[t][j] = scale * s of it, renormalised
- * if asked.  The ranking is that of exactly evaluated scores: without a bias the
- * logits themselves are compared, and where 32 bits cannot tell two scores apart the
- * row is decided in 64 bits.
+ * if asked.  The ranking is that of the scores in 64 bits: where 32 bits cannot tell two
+ * apart the row is decided there, and without a bias the logits themselves are compared.
  * A logit of -inf masks its expert: score 0, never chosen.  Where fewer than top_k
  * experts are left the remaining entries are expert -1, weight 0 (a row of -inf, the
  * padding of a batch, names no expert at all).  A row with a NaN or +inf logit under
@@ -565,8 +564,8 @@ KAPYB_API kapyb_status kapyb_route(kapyb_handle h, const kapyb_tensor2d *logits,
  * grad_weights f32 [rows, top_k], grad_logits f16 / bf16 / f32 [rows, experts], any
  * strides, written whole.  The choice itself and the bias have no gradient; masked
  * experts get 0, and so do experts that were not chosen except under a softmax that
- * is not renormalised.  An expert named twice counts twice, an index outside
- * 0 .. experts-1 not at all. */
+ * is not renormalised (the only one for which more than the chosen logits is read).  An
+ * expert named twice counts twice, an index outside 0 .. experts-1 not at all. */
 KAPYB_API kapyb_status kapyb_route_backward(kapyb_handle h, const kapyb_tensor2d *logits,
                                             const kapyb_routing *routing, const int32_t *experts,
                                             const float *grad_weights,
@@ -596,8 +595,10 @@ KAPYB_API kapyb_status kapyb_plan_rows(kapyb_handle h, const int32_t *index, int
  * (dense [groups, columns of rhs], bias_axis 1), activation, rounding; NULL = none.
  * lhs and rhs: both f16, both bf16 (tensor cores) or both f32 (CUDA cores, multiplied
  * as f32), out f16 / bf16 / f32; sums in f32.  16-bit operands with 16-byte aligned
- * bases, leading dimensions and group stride, lhs with unit stride on K, run on
- * tcgen05; any other strides run on CUDA cores.  Up to 1024 groups.  The same bits on
+ * bases, leading dimensions and group stride, lhs with unit stride on K and out on its
+ * columns, run on tcgen05 (gated weights with their unit stride on the columns: N a multiple
+ * of 8 as well, since the up columns are fetched from a 16-byte boundary); any other strides
+ * run on CUDA cores, some 30 times as long.  Up to 1024 groups.  The same bits on
  * every run.  (The tensor cores' f32 additions truncate: a sum of K terms is off by about
  * K * 1e-9 of itself, as in kapyb_matmul.) */
 KAPYB_API kapyb_status kapyb_matmul_grouped(kapyb_handle h, const kapyb_tensor2d *lhs,
@@ -614,7 +615,8 @@ KAPYB_API kapyb_status kapyb_matmul_grouped(kapyb_handle h, const kapyb_tensor2d
  * f32, of one type), offsets / order / fan as in kapyb_matmul_grouped; a row that does not
  * exist counts as zeros.  Groups of out must not overlap (out_group_stride at least one
  * group's extent).  Sums in f32 (on the tensor cores, for an f32 out, 1024 positions at a
- * time, so that long groups keep f32's precision), rounded once to out's type.  The same bits on every run. */
+ * time, so that long groups keep f32's precision; a 16-bit out is summed at once and off by
+ * about 1e-9 of itself per position), rounded once to out's type.  The same bits on every run. */
 KAPYB_API kapyb_status kapyb_matmul_grouped_grad(kapyb_handle h, const kapyb_tensor2d *lhs,
                                                  const kapyb_tensor2d *grad, int32_t groups,
                                                  const int32_t *offsets, const int32_t *order,
@@ -656,8 +658,8 @@ KAPYB_API kapyb_status kapyb_combine_rows_backward(kapyb_handle h, const kapyb_t
  * row's own adapter or values hold, NaN and infinities included, reaches no other row.  16-bit
  * operands TMA can describe (as in kapyb_matmul_grouped; up to 256 rows only lhs and rhs, and
  * any alpha; beyond, all four and an alpha of magnitude 1/256 .. 256) run on tcgen05, the
- * rest on CUDA cores.  The same bits on every run.  An inference operator: it has no gradient here
- * (rhs, down and up of a training step are ordinary kapyb_matmul problems).
+ * rest on CUDA cores.  The same bits on every run.  An inference operator: it has no
+ * gradient here (rhs, down and up of a training step are ordinary kapyb_matmul problems).
  * scratch: device memory of kapyb_matmul_adapters_scratch() bytes, 256-byte aligned,
  * the call's own until it has run on `stream`. */
 KAPYB_API kapyb_status kapyb_matmul_adapters(kapyb_handle h, const kapyb_tensor2d *lhs,

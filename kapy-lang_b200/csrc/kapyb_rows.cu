@@ -68,11 +68,11 @@ kapyb_status allow_smem(kapyb_handle h, int bytes) {
   return KAPYB_OK;
 }
 
-kapyb_status launched(kapyb_handle h, const char *name, int kernels = 1) {
+kapyb_status launched(kapyb_handle h, const char *name) {
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(h, KAPYB_CUDA_ERROR, "%s: launch failed: %s", name, cudaGetErrorString(e));
   h->last_kernel = name;
-  h->launches += kernels;
+  h->launches += 1;
   return KAPYB_OK;
 }
 
@@ -144,8 +144,9 @@ const kapyb_epilogue kPlainEpilogue = {1.0f, nullptr, KAPYB_F32, 1, KAPYB_ACT_NO
 // while the kernel in front ends, and every one of them waits for its end
 // (griddepcontrol.wait) before it reads or writes what another kernel may hold.  Each such
 // kernel has a thread that waits, so one that has ended vouches for all in front of it.
-// (Plan and product of 5331 rows 36.5 -> 31.4 us; a layer of 64 tokens x 2 of 8 experts in a
-// graph 35.3 -> 33.8 us, 512 x 2 of 16 68.6 -> 65.3; one token 29.2 -> 29.0.)
+// (In replayed graphs: plan and product of 5331 rows 30.3 -> 28.6 us; a layer of one token x 2
+// of 8 experts 29.8 -> 29.0, 64 x 2 of 8 32.7 -> 32.5, 512 x 2 of 16 65.3 -> 64.4; adapters of
+// one row 14.5 -> 11.4.)
 
 // ------------------------------------------------------------------- routing
 
